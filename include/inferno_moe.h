@@ -52,9 +52,14 @@ enum inferno_quant {
   INFERNO_Q6_K = 14
 };
 
-enum inferno_dtype { INFERNO_F32 = 0, INFERNO_BF16 = 1 };
+/* INFERNO_I8: activations of the 4-bit products only. */
+enum inferno_dtype { INFERNO_F32 = 0, INFERNO_BF16 = 1, INFERNO_I8 = 2 };
 
 enum inferno_score_fn { INFERNO_SCORE_SIGMOID = 0, INFERNO_SCORE_SOFTMAX = 1 };
+
+/* A group of experts counts as its largest selection value, or as the sum of
+ * its two largest (of its one, if it has no two). */
+enum inferno_group_score { INFERNO_GROUP_MAX = 0, INFERNO_GROUP_TOP2 = 1 };
 
 /* Last error message of the calling thread ("" if none). */
 const char* inferno_last_error(void);
@@ -101,6 +106,21 @@ int inferno_moe_router_topk(void* stream, const float* logits, const float* bias
                             size_t E, size_t k, int score_fn, int norm_topk_prob,
                             float routed_scaling_factor, uint32_t* expert_ids,
                             float* expert_weights, uint32_t* token_indices);
+
+/* The same top-k over the best groups of experts: expert e is in group
+ * e / (E / n_group); the topk_group groups of the highest group_score stay open
+ * (ties go to the lower group), the others' experts are not selected.
+ * Selection values are sigmoid(l) + bias, or l + bias (softmax), compared in 64
+ * bits; -0 equals +0 and a NaN lies above +infinity, for its group too. Weights
+ * as above; softmax scores are normalised over all E experts, open or not, and
+ * a row of -infinity has weights 0. bias and token_indices may be NULL.
+ * n_group divides E, E <= 256, k <= min(16, topk_group * E / n_group).
+ * T = 0 does nothing. */
+int inferno_moe_router_group_topk(void* stream, const float* logits, const float* bias, size_t T,
+                                  size_t E, size_t k, int score_fn, int norm_topk_prob,
+                                  float routed_scaling_factor, size_t n_group, size_t topk_group,
+                                  int group_score, uint32_t* expert_ids, float* expert_weights,
+                                  uint32_t* token_indices);
 
 /* --------------------------------------------------------------- dispatch */
 
@@ -179,6 +199,65 @@ int inferno_q8_0_matvec_add2(void* stream, const void* w, size_t w_bytes, const 
                              size_t In, size_t O, float* out, void* workspace,
                              size_t workspace_bytes);
 
+/* ------------------------------------------------- 4-bit group-scaled weights */
+
+/* A matrix of 4-bit codes with one scale, and optionally one zero point, per
+ * `group` consecutive columns of a row, or `experts` such matrices one after
+ * another:
+ *   W[r, c] = scales[r, c / group] * (code[r, c] - zeros[r, c / group])
+ * codes: [experts * rows][cols / 2] bytes, column 2 j in the low nibble of byte
+ * j and column 2 j + 1 in the high one; scales: [experts * rows][cols / group]
+ * F32 or BF16; zeros: the same number of bytes, any value, or NULL: 8.
+ * cols is a multiple of 32 and of group; group is 32, 64 or a multiple of 128.
+ * codes lie at a multiple of 16 bytes. The byte lengths are checked. */
+typedef struct inferno_w4 {
+  size_t experts; /* 1: a plain matrix */
+  size_t rows, cols, group;
+  int scale_dtype; /* INFERNO_F32 or INFERNO_BF16 */
+  const void* codes;
+  const void* scales;
+  const void* zeros; /* or NULL */
+  size_t codes_bytes, scales_bytes, zeros_bytes;
+} inferno_w4;
+
+/* Activations x [T, cols] of the products below: F32, BF16, or I8 with
+ * x_scales [T, cols / x_group] fp32 (x = value * scale; x_group a multiple of
+ * 128 that divides cols, or 0: one scale per row; what
+ * inferno_add_rms_norm_q8 writes). x lies at a multiple of 16 bytes; x_scales
+ * and x_group are not read for F32 and BF16. The products of codes and
+ * activations are summed exactly within a group: bf16 activations enter whole
+ * (down to 2^-14 of the largest of their 128 columns), fp32 ones rounded to
+ * 2^-23 of it. A NaN or an infinity in x makes its token's outputs NaN.
+ * T = 0 does nothing. */
+
+/* Workspace bytes of the two dense products over T tokens of `cols` columns. */
+size_t inferno_w4_workspace_bytes(size_t T, size_t cols);
+
+/* out[T,rows] = residual_a + residual_b + W x, fp32; the residuals may be
+ * NULL, and out may be one of them. */
+int inferno_w4_matvec_add2(void* stream, const inferno_w4* w, const void* x, int x_dtype,
+                           const float* x_scales, size_t x_group, const float* residual_a,
+                           const float* residual_b, size_t T, float* out, void* workspace,
+                           size_t workspace_bytes);
+
+/* out[T,rows] = silu(W_gate x) * (W_up x). Both matrices have the same sizes,
+ * group, scale type, and both or neither have zero points. */
+int inferno_w4_gate_up_swiglu(void* stream, const inferno_w4* gate, const inferno_w4* up,
+                              const void* x, int x_dtype, const float* x_scales, size_t x_group,
+                              size_t T, float* out, void* workspace, size_t workspace_bytes);
+
+size_t inferno_w4_moe_workspace_bytes(size_t T, size_t k, size_t E, size_t H, size_t I);
+
+/* Routed experts: out[T,H] = sum_{r<k} W_down[e] (silu(W_gate[e] x_t) *
+ * (W_up[e] x_t)) * w, e and w the token's r-th id and weight, the ranks summed
+ * in a fixed order. gate, up: [experts][I][H]; down: [experts][H][I], which may
+ * have another group, scale type and zero points. experts <= 256, k <= 16.
+ * Ids of no expert count nothing. out must not alias an input. */
+int inferno_w4_moe(void* stream, const inferno_w4* gate, const inferno_w4* up,
+                   const inferno_w4* down, const void* x, int x_dtype, const float* x_scales,
+                   size_t x_group, const uint32_t* expert_ids, const float* expert_weights,
+                   size_t T, size_t k, float* out, void* workspace, size_t workspace_bytes);
+
 /* --------------------------------------------------------------- combine */
 
 /* out[T,H] = shared + residual + sum_{r<k} expert_outputs[t*k+r] * w[t*k+r],
@@ -208,6 +287,22 @@ int inferno_moe_gather_tokens(void* stream, const float* x, const uint32_t* toke
  * Replaces Backend::rms_norm (reference_rms_norm_f32, backend.rs:10211). */
 int inferno_rms_norm(void* stream, const float* x, const float* w, size_t rows, size_t H,
                      float eps, float* out);
+
+/* Residual addition, RMSNorm and 8-bit activations in one pass, per row:
+ *   s = x + residual (fp32; residual may be NULL: s = x);
+ *   y = s / sqrt(mean(s^2) + eps) * w, rounded to act_dtype (F32 or BF16);
+ *   q = rint(127 y / A), scale = A / 127, A = max |y| over each `group` columns
+ *     (32, 64 or 128, which divides H; 0: the row), so that y ~ q * scale. q is
+ *     the rounding of the exact quotient, ties to even.
+ * x is [rows,H] f32 or bf16. sum_out receives s, normed_out y, q_out [rows,H]
+ * int8 and scales_out [rows, H/group]; each may be NULL, q_out and scales_out
+ * together. sum_out may be residual, or an fp32 x; no other overlap. A group
+ * with a NaN or an infinity has q = 0 and a scale that is not finite. A group
+ * of zeros has q = 0, scale = 0. rows = 0 does nothing. */
+int inferno_add_rms_norm_q8(void* stream, const void* x, int x_dtype, const float* residual,
+                            const float* w, float eps, size_t rows, size_t H, size_t group,
+                            int act_dtype, float* sum_out, void* normed_out, int8_t* q_out,
+                            float* scales_out);
 
 /* Workspace bytes of inferno_rms_norm_router_topk with the top-k (T ticket
  * words, 256-byte aligned). The workspace must be zero-filled before its

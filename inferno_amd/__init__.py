@@ -7,7 +7,7 @@ benchmarks. There is no CPU fallback: if the library is missing, every call
 raises.
 """
 from ._lib import (  # noqa: F401
-    BF16, F32, Q2_K, Q3_K, Q4_K, Q6_K, Q8_0, SCORE_SIGMOID, SCORE_SOFTMAX,
-    InfernoError, LayerDesc, lib, lib_path, EXPORTED_SYMBOLS,
+    BF16, F32, GROUP_MAX, GROUP_TOP2, I8, Q2_K, Q3_K, Q4_K, Q6_K, Q8_0, SCORE_SIGMOID,
+    SCORE_SOFTMAX, InfernoError, LayerDesc, W4Desc, lib, lib_path, EXPORTED_SYMBOLS,
 )
 from . import ops  # noqa: F401

@@ -4,9 +4,10 @@ from pathlib import Path
 
 lib_path = Path(__file__).resolve().parent / "libinferno_moe.so"
 
-F32, BF16 = 0, 1
+F32, BF16, I8 = 0, 1, 2
 Q8_0, Q2_K, Q3_K, Q4_K, Q6_K = 8, 10, 11, 12, 14
 SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
 
 _vp, _sz, _i, _f, _u64 = C.c_void_p, C.c_size_t, C.c_int, C.c_float, C.c_uint64
 
@@ -31,6 +32,15 @@ class LayerDesc(C.Structure):
     ]
 
 
+class W4Desc(C.Structure):
+    """Mirror of `struct inferno_w4`."""
+    _fields_ = [
+        ("experts", _sz), ("rows", _sz), ("cols", _sz), ("group", _sz), ("scale_dtype", _i),
+        ("codes", _vp), ("scales", _vp), ("zeros", _vp),
+        ("codes_bytes", _sz), ("scales_bytes", _sz), ("zeros_bytes", _sz),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES = {
     "inferno_last_error": (C.c_char_p, []),
@@ -43,6 +53,8 @@ SIGNATURES = {
     "inferno_gguf_dequantize": (_i, [_vp, _i, _vp, _sz, _vp]),
     "inferno_router_logits": (_i, [_vp, _vp, _i, _vp, _sz, _sz, _sz, _vp]),
     "inferno_moe_router_topk": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _i, _i, _f, _vp, _vp, _vp]),
+    "inferno_moe_router_group_topk": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _i, _i, _f, _sz, _sz, _i,
+                                           _vp, _vp, _vp]),
     "inferno_moe_dispatch": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp]),
     "inferno_gguf_moe_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz]),
     "inferno_gguf_moe": (_i, [_vp, _i, _i, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _i, _vp, _vp,
@@ -60,9 +72,19 @@ SIGNATURES = {
     "inferno_moe_weighted_index_add_combine": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp]),
     "inferno_moe_gather_tokens": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _vp]),
     "inferno_rms_norm": (_i, [_vp, _vp, _vp, _sz, _sz, _f, _vp]),
+    "inferno_add_rms_norm_q8": (_i, [_vp, _vp, _i, _vp, _vp, _f, _sz, _sz, _sz, _i, _vp, _vp, _vp,
+                                     _vp]),
     "inferno_rms_norm_router_topk_workspace_bytes": (_sz, [_sz]),
     "inferno_rms_norm_router_topk": (_i, [_vp, _vp, _vp, _f, _vp, _vp, _sz, _sz, _sz, _sz, _i, _i,
                                           _f, _i, _vp, _vp, _vp, _vp, _vp, _sz]),
+    "inferno_w4_workspace_bytes": (_sz, [_sz, _sz]),
+    "inferno_w4_matvec_add2": (_i, [_vp, C.POINTER(W4Desc), _vp, _i, _vp, _sz, _vp, _vp, _sz, _vp,
+                                    _vp, _sz]),
+    "inferno_w4_gate_up_swiglu": (_i, [_vp, C.POINTER(W4Desc), C.POINTER(W4Desc), _vp, _i, _vp,
+                                       _sz, _sz, _vp, _vp, _sz]),
+    "inferno_w4_moe_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz]),
+    "inferno_w4_moe": (_i, [_vp, C.POINTER(W4Desc), C.POINTER(W4Desc), C.POINTER(W4Desc), _vp, _i,
+                            _vp, _sz, _vp, _vp, _sz, _sz, _vp, _vp, _sz]),
     "inferno_moe_layer_workspace_bytes": (_sz, [C.POINTER(LayerDesc), _sz]),
     "inferno_moe_layer_forward": (_i, [_vp, C.POINTER(LayerDesc), _vp, _i, _vp, _sz, _vp, _vp,
                                        _vp, _vp, _sz]),

@@ -9,6 +9,7 @@
 #include <string>
 #include <vector>
 
+#include "abi_common.hpp"
 #include "decode.hpp"
 #include "dense_q8.hpp"
 #include "prefill.hpp"
@@ -23,22 +24,6 @@ void set_error(const std::string& msg) { g_last_error = msg; }
 void clear_error() { g_last_error.clear(); }
 
 namespace {
-
-hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
-
-size_t align_up(size_t v) { return (v + 255) & ~size_t(255); }
-
-// Carves aligned sub-buffers out of a caller workspace.
-struct Carver {
-  char* base;
-  size_t used = 0;
-  template <typename T>
-  T* take(size_t count) {
-    T* p = reinterpret_cast<T*>(base ? base + used : nullptr);
-    used += align_up(count * sizeof(T));
-    return p;
-  }
-};
 
 bool is_routed_quant(int q) {
   return q == INFERNO_Q2_K || q == INFERNO_Q3_K || q == INFERNO_Q4_K;
@@ -175,29 +160,6 @@ int run_routed(hipStream_t s, int quant, int down_quant, const void* gate, const
   });
 }
 
-// The reference returns Ok(None) ("unsupported here, the caller may fall
-// back") when no native device backs the backend (backend.rs:6688-6692 and
-// the non-Metal branches); the counterpart here is INFERNO_UNSUPPORTED when
-// the process sees no HIP device. Argument errors are reported before this
-// check, as the reference validates before it looks for the device.
-int require_device() {
-  static const int count = [] {
-    int n = 0;
-    return hipGetDeviceCount(&n) == hipSuccess ? n : 0;
-  }();
-  if (count > 0) return INFERNO_OK;
-  set_error("no HIP device is available (unsupported here; the caller may fall back)");
-  return INFERNO_UNSUPPORTED;
-}
-
-int need_ws(void* ws, size_t have, size_t need) {
-  if (need > 0 && (ws == nullptr || have < need)) {
-    set_error("workspace too small: need " + std::to_string(need) + " bytes");
-    return INFERNO_ERR_SIZE;
-  }
-  return INFERNO_OK;
-}
-
 }  // namespace
 }  // namespace inferno
 
@@ -289,6 +251,35 @@ int inferno_moe_router_topk(void* stream, const float* logits, const float* bias
   if (int st_ = require_device()) return st_;
   return launch_router_topk(as_stream(stream), logits, bias, T, E, k, score_fn, norm_topk_prob,
                             routed_scaling_factor, expert_ids, expert_weights, token_indices);
+}
+
+int inferno_moe_router_group_topk(void* stream, const float* logits, const float* bias, size_t T,
+                                  size_t E, size_t k, int score_fn, int norm_topk_prob,
+                                  float routed_scaling_factor, size_t n_group, size_t topk_group,
+                                  int group_score, uint32_t* expert_ids, float* expert_weights,
+                                  uint32_t* token_indices) {
+  clear_error();
+  INF_CHECK_ARG(E > 0 && E <= size_t(kMaxExperts), "expert_count must be in 1..=256");
+  INF_CHECK_ARG(n_group > 0 && E % n_group == 0, "the groups must divide the experts evenly");
+  INF_CHECK_ARG(topk_group > 0 && topk_group <= n_group, "topk_group must be in 1..=n_group");
+  INF_CHECK_ARG(k > 0 && k <= size_t(kMaxTopK), "top_k must be in 1..=16");
+  if (k > topk_group * (E / n_group)) {
+    set_error("top_k " + std::to_string(k) + " exceeds the " +
+              std::to_string(topk_group * (E / n_group)) + " experts of the selected groups");
+    return INFERNO_ERR_INVALID;
+  }
+  INF_CHECK_ARG(score_fn == INFERNO_SCORE_SIGMOID || score_fn == INFERNO_SCORE_SOFTMAX,
+                "score_fn must be SIGMOID or SOFTMAX");
+  INF_CHECK_ARG(group_score == INFERNO_GROUP_MAX || group_score == INFERNO_GROUP_TOP2,
+                "group_score must be GROUP_MAX or GROUP_TOP2");
+  INF_CHECK_ARG(std::isfinite(routed_scaling_factor), "routed scaling factor must be finite");
+  INF_CHECK_ARG(T < (size_t(1) << 26), "too many tokens");
+  if (T == 0) return INFERNO_OK;
+  INF_CHECK_ARG(logits && expert_ids && expert_weights, "null pointer");
+  if (int st_ = require_device()) return st_;
+  return launch_group_topk(as_stream(stream), logits, bias, T, E, k, score_fn, norm_topk_prob,
+                           routed_scaling_factor, n_group, topk_group, group_score, expert_ids,
+                           expert_weights, token_indices);
 }
 
 int inferno_moe_dispatch(void* stream, const uint32_t* expert_ids, size_t T, size_t k, size_t E,
@@ -488,6 +479,30 @@ int inferno_rms_norm(void* stream, const float* x, const float* w, size_t rows, 
   INF_CHECK_ARG(rows == 0 || (x && w && out), "null pointer");
   if (int st_ = require_device()) return st_;
   return launch_rms_norm(as_stream(stream), x, w, rows, H, eps, out, INFERNO_F32);
+}
+
+int inferno_add_rms_norm_q8(void* stream, const void* x, int x_dtype, const float* residual,
+                            const float* w, float eps, size_t rows, size_t H, size_t group,
+                            int act_dtype, float* sum_out, void* normed_out, int8_t* q_out,
+                            float* scales_out) {
+  clear_error();
+  INF_CHECK_ARG(x_dtype == INFERNO_F32 || x_dtype == INFERNO_BF16, "x dtype must be F32 or BF16");
+  INF_CHECK_ARG(act_dtype == INFERNO_F32 || act_dtype == INFERNO_BF16,
+                "act dtype must be F32 or BF16");
+  INF_CHECK_ARG(H > 0 && eps >= 0.f && std::isfinite(eps),
+                "the norm needs a positive width and a finite eps >= 0");
+  INF_CHECK_ARG(group == 0 || group == 32 || group == 64 || group == 128,
+                "group must be 0 (the row), 32, 64 or 128");
+  INF_CHECK_ARG(group == 0 || H % group == 0, "the width must be a multiple of the group");
+  INF_CHECK_ARG(rows < (size_t(1) << 24), "too many rows");
+  INF_CHECK_ARG((q_out == nullptr) == (scales_out == nullptr),
+                "8-bit values and their scales are asked for together");
+  if (rows == 0) return INFERNO_OK;
+  INF_CHECK_ARG(x && w, "null pointer");
+  if (int st_ = require_device()) return st_;
+  return launch_add_norm_q8(as_stream(stream), AddNormQ8{x, x_dtype, residual, w, eps, rows, H,
+                                                         group, act_dtype, sum_out, normed_out,
+                                                         q_out, scales_out});
 }
 
 size_t inferno_rms_norm_router_topk_workspace_bytes(size_t T) {

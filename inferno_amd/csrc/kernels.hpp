@@ -68,6 +68,29 @@ int launch_gather(hipStream_t s, const float* x, const uint32_t* token_idx, size
 int launch_rms_norm(hipStream_t s, const float* x, const float* w, size_t rows, size_t H,
                     float eps, void* out, int out_dtype = INFERNO_F32);
 
+// Residual addition, RMSNorm and 8-bit activations (add_norm_q8.hip). residual,
+// sum, normed, and q with scales may be null; sum may be residual or x.
+struct AddNormQ8 {
+  const void* x;
+  int x_dtype;
+  const float* residual;
+  const float* w;
+  float eps;
+  size_t rows, H, group;  // group 0: the row
+  int act_dtype;          // of normed
+  float* sum;
+  void* normed;
+  int8_t* q;
+  float* scales;
+};
+int launch_add_norm_q8(hipStream_t s, const AddNormQ8& p);
+
+// Top-k over the topk_group best of `groups` groups of experts (group_topk.hip).
+int launch_group_topk(hipStream_t s, const float* logits, const float* bias, size_t T, size_t E,
+                      size_t k, int score_fn, int norm, float scale, size_t groups,
+                      size_t topk_group, int rule, uint32_t* ids, float* weights,
+                      uint32_t* token_idx);
+
 // RMSNorm -> router logits (-> top-k when ids is not null) in one launch
 // (norm_router.hip); tickets: T words, zero on entry, left zero.
 bool norm_router_supported(size_t T, size_t H, size_t E, size_t k);

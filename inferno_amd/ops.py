@@ -7,7 +7,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import BF16, F32, Q8_0, LayerDesc, check, lib
+from ._lib import BF16, F32, I8, Q8_0, LayerDesc, W4Desc, check, lib
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
 
@@ -167,6 +167,180 @@ def rms_norm(x, w, eps):
     rows, H = x.shape
     out = torch.empty_like(x)
     check(lib().inferno_rms_norm(_s(), _p(_dev(x)), _p(w), rows, H, float(eps), _p(out)))
+    return out
+
+
+def _like(x, name, t, dtype, *shape):
+    """Refuses a tensor that an entry point cannot take: on another device than
+    x, not of this type and shape, or not contiguous."""
+    if t.dtype != dtype or t.shape != shape or t.device != x.device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on "
+                         f"{x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}"
+                         f"{'' if t.is_contiguous() else ', not contiguous'}")
+
+
+def _rows_of(x, name, dtypes):
+    if x.dim() != 2 or x.dtype not in dtypes or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous 2-D tensor of one of {dtypes}, got "
+                         f"{x.dtype} {tuple(x.shape)}"
+                         f"{'' if x.is_contiguous() else ', not contiguous'}")
+
+
+def _run(x, fn, *args):
+    """fn(stream, *args) on x's device and that device's current stream."""
+    _dev(x)
+    if x.get_device() == torch.cuda.current_device():
+        check(fn(_s(), *args))
+    else:
+        with torch.cuda.device(x.device):
+            check(fn(_s(), *args))
+
+
+def add_rms_norm_q8(x, residual, w, eps, group=0, act_dtype=torch.float32, out=None):
+    """Residual addition, RMSNorm and 8-bit activations (inferno_add_rms_norm_q8):
+    s = x + residual (None: x), y = s / sqrt(mean(s^2) + eps) * w, and y in int8
+    with one fp32 scale per ``group`` columns (32, 64, 128; 0: the row). Returns
+    (s, y in act_dtype, q, scales); ``out`` (fp32, may be ``residual``) receives s."""
+    _rows_of(x, "x", tuple(_DT))
+    T, H = x.shape
+    if group and (group not in (32, 64, 128) or H % group):
+        raise ValueError(f"group must be 0, 32, 64 or 128 and divide the width {H}, got {group}")
+    if act_dtype not in _DT:
+        raise ValueError(f"act_dtype must be one of {tuple(_DT)}, got {act_dtype}")
+    if residual is not None:
+        _like(x, "residual", residual, torch.float32, T, H)
+    _like(x, "w", w, torch.float32, H)
+    if out is None:
+        out = torch.empty(T, H, dtype=torch.float32, device=x.device)
+    else:
+        _like(x, "out", out, torch.float32, T, H)
+    normed = torch.empty(T, H, dtype=act_dtype, device=x.device)
+    q = torch.empty(T, H, dtype=torch.int8, device=x.device)
+    scales = torch.empty(T, H // group if group else 1, dtype=torch.float32, device=x.device)
+    _run(x, lib().inferno_add_rms_norm_q8, _p(x), _DT[x.dtype], _p(residual), _p(w), float(eps), T,
+         H, group, _DT[act_dtype], _p(out), _p(normed), _p(q), _p(scales))
+    return out, normed, q, scales
+
+
+def router_group_topk(logits, bias, k, score_fn, norm, scale, n_group, topk_group, group_score):
+    """``router_topk`` over the ``topk_group`` best of ``n_group`` groups of
+    experts (inferno_moe_router_group_topk)."""
+    _rows_of(logits, "logits", (torch.float32,))
+    T, E = logits.shape
+    if bias is not None:
+        _like(logits, "bias", bias, torch.float32, E)
+    if k < 0 or n_group < 0 or topk_group < 0:
+        raise ValueError("k, n_group and topk_group must not be negative")
+    ids = torch.empty(T * k, dtype=torch.int32, device=logits.device)
+    w = torch.empty(T * k, dtype=torch.float32, device=logits.device)
+    tok = torch.empty(T * k, dtype=torch.int32, device=logits.device)
+    _run(logits, lib().inferno_moe_router_group_topk, _p(logits), _p(bias), T, E, k, score_fn,
+         int(norm), float(scale), n_group, topk_group, group_score, _p(ids), _p(w), _p(tok))
+    return ids, w, tok
+
+
+class W4:
+    """4-bit weights with group scales (struct inferno_w4): one matrix [rows,
+    cols], or one per expert [E, rows, cols]. ``codes`` holds two columns a byte
+    (uint8 [..., cols / 2], the even column in the low nibble), ``scales`` one
+    factor per cols / scales.shape[-1] columns (fp32 or bf16), ``zeros`` a zero
+    point for each scale (uint8; None: 8). The tensors are used as they are."""
+
+    def __init__(self, codes, scales, zeros=None):
+        if codes.dtype != torch.uint8 or codes.dim() not in (2, 3) or not codes.is_contiguous():
+            raise ValueError("codes must be a contiguous 2-D or 3-D uint8 tensor, got "
+                             f"{codes.dtype} {tuple(codes.shape)}")
+        if scales.dtype not in _DT:
+            raise ValueError(f"scales must be one of {tuple(_DT)}, got {scales.dtype}")
+        rows, cols = codes.shape[-2], 2 * codes.shape[-1]
+        groups = scales.shape[-1] if scales.dim() else 0
+        if groups == 0 or cols % groups:
+            raise ValueError(f"{groups} scales a row do not divide {cols} columns")
+        _like(codes, "scales", scales, scales.dtype, *codes.shape[:-1], groups)
+        if zeros is not None:
+            _like(codes, "zeros", zeros, torch.uint8, *codes.shape[:-1], groups)
+        self.tensors = (codes, scales, zeros)
+        self.device = codes.device
+        self.experts = codes.shape[0] if codes.dim() == 3 else 1
+        self.rows, self.cols, self.group = rows, cols, cols // groups
+        self.desc = W4Desc(
+            self.experts, rows, cols, self.group, _DT[scales.dtype], codes.data_ptr(),
+            scales.data_ptr(), zeros.data_ptr() if zeros is not None else None, codes.numel(),
+            scales.numel() * scales.element_size(), zeros.numel() if zeros is not None else 0)
+        self.ref = C.byref(self.desc)
+
+
+_ACT = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: I8}
+
+
+def _w4_x(w, x, x_scales):
+    """Checks activations of a 4-bit product; their type, scales and group."""
+    _rows_of(x, "x", tuple(_ACT))
+    if x.shape[1] != w.cols or x.device != w.device:
+        raise ValueError(f"x must be [tokens, {w.cols}] on {w.device}, got {tuple(x.shape)} on "
+                         f"{x.device}")
+    if x.dtype != torch.int8:
+        if x_scales is not None:
+            raise ValueError("x_scales belong to int8 activations")
+        return _ACT[x.dtype], None, 0
+    if x_scales is None or x_scales.dim() != 2 or not x_scales.shape[1] or \
+            w.cols % x_scales.shape[1]:
+        raise ValueError("int8 activations need x_scales [tokens, groups], groups dividing "
+                         f"{w.cols}")
+    _like(x, "x_scales", x_scales, torch.float32, x.shape[0], x_scales.shape[1])
+    return I8, _p(x_scales), w.cols // x_scales.shape[1]
+
+
+def _w4_ws(x, n):
+    return torch.empty(n, dtype=torch.uint8, device=x.device)
+
+
+def w4_matvec_add2(w, x, residual_a=None, residual_b=None, x_scales=None):
+    """residual_a + residual_b + x W^T for a 4-bit matrix (inferno_w4_matvec_add2).
+    x: fp32, bf16, or int8 with ``x_scales`` (add_rms_norm_q8's, group 128 or 0)."""
+    dt, xs, xg = _w4_x(w, x, x_scales)
+    T = x.shape[0]
+    for name, r in (("residual_a", residual_a), ("residual_b", residual_b)):
+        if r is not None:
+            _like(x, name, r, torch.float32, T, w.rows)
+    out = torch.empty(T, w.rows, dtype=torch.float32, device=x.device)
+    n = lib().inferno_w4_workspace_bytes(T, w.cols)
+    ws = _w4_ws(x, n)
+    _run(x, lib().inferno_w4_matvec_add2, w.ref, _p(x), dt, xs, xg, _p(residual_a),
+         _p(residual_b), T, _p(out), _p(ws), n)
+    return out
+
+
+def w4_gate_up_swiglu(gate, up, x, x_scales=None):
+    """silu(x W_gate^T) * (x W_up^T) for 4-bit matrices (inferno_w4_gate_up_swiglu)."""
+    dt, xs, xg = _w4_x(gate, x, x_scales)
+    if up.device != x.device:
+        raise ValueError(f"the up matrix must be on {x.device}, got {up.device}")
+    T = x.shape[0]
+    out = torch.empty(T, gate.rows, dtype=torch.float32, device=x.device)
+    n = lib().inferno_w4_workspace_bytes(T, gate.cols)
+    ws = _w4_ws(x, n)
+    _run(x, lib().inferno_w4_gate_up_swiglu, gate.ref, up.ref, _p(x), dt, xs, xg, T, _p(out),
+         _p(ws), n)
+    return out
+
+
+def w4_moe(gate, up, down, x, ids, weights, k, x_scales=None):
+    """Routed experts with 4-bit weights (inferno_w4_moe): gate and up [E, I, H],
+    down [E, H, I]; ids and weights [T * k] as ``router_topk`` returns them."""
+    dt, xs, xg = _w4_x(gate, x, x_scales)
+    if up.device != x.device or down.device != x.device:
+        raise ValueError(f"the expert matrices must be on {x.device}")
+    T, H = x.shape
+    if k < 1:
+        raise ValueError(f"k must be positive, got {k}")
+    _like(x, "ids", ids, torch.int32, T * k)
+    _like(x, "weights", weights, torch.float32, T * k)
+    out = torch.empty(T, H, dtype=torch.float32, device=x.device)
+    n = lib().inferno_w4_moe_workspace_bytes(T, k, gate.experts, H, gate.rows)
+    ws = _w4_ws(x, n)
+    _run(x, lib().inferno_w4_moe, gate.ref, up.ref, down.ref, _p(x), dt, xs, xg, _p(ids),
+         _p(weights), T, k, _p(out), _p(ws), n)
     return out
 
 

@@ -1,0 +1,171 @@
+"""Grouped routing (inferno_moe_router_group_topk) against its definition in
+64 bits, evaluated on the host by sorting.
+
+Bars. Ids: equal, ties to the lower group and the lower id (64-bit values of
+fp32 logits are equal only where the inputs are). Weights: a score is off by at
+most 4 roundings of 2^-24 (the exponential's argument l - max rounds to 2^-24
+of itself, which moves the score by |l - max| 2^-24 more), the sum of k or 256
+scores adds at most k + 10 roundings, quotient and scale one each."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from inferno_amd import GROUP_MAX, GROUP_TOP2, SCORE_SIGMOID, SCORE_SOFTMAX, lib, ops
+
+
+def _definition(logits, bias, k, score_fn, norm, scale, n_group, topk_group, rule):
+    T, E = logits.shape
+    l = logits.astype(np.float64)
+    with np.errstate(over="ignore", invalid="ignore"):
+        if score_fn == SCORE_SIGMOID:
+            score = 1.0 / (1.0 + np.exp(-l))
+            value = score
+        else:
+            top = l.max(1, keepdims=True)
+            score = np.where(np.isneginf(top), 0.0, np.exp(l - np.where(np.isneginf(top), 0, top)))
+            value = l
+    value = value + (0.0 if bias is None else bias.astype(np.float64))
+    size = E // n_group
+    ids = np.empty((T, k), np.int64)
+    for t in range(T):
+        v = value[t].tolist()
+        best = []
+        for g in range(n_group):
+            m = sorted(v[g * size:(g + 1) * size], reverse=True)
+            best.append(m[0] if rule == GROUP_MAX or size == 1 else m[0] + m[1])
+        kept = sorted(range(n_group), key=lambda g: (-best[g], g))[:topk_group]
+        live = [e for e in range(E) if e // size in kept]
+        ids[t] = sorted(live, key=lambda e: (-v[e], e))[:k]
+    w = np.take_along_axis(score, ids, 1)
+    total = w.sum(1, keepdims=True) if norm else score.sum(1, keepdims=True)
+    if norm or score_fn == SCORE_SOFTMAX:
+        w = np.where(total > 0, w / np.where(total > 0, total, 1.0), w)
+    return ids, w * scale
+
+
+def _check(logits, bias, k, score_fn, norm, scale, n_group, topk_group, rule):
+    ids, w, tok = ops.router_group_topk(logits, bias, k, score_fn, norm, scale, n_group,
+                                        topk_group, rule)
+    T = logits.shape[0]
+    l = logits.cpu().numpy()
+    want, ww = _definition(l, None if bias is None else bias.cpu().numpy(), k, score_fn, norm,
+                           scale, n_group, topk_group, rule)
+    got = ids.view(T, k).cpu().numpy()
+    assert np.array_equal(got, want), np.nonzero((got != want).any(1))[0][:5]
+    finite = l[np.isfinite(l)]
+    far = float(finite.max() - finite.min()) if score_fn == SCORE_SOFTMAX and finite.size else 0.0
+    bar = (4 + 2 * far + k + 10 + 2) * 2.0 ** -24
+    np.testing.assert_allclose(w.view(T, k).cpu().numpy(), ww, rtol=bar, atol=1e-38)
+    assert torch.equal(tok.view(T, k).cpu(), torch.arange(T, dtype=torch.int32).repeat_interleave(k)
+                       .view(T, k))
+    return ids, w
+
+
+SHAPES = [  # E, groups, kept groups, k
+    (256, 8, 4, 8), (256, 8, 3, 16), (64, 4, 2, 6), (160, 8, 3, 6), (256, 1, 1, 8), (60, 5, 2, 4),
+    (255, 15, 7, 9), (7, 7, 3, 3), (1, 1, 1, 1), (256, 256, 16, 16), (132, 3, 1, 16), (48, 16, 1, 3),
+    (256, 2, 1, 10), (100, 50, 20, 16), (65, 13, 13, 1), (250, 125, 3, 5), (128, 8, 8, 4)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,groups,kept,k", SHAPES)
+@pytest.mark.parametrize("score_fn", [SCORE_SIGMOID, SCORE_SOFTMAX])
+@pytest.mark.parametrize("rule", [GROUP_MAX, GROUP_TOP2])
+def test_against_the_definition(cuda, E, groups, kept, k, score_fn, rule):
+    g = torch.Generator().manual_seed(E * 7 + groups)
+    for T, norm, with_bias in ((1, True, True), (5, False, True), (33, True, False),
+                               (130, False, False)):
+        logits = (2.0 * torch.randn(T, E, generator=g)).to(cuda)
+        bias = (0.2 * torch.randn(E, generator=g)).to(cuda) if with_bias else None
+        _check(logits, bias, k, score_fn, norm, 2.5, groups, kept, rule)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score_fn", [SCORE_SIGMOID, SCORE_SOFTMAX])
+@pytest.mark.parametrize("rule", [GROUP_MAX, GROUP_TOP2])
+def test_ties_and_neighbours(cuda, score_fn, rule):
+    # a few distinct values (ties of experts and of groups), then values one
+    # fp32 step apart, whose sigmoids are equal in fp32 but not in 64 bits
+    g = torch.Generator().manual_seed(3)
+    few = torch.randint(0, 3, (40, 96), generator=g).float()
+    _check(few.to(cuda), None, 7, score_fn, True, 1.0, 12, 5, rule)
+    _check(torch.zeros(3, 96, device=cuda), None, 7, score_fn, True, 1.0, 12, 5, rule)
+    near = torch.full((40, 96), 5.0) + torch.randint(0, 40, (40, 96), generator=g) * 2.0 ** -21
+    _check(near.to(cuda), None, 7, score_fn, True, 1.0, 12, 5, rule)
+    bias = torch.randint(0, 3, (96,), generator=g).float() * 0.25
+    _check(near.to(cuda), bias.to(cuda), 7, score_fn, False, 1.0, 12, 5, rule)
+    # sums of a value and a bias that round to one fp32 number
+    wide = torch.randint(0, 9, (40, 96), generator=g) * 2.0 ** -30
+    _check(wide.to(cuda), torch.ones(96, device=cuda), 7, score_fn, True, 1.0, 12, 5, rule)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score_fn", [SCORE_SIGMOID, SCORE_SOFTMAX])
+def test_closed_and_empty_rows(cuda, score_fn):
+    g = torch.Generator().manual_seed(4)
+    logits = torch.randn(6, 32, generator=g)
+    inf = float("inf")
+    logits[0, 4:] = -inf      # fewer experts than are chosen
+    logits[1] = -inf          # nothing
+    logits[2, ::2] = -3e38    # the lowest finite values
+    logits[3] = 200.0
+    logits[4, 5] = 90.0       # the others' softmax scores vanish
+    for rule in (GROUP_MAX, GROUP_TOP2):
+        ids, w = _check(logits.to(cuda), None, 6, score_fn, True, 1.0, 8, 3, rule)
+        assert w.isfinite().all() and not w.view(6, 6)[1].any()
+
+
+@pytest.mark.gpu
+def test_nan_rows_keep_valid_ids(cuda):
+    logits = torch.randn(8, 64, generator=torch.Generator().manual_seed(5)).to(cuda)
+    clean = ops.router_group_topk(logits, None, 5, 0, True, 1.0, 8, 2, GROUP_TOP2)
+    bad = logits.clone()
+    bad[3, 17] = float("nan")
+    bad[5] = float("nan")
+    ids, w, _ = ops.router_group_topk(bad, None, 5, 0, True, 1.0, 8, 2, GROUP_TOP2)
+    ids, w = ids.view(8, 5), w.view(8, 5)
+    assert ids[3, 0] == 17  # above +infinity
+    assert ids[5].tolist() == [0, 1, 2, 3, 4]
+    for t in range(8):
+        assert len(set(ids[t].tolist())) == 5 and 0 <= int(ids[t].min()) <= int(ids[t].max()) < 64
+        if t not in (3, 5):
+            assert torch.equal(ids[t], clean[0].view(8, 5)[t]) and torch.equal(w[t], clean[1].view(8, 5)[t])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score_fn", [SCORE_SIGMOID, SCORE_SOFTMAX])
+def test_one_group_is_the_plain_top_k(cuda, score_fn):
+    logits = torch.randn(50, 128, generator=torch.Generator().manual_seed(6)).to(cuda)
+    a = ops.router_topk(logits, None, 8, score_fn, True, 1.5)
+    b = ops.router_group_topk(logits, None, 8, score_fn, True, 1.5, 1, 1, GROUP_MAX)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2])
+    assert torch.allclose(a[1], b[1], rtol=32 * 2.0 ** -24, atol=0)
+
+
+def test_refusals():
+    logits = torch.zeros(2, 32)
+    ok = dict(bias=None, k=4, score_fn=0, norm=True, scale=1.0, n_group=4, topk_group=2,
+              group_score=0)
+    with pytest.raises(ValueError, match="GPU tensors"):
+        ops.router_group_topk(logits, **ok)
+    with pytest.raises(ValueError, match="bias"):
+        ops.router_group_topk(logits, **dict(ok, bias=torch.zeros(31)))
+    with pytest.raises(ValueError, match="logits"):
+        ops.router_group_topk(logits.bfloat16(), **ok)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.router_group_topk(torch.zeros(32, 2).T, **ok)
+    with pytest.raises(ValueError, match="negative"):
+        ops.router_group_topk(logits, **dict(ok, k=-1))
+    f = lib().inferno_moe_router_group_topk
+
+    def status(T=1, E=32, k=4, score=0, scale=1.0, groups=4, kept=2, rule=0, p=16):
+        return f(None, p, None, T, E, k, score, 1, scale, groups, kept, rule, 16, 16, None)
+
+    for bad in (dict(E=0), dict(E=257, groups=1), dict(groups=0), dict(groups=5), dict(kept=0),
+                dict(kept=5), dict(k=0), dict(k=17), dict(score=2), dict(rule=2),
+                dict(scale=math.inf), dict(p=None), dict(T=1 << 26), dict(k=9, kept=1)):
+        assert status(**bad) == -1, bad
+    assert b"exceeds the 8 experts" in lib().inferno_last_error()
+    assert status(T=0, p=None) == 0

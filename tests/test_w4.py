@@ -1,0 +1,401 @@
+"""Products with 4-bit group-scaled weights against 64 bits (bars:
+w4_reference.py), their refusals, and the calls that share a GPU."""
+import pytest
+import torch
+
+import w4_reference as ref
+from inferno_amd import InfernoError, W4Desc, lib, ops
+
+F32, BF16, I8 = torch.float32, torch.bfloat16, torch.int8
+
+
+def _x(g, T, K, dtype, x_group=0, device="cuda", std=1.0):
+    x = std * torch.randn(T, K, generator=g)
+    x[:, ::61] *= 12.0  # loud channels
+    if dtype != I8:
+        return x.to(dtype).to(device), None
+    n = x_group or K
+    v = x.view(T, K // n, n)
+    s = v.abs().amax(2, keepdim=True) / 127.0
+    q = torch.round(v / s).clamp(-128, 127).to(I8).view(T, K).contiguous()
+    q[:, 5::50] = -128
+    return q.to(device), s.view(T, K // n).contiguous().to(device)
+
+
+def _near(got, want, bar):
+    got = got.cpu().double()
+    worst = ((got - want).abs() / (bar + 1e-300)).max().item()
+    assert worst <= 1.0, worst
+
+
+SHAPES = [  # T, rows, cols, group
+    (1, 16, 128, 128), (1, 1, 32, 32), (1, 17, 96, 32), (2, 33, 160, 32), (3, 250, 192, 64),
+    (4, 64, 2048, 128), (5, 16, 1056, 32), (7, 130, 640, 128), (16, 48, 512, 256), (17, 31, 384, 64),
+    (33, 20, 1024, 1024), (64, 96, 256, 64), (70, 257, 288, 32), (128, 128, 512, 128),
+    (130, 70, 1152, 384), (300, 129, 448, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N,K,group", SHAPES)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, I8])
+def test_matvec_add2(cuda, T, N, K, group, zeros, dtype):
+    g = torch.Generator().manual_seed(T * 1000 + N + K)
+    for scales in (F32, BF16):
+        m = ref.make(g, N, K, group, zeros=zeros, scales=scales)
+        w = ops.W4(*m)
+        assert (w.rows, w.cols, w.group) == (N, K, group)
+        x, xs = _x(g, T, K, dtype, 128 if K % 128 == 0 and scales == F32 else 0)
+        a, b = (torch.randn(T, N, generator=g).cuda() for _ in range(2))
+        want, bar = ref.linear(ref.dense(*m), ref.values(x, xs), dtype != I8)
+        _near(ops.w4_matvec_add2(w, x, x_scales=xs), want, bar)
+        want, bar = ref.linear(ref.dense(*m), ref.values(x, xs), dtype != I8,
+                               extra=(a.abs() + b.abs()).cpu().double())
+        _near(ops.w4_matvec_add2(w, x, a, b, x_scales=xs), want + (a.cpu().double() + b.cpu()), bar)
+        want = want + b.cpu()
+        _near(ops.w4_matvec_add2(w, x, residual_b=b, x_scales=xs), want, bar)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N,K,group", SHAPES)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, I8])
+def test_gate_up_swiglu(cuda, T, N, K, group, zeros, dtype):
+    g = torch.Generator().manual_seed(T * 1000 + N + K + 1)
+    mg, mu = (ref.make(g, N, K, group, zeros=zeros) for _ in range(2))
+    x, xs = _x(g, T, K, dtype)
+    want, bar = ref.swiglu(ref.dense(*mg), ref.dense(*mu), ref.values(x, xs), dtype != I8)
+    _near(ops.w4_gate_up_swiglu(ops.W4(*mg), ops.W4(*mu), x, x_scales=xs), want, bar)
+
+
+def _experts(g, E, H, I, group, group2=None, zeros=False, zeros2=False, scales=BF16):
+    return (ref.make(g, I, H, group, E, zeros, scales), ref.make(g, I, H, group, E, zeros, scales),
+            ref.make(g, H, I, group2 or group, E, zeros2))
+
+
+def _moe(mats, x, xs, ids, w, k):
+    """The entry point's result, checked against 64 bits."""
+    got = ops.w4_moe(*(ops.W4(*m) for m in mats), x, ids, w, k, x_scales=xs)
+    d = [[ref.dense(*(None if v is None else v[e] for v in m)) for e in range(m[0].shape[0])]
+         for m in mats]
+    want, bar = ref.moe(*d, ref.values(x, xs), ids, w, k, x.dtype != I8)
+    _near(got, want, bar)
+    return got
+
+
+def _routing(g, T, E, k):
+    top = torch.randn(T, E, generator=g).topk(k, 1)
+    return (top.indices.int().flatten().cuda(),
+            torch.softmax(top.values, 1).flatten().contiguous().cuda())
+
+
+MOE = [  # T, E, k, H, I, group of gate and up, of down
+    (1, 8, 2, 128, 64, 64, 32), (1, 256, 16, 64, 32, 32, 32), (1, 16, 4, 2048, 768, 128, 128),
+    (2, 8, 8, 96, 160, 32, 32), (3, 5, 2, 256, 384, 128, 128), (5, 16, 3, 288, 96, 32, 32),
+    (16, 4, 2, 512, 256, 128, 64), (20, 64, 6, 384, 192, 64, 64), (40, 3, 1, 160, 224, 32, 32),
+    (70, 2, 2, 256, 128, 256, 128), (130, 8, 3, 384, 256, 128, 128), (257, 6, 2, 224, 288, 32, 32)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,k,H,I,group,group2", MOE)
+@pytest.mark.parametrize("dtype,zeros", [(F32, False), (BF16, True), (I8, False), (BF16, False)])
+def test_moe(cuda, T, E, k, H, I, group, group2, dtype, zeros):
+    g = torch.Generator().manual_seed(T + E + H)
+    mats = _experts(g, E, H, I, group, group2, zeros, not zeros, F32 if zeros else BF16)
+    x, xs = _x(g, T, H, dtype, 128 if H % 128 == 0 else 0)
+    _moe(mats, x, xs, *_routing(g, T, E, k), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 6, 90])
+def test_moe_any_ids(cuda, T):
+    # repeated experts in a token, ids of no expert, one expert for all, none
+    g = torch.Generator().manual_seed(T)
+    E, k, H, I = 7, 4, 256, 160
+    mats = _experts(g, E, H, I, 32)
+    x, _ = _x(g, T, H, BF16)
+    w = torch.rand(T * k, generator=g).cuda()
+    some = torch.randint(0, E, (T * k,), generator=g).int()
+    some[1::5] = E
+    some[3::7] = -1
+    some[::11] = 2 ** 31 - 1
+    _moe(mats, x, None, some.cuda(), w, k)
+    _moe(mats, x, None, torch.full((T * k,), 3).int().cuda(), w, k)
+    out = _moe(mats, x, None, torch.full((T * k,), E).int().cuda(), w, k)
+    assert not out.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("std", [1e-38, 1e-30, 1e-18, 1e18, 1e30])
+def test_sizes_of_the_values(cuda, dtype, std):
+    # activations below 2^-96 share the step of that size: 2^-118 and half of
+    # it as an error, which the bar takes in as such
+    g = torch.Generator().manual_seed(5)
+    for T in (1, 20):
+        m = ref.make(g, 40, 416, 32)
+        x, _ = _x(g, T, 416, dtype, std=std)
+        w, v = ref.dense(*m), ref.values(x)
+        want, bar = ref.linear(w, v)
+        bar = bar + 2.0 ** -119 * w.abs().sum(1) + 2.0 ** -149 * 20
+        _near(ops.w4_matvec_add2(ops.W4(*m), x), want, bar)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 128])
+def test_extreme_codes_and_zero_points(cuda, group):
+    # the largest sums: every code 0 or 15, zero points of any byte, digits of
+    # one sign
+    for T in (1, 8, 40):
+        for code in (0x00, 0xff, 0xf0):
+            for z in (None, 0, 15, 255):
+                codes = torch.full((24, 128), code, dtype=torch.uint8, device=cuda)
+                s = torch.full((24, 256 // group), 0.5, device=cuda)
+                zp = None if z is None else torch.full_like(s, z).to(torch.uint8)
+                for x, xs in ((torch.full((T, 256), 127, dtype=I8, device=cuda),
+                               torch.ones(T, 1, device=cuda)),
+                              (torch.full((T, 256), -128, dtype=I8, device=cuda),
+                               torch.ones(T, 1, device=cuda)),
+                              (torch.full((T, 256), 1.9921875, device=cuda), None),
+                              (torch.full((T, 256), -1.9999999, device=cuda), None)):
+                    want, bar = ref.linear(ref.dense(codes, s, zp), ref.values(x, xs), xs is None)
+                    _near(ops.w4_matvec_add2(ops.W4(codes, s, zp), x, x_scales=xs), want, bar)
+
+
+@pytest.mark.gpu
+def test_digits_hold_bf16_whole(cuda):
+    # one column at a time through a matrix of ones: values down to 2^-14 of
+    # their chunk's largest come back as they are
+    K = 128
+    x = torch.zeros(64, K)
+    i = torch.arange(64)
+    x[:, 0] = 1.9921875                                # the chunk's largest
+    x[i, 1 + i] = (1 + i / 64.0) * 2.0 ** -(i % 15)
+    x = x.to(BF16)
+    codes = torch.full((16, K // 2), 0x99, dtype=torch.uint8)  # 9 - 8 = 1
+    codes[:, 0] = 0x98                                 # column 0: 0
+    w = ops.W4(codes.cuda(), torch.ones(16, 1, device=cuda))
+    want = x[:, 1:].double().sum(1, keepdim=True).expand(-1, 16)
+    for T in (1, 4, 64):
+        assert torch.equal(ops.w4_matvec_add2(w, x[:T].cuda()).cpu().double(), want[:T])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 3, 9, 40, 100])
+@pytest.mark.parametrize("group", [32, 128])
+def test_not_finite_and_zero_rows(cuda, T, group):
+    g = torch.Generator().manual_seed(T)
+    E, k, H, I = 6, 2, 256, 128
+    mats = _experts(g, E, H, I, group)
+    ws = [ops.W4(*m) for m in mats]
+    x, _ = _x(g, T, H, F32)
+    ids, w = _routing(g, T, E, k)
+    clean = ops.w4_moe(*ws, x, ids, w, k)
+    bad = x.clone()
+    bad[0, 200] = float("nan")
+    bad[T // 2, 3] = float("inf")
+    if T > 2:
+        bad[T - 1] = 0.0
+    out = ops.w4_moe(*ws, bad, ids, w, k)
+    lin = ops.w4_matvec_add2(ops.W4(*(v[0].contiguous() for v in mats[0] if v is not None)), bad)
+    for t in range(T):
+        if t in (0, T // 2):
+            assert out[t].isnan().all() and lin[t].isnan().all()
+        elif t == T - 1 and T > 2:
+            assert not out[t].any() and not lin[t].any()
+        else:
+            assert torch.equal(out[t], clean[t])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 4, 16, 65, 200])
+def test_same_bits_again_and_rows_by_themselves(cuda, T):
+    # the same call twice gives the same bits
+    g = torch.Generator().manual_seed(2)
+    mats = _experts(g, 8, 256, 192, 64)
+    ws = [ops.W4(*m) for m in mats]
+    x, _ = _x(g, T, 256, BF16)
+    ids, w = _routing(g, T, 8, 3)
+    a = ops.w4_moe(*ws, x, ids, w, 3)
+    for _ in range(3):
+        assert torch.equal(a, ops.w4_moe(*ws, x, ids, w, 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 5, 33])
+def test_only_the_outputs_are_written(cuda, T):
+    # the library's call with outputs inside a larger buffer and a workspace of
+    # exactly the size asked for, both with a border that has to stay
+    g = torch.Generator().manual_seed(8)
+    E, k, H, I = 5, 2, 160, 96
+    mats = _experts(g, E, H, I, 32, zeros=True)
+    ws = [ops.W4(*m) for m in mats]
+    x, _ = _x(g, T, H, F32)
+    ids, w = _routing(g, T, E, k)
+    want = ops.w4_moe(*ws, x, ids, w, k)
+    n = lib().inferno_w4_moe_workspace_bytes(T, k, E, H, I)
+    buf = torch.full((n + 512,), 171, dtype=torch.uint8, device=cuda)
+    out = torch.full((T + 2, H), 5.0, device=cuda)
+    s = torch.cuda.current_stream().cuda_stream
+    assert lib().inferno_w4_moe(s, ws[0].ref, ws[1].ref, ws[2].ref, x.data_ptr(), 0, None, 0,
+                                ids.data_ptr(), w.data_ptr(), T, k, out[1:].data_ptr(),
+                                buf[256:].data_ptr(), n) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out[1:-1], want) and (out[0] == 5).all() and (out[-1] == 5).all()
+    assert (buf[:256] == 171).all() and (buf[-256:] == 171).all()
+
+
+@pytest.mark.gpu
+def test_residual_in_place(cuda):
+    g = torch.Generator().manual_seed(9)
+    m = ref.make(g, 64, 256, 64)
+    w = ops.W4(*m)
+    for T in (1, 20, 100):
+        x, _ = _x(g, T, 256, BF16)
+        r = torch.randn(T, 64, generator=g).cuda()
+        want = ops.w4_matvec_add2(w, x, r)
+        n = lib().inferno_w4_workspace_bytes(T, 256)
+        ws = torch.empty(n, dtype=torch.uint8, device=cuda)
+        s = torch.cuda.current_stream().cuda_stream
+        assert lib().inferno_w4_matvec_add2(s, w.ref, x.data_ptr(), 1, None, 0, r.data_ptr(), None,
+                                            T, r.data_ptr(), ws.data_ptr(), n) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(r, want)
+
+
+@pytest.mark.gpu
+def test_no_tokens(cuda):
+    g = torch.Generator().manual_seed(1)
+    mats = _experts(g, 4, 64, 32, 32)
+    ws = [ops.W4(*m) for m in mats]
+    x = torch.zeros(0, 64, device=cuda)
+    ids, w = torch.zeros(0, dtype=torch.int32, device=cuda), torch.zeros(0, device=cuda)
+    assert ops.w4_moe(*ws, x, ids, w, 2).shape == (0, 64)
+    one = ops.W4(*ref.make(g, 48, 64, 32))
+    assert ops.w4_matvec_add2(one, x).shape == (0, 48)
+    assert ops.w4_gate_up_swiglu(one, one, x).shape == (0, 48)
+
+
+def _cpu(rows=16, cols=64, group=32, experts=0, **kw):
+    return ref.make(torch.Generator().manual_seed(0), rows, cols, group, experts, device="cpu", **kw)
+
+
+def test_refusals_of_the_wrappers():
+    codes, scales, _ = _cpu()
+    with pytest.raises(ValueError, match="codes"):
+        ops.W4(codes.int(), scales)
+    with pytest.raises(ValueError, match="codes"):
+        ops.W4(codes.T, scales)
+    with pytest.raises(ValueError, match="scales"):
+        ops.W4(codes, scales.half())
+    with pytest.raises(ValueError, match="scales"):
+        ops.W4(codes, scales[:-1])
+    with pytest.raises(ValueError, match="do not divide"):
+        ops.W4(codes, torch.zeros(16, 3))
+    with pytest.raises(ValueError, match="zeros"):
+        ops.W4(codes, scales, torch.zeros(16, 2, dtype=torch.int8))
+    w = ops.W4(codes, scales)
+    x = torch.zeros(2, 64)
+    with pytest.raises(ValueError, match="GPU tensors"):
+        ops.w4_matvec_add2(w, x)
+    with pytest.raises(ValueError, match="x must"):
+        ops.w4_matvec_add2(w, torch.zeros(2, 32))
+    with pytest.raises(ValueError, match="x must"):
+        ops.w4_matvec_add2(w, x.half())
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.w4_matvec_add2(w, torch.zeros(64, 2).T)
+    with pytest.raises(ValueError, match="x_scales"):
+        ops.w4_matvec_add2(w, x.to(I8))
+    with pytest.raises(ValueError, match="x_scales"):
+        ops.w4_matvec_add2(w, x.to(I8), x_scales=torch.zeros(2, 3))
+    with pytest.raises(ValueError, match="x_scales"):
+        ops.w4_matvec_add2(w, x.to(I8), x_scales=torch.zeros(3, 1))
+    with pytest.raises(ValueError, match="belong"):
+        ops.w4_matvec_add2(w, x, x_scales=torch.zeros(2, 1))
+    with pytest.raises(ValueError, match="residual_a"):
+        ops.w4_matvec_add2(w, x, torch.zeros(2, 15))
+    mats = [ops.W4(*_cpu(32, 64, experts=4)) for _ in range(2)] + [ops.W4(*_cpu(64, 32, experts=4))]
+    ids, wt = torch.zeros(4, dtype=torch.int32), torch.zeros(4)
+    with pytest.raises(ValueError, match="ids"):
+        ops.w4_moe(*mats, x, ids.long(), wt, 2)
+    with pytest.raises(ValueError, match="ids"):
+        ops.w4_moe(*mats, x, ids, wt, 3)
+    with pytest.raises(ValueError, match="weights"):
+        ops.w4_moe(*mats, x, ids, wt[:3], 2)
+    with pytest.raises(ValueError, match="k must"):
+        ops.w4_moe(*mats, x, ids, wt, 0)
+
+
+def _desc(experts=1, rows=16, cols=64, group=32, p=16, **more):
+    d = W4Desc(experts, rows, cols, group, 0, p, p, None, experts * rows * cols // 2,
+               experts * rows * (cols // group if group else 0) * 4, 0)
+    for name, v in more.items():
+        setattr(d, name, v)
+    return d
+
+
+def test_refusals_of_the_library():
+    # every one before any device work
+    L = lib()
+
+    def matvec(d, x=16, dt=0, xs=None, xg=0, T=1, out=16, ws=16, n=1 << 30):
+        return L.inferno_w4_matvec_add2(None, d, x, dt, xs, xg, None, None, T, out, ws, n)
+
+    for d in (_desc(rows=0), _desc(cols=0), _desc(experts=0), _desc(group=0), _desc(group=48),
+              _desc(group=128), _desc(group=96, cols=96), _desc(cols=48, group=16),
+              _desc(scale_dtype=2), _desc(codes=None), _desc(codes=24), _desc(scales=18),
+              _desc(experts=2), _desc(experts=257)):
+        assert matvec(d) == -1, L.inferno_last_error()
+    for d in (_desc(codes_bytes=1), _desc(scales_bytes=64), _desc(zeros=16, zeros_bytes=3)):
+        assert matvec(d) == -2
+    d = _desc()
+    assert matvec(d, x=None) == -1 and matvec(d, x=20) == -1 and matvec(d, dt=3) == -1
+    assert matvec(d, out=None) == -1 and matvec(d, ws=None) == -2 and matvec(d, n=100) == -2
+    assert matvec(d, ws=24) == -1 and matvec(d, T=1 << 31) == -1
+    assert matvec(d, dt=2) == -1  # no scales
+    big = _desc(cols=512, group=128)
+    for xg in (64, 192, 1024, 32):
+        assert matvec(big, dt=2, xs=16, xg=xg) == -1
+    assert matvec(d, x=None, T=0, out=None, ws=None, n=0) == 0
+
+    def pair(a, b):
+        return L.inferno_w4_gate_up_swiglu(None, a, b, 16, 0, None, 0, 1, 16, 16, 1 << 30)
+
+    other = _desc(zeros=16, zeros_bytes=32)
+    for b in (_desc(rows=32), _desc(cols=128), _desc(group=64), other):
+        assert pair(d, b) == -1 and b"same" in L.inferno_last_error()
+    half = _desc(scale_dtype=1, scales_bytes=64)
+    assert pair(d, half) == -1
+
+    def moe(g, u, dn, ids=16, k=2, T=1, n=1 << 30):
+        return L.inferno_w4_moe(None, g, u, dn, 16, 0, None, 0, ids, 16, T, k, 16, 16, n)
+
+    g, dn = _desc(4, 32, 64), _desc(4, 64, 32)
+    for down in (_desc(3, 64, 32), _desc(4, 32, 32), _desc(4, 64, 64)):
+        assert moe(g, g, down) == -1 and b"changed over" in L.inferno_last_error()
+    assert moe(g, g, dn, k=0) == -1 and moe(g, g, dn, k=17) == -1
+    assert moe(g, g, dn, ids=None) == -1 and moe(g, g, dn, n=10) == -2
+    assert moe(g, g, dn, T=1 << 27) == -1
+    assert moe(g, g, dn, T=0) == 0
+
+
+def test_workspace_does_not_fall():
+    L = lib()
+    for K in (32, 160, 4096):
+        need = [L.inferno_w4_workspace_bytes(T, K) for T in range(0, 300)]
+        assert need == sorted(need)
+        need = [L.inferno_w4_moe_workspace_bytes(T, 8, 64, K, 96) for T in range(0, 300)]
+        assert need == sorted(need)
+
+
+@pytest.mark.gpu
+def test_library_errors_reach_the_caller(cuda):
+    g = torch.Generator().manual_seed(1)
+    a, b = ops.W4(*ref.make(g, 16, 64, 32)), ops.W4(*ref.make(g, 16, 64, 64))
+    with pytest.raises(InfernoError, match="same group"):
+        ops.w4_gate_up_swiglu(a, b, torch.zeros(1, 64, device=cuda))
+    with pytest.raises(InfernoError, match="group"):
+        ops.w4_matvec_add2(ops.W4(*ref.make(g, 16, 96, 96)), torch.zeros(1, 96, device=cuda))
+    buf = torch.zeros(65, device=cuda)
+    with pytest.raises(InfernoError, match="multiple of 16"):
+        ops.w4_matvec_add2(a, buf[1:].view(1, 64))
