@@ -207,7 +207,7 @@ int inferno_q8_0_matvec_add2(void* stream, const void* w, size_t w_bytes, const 
  *   W[r, c] = scales[r, c / group] * (code[r, c] - zeros[r, c / group])
  * codes: [experts * rows][cols / 2] bytes, column 2 j in the low nibble of byte
  * j and column 2 j + 1 in the high one; scales: [experts * rows][cols / group]
- * F32 or BF16; zeros: the same number of bytes, any value, or NULL: 8.
+ * F32 or BF16; zeros: as many bytes (one above 127 counts as 127), or NULL: 8.
  * cols is a multiple of 32 and of group; group is 32, 64 or a multiple of 128.
  * codes lie at a multiple of 16 bytes. The byte lengths are checked. */
 typedef struct inferno_w4 {

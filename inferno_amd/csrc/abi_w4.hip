@@ -79,13 +79,12 @@ int check_tokens(size_t rows, size_t cols) {
   return INFERNO_OK;
 }
 
-// Room for three digits and zero points' sums, which any call fits.
+// Room for three digits, which any call fits.
 W4Acts carve_acts(Carver& c, size_t rows, size_t cols) {
   const size_t n = rows * w4_chunks(cols);
   W4Acts a{};
   a.planes = c.take<int8_t>(n * 3 * kW4Chunk);
   a.xs = c.take<float>(n);
-  a.sums = c.take<int>(n * 16);
   return a;
 }
 
@@ -93,7 +92,6 @@ W4Acts carve_acts(Carver& c, size_t rows, size_t cols) {
 W4Acts acts_for(W4Acts a, const inferno_w4* w, int x_dtype) {
   a.P = x_dtype == INFERNO_I8 ? 1 : 3;
   a.fine = w->group < size_t(kW4Chunk);
-  if (!w->zeros) a.sums = nullptr;
   return a;
 }
 

@@ -14,19 +14,16 @@ struct W4Mat {
 };
 
 // Activations as int8 digits, the operands of the integer matrix cores.
-// A value of a 128-column chunk is (65536 d0 + 256 d1 + d2) * 16 xs (3 planes;
-// d in [-128, 127]), or d0 * 16 xs (1 plane, int8 activations).
+// A value of a 128-column chunk is (65536 d0 + 256 d1 + d2) xs (3 planes; d in
+// [-128, 127]), or d0 xs (1 plane, int8 activations).
 //   planes [rows][chunks][planes][128]: the digits of one chunk in the order
-//     in which the lanes of the weights' tile hold its columns (w4_column);
-//   xs [rows][chunks];
-//   sums [rows][chunks][blocks][planes padded to 4 | 1]: digit sums of the
-//     chunk (blocks = 1) or of its 32-column blocks (4), for zero points.
+//     in which the lanes of the weights' tile hold its columns;
+//   xs [rows][chunks].
 struct W4Acts {
   int8_t* planes;
   float* xs;
-  int* sums;
-  int P;        // planes: 3 or 1
-  bool fine;    // groups of 32 or 64 columns
+  int P;      // planes: 3 or 1
+  bool fine;  // groups of 32 or 64 columns
 };
 
 inline size_t w4_chunks(size_t K) { return (K + kW4Chunk - 1) / kW4Chunk; }

@@ -34,7 +34,7 @@ def dense(codes, scales, zeros=None):
     q[..., 0::2] = (codes & 15).double()
     q[..., 1::2] = (codes >> 4).double()
     of = torch.arange(cols) // (cols // scales.shape[-1])
-    q -= 8.0 if zeros is None else zeros.cpu().double()[..., of]
+    q -= 8.0 if zeros is None else zeros.cpu().clamp(max=127).double()[..., of]
     return q * scales.double()[..., of]
 
 
