@@ -205,20 +205,32 @@ int inferno_q8_0_matvec_add2(void* stream, const void* w, size_t w_bytes, const 
  * `group` consecutive columns of a row, or `experts` such matrices one after
  * another:
  *   W[r, c] = scales[r, c / group] * (code[r, c] - zeros[r, c / group])
- * codes: [experts * rows][cols / 2] bytes, column 2 j in the low nibble of byte
- * j and column 2 j + 1 in the high one; scales: [experts * rows][cols / group]
- * F32 or BF16; zeros: as many bytes (one above 127 counts as 127), or NULL: 8.
- * cols is a multiple of 32 and of group; group is 32, 64 or a multiple of 128.
- * codes lie at a multiple of 16 bytes. The byte lengths are checked. */
+ * without zero points 8 in their place. cols is a multiple of 32 and of group;
+ * group is 32, 64 or a multiple of 128; one matrix has less than 2^33 codes,
+ * experts <= 256. The products read a packed form, which inferno_w4_pack writes
+ * once; it takes inferno_w4_packed_bytes at a multiple of 16 bytes. */
 typedef struct inferno_w4 {
   size_t experts; /* 1: a plain matrix */
   size_t rows, cols, group;
   int scale_dtype; /* INFERNO_F32 or INFERNO_BF16 */
-  const void* codes;
-  const void* scales;
-  const void* zeros; /* or NULL */
-  size_t codes_bytes, scales_bytes, zeros_bytes;
+  int has_zeros;
+  const void* packed;
+  size_t packed_bytes;
 } inferno_w4;
+
+/* Bytes of the packed form (rows to a multiple of 16, columns to one of 128;
+ * for groups of 64 a scale is stored twice); 0 if the sizes are refused. Does
+ * not read `packed`. Host-only, no GPU needed. */
+size_t inferno_w4_packed_bytes(const inferno_w4* w);
+
+/* Packs a matrix of w's sizes into `packed` (w->packed is not read,
+ * w->packed_bytes is its size). codes: [experts * rows][cols / 2] bytes, column
+ * 2 j in the low nibble of byte j, column 2 j + 1 in the high one; scales:
+ * [experts * rows][cols / group] of scale_dtype; zeros: as many bytes (one above
+ * 127 counts as 127), read with has_zeros. The byte lengths are checked. */
+int inferno_w4_pack(void* stream, const inferno_w4* w, const void* codes, size_t codes_bytes,
+                    const void* scales, size_t scales_bytes, const void* zeros, size_t zeros_bytes,
+                    void* packed);
 
 /* Activations x [T, cols] of the products below: F32, BF16, or I8 with
  * x_scales [T, cols / x_group] fp32 (x = value * scale; x_group a multiple of

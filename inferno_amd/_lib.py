@@ -36,8 +36,7 @@ class W4Desc(C.Structure):
     """Mirror of `struct inferno_w4`."""
     _fields_ = [
         ("experts", _sz), ("rows", _sz), ("cols", _sz), ("group", _sz), ("scale_dtype", _i),
-        ("codes", _vp), ("scales", _vp), ("zeros", _vp),
-        ("codes_bytes", _sz), ("scales_bytes", _sz), ("zeros_bytes", _sz),
+        ("has_zeros", _i), ("packed", _vp), ("packed_bytes", _sz),
     ]
 
 
@@ -77,6 +76,8 @@ SIGNATURES = {
     "inferno_rms_norm_router_topk_workspace_bytes": (_sz, [_sz]),
     "inferno_rms_norm_router_topk": (_i, [_vp, _vp, _vp, _f, _vp, _vp, _sz, _sz, _sz, _sz, _i, _i,
                                           _f, _i, _vp, _vp, _vp, _vp, _vp, _sz]),
+    "inferno_w4_packed_bytes": (_sz, [C.POINTER(W4Desc)]),
+    "inferno_w4_pack": (_i, [_vp, C.POINTER(W4Desc), _vp, _sz, _vp, _sz, _vp, _sz, _vp]),
     "inferno_w4_workspace_bytes": (_sz, [_sz, _sz]),
     "inferno_w4_matvec_add2": (_i, [_vp, C.POINTER(W4Desc), _vp, _i, _vp, _sz, _vp, _vp, _sz, _vp,
                                     _vp, _sz]),

@@ -18,11 +18,16 @@ int check_bytes(const char* what, const char* part, size_t got, size_t want) {
   return INFERNO_ERR_SIZE;
 }
 
-int check_w4(const char* what, const inferno_w4* w) {
+W4Mat mat(const inferno_w4* w) {
+  return W4Mat{w->experts, w->rows,           w->cols,  w->group,
+               w->scale_dtype, w->has_zeros != 0, w->packed};
+}
+
+int check_shape(const char* what, const inferno_w4* w) {
   INF_CHECK_ARG(w != nullptr, "null 4-bit matrix");
   const size_t most = size_t(1) << 31;
   if (w->experts == 0 || w->rows == 0 || w->cols == 0 || w->rows >= most || w->cols >= most ||
-      w->experts > size_t(kMaxExperts)) {
+      w->experts > size_t(kMaxExperts) || w->rows * w->cols >= 4 * most) {
     set_error(std::string("4-bit ") + what + " matrix: sizes out of range, experts=" +
               std::to_string(w->experts) + ", rows=" + std::to_string(w->rows) + ", cols=" +
               std::to_string(w->cols));
@@ -35,16 +40,15 @@ int check_w4(const char* what, const inferno_w4* w) {
                 "the columns of a 4-bit matrix must be a multiple of 32 and of its group");
   INF_CHECK_ARG(w->scale_dtype == INFERNO_F32 || w->scale_dtype == INFERNO_BF16,
                 "scales must be F32 or BF16");
-  const size_t rows = w->experts * w->rows, groups = rows * (w->cols / g);
-  const size_t each = w->scale_dtype == INFERNO_BF16 ? 2 : 4;
+  return INFERNO_OK;
+}
+
+int check_w4(const char* what, const inferno_w4* w) {
   int st;
-  if ((st = check_bytes(what, "codes", w->codes_bytes, rows * (w->cols / 2)))) return st;
-  if ((st = check_bytes(what, "scales", w->scales_bytes, groups * each))) return st;
-  if (w->zeros && (st = check_bytes(what, "zero points", w->zeros_bytes, groups))) return st;
-  INF_CHECK_ARG(w->codes && w->scales, "null pointer in a 4-bit matrix");
-  INF_CHECK_ARG(aligned(w->codes, 16) && aligned(w->scales, each),
-                "the codes of a 4-bit matrix must lie at a multiple of 16 bytes, its scales at "
-                "one of their size");
+  if ((st = check_shape(what, w))) return st;
+  if ((st = check_bytes(what, "packed form", w->packed_bytes, w4_layout(mat(w)).bytes))) return st;
+  INF_CHECK_ARG(w->packed != nullptr, "null pointer in a 4-bit matrix");
+  INF_CHECK_ARG(aligned(w->packed, 16), "a packed matrix must lie at a multiple of 16 bytes");
   return INFERNO_OK;
 }
 
@@ -56,7 +60,7 @@ int check_pair(const inferno_w4* gate, const inferno_w4* up) {
   INF_CHECK_ARG(gate->experts == up->experts && gate->rows == up->rows && gate->cols == up->cols,
                 "the gate and up matrices must have the same sizes");
   INF_CHECK_ARG(gate->group == up->group && gate->scale_dtype == up->scale_dtype &&
-                    (gate->zeros == nullptr) == (up->zeros == nullptr),
+                    (gate->has_zeros != 0) == (up->has_zeros != 0),
                 "the gate and up matrices must have the same group, scale type and zero points");
   return INFERNO_OK;
 }
@@ -91,23 +95,14 @@ W4Acts carve_acts(Carver& c, size_t rows, size_t cols) {
 // The same region for the matrices and activations of one call.
 W4Acts acts_for(W4Acts a, const inferno_w4* w, int x_dtype) {
   a.P = x_dtype == INFERNO_I8 ? 1 : 3;
-  a.fine = w->group < size_t(kW4Chunk);
+  a.fine = mat(w).fine();
   return a;
-}
-
-W4Mat mat(const inferno_w4* w) {
-  return W4Mat{static_cast<const uint8_t*>(w->codes), w->scales,
-               static_cast<const uint8_t*>(w->zeros)};
 }
 
 W4Product product(const inferno_w4* w, const W4Acts& x, size_t T, float* out) {
   W4Product p{};
   p.m[0] = mat(w);
   p.mats = 1;
-  p.scale_dtype = w->scale_dtype;
-  p.K = w->cols;
-  p.N = w->rows;
-  p.group = w->group;
   p.x = x;
   p.T = T;
   p.out = out;
@@ -147,6 +142,33 @@ int check_ws(void* workspace, size_t have, size_t need) {
 using namespace inferno;
 
 extern "C" {
+
+size_t inferno_w4_packed_bytes(const inferno_w4* w) {
+  clear_error();
+  return check_shape("given", w) ? 0 : w4_layout(mat(w)).bytes;
+}
+
+int inferno_w4_pack(void* stream, const inferno_w4* w, const void* codes, size_t codes_bytes,
+                    const void* scales, size_t scales_bytes, const void* zeros, size_t zeros_bytes,
+                    void* packed) {
+  clear_error();
+  int st;
+  if ((st = check_shape("given", w))) return st;
+  const size_t rows = w->experts * w->rows, groups = rows * (w->cols / w->group);
+  const size_t each = w->scale_dtype == INFERNO_BF16 ? 2 : 4;
+  if ((st = check_bytes("given", "codes", codes_bytes, rows * (w->cols / 2)))) return st;
+  if ((st = check_bytes("given", "scales", scales_bytes, groups * each))) return st;
+  if (w->has_zeros && (st = check_bytes("given", "zero points", zeros_bytes, groups))) return st;
+  if ((st = check_bytes("given", "packed form", w->packed_bytes, w4_layout(mat(w)).bytes))) return st;
+  INF_CHECK_ARG(codes && scales && packed && (zeros || !w->has_zeros), "null pointer");
+  INF_CHECK_ARG(aligned(codes, 4) && aligned(scales, each),
+                "codes must lie at a multiple of 4 bytes, scales at one of their size");
+  INF_CHECK_ARG(aligned(packed, 16), "a packed matrix must lie at a multiple of 16 bytes");
+  INF_CHECK_ARG(rows * w->cols < (size_t(1) << 42), "too many codes");
+  if (int st_ = require_device()) return st_;
+  return launch_w4_pack(as_stream(stream), mat(w), codes, scales, w->has_zeros ? zeros : nullptr,
+                        packed);
+}
 
 size_t inferno_w4_workspace_bytes(size_t T, size_t cols) {
   Carver c{nullptr};
@@ -241,7 +263,6 @@ int inferno_w4_moe(void* stream, const inferno_w4* gate, const inferno_w4* up,
   g.sorted = m.sorted;
   g.active = m.active;
   g.k = k;
-  g.E = E;
   g.route_w = expert_weights;
   if ((st = launch_w4_product(s, g))) return st;
   if ((st = launch_w4_stage(s, m.h, INFERNO_F32, nullptr, 0, T * k, I, ha))) return st;
@@ -250,7 +271,6 @@ int inferno_w4_moe(void* stream, const inferno_w4* gate, const inferno_w4* up,
   d.sorted = m.sorted;
   d.active = m.active;
   d.k = k;
-  d.E = E;
   d.x_by_assignment = true;
   if ((st = launch_w4_product(s, d))) return st;
   return launch_w4_combine(s, m.y, expert_ids, T, H, k, E, out);

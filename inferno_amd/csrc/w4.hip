@@ -12,9 +12,12 @@
 //
 // Tile: 16 weight rows (the 16 columns of a 16x16 MFMA result) by 16 digit
 // rows. A lane holds 32 codes of its row per chunk (16 bytes: low nibbles are
-// the even columns, high nibbles the odd ones). Any order of the columns
-// inside a group gives the same sum, so the codes are used as they lie and the
+// the even columns, high nibbles the odd ones); the packed matrix has the 1 KB
+// of a tile's chunk together in the lanes' order. Any order of the columns
+// inside a group gives the same sum, so no code moves inside its bytes, and the
 // digits are laid out to match.
+#include <type_traits>
+
 #include "w4.hpp"
 
 namespace inferno {
@@ -143,14 +146,63 @@ __global__ void __launch_bounds__(256) w4_stage_kernel(Stage p) {
   if (b == 0) p.a.xs[rc] = xs;
 }
 
+// -------------------------------------------------------------------- pack
+
+struct Pack {
+  const uint8_t* codes;
+  const void* scales;
+  const uint8_t* zeros;
+  uint8_t* to;
+  size_t scales_at, zeros_at;  // byte offsets in `to`
+  uint32_t tiles;              // all experts'
+  uint32_t row_tiles, N, K, C, group, groups;
+  bool fine;
+};
+
+// One wavefront per tile and chunk. Rows behind N and columns behind K get the
+// code, the scale and the zero point that count nothing.
+template <typename ST>
+__global__ void __launch_bounds__(256) w4_pack_kernel(Pack p) {
+  const size_t tc = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (tc >= size_t(p.tiles) * p.C) return;
+  const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+  const uint32_t tile = uint32_t(tc / p.C), c = uint32_t(tc % p.C);
+  const uint32_t row = tile % p.row_tiles * 16 + n;
+  const size_t mrow = size_t(tile / p.row_tiles) * p.N + min(row, p.N - 1);
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(p.codes + mrow * (p.K / 2));
+  v4u v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    // coarse groups: block `quad`; fine ones: dword `quad` of every block
+    const int block = p.fine ? j : quad, word = p.fine ? quad : j;
+    const uint32_t col = c * kW4Chunk + 32 * block;
+    const bool in = row < p.N && col < p.K;
+    const uint32_t u = src[in ? col / 8 + word : 0];
+    v[j] = p.zeros ? (in ? u : 0u) : (in ? u ^ 0x88888888u : 0u);  // q, or q - 8
+  }
+  *reinterpret_cast<v4u*>(p.to + tc * 1024 + lane * 16) = v;
+  // lane (n, quad): the scale of block `quad`, or for coarse groups of all
+  if (!p.fine && quad) return;
+  const uint32_t col = c * kW4Chunk + 32 * quad;
+  const bool in = row < p.N && col < p.K;
+  const size_t from = mrow * p.groups + (in ? col / p.group : 0);
+  const size_t at = p.fine ? (tc * 16 + n) * 4 + quad : tc * 16 + n;
+  const ST s = static_cast<const ST*>(p.scales)[from];
+  reinterpret_cast<ST*>(p.to + p.scales_at)[at] = in ? s : ST(0);
+  if (p.zeros) p.to[p.zeros_at + at] = in ? uint8_t(min(uint32_t(p.zeros[from]), 127u)) : 0;
+}
+
 // ----------------------------------------------------------------- product
 
+struct Mat {
+  const uint8_t* codes;   // [tiles][chunks][64][16]
+  const uint8_t* scales;  // [tiles][chunks][16][1 or 4] of the scale type
+  const uint8_t* zeros;   // likewise, bytes
+};
+
 struct Product {
-  W4Mat m[2];
-  int scale_bf16;
-  uint32_t K, N, C, groups;  // columns, rows, chunks, groups per row
-  uint32_t log2_group;       // fine groups
-  uint32_t chunks_per_group; // coarse groups
+  Mat m[2];
+  uint32_t N, C, row_tiles;  // rows, chunks and row tiles of one expert's matrix
   const int8_t* planes;
   const float* xs;
   uint32_t T;
@@ -165,342 +217,326 @@ struct Product {
   float* out;
 };
 
-__device__ __forceinline__ float load_scale(const void* p, int bf16, size_t i) {
-  return bf16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i])
-              : static_cast<const float*>(p)[i];
-}
-
-// 4x4 transpose of the dwords that the four 16-lane rows of a wavefront hold:
-// dword j of row q becomes dword q of row j.
-__device__ __forceinline__ void transpose4(uint32_t (&d)[4]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const auto r = __builtin_amdgcn_permlane32_swap(d[j], d[j + 2], false, false);
-    d[j] = r[0];
-    d[j + 2] = r[1];
-  }
-#pragma unroll
-  for (int j = 0; j < 4; j += 2) {
-    const auto r = __builtin_amdgcn_permlane16_swap(d[j], d[j + 1], false, false);
-    d[j] = r[0];
-    d[j + 1] = r[1];
-  }
-}
-
-enum Kind { kPack3, kOne, kWide3 };
-
-// Tokens of one tile: kPack3 holds a token's three digits in rows 4 t, 4 t + 1,
-// 4 t + 2 of one 16x16 result (one lane then has all three sums of a token);
-// kOne and kWide3 hold 16 tokens, kWide3 in three results, one per digit.
-template <int KIND>
-struct KindOf {
-  static constexpr int P = KIND == kOne ? 1 : 3;
-  static constexpr int tokens = KIND == kPack3 ? 4 : 16;
-  static constexpr int tiles = KIND == kWide3 ? 3 : 1;
-  static constexpr int values = KIND == kPack3 ? 1 : 4;  // tokens per lane
+// The expert of this workgroup (blockIdx.y) and its assignments, or all tokens;
+// false: none. Uniform values.
+struct Slot {
+  uint32_t expert, first, end;
 };
+__device__ __forceinline__ bool slot_of(const Product& p, Slot& s) {
+  s = Slot{0, 0, p.T};
+  if (!p.offsets) return true;
+  if (blockIdx.y >= p.active[0]) return false;
+  s.expert = __builtin_amdgcn_readfirstlane(p.active[1 + blockIdx.y]);
+  s.first = __builtin_amdgcn_readfirstlane(p.offsets[s.expert]);
+  s.end = __builtin_amdgcn_readfirstlane(p.offsets[s.expert + 1]);
+  return true;
+}
+
+// Activation row of assignment (or token) i of a slot; the last one's behind it.
+__device__ __forceinline__ size_t x_row(const Product& p, const Slot& s, uint32_t i) {
+  const uint32_t j = min(i, s.end - 1);
+  if (!p.offsets) return j;
+  const uint32_t a = p.sorted[j];
+  return p.x_by_assignment ? a : a / p.k;
+}
+
+__device__ __forceinline__ void store_result(const Product& p, uint32_t j, uint32_t row, float g,
+                                             const float* u) {
+  const size_t a = p.offsets ? p.sorted[j] : j;
+  float y = u ? g / (1.f + expf(-g)) * *u : g;
+  if (p.route_w) y *= p.route_w[a];
+  const size_t at = a * p.N + row;
+  if (p.res_a) y += p.res_a[at];
+  if (p.res_b) y += p.res_b[at];
+  p.out[at] = y;
+}
+
+// One chunk of one weight tile on its way: codes, and the scales and zero
+// points of this lane's row (of its four blocks for fine groups).
+template <bool FINE, bool ZEROS, typename ST>
+struct Codes {
+  static constexpr int B = FINE ? 4 : 1;
+  typedef ST SV __attribute__((ext_vector_type(B)));
+  v4u q;
+  SV s;
+  uint32_t z;
+
+  // tc: the tile's chunk
+  __device__ __forceinline__ void load(const Mat& m, size_t tc, int lane) {
+    q = reinterpret_cast<const v4u*>(m.codes)[tc * 64 + lane];
+    s = reinterpret_cast<const SV*>(m.scales)[tc * 16 + (lane & 15)];
+    if (ZEROS) {
+      if (FINE) z = reinterpret_cast<const uint32_t*>(m.zeros)[tc * 16 + (lane & 15)];
+      else z = m.zeros[tc * 16 + (lane & 15)];
+    }
+  }
+  // Even and odd columns as int8: 16 (q - 8), or q - z with zero points (z is at
+  // most 127: no byte borrows from the next).
+  __device__ __forceinline__ void widen(v4i& even, v4i& odd) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (ZEROS) {
+        const uint32_t zz = (FINE ? (z >> (8 * j)) & 255u : z) * 0x01010101u;
+        even[j] = int((((q[j] & 0x0f0f0f0fu) | 0x80808080u) - zz) ^ 0x80808080u);
+        odd[j] = int(((((q[j] >> 4) & 0x0f0f0f0fu) | 0x80808080u) - zz) ^ 0x80808080u);
+      } else {
+        even[j] = int((q[j] << 4) & 0xf0f0f0f0u);
+        odd[j] = int(q[j] & 0xf0f0f0f0u);
+      }
+    }
+  }
+  // Scale of block b for widen's values; 0 for a chunk that is not `there`.
+  __device__ __forceinline__ float scale(int b, bool there) const {
+    float v;
+    if constexpr (sizeof(ST) == 2) v = bf16_bits_to_f32(s[b]);
+    else v = s[b];
+    return there ? (ZEROS ? v : v * 0.0625f) : 0.f;
+  }
+};
+
+__device__ __forceinline__ long two(uint32_t a, uint32_t b) {
+  return long((uint64_t(b) << 32) | a);
+}
+
+// Sums of one chunk's block b: 16 digit rows (the two halves x0, x1 of a plane)
+// by 16 weight rows.
+template <bool FINE>
+__device__ __forceinline__ v4i dot(const v4u& x0, const v4u& x1, const v4i& even, const v4i& odd,
+                                   int b) {
+  v4i s = {0, 0, 0, 0};
+  if (FINE) {
+    const v4u& u = b < 2 ? x0 : x1;
+    return __builtin_amdgcn_mfma_i32_16x16x32_i8(two(u[2 * (b % 2)], u[2 * (b % 2) + 1]),
+                                                 two(uint32_t(even[b]), uint32_t(odd[b])), s, 0, 0,
+                                                 0);
+  }
+  s = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, x0), even, s, 0, 0, 0);
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, x1), odd, s, 0, 0, 0);
+}
 
 // Sum of a token's digits' sums as a float; a sum is at most 2^21.
 __device__ __forceinline__ float join(int hi, int mid, int lo) {
   return fmaf(float((hi << 8) + mid), 256.f, float(lo));
 }
 
-// Four even and four odd columns of a dword of codes as int8: 16 (q - 8), or
-// q - z with zero points (zz: z in every byte, at most 127, so that no byte
-// borrows from the next).
-template <bool ZEROS>
-__device__ __forceinline__ void widen(uint32_t d, uint32_t zz, int& even, int& odd) {
-  if (ZEROS) {
-    even = int((((d & 0x0f0f0f0fu) | 0x80808080u) - zz) ^ 0x80808080u);
-    odd = int(((((d >> 4) & 0x0f0f0f0fu) | 0x80808080u) - zz) ^ 0x80808080u);
-  } else {
-    const uint32_t u = d ^ 0x88888888u;
-    even = int((u << 4) & 0xf0f0f0f0u);
-    odd = int(u & 0xf0f0f0f0u);
-  }
-}
+// Token tiles of the rows kernel. kPack3 holds a token's three digits in rows
+// 4 t, 4 t + 1, 4 t + 2 of one 16x16 result (one lane then has all three sums of
+// a token); kOne and kWide3 hold 16 tokens, kWide3 in three results, one per
+// digit.
+enum Kind { kPack3, kOne, kWide3 };
 
-__device__ __forceinline__ uint32_t spread(uint32_t z) { return min(z, 127u) * 0x01010101u; }
-
-// The scale of one group, for widen's codes.
-template <bool ZEROS>
-__device__ __forceinline__ float code_scale(const Product& p, int m, size_t i) {
-  return load_scale(p.m[m].scales, p.scale_bf16, i) * (ZEROS ? 1.f : 0.0625f);
-}
-
-__device__ __forceinline__ long two(uint32_t a, uint32_t b) {
-  return long((uint64_t(b) << 32) | a);
-}
-
-// One workgroup: 16 rows of the matrices (the same rows of both), all tokens
-// of one expert (or of the batch) in tiles; the four wavefronts share the
-// chunks and add their sums in order.
-template <bool FINE, int MATS, int KIND, bool ZEROS>
+// Few tokens. One workgroup: 16 rows of the matrices (the same rows of both),
+// all tokens of one expert (or of the batch) in tiles; the four wavefronts
+// share the chunks and add their sums in order.
+template <bool FINE, int MATS, int P, bool ZEROS, typename ST>
 __global__ void __launch_bounds__(256) w4_rows_kernel(Product p) {
-  using KO = KindOf<KIND>;
-  constexpr int P = KO::P, TT = KO::tokens, NT = KO::tiles, NV = KO::values;
-  __shared__ float part[4][MATS * NV][kWave];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int B = FINE ? 4 : 1;
+  __shared__ float part[4][MATS * 4][kWave];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;
-  size_t expert = 0;
-  uint32_t first = 0, end = p.T;
-  if (p.offsets) {
-    if (blockIdx.y >= p.active[0]) return;
-    expert = p.active[1 + blockIdx.y];
-    first = p.offsets[expert];
-    end = p.offsets[expert + 1];
-  }
+  Slot slot;
+  if (!slot_of(p, slot)) return;
+  const uint32_t end = slot.end;
   const uint32_t row = blockIdx.x * 16 + n;
-  const size_t mrow = expert * p.N + min(row, p.N - 1);
+  const size_t tile = (size_t(slot.expert) * p.row_tiles + blockIdx.x) * p.C;
   const uint32_t c0 = p.C * wave / 4, c1 = p.C * (wave + 1) / 4;
-  // activation row of assignment (or token) i
-  auto x_row = [&](uint32_t i) -> size_t {
-    const uint32_t j = min(i, end - 1);
-    if (!p.offsets) return j;
-    const uint32_t a = p.sorted[j];
-    return p.x_by_assignment ? a : a / p.k;
-  };
-  for (uint32_t t0 = first; t0 < end; t0 += TT) {
+  uint32_t t0 = slot.first;
+  auto run = [&](auto kind) __attribute__((always_inline)) {
+    constexpr int KIND = decltype(kind)::value;
+    constexpr int NT = KIND == kWide3 ? 3 : 1;   // results
+    constexpr int NV = KIND == kPack3 ? 1 : 4;   // tokens per lane
     // this lane's operand row, and the tokens whose sums it gets
-    const size_t xr = x_row(t0 + (KIND == kPack3 ? n / 4 : n));
-    const int plane = KIND == kPack3 ? min(n & 3, 2) : 0;
-    size_t vr[NV];
+    const int8_t* xp = p.planes + x_row(p, slot, t0 + (KIND == kPack3 ? n / 4 : n)) * p.C *
+                                      (P * kW4Chunk) +
+                       (KIND == kPack3 ? min(n & 3, 2) * kW4Chunk : 0) + quad * 16;
+    const float* sp[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) vr[i] = x_row(t0 + (KIND == kPack3 ? quad : 4 * quad + i));
+    for (int i = 0; i < NV; ++i)
+      sp[i] = p.xs + x_row(p, slot, t0 + (KIND == kPack3 ? quad : 4 * quad + i)) * p.C;
     float acc[MATS][NV];
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
 #pragma unroll
       for (int i = 0; i < NV; ++i) acc[m][i] = 0.f;
-    for (uint32_t c = c0; c < c1; ++c) {
-      v4u xe[NT], xo[NT];
+    // loads on their way, of two chunks
+    Codes<FINE, ZEROS, ST> w[2][MATS];
+    v4u x[2][NT][2];
+    float xs[2][NV];
+    auto load = [&](uint32_t chunk, int to) {
+      const uint32_t c = min(chunk, p.C - 1);
+#pragma unroll
+      for (int m = 0; m < MATS; ++m) w[to][m].load(p.m[m], tile + c, lane);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const v4u* x = reinterpret_cast<const v4u*>(
-            p.planes + ((xr * p.C + c) * P + plane + t) * kW4Chunk + quad * 16);
-        xe[t] = x[0];
-        xo[t] = x[4];
+        const v4u* at =
+            reinterpret_cast<const v4u*>(xp + size_t(c) * (P * kW4Chunk) + t * kW4Chunk);
+        x[to][t][0] = at[0];
+        x[to][t][1] = at[4];
       }
-      float xs[NV];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) xs[i] = p.xs[vr[i] * p.C + c];
+      for (int i = 0; i < NV; ++i) xs[to][i] = sp[i][c];
+    };
+    auto step = [&](uint32_t c, int cur) {
 #pragma unroll
       for (int m = 0; m < MATS; ++m) {
-        uint32_t d[4] = {0, 0, 0, 0};
-        if (c * kW4Chunk + quad * 32 < p.K) {
-          const v4u v = *reinterpret_cast<const v4u*>(p.m[m].codes + mrow * (p.K / 2) +
-                                                      c * (kW4Chunk / 2) + quad * 16);
-          d[0] = v[0]; d[1] = v[1]; d[2] = v[2]; d[3] = v[3];
-        }
-        if (FINE) transpose4(d);
-        v4i lo, hi;
-        float ws[FINE ? 4 : 1];
-#pragma unroll
-        for (int b = 0; b < (FINE ? 4 : 1); ++b) {
-          const uint32_t g = FINE ? min((c * kW4Chunk + 32 * b) >> p.log2_group, p.groups - 1)
-                                  : c / p.chunks_per_group;
-          ws[b] = code_scale<ZEROS>(p, m, mrow * p.groups + g);
-          const uint32_t zz = ZEROS ? spread(p.m[m].zeros[mrow * p.groups + g]) : 0u;
-          if (FINE) {
-            int l, h;
-            widen<ZEROS>(d[b], zz, l, h);
-            lo[b] = l;
-            hi[b] = h;
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              int l, h;
-              widen<ZEROS>(d[j], zz, l, h);
-              lo[j] = l;
-              hi[j] = h;
-            }
-          }
-        }
+        v4i even, odd;
+        w[cur][m].widen(even, odd);
         float value[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) value[i] = 0.f;
-#pragma unroll
-        for (int b = 0; b < (FINE ? 4 : 1); ++b) {
+        for (int b = 0; b < B; ++b) {
           v4i sum[NT];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            sum[t] = v4i{0, 0, 0, 0};
-            if (FINE) {
-              const long xb = b < 2 ? two(xe[t][2 * b], xe[t][2 * b + 1])
-                                    : two(xo[t][2 * b - 4], xo[t][2 * b - 3]);
-              sum[t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
-                  xb, two(uint32_t(lo[b]), uint32_t(hi[b])), sum[t], 0, 0, 0);
-            } else {
-              sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, xe[t]), lo,
-                                                             sum[t], 0, 0, 0);
-              sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, xo[t]), hi,
-                                                             sum[t], 0, 0, 0);
-            }
-          }
+          for (int t = 0; t < NT; ++t)
+            sum[t] = dot<FINE>(x[cur][t][0], x[cur][t][1], even, odd, b);
+          const float ws = w[cur][m].scale(b, c < c1);
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
             float f;
             if (KIND == kPack3) f = join(sum[0][0], sum[0][1], sum[0][2]);
             else if (KIND == kOne) f = float(sum[0][i]);
-            else f = join(sum[0][i], sum[NT > 1 ? 1 : 0][i], sum[NT > 2 ? 2 : 0][i]);
-            value[i] = fmaf(ws[b], f, value[i]);
+            else f = join(sum[0][i], sum[NT / 2][i], sum[NT - 1][i]);
+            value[i] = b == 0 ? ws * f : fmaf(ws, f, value[i]);
           }
         }
 #pragma unroll
-        for (int i = 0; i < NV; ++i) acc[m][i] = fmaf(value[i], xs[i], acc[m][i]);
+        for (int i = 0; i < NV; ++i) acc[m][i] = fmaf(value[i], xs[cur][i], acc[m][i]);
+      }
+      load(c + 2, cur);
+    };
+    if (c0 < c1) {
+      load(c0, 0);
+      load(c0 + 1, 1);
+      // two at a time without a way past the second (a chunk behind the end has
+      // scales of 0): the wait counts of a loop hold for its shortest path
+      for (uint32_t c = c0; c < c1; c += 2) {
+        step(c, 0);
+        step(c + 1, 1);
       }
     }
-    __syncthreads();  // the last tile's sums are read
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
 #pragma unroll
       for (int i = 0; i < NV; ++i) part[wave][m * NV + i][lane] = acc[m][i];
     __syncthreads();
     // wavefront i writes token value i of every lane
-    if (wave < NV && row < p.N) {
-      const int i = wave;
-      const uint32_t t = t0 + (KIND == kPack3 ? quad : 4 * quad + i);
-      if (t < end) {
-        float v[MATS];
+    const uint32_t j = t0 + (KIND == kPack3 ? quad : 4 * quad + wave);
+    if (wave < NV && row < p.N && j < end) {
+      float v[MATS];
 #pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-          v[m] = part[0][m * NV + i][lane];
-          for (int w = 1; w < 4; ++w) v[m] += part[w][m * NV + i][lane];
-        }
-        const size_t a = p.offsets ? p.sorted[t] : t;
-        float y = v[0];
-        if (MATS == 2) y = v[0] / (1.f + expf(-v[0])) * v[MATS - 1];
-        if (p.route_w) y *= p.route_w[a];
-        const size_t at = a * p.N + row;
-        if (p.res_a) y += p.res_a[at];
-        if (p.res_b) y += p.res_b[at];
-        p.out[at] = y;
+      for (int m = 0; m < MATS; ++m) {
+        v[m] = part[0][m * NV + wave][lane];
+        for (int i = 1; i < 4; ++i) v[m] += part[i][m * NV + wave][lane];
       }
+      store_result(p, j, row, v[0], MATS == 2 ? &v[MATS - 1] : nullptr);
+    }
+    __syncthreads();  // before the next tokens' sums
+    t0 += KIND == kPack3 ? 4 : 16;
+  };
+  while (t0 < end) {
+    if constexpr (P == 1) {
+      run(std::integral_constant<int, kOne>{});
+    } else {
+      if (end - t0 <= 4) run(std::integral_constant<int, kPack3>{});
+      else run(std::integral_constant<int, kWide3>{});
     }
   }
 }
 
-template <bool FINE, int MATS, bool ZEROS>
-void run_rows(hipStream_t s, const Product& p, dim3 grid, int kind) {
-  if (kind == kPack3) w4_rows_kernel<FINE, MATS, kPack3, ZEROS><<<grid, 256, 0, s>>>(p);
-  else if (kind == kOne) w4_rows_kernel<FINE, MATS, kOne, ZEROS><<<grid, 256, 0, s>>>(p);
-  else w4_rows_kernel<FINE, MATS, kWide3, ZEROS><<<grid, 256, 0, s>>>(p);
-}
-
-// Many tokens. One workgroup: 64 tokens by 64 RT rows of the matrices; a
+// Many tokens. One workgroup: 64 tokens by 128 RT rows of the matrices; a
 // wavefront takes RT tiles of 16 rows of each matrix against all tokens. The
-// weights go from memory to the wavefront that owns them, one chunk ahead; the
-// tokens' digits go through LDS (two buffers, filled by the LDS DMA one chunk
-// ahead) in the order in which the matrix instructions' lanes read them, so
-// that a read is 1 KB without bank conflicts. Tiles of 16 tokens that an
-// expert does not have are left out.
-typedef const __attribute__((address_space(1))) void* gptr_t;
-typedef __attribute__((address_space(3))) void* lptr_t;
-
+// weights go from memory to the wavefront that owns them; the tokens' digits go
+// through LDS (two buffers of one chunk) in the order in which the matrix
+// instructions' lanes read them, so that a read is 1 KB without bank conflicts.
+// Both are two chunks ahead in registers, since a chunk's loads take longer
+// than its arithmetic (copies to LDS that bypass registers would have to be
+// complete before any LDS read). Tiles of 16 tokens that an expert does not
+// have are left out.
 constexpr int kTileTokens = 64;
+constexpr int kTileWaves = 8;
 
-template <bool FINE, int MATS, int P, bool ZEROS, int RT>
-__global__ void __launch_bounds__(256, 2) w4_tile_kernel(Product p) {
+template <bool FINE, int MATS, int P, bool ZEROS, typename ST, int RT>
+__global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p) {
   constexpr int F = MATS * RT, TT = kTileTokens / 16, B = FINE ? 4 : 1;
   __shared__ __align__(16) int8_t xt[2][TT][2 * P][kWave * 16];
   __shared__ __align__(16) float xst[2][kTileTokens];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;
-  size_t expert = 0;
-  uint32_t first = 0, end = p.T;
-  if (p.offsets) {
-    if (blockIdx.y >= p.active[0]) return;
-    expert = p.active[1 + blockIdx.y];
-    first = p.offsets[expert];
-    end = p.offsets[expert + 1];
-  }
-  const uint32_t row0 = (blockIdx.x * 4 + wave) * (16 * RT) + n;
-  const uint8_t* codes[F];
-  size_t group0[RT];  // of the row's first group
+  Slot slot;
+  if (!slot_of(p, slot)) return;
+  const uint32_t end = slot.end;
+  // this wavefront's row tiles; those behind the last are the last one again
+  const uint32_t tile0 = (blockIdx.x * kTileWaves + wave) * RT;
+  size_t tile[RT];
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const size_t mrow = expert * p.N + min(row0 + 16 * r, p.N - 1);
-    group0[r] = mrow * p.groups;
-#pragma unroll
-    for (int m = 0; m < MATS; ++m) codes[m * RT + r] = p.m[m].codes + mrow * (p.K / 2);
-  }
-  auto x_row = [&](uint32_t i) -> size_t {
-    const uint32_t j = min(i, end - 1);
-    if (!p.offsets) return j;
-    const uint32_t a = p.sorted[j];
-    return p.x_by_assignment ? a : a / p.k;
-  };
-  for (uint32_t t0 = first + blockIdx.z * kTileTokens; t0 < end; t0 += gridDim.z * kTileTokens) {
+  for (int r = 0; r < RT; ++r)
+    tile[r] = (size_t(slot.expert) * p.row_tiles + min(tile0 + r, p.row_tiles - 1)) * p.C;
+  for (uint32_t t0 = slot.first + blockIdx.z * kTileTokens; t0 < end;
+       t0 += gridDim.z * kTileTokens) {
     const uint32_t tokens = min(end - t0, uint32_t(kTileTokens));
-    // wavefront w copies the digits of token tile w, the first one the scales
-    const int8_t* xp = p.planes + x_row(t0 + 16 * wave + n) * p.C * (P * kW4Chunk) + quad * 16;
-    const float* sp = p.xs + x_row(t0 + lane) * p.C;
-    float acc[F][TT][4];
+    auto run = [&](auto token_tiles) __attribute__((always_inline)) {
+      constexpr int NT = decltype(token_tiles)::value;
+      // kTileWaves / 4 wavefronts bring the digits of a token tile, the first of
+      // them its scales
+      constexpr int kPieces = 8 * P / kTileWaves;
+      const int ct = wave * 4 / kTileWaves, cp = wave * kPieces % (2 * P);
+      const bool brings = 16u * ct < tokens;
+      const size_t xr = x_row(p, slot, t0 + 16 * ct + n) * p.C;
+      const int8_t* xp = p.planes + xr * (P * kW4Chunk) + cp * 64 + quad * 16;
+      const float* sp = p.xs + xr;
+      float acc[F][NT][4];
 #pragma unroll
-    for (int f = 0; f < F; ++f)
+      for (int f = 0; f < F; ++f)
 #pragma unroll
-      for (int t = 0; t < TT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[f][t][i] = 0.f;
-    auto copy = [&](uint32_t c) {
-      if (16u * wave < tokens) {
+          for (int i = 0; i < 4; ++i) acc[f][t][i] = 0.f;
+      // Loads on their way, of even and odd chunks. A chunk behind the end is the
+      // last one again.
+      Codes<FINE, ZEROS, ST> w[2][F];
+      v4u digits[2][kPieces];
+      float digit_s[2];
+      auto load_digits = [&](uint32_t chunk, int to) {
+        const uint32_t c = min(chunk, p.C - 1);
+        if (brings) {
 #pragma unroll
-        for (int i = 0; i < 2 * P; ++i)
-          __builtin_amdgcn_global_load_lds((gptr_t)(xp + size_t(c) * (P * kW4Chunk) + i * 64),
-                                           (lptr_t)&xt[c & 1][wave][i][0], 16, 0, 0);
-      }
-      if (wave == 0)
-        __builtin_amdgcn_global_load_lds((gptr_t)(sp + c), (lptr_t)&xst[c & 1][0], 4, 0, 0);
-    };
-    v4u next[F];
-    float next_s[F][B];
-    uint32_t next_z[F][B];
-    auto fetch = [&](uint32_t c) {
-      // columns behind K meet digits of 0: any codes do
-      const uint32_t at = min(c * (kW4Chunk / 2) + quad * 16, p.K / 2 - 16);
-#pragma unroll
-      for (int m = 0; m < MATS; ++m)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const int f = m * RT + r;
-          next[f] = *reinterpret_cast<const v4u*>(codes[f] + at);
-#pragma unroll
-          for (int b = 0; b < B; ++b) {
-            const uint32_t g = FINE ? min((c * kW4Chunk + 32 * b) >> p.log2_group, p.groups - 1)
-                                    : c / p.chunks_per_group;
-            next_s[f][b] = code_scale<ZEROS>(p, m, group0[r] + g);
-            next_z[f][b] = ZEROS ? p.m[m].zeros[group0[r] + g] : 0u;
-          }
+          for (int i = 0; i < kPieces; ++i)
+            digits[to][i] =
+                *reinterpret_cast<const v4u*>(xp + size_t(c) * (P * kW4Chunk) + i * 64);
+          digit_s[to] = sp[c];
         }
-    };
-    copy(0);
-    fetch(0);
-    for (uint32_t c = 0; c < p.C; ++c) {
-      v4i lo[F], hi[F];
-      float ws[F][B];
+      };
+      auto store_digits = [&](uint32_t c, int from) {
+        if (brings) {
 #pragma unroll
-      for (int f = 0; f < F; ++f) {
-        uint32_t d[4] = {next[f][0], next[f][1], next[f][2], next[f][3]};
-        if (FINE) transpose4(d);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          int l, h;
-          widen<ZEROS>(d[j], ZEROS ? spread(next_z[f][FINE ? j : 0]) : 0u, l, h);
-          lo[f][j] = l;
-          hi[f][j] = h;
+          for (int i = 0; i < kPieces; ++i)
+            *reinterpret_cast<v4u*>(&xt[c & 1][ct][cp + i][lane * 16]) = digits[from][i];
+          if (cp == 0 && lane < 16) xst[c & 1][16 * ct + n] = digit_s[from];
         }
+      };
+      auto load_codes = [&](uint32_t chunk, int to) {
+        const uint32_t c = min(chunk, p.C - 1);
 #pragma unroll
-        for (int b = 0; b < B; ++b) ws[f][b] = next_s[f][b];
-      }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wavefront's copies are in LDS
-      __builtin_amdgcn_s_barrier();  // everybody's are, and chunk c - 1 is read
-      if (c + 1 < p.C) {
-        copy(c + 1);
-        fetch(c + 1);
-      }
+        for (int f = 0; f < F; ++f) w[to][f].load(p.m[f / RT], tile[f % RT] + c, lane);
+      };
+      auto step = [&](uint32_t c, int cur) {
+        // everybody has stored chunk c, and has read chunk c - 1
+        __syncthreads();
+        store_digits(c + 1, cur ^ 1);
+        load_digits(c + 3, cur ^ 1);
+        v4i even[F], odd[F];
+        float ws[F][B];
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        if (16u * t < tokens) {  // uniform
+        for (int f = 0; f < F; ++f) {
+          w[cur][f].widen(even[f], odd[f]);
+#pragma unroll
+          for (int b = 0; b < B; ++b) ws[f][b] = w[cur][f].scale(b, c < p.C);
+        }
+        load_codes(c + 2, cur);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
           v4u x[2 * P];
 #pragma unroll
           for (int i = 0; i < 2 * P; ++i)
@@ -514,20 +550,8 @@ __global__ void __launch_bounds__(256, 2) w4_tile_kernel(Product p) {
             for (int b = 0; b < B; ++b) {
               v4i sum[P];
 #pragma unroll
-              for (int q = 0; q < P; ++q) {
-                sum[q] = v4i{0, 0, 0, 0};
-                if (FINE) {
-                  const v4u u = x[2 * q + b / 2];
-                  sum[q] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
-                      two(u[2 * (b % 2)], u[2 * (b % 2) + 1]),
-                      two(uint32_t(lo[f][b]), uint32_t(hi[f][b])), sum[q], 0, 0, 0);
-                } else {
-                  sum[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                      __builtin_bit_cast(v4i, x[2 * q]), lo[f], sum[q], 0, 0, 0);
-                  sum[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                      __builtin_bit_cast(v4i, x[2 * q + 1]), hi[f], sum[q], 0, 0, 0);
-                }
-              }
+              for (int q = 0; q < P; ++q)
+                sum[q] = dot<FINE>(x[2 * q], x[2 * q + 1], even[f], odd[f], b);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const float v = P == 3 ? join(sum[0][i], sum[P / 2][i], sum[P - 1][i])
@@ -537,48 +561,63 @@ __global__ void __launch_bounds__(256, 2) w4_tile_kernel(Product p) {
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[f][t][i] = fmaf(value[i], xs[i], acc[f][t][i]);
+            if (FINE) __builtin_amdgcn_sched_barrier(0);  // (registers)
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      load_digits(0, 0);
+      load_digits(1, 1);
+      load_codes(0, 0);
+      load_codes(1, 1);
+      store_digits(0, 0);
+      load_digits(2, 0);
+      // two at a time without a way past the second (a chunk behind the end has
+      // scales of 0): the wait counts of a loop hold for its shortest path
+      for (uint32_t c = 0; c < p.C; c += 2) {
+        step(c, 0);
+        step(c + 1, 1);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t j = t0 + 16 * t + 4 * quad + i;
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const uint32_t row = (tile0 + r) * 16 + n;
+            if (j < end && row < p.N)
+              store_result(p, j, row, acc[r][t][i],
+                           MATS == 2 ? &acc[(MATS - 1) * RT + r][t][i] : nullptr);
           }
         }
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t j = t0 + 16 * t + 4 * quad + i;
-        if (j >= end) continue;
-        const size_t a = p.offsets ? p.sorted[j] : j;
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const uint32_t row = row0 + 16 * r;
-          if (row >= p.N) continue;
-          float y = acc[r][t][i];
-          if (MATS == 2) y = y / (1.f + expf(-y)) * acc[(MATS - 1) * RT + r][t][i];
-          if (p.route_w) y *= p.route_w[a];
-          const size_t at = a * p.N + row;
-          if (p.res_a) y += p.res_a[at];
-          if (p.res_b) y += p.res_b[at];
-          p.out[at] = y;
-        }
-      }
-    }
+    };
+    // a loop for each number of token tiles: a branch for each tile inside one
+    // loop takes twice the registers
+    if (tokens > 48) run(std::integral_constant<int, 4>{});
+    else if (tokens > 32) run(std::integral_constant<int, 3>{});
+    else if (tokens > 16) run(std::integral_constant<int, 2>{});
+    else run(std::integral_constant<int, 1>{});
     __syncthreads();  // the last chunk is read: the next tokens' first may come
   }
 }
 
-template <bool FINE, int MATS, int P, bool ZEROS>
-void run_tiles(hipStream_t s, const Product& p, unsigned slots, unsigned blocks) {
-  constexpr int RT = MATS == 2 ? 2 : 4;
-  const dim3 grid((p.N + 64 * RT - 1) / (64 * RT), slots, blocks);
-  w4_tile_kernel<FINE, MATS, P, ZEROS, RT><<<grid, 256, 0, s>>>(p);
-}
-
-template <bool FINE, bool ZEROS>
-void run_tiles(hipStream_t s, const Product& p, int mats, int P, unsigned slots, unsigned blocks) {
-  if (mats == 2 && P == 3) run_tiles<FINE, 2, 3, ZEROS>(s, p, slots, blocks);
-  else if (mats == 2) run_tiles<FINE, 2, 1, ZEROS>(s, p, slots, blocks);
-  else if (P == 3) run_tiles<FINE, 1, 3, ZEROS>(s, p, slots, blocks);
-  else run_tiles<FINE, 1, 1, ZEROS>(s, p, slots, blocks);
+// Calls f with the instance's constants: (fine groups, matrices, zero points,
+// scale type) as values of integral_constant and a scale.
+template <typename Fn>
+void by_format(const W4Product& q, Fn f) {
+  auto scale = [&](auto fine, auto mats, auto zeros) {
+    q.m[0].scale_dtype == INFERNO_BF16 ? f(fine, mats, zeros, uint16_t{})
+                                       : f(fine, mats, zeros, 0.f);
+  };
+  auto zero = [&](auto fine, auto mats) {
+    q.m[0].zeros ? scale(fine, mats, std::true_type{}) : scale(fine, mats, std::false_type{});
+  };
+  auto mat = [&](auto fine) {
+    q.mats == 2 ? zero(fine, std::integral_constant<int, 2>{})
+                : zero(fine, std::integral_constant<int, 1>{});
+  };
+  q.m[0].fine() ? mat(std::true_type{}) : mat(std::false_type{});
 }
 
 // ----------------------------------------------------------------- combine
@@ -610,17 +649,52 @@ int launch_w4_stage(hipStream_t s, const void* x, int x_dtype, const float* x_sc
   return INFERNO_OK;
 }
 
+W4Layout w4_layout(const W4Mat& m) {
+  const size_t per = m.fine() ? 4 : 1;
+  const size_t tc = m.experts * ((m.rows + 15) / 16) * w4_chunks(m.cols);
+  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  W4Layout l;
+  l.scales = up(tc * 1024);
+  l.zeros = l.scales + up(tc * 16 * per * (m.scale_dtype == INFERNO_BF16 ? 2 : 4));
+  l.bytes = l.zeros + (m.zeros ? up(tc * 16 * per) : 0);
+  return l;
+}
+
+int launch_w4_pack(hipStream_t s, const W4Mat& m, const void* codes, const void* scales,
+                   const void* zeros, void* packed) {
+  const W4Layout l = w4_layout(m);
+  Pack p{};
+  p.codes = static_cast<const uint8_t*>(codes);
+  p.scales = scales;
+  p.zeros = static_cast<const uint8_t*>(zeros);
+  p.to = static_cast<uint8_t*>(packed);
+  p.scales_at = l.scales;
+  p.zeros_at = l.zeros;
+  p.row_tiles = uint32_t((m.rows + 15) / 16);
+  p.tiles = uint32_t(m.experts * p.row_tiles);
+  p.N = uint32_t(m.rows);
+  p.K = uint32_t(m.cols);
+  p.C = uint32_t(w4_chunks(m.cols));
+  p.group = uint32_t(m.group);
+  p.groups = uint32_t(m.cols / m.group);
+  p.fine = m.fine();
+  const unsigned grid = unsigned((size_t(p.tiles) * p.C + 3) / 4);
+  if (m.scale_dtype == INFERNO_BF16) w4_pack_kernel<uint16_t><<<grid, 256, 0, s>>>(p);
+  else w4_pack_kernel<float><<<grid, 256, 0, s>>>(p);
+  INF_LAUNCHED();
+  return INFERNO_OK;
+}
+
 int launch_w4_product(hipStream_t s, const W4Product& q) {
   Product p{};
-  p.m[0] = q.m[0];
-  p.m[1] = q.m[1];
-  p.scale_bf16 = q.scale_dtype == INFERNO_BF16;
-  p.K = uint32_t(q.K);
-  p.N = uint32_t(q.N);
-  p.C = uint32_t(w4_chunks(q.K));
-  p.groups = uint32_t(q.K / q.group);
-  p.log2_group = q.group == 32 ? 5 : 6;
-  p.chunks_per_group = uint32_t(q.group / kW4Chunk);
+  for (int m = 0; m < q.mats; ++m) {
+    const W4Layout l = w4_layout(q.m[m]);
+    const uint8_t* at = static_cast<const uint8_t*>(q.m[m].packed);
+    p.m[m] = Mat{at, at + l.scales, at + l.zeros};
+  }
+  p.N = uint32_t(q.m[0].rows);
+  p.C = uint32_t(w4_chunks(q.m[0].cols));
+  p.row_tiles = (p.N + 15) / 16;
   p.planes = q.x.planes;
   p.xs = q.x.xs;
   p.T = uint32_t(q.T);
@@ -633,34 +707,35 @@ int launch_w4_product(hipStream_t s, const W4Product& q) {
   p.res_a = q.res_a;
   p.res_b = q.res_b;
   p.out = q.out;
-  const unsigned slots = q.offsets ? unsigned(std::min(q.E, q.T * q.k)) : 1u;
-  const bool zeros = q.m[0].zeros != nullptr;
+  const unsigned slots = q.offsets ? unsigned(std::min(q.m[0].experts, q.T * q.k)) : 1u;
   const size_t per_slot = q.T * (q.offsets ? q.k : 1) / slots;
+  const bool one = q.x.P == 1;
   if (per_slot > 16) {
     // workgroups of a slot beyond its tokens end at once; a slot with more
     // tokens than they take goes round again
     const size_t blocks = q.offsets ? std::min<size_t>(2 * per_slot / kTileTokens + 1, 8)
                                     : (q.T + kTileTokens - 1) / kTileTokens;
-    const unsigned z = unsigned(std::min<size_t>(blocks, 65535));
-    if (q.x.fine) zeros ? run_tiles<true, true>(s, p, q.mats, q.x.P, slots, z)
-                        : run_tiles<true, false>(s, p, q.mats, q.x.P, slots, z);
-    else zeros ? run_tiles<false, true>(s, p, q.mats, q.x.P, slots, z)
-               : run_tiles<false, false>(s, p, q.mats, q.x.P, slots, z);
-    INF_LAUNCHED();
-    return INFERNO_OK;
-  }
-  const dim3 grid(unsigned((q.N + 15) / 16), slots);
-  const int kind = q.x.P == 1 ? kOne : q.T <= 4 ? kPack3 : kWide3;
-  if (q.x.fine) {
-    if (q.mats == 2) zeros ? run_rows<true, 2, true>(s, p, grid, kind)
-                           : run_rows<true, 2, false>(s, p, grid, kind);
-    else zeros ? run_rows<true, 1, true>(s, p, grid, kind)
-               : run_rows<true, 1, false>(s, p, grid, kind);
+    by_format(q, [&](auto fine, auto mats, auto zeros, auto st) {
+      constexpr int M = decltype(mats)::value, RT = M == 2 ? 1 : 2;
+      constexpr unsigned tiles = RT * kTileWaves;
+      const dim3 grid((p.row_tiles + tiles - 1) / tiles, slots,
+                      unsigned(std::min<size_t>(blocks, 65535)));
+      using ST = decltype(st);
+      if (one)
+        w4_tile_kernel<fine.value, M, 1, zeros.value, ST, RT>
+            <<<grid, kTileWaves * kWave, 0, s>>>(p);
+      else
+        w4_tile_kernel<fine.value, M, 3, zeros.value, ST, RT>
+            <<<grid, kTileWaves * kWave, 0, s>>>(p);
+    });
   } else {
-    if (q.mats == 2) zeros ? run_rows<false, 2, true>(s, p, grid, kind)
-                           : run_rows<false, 2, false>(s, p, grid, kind);
-    else zeros ? run_rows<false, 1, true>(s, p, grid, kind)
-               : run_rows<false, 1, false>(s, p, grid, kind);
+    by_format(q, [&](auto fine, auto mats, auto zeros, auto st) {
+      constexpr int M = decltype(mats)::value;
+      const dim3 grid(p.row_tiles, slots);
+      using ST = decltype(st);
+      if (one) w4_rows_kernel<fine.value, M, 1, zeros.value, ST><<<grid, 256, 0, s>>>(p);
+      else w4_rows_kernel<fine.value, M, 3, zeros.value, ST><<<grid, 256, 0, s>>>(p);
+    });
   }
   INF_LAUNCHED();
   return INFERNO_OK;

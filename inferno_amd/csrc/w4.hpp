@@ -6,12 +6,28 @@ namespace inferno {
 
 constexpr int kW4Chunk = 128;  // columns of one step: 64 bytes of codes per row
 
-// One matrix, or one per expert, as the caller stores it.
+// One matrix, or one per expert, packed: for every tile of 16 rows and chunk of
+// 128 columns the 1024 bytes of codes that a wavefront's lanes take in one load
+// (16 each), then for all of them the scales of the 16 rows (one each, or four
+// for groups of 32 and 64: one per 32 columns), then likewise the zero points.
+// Rows behind the last and columns behind cols count nothing.
 struct W4Mat {
-  const uint8_t* codes;  // [rows, K/2], the even column in the low nibble
-  const void* scales;    // [rows, K/group] fp32 or bf16
-  const uint8_t* zeros;  // [rows, K/group], or null: 8
+  size_t experts, rows, cols, group;
+  int scale_dtype;
+  bool zeros;
+  const void* packed;
+  bool fine() const { return group < size_t(kW4Chunk); }
 };
+struct W4Layout {
+  size_t scales, zeros, bytes;  // byte offsets, and the size
+};
+W4Layout w4_layout(const W4Mat& m);
+inline size_t w4_chunks(size_t K) { return (K + kW4Chunk - 1) / kW4Chunk; }
+
+// Packs codes [rows, cols/2] (the even column in the low nibble), scales [rows,
+// cols/group] and zeros [rows, cols/group] or null (8).
+int launch_w4_pack(hipStream_t s, const W4Mat& m, const void* codes, const void* scales,
+                   const void* zeros, void* packed);
 
 // Activations as int8 digits, the operands of the integer matrix cores.
 // A value of a 128-column chunk is (65536 d0 + 256 d1 + d2) xs (3 planes; d in
@@ -26,8 +42,6 @@ struct W4Acts {
   bool fine;  // groups of 32 or 64 columns
 };
 
-inline size_t w4_chunks(size_t K) { return (K + kW4Chunk - 1) / kW4Chunk; }
-
 // Writes the activations' digits. x: fp32, bf16, or int8 with x_scales
 // [R, K / x_group] (x_group 0: one per row).
 int launch_w4_stage(hipStream_t s, const void* x, int x_dtype, const float* x_scales,
@@ -37,16 +51,14 @@ int launch_w4_stage(hipStream_t s, const void* x, int x_dtype, const float* x_sc
 // expert (dispatch outputs), activation rows by token or by assignment.
 struct W4Product {
   W4Mat m[2];
-  int mats;         // 2: silu(m0 x) * (m1 x) [* weight]
-  int scale_dtype;
-  size_t K, N, group;
+  int mats;         // 2: silu(m0 x) * (m1 x) [* weight], both of one format
   W4Acts x;
   size_t T;         // tokens
   // routed (offsets not null): assignments sorted by expert
   const uint32_t* offsets;
   const uint32_t* sorted;
   const uint32_t* active;
-  size_t k, E;
+  size_t k;
   bool x_by_assignment;
   const float* route_w;  // [T*k], multiplied into the result, or null
   const float* res_a;    // added (dense), or null

@@ -244,7 +244,8 @@ class W4:
     cols], or one per expert [E, rows, cols]. ``codes`` holds two columns a byte
     (uint8 [..., cols / 2], the even column in the low nibble), ``scales`` one
     factor per cols / scales.shape[-1] columns (fp32 or bf16), ``zeros`` a zero
-    point for each scale (uint8; None: 8). The tensors are used as they are."""
+    point for each scale (uint8; None: 8). Packed once, here (inferno_w4_pack);
+    the tensors are not kept."""
 
     def __init__(self, codes, scales, zeros=None):
         if codes.dtype != torch.uint8 or codes.dim() not in (2, 3) or not codes.is_contiguous():
@@ -259,15 +260,18 @@ class W4:
         _like(codes, "scales", scales, scales.dtype, *codes.shape[:-1], groups)
         if zeros is not None:
             _like(codes, "zeros", zeros, torch.uint8, *codes.shape[:-1], groups)
-        self.tensors = (codes, scales, zeros)
         self.device = codes.device
         self.experts = codes.shape[0] if codes.dim() == 3 else 1
         self.rows, self.cols, self.group = rows, cols, cols // groups
-        self.desc = W4Desc(
-            self.experts, rows, cols, self.group, _DT[scales.dtype], codes.data_ptr(),
-            scales.data_ptr(), zeros.data_ptr() if zeros is not None else None, codes.numel(),
-            scales.numel() * scales.element_size(), zeros.numel() if zeros is not None else 0)
-        self.ref = C.byref(self.desc)
+        d = W4Desc(self.experts, rows, cols, self.group, _DT[scales.dtype], int(zeros is not None),
+                   None, 0)
+        self.desc, self.ref = d, C.byref(d)
+        d.packed_bytes = lib().inferno_w4_packed_bytes(self.ref)
+        self.packed = torch.empty(d.packed_bytes, dtype=torch.uint8, device=codes.device)
+        _run(codes, lib().inferno_w4_pack, self.ref, _p(codes), codes.numel(), _p(scales),
+             scales.numel() * scales.element_size(), _p(zeros),
+             zeros.numel() if zeros is not None else 0, _p(self.packed))
+        d.packed = self.packed.data_ptr()
 
 
 _ACT = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: I8}

@@ -280,6 +280,14 @@ def _cpu(rows=16, cols=64, group=32, experts=0, **kw):
     return ref.make(torch.Generator().manual_seed(0), rows, cols, group, experts, device="cpu", **kw)
 
 
+def _unpacked(rows=16, cols=64, experts=1):
+    """A handle of these sizes without its matrix: the checks come first."""
+    w = object.__new__(ops.W4)
+    w.rows, w.cols, w.experts, w.device = rows, cols, experts, torch.device("cpu")
+    w.ref = _desc(experts, rows, cols)
+    return w
+
+
 def test_refusals_of_the_wrappers():
     codes, scales, _ = _cpu()
     with pytest.raises(ValueError, match="codes"):
@@ -294,7 +302,9 @@ def test_refusals_of_the_wrappers():
         ops.W4(codes, torch.zeros(16, 3))
     with pytest.raises(ValueError, match="zeros"):
         ops.W4(codes, scales, torch.zeros(16, 2, dtype=torch.int8))
-    w = ops.W4(codes, scales)
+    with pytest.raises(ValueError, match="GPU tensors"):
+        ops.W4(codes, scales)
+    w = _unpacked()
     x = torch.zeros(2, 64)
     with pytest.raises(ValueError, match="GPU tensors"):
         ops.w4_matvec_add2(w, x)
@@ -314,7 +324,7 @@ def test_refusals_of_the_wrappers():
         ops.w4_matvec_add2(w, x, x_scales=torch.zeros(2, 1))
     with pytest.raises(ValueError, match="residual_a"):
         ops.w4_matvec_add2(w, x, torch.zeros(2, 15))
-    mats = [ops.W4(*_cpu(32, 64, experts=4)) for _ in range(2)] + [ops.W4(*_cpu(64, 32, experts=4))]
+    mats = [_unpacked(32, 64, 4), _unpacked(32, 64, 4), _unpacked(64, 32, 4)]
     ids, wt = torch.zeros(4, dtype=torch.int32), torch.zeros(4)
     with pytest.raises(ValueError, match="ids"):
         ops.w4_moe(*mats, x, ids.long(), wt, 2)
@@ -327,28 +337,62 @@ def test_refusals_of_the_wrappers():
 
 
 def _desc(experts=1, rows=16, cols=64, group=32, p=16, **more):
-    d = W4Desc(experts, rows, cols, group, 0, p, p, None, experts * rows * cols // 2,
-               experts * rows * (cols // group if group else 0) * 4, 0)
+    d = W4Desc(experts, rows, cols, group, 0, 0, p, 0)
+    d.packed_bytes = lib().inferno_w4_packed_bytes(d)
     for name, v in more.items():
         setattr(d, name, v)
     return d
+
+
+BAD_SIZES = [dict(rows=0), dict(cols=0), dict(experts=0), dict(group=0), dict(group=48),
+             dict(group=128), dict(group=96, cols=96), dict(cols=48, group=16),
+             dict(scale_dtype=2), dict(experts=257), dict(rows=1 << 20, cols=1 << 13, group=128),
+             dict(rows=1 << 31), dict(cols=1 << 31)]
+
+
+def test_packed_bytes():
+    L = lib()
+
+    def size(zeros=0, dtype=0, **kw):
+        d = _desc(**kw)
+        d.has_zeros, d.scale_dtype = zeros, dtype
+        return L.inferno_w4_packed_bytes(d)
+
+    # 16 rows by 128 columns: 1024 bytes of codes, 16 scales or 16 times 4
+    assert size(rows=16, cols=128, group=128, dtype=1) == 1024 + 256
+    assert size(rows=17, cols=160, group=32, dtype=1) == 4 * 1024 + 4 * 128
+    assert size(rows=64, cols=1024, group=64, dtype=0, zeros=1) == 32 * (1024 + 256 + 64)
+    assert size(experts=3, rows=16, cols=256, group=256, dtype=0, zeros=1) == 6 * 1024 + 512 + 256
+    for kw in BAD_SIZES:
+        assert L.inferno_w4_packed_bytes(_desc(**kw)) == 0, kw
 
 
 def test_refusals_of_the_library():
     # every one before any device work
     L = lib()
 
+    def pack(d, codes=16, nc=512, scales=16, ns=128, zeros=None, nz=0, to=16):
+        return L.inferno_w4_pack(None, d, codes, nc, scales, ns, zeros, nz, to)
+
+    d = _desc()
+    for bad in (dict(codes=None), dict(codes=18), dict(scales=None), dict(scales=18), dict(to=None),
+                dict(to=24)):
+        assert pack(d, **bad) == -1, bad
+    for bad in (dict(nc=511), dict(ns=64)):
+        assert pack(d, **bad) == -2, bad
+    z = _desc(has_zeros=1)
+    z.packed_bytes = L.inferno_w4_packed_bytes(z)
+    assert pack(z, nz=32) == -1 and pack(z, zeros=16, nz=31) == -2
+    assert pack(_desc(packed_bytes=10)) == -2
+    for kw in BAD_SIZES:
+        assert pack(_desc(**kw)) == -1, kw
+
     def matvec(d, x=16, dt=0, xs=None, xg=0, T=1, out=16, ws=16, n=1 << 30):
         return L.inferno_w4_matvec_add2(None, d, x, dt, xs, xg, None, None, T, out, ws, n)
 
-    for d in (_desc(rows=0), _desc(cols=0), _desc(experts=0), _desc(group=0), _desc(group=48),
-              _desc(group=128), _desc(group=96, cols=96), _desc(cols=48, group=16),
-              _desc(scale_dtype=2), _desc(codes=None), _desc(codes=24), _desc(scales=18),
-              _desc(experts=2), _desc(experts=257)):
-        assert matvec(d) == -1, L.inferno_last_error()
-    for d in (_desc(codes_bytes=1), _desc(scales_bytes=64), _desc(zeros=16, zeros_bytes=3)):
-        assert matvec(d) == -2
-    d = _desc()
+    for kw in BAD_SIZES + [dict(packed=None), dict(packed=24), dict(experts=2)]:
+        assert matvec(_desc(**kw)) == -1, kw
+    assert matvec(_desc(packed_bytes=1024)) == -2 and matvec(_desc(has_zeros=1)) == -2
     assert matvec(d, x=None) == -1 and matvec(d, x=20) == -1 and matvec(d, dt=3) == -1
     assert matvec(d, out=None) == -1 and matvec(d, ws=None) == -2 and matvec(d, n=100) == -2
     assert matvec(d, ws=24) == -1 and matvec(d, T=1 << 31) == -1
@@ -361,11 +405,11 @@ def test_refusals_of_the_library():
     def pair(a, b):
         return L.inferno_w4_gate_up_swiglu(None, a, b, 16, 0, None, 0, 1, 16, 16, 1 << 30)
 
-    other = _desc(zeros=16, zeros_bytes=32)
-    for b in (_desc(rows=32), _desc(cols=128), _desc(group=64), other):
+    half = _desc()
+    half.scale_dtype = 1
+    half.packed_bytes = L.inferno_w4_packed_bytes(half)
+    for b in (_desc(rows=32), _desc(cols=128), _desc(group=64), z, half):
         assert pair(d, b) == -1 and b"same" in L.inferno_last_error()
-    half = _desc(scale_dtype=1, scales_bytes=64)
-    assert pair(d, half) == -1
 
     def moe(g, u, dn, ids=16, k=2, T=1, n=1 << 30):
         return L.inferno_w4_moe(None, g, u, dn, 16, 0, None, 0, ids, 16, T, k, 16, 16, n)
@@ -395,7 +439,9 @@ def test_library_errors_reach_the_caller(cuda):
     with pytest.raises(InfernoError, match="same group"):
         ops.w4_gate_up_swiglu(a, b, torch.zeros(1, 64, device=cuda))
     with pytest.raises(InfernoError, match="group"):
-        ops.w4_matvec_add2(ops.W4(*ref.make(g, 16, 96, 96)), torch.zeros(1, 96, device=cuda))
+        ops.W4(*ref.make(g, 16, 96, 96))
+    with pytest.raises(InfernoError, match="plain product"):
+        ops.w4_matvec_add2(ops.W4(*ref.make(g, 16, 64, 32, 2)), torch.zeros(1, 64, device=cuda))
     buf = torch.zeros(65, device=cuda)
     with pytest.raises(InfernoError, match="multiple of 16"):
         ops.w4_matvec_add2(a, buf[1:].view(1, 64))
