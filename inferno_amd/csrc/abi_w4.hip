@@ -88,7 +88,7 @@ W4Acts carve_acts(Carver& c, size_t rows, size_t cols) {
   const size_t n = rows * w4_chunks(cols);
   W4Acts a{};
   a.planes = c.take<int8_t>(n * 3 * kW4Chunk);
-  a.xs = c.take<float>(n);
+  a.xs = c.take<float>(rows * w4_xs_stride(cols));
   return a;
 }
 

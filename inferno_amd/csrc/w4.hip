@@ -34,7 +34,7 @@ struct Stage {
   const void* x;
   const float* x_scales;
   size_t x_group;  // > 0
-  size_t R, K, C;
+  size_t R, K, C, xs_stride;
   W4Acts a;
 };
 
@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(256) w4_stage_kernel(Stage p) {
             make_uint4(w[o][0], w[o][1], w[o][2], w[o][3]);
     }
   }
-  if (b == 0) p.a.xs[rc] = xs;
+  if (b == 0) p.a.xs[r * p.xs_stride + c] = xs;
+  if (b == 1 && c + 1 == p.C && p.C < p.xs_stride) p.a.xs[r * p.xs_stride + p.C] = 0.f;
 }
 
 // -------------------------------------------------------------------- pack
@@ -205,6 +206,7 @@ struct Product {
   uint32_t N, C, row_tiles;  // rows, chunks and row tiles of one expert's matrix
   const int8_t* planes;
   const float* xs;
+  uint32_t xs_stride;
   uint32_t T;
   const uint32_t* offsets;
   const uint32_t* sorted;
@@ -325,22 +327,28 @@ __device__ __forceinline__ float join(int hi, int mid, int lo) {
 // digit.
 enum Kind { kPack3, kOne, kWide3 };
 
-// Few tokens. One workgroup: 16 rows of the matrices (the same rows of both),
-// all tokens of one expert (or of the batch) in tiles; the four wavefronts
-// share the chunks and add their sums in order.
-template <bool FINE, int MATS, int P, bool ZEROS, typename ST>
-__global__ void __launch_bounds__(256) w4_rows_kernel(Product p) {
-  constexpr int B = FINE ? 4 : 1;
-  __shared__ float part[4][MATS * 4][kWave];
+// Few tokens. A wavefront takes RT tiles of 16 rows of the matrices (the same
+// rows of both) and all tokens of one expert (or of the batch) in tiles. `split`
+// wavefronts share the chunks of these rows and add their sums in order; a
+// workgroup's four cover 4 RT / split tiles.
+template <bool FINE, int MATS, int P, bool ZEROS, typename ST, int RT>
+__global__ void __launch_bounds__(256) w4_rows_kernel(Product p, int split) {
+  constexpr int B = FINE ? 4 : 1, F = MATS * RT;
+  __shared__ float part[4][F * 4][kWave];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;
   Slot slot;
   if (!slot_of(p, slot)) return;
   const uint32_t end = slot.end;
-  const uint32_t row = blockIdx.x * 16 + n;
-  const size_t tile = (size_t(slot.expert) * p.row_tiles + blockIdx.x) * p.C;
-  const uint32_t c0 = p.C * wave / 4, c1 = p.C * (wave + 1) / 4;
+  const uint32_t tile0 = (blockIdx.x * (4 / split) + wave / split) * RT;
+  size_t tile[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+    tile[i] = (size_t(slot.expert) * p.row_tiles + min(tile0 + i, p.row_tiles - 1)) * p.C;
+  // chunks in pairs
+  const uint32_t pairs = (p.C + 1) / 2, share = wave % split;
+  const uint32_t c0 = pairs * share / split * 2, c1 = pairs * (share + 1) / split * 2;
   uint32_t t0 = slot.first;
   auto run = [&](auto kind) __attribute__((always_inline)) {
     constexpr int KIND = decltype(kind)::value;
@@ -353,20 +361,20 @@ __global__ void __launch_bounds__(256) w4_rows_kernel(Product p) {
     const float* sp[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      sp[i] = p.xs + x_row(p, slot, t0 + (KIND == kPack3 ? quad : 4 * quad + i)) * p.C;
-    float acc[MATS][NV];
+      sp[i] = p.xs + x_row(p, slot, t0 + (KIND == kPack3 ? quad : 4 * quad + i)) * p.xs_stride;
+    float acc[F][NV];
 #pragma unroll
-    for (int m = 0; m < MATS; ++m)
+    for (int f = 0; f < F; ++f)
 #pragma unroll
-      for (int i = 0; i < NV; ++i) acc[m][i] = 0.f;
+      for (int i = 0; i < NV; ++i) acc[f][i] = 0.f;
     // loads on their way, of two chunks
-    Codes<FINE, ZEROS, ST> w[2][MATS];
+    Codes<FINE, ZEROS, ST> w[2][F];
     v4u x[2][NT][2];
-    float xs[2][NV];
+    float2 xs[NV], next_xs[NV];
     auto load = [&](uint32_t chunk, int to) {
       const uint32_t c = min(chunk, p.C - 1);
 #pragma unroll
-      for (int m = 0; m < MATS; ++m) w[to][m].load(p.m[m], tile + c, lane);
+      for (int f = 0; f < F; ++f) w[to][f].load(p.m[f / RT], tile[f % RT] + c, lane);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const v4u* at =
@@ -374,14 +382,17 @@ __global__ void __launch_bounds__(256) w4_rows_kernel(Product p) {
         x[to][t][0] = at[0];
         x[to][t][1] = at[4];
       }
+    };
+    auto load_xs = [&](uint32_t pair_at) {
+      const uint32_t c = min(pair_at, 2 * pairs - 2);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) xs[to][i] = sp[i][c];
+      for (int i = 0; i < NV; ++i) next_xs[i] = *reinterpret_cast<const float2*>(sp[i] + c);
     };
     auto step = [&](uint32_t c, int cur) {
 #pragma unroll
-      for (int m = 0; m < MATS; ++m) {
+      for (int f = 0; f < F; ++f) {
         v4i even, odd;
-        w[cur][m].widen(even, odd);
+        w[cur][f].widen(even, odd);
         float value[NV];
 #pragma unroll
         for (int b = 0; b < B; ++b) {
@@ -389,49 +400,70 @@ __global__ void __launch_bounds__(256) w4_rows_kernel(Product p) {
 #pragma unroll
           for (int t = 0; t < NT; ++t)
             sum[t] = dot<FINE>(x[cur][t][0], x[cur][t][1], even, odd, b);
-          const float ws = w[cur][m].scale(b, c < c1);
+          const float ws = w[cur][f].scale(b, c < p.C);
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
-            float f;
-            if (KIND == kPack3) f = join(sum[0][0], sum[0][1], sum[0][2]);
-            else if (KIND == kOne) f = float(sum[0][i]);
-            else f = join(sum[0][i], sum[NT / 2][i], sum[NT - 1][i]);
-            value[i] = b == 0 ? ws * f : fmaf(ws, f, value[i]);
+            float v;
+            if (KIND == kPack3) v = join(sum[0][0], sum[0][1], sum[0][2]);
+            else if (KIND == kOne) v = float(sum[0][i]);
+            else v = join(sum[0][i], sum[NT / 2][i], sum[NT - 1][i]);
+            value[i] = b == 0 ? ws * v : fmaf(ws, v, value[i]);
           }
         }
 #pragma unroll
-        for (int i = 0; i < NV; ++i) acc[m][i] = fmaf(value[i], xs[cur][i], acc[m][i]);
+        for (int i = 0; i < NV; ++i)
+          acc[f][i] = fmaf(value[i], cur ? xs[i].y : xs[i].x, acc[f][i]);
       }
       load(c + 2, cur);
     };
     if (c0 < c1) {
+      load_xs(c0);
       load(c0, 0);
       load(c0 + 1, 1);
       // two at a time without a way past the second (a chunk behind the end has
       // scales of 0): the wait counts of a loop hold for its shortest path
       for (uint32_t c = c0; c < c1; c += 2) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) xs[i] = next_xs[i];
+        load_xs(c + 2);
         step(c, 0);
         step(c + 1, 1);
       }
     }
+    const uint32_t j0 = t0 + (KIND == kPack3 ? quad : 4 * quad);
+    t0 += KIND == kPack3 ? 4 : 16;
+    if (split == 1) {
 #pragma unroll
-    for (int m = 0; m < MATS; ++m)
+      for (int r = 0; r < RT; ++r) {
+        const uint32_t row = (tile0 + r) * 16 + n;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) part[wave][m * NV + i][lane] = acc[m][i];
+        for (int i = 0; i < NV; ++i)
+          if (row < p.N && j0 + i < end)
+            store_result(p, j0 + i, row, acc[r][i],
+                         MATS == 2 ? &acc[(MATS - 1) * RT + r][i] : nullptr);
+      }
+      return;
+    }
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) part[wave][f * NV + i][lane] = acc[f][i];
     __syncthreads();
-    // wavefront i writes token value i of every lane
-    const uint32_t j = t0 + (KIND == kPack3 ? quad : 4 * quad + wave);
-    if (wave < NV && row < p.N && j < end) {
-      float v[MATS];
+    // the wavefronts of a tile write the token values in turn
+    for (int v = int(share); v < RT * NV; v += split) {
+      const int r = v / NV, i = v % NV;
+      const uint32_t row = (tile0 + r) * 16 + n;
+      if (row >= p.N || j0 + i >= end) continue;
+      float y[MATS];
 #pragma unroll
       for (int m = 0; m < MATS; ++m) {
-        v[m] = part[0][m * NV + wave][lane];
-        for (int i = 1; i < 4; ++i) v[m] += part[i][m * NV + wave][lane];
+        const int f = m * RT + r;
+        y[m] = part[wave - share][f * NV + i][lane];
+        for (int k = 1; k < split; ++k) y[m] += part[wave - share + k][f * NV + i][lane];
       }
-      store_result(p, j, row, v[0], MATS == 2 ? &v[MATS - 1] : nullptr);
+      store_result(p, j0 + i, row, y[0], MATS == 2 ? &y[MATS - 1] : nullptr);
     }
     __syncthreads();  // before the next tokens' sums
-    t0 += KIND == kPack3 ? 4 : 16;
   };
   while (t0 < end) {
     if constexpr (P == 1) {
@@ -482,9 +514,9 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
       constexpr int kPieces = 8 * P / kTileWaves;
       const int ct = wave * 4 / kTileWaves, cp = wave * kPieces % (2 * P);
       const bool brings = 16u * ct < tokens;
-      const size_t xr = x_row(p, slot, t0 + 16 * ct + n) * p.C;
-      const int8_t* xp = p.planes + xr * (P * kW4Chunk) + cp * 64 + quad * 16;
-      const float* sp = p.xs + xr;
+      const size_t xr = x_row(p, slot, t0 + 16 * ct + n);
+      const int8_t* xp = p.planes + xr * p.C * (P * kW4Chunk) + cp * 64 + quad * 16;
+      const float* sp = p.xs + xr * p.xs_stride;
       float acc[F][NT][4];
 #pragma unroll
       for (int f = 0; f < F; ++f)
@@ -640,7 +672,7 @@ __global__ void __launch_bounds__(256)
 
 int launch_w4_stage(hipStream_t s, const void* x, int x_dtype, const float* x_scales,
                     size_t x_group, size_t R, size_t K, const W4Acts& a) {
-  const Stage p{x, x_scales, x_group ? x_group : K, R, K, w4_chunks(K), a};
+  const Stage p{x, x_scales, x_group ? x_group : K, R, K, w4_chunks(K), w4_xs_stride(K), a};
   const unsigned grid = unsigned((R * p.C * 4 + 255) / 256);
   if (x_dtype == INFERNO_F32) w4_stage_kernel<float, 3><<<grid, 256, 0, s>>>(p);
   else if (x_dtype == INFERNO_BF16) w4_stage_kernel<uint16_t, 3><<<grid, 256, 0, s>>>(p);
@@ -697,6 +729,7 @@ int launch_w4_product(hipStream_t s, const W4Product& q) {
   p.row_tiles = (p.N + 15) / 16;
   p.planes = q.x.planes;
   p.xs = q.x.xs;
+  p.xs_stride = uint32_t(w4_xs_stride(q.m[0].cols));
   p.T = uint32_t(q.T);
   p.offsets = q.offsets;
   p.sorted = q.sorted;
@@ -729,12 +762,31 @@ int launch_w4_product(hipStream_t s, const W4Product& q) {
             <<<grid, kTileWaves * kWave, 0, s>>>(p);
     });
   } else {
+    // Measured over 81 to 32768 row tiles (whole passes, rt / split): enough
+    // tiles take two or four together, which share the loads of the digits (16
+    // assignments of 128 experts, down: 1/1 209, 2/2 193, 4/2 190 us; 64 tokens:
+    // 1/1 360, 2/2 325, 4/2 298; 81 tiles of one matrix: 1/4 12.6, 2/4 15.5);
+    // int8 tokens have fewer digits to share (gate and up 1/1 345, 2/2 380). A
+    // tile's chunks are split so that neighbouring wavefronts read neighbouring
+    // memory, but short matrices less (one token, down: 2/2 42.5, 2/4 43.8).
+    const size_t tiles = size_t(p.row_tiles) * slots;
+    const int rt = tiles < 384 || (one && q.mats == 2) ? 1 : q.mats == 1 && tiles >= 16384 ? 4 : 2;
+    const int split = q.mats == 1 ? (tiles >= 2048 ? 2 : 4) : one && tiles >= 8192 ? 1 : 4;
     by_format(q, [&](auto fine, auto mats, auto zeros, auto st) {
       constexpr int M = decltype(mats)::value;
-      const dim3 grid(p.row_tiles, slots);
+      const unsigned units = (p.row_tiles + rt - 1) / rt;
+      const dim3 grid((units * split + 3) / 4, slots);
       using ST = decltype(st);
-      if (one) w4_rows_kernel<fine.value, M, 1, zeros.value, ST><<<grid, 256, 0, s>>>(p);
-      else w4_rows_kernel<fine.value, M, 3, zeros.value, ST><<<grid, 256, 0, s>>>(p);
+      auto go = [&](auto tiles) {
+        constexpr int RT = decltype(tiles)::value;
+        if (one)
+          w4_rows_kernel<fine.value, M, 1, zeros.value, ST, RT><<<grid, 256, 0, s>>>(p, split);
+        else
+          w4_rows_kernel<fine.value, M, 3, zeros.value, ST, RT><<<grid, 256, 0, s>>>(p, split);
+      };
+      if (rt == 4 && M == 1) go(std::integral_constant<int, M == 1 ? 4 : 1>{});
+      else if (rt == 2) go(std::integral_constant<int, 2>{});
+      else go(std::integral_constant<int, 1>{});
     });
   }
   INF_LAUNCHED();

@@ -34,7 +34,8 @@ int launch_w4_pack(hipStream_t s, const W4Mat& m, const void* codes, const void*
 // [-128, 127]), or d0 xs (1 plane, int8 activations).
 //   planes [rows][chunks][planes][128]: the digits of one chunk in the order
 //     in which the lanes of the weights' tile hold its columns;
-//   xs [rows][chunks].
+//   xs [rows][chunks, to a multiple of 2 with 0].
+inline size_t w4_xs_stride(size_t K) { return (w4_chunks(K) + 1) / 2 * 2; }
 struct W4Acts {
   int8_t* planes;
   float* xs;

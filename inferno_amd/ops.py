@@ -11,6 +11,10 @@ from ._lib import BF16, F32, I8, Q8_0, LayerDesc, W4Desc, check, lib
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
 
+# a device's current stream as an integer, without a Stream object (3 us each)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
 
 def _p(t):
     return None if t is None else C.c_void_p(t.data_ptr())
@@ -186,14 +190,18 @@ def _rows_of(x, name, dtypes):
                          f"{'' if x.is_contiguous() else ', not contiguous'}")
 
 
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 def _run(x, fn, *args):
     """fn(stream, *args) on x's device and that device's current stream."""
-    _dev(x)
-    if x.get_device() == torch.cuda.current_device():
-        check(fn(_s(), *args))
+    dev = _dev(x).get_device()
+    if dev == torch.cuda.current_device():
+        check(fn(_raw_stream(dev), *args))
     else:
-        with torch.cuda.device(x.device):
-            check(fn(_s(), *args))
+        with torch.cuda.device(dev):
+            check(fn(_raw_stream(dev), *args))
 
 
 def add_rms_norm_q8(x, residual, w, eps, group=0, act_dtype=torch.float32, out=None):
@@ -217,8 +225,8 @@ def add_rms_norm_q8(x, residual, w, eps, group=0, act_dtype=torch.float32, out=N
     normed = torch.empty(T, H, dtype=act_dtype, device=x.device)
     q = torch.empty(T, H, dtype=torch.int8, device=x.device)
     scales = torch.empty(T, H // group if group else 1, dtype=torch.float32, device=x.device)
-    _run(x, lib().inferno_add_rms_norm_q8, _p(x), _DT[x.dtype], _p(residual), _p(w), float(eps), T,
-         H, group, _DT[act_dtype], _p(out), _p(normed), _p(q), _p(scales))
+    _run(x, lib().inferno_add_rms_norm_q8, _at(x), _DT[x.dtype], _at(residual), _at(w), float(eps), T,
+         H, group, _DT[act_dtype], _at(out), _at(normed), _at(q), _at(scales))
     return out, normed, q, scales
 
 
@@ -234,8 +242,8 @@ def router_group_topk(logits, bias, k, score_fn, norm, scale, n_group, topk_grou
     ids = torch.empty(T * k, dtype=torch.int32, device=logits.device)
     w = torch.empty(T * k, dtype=torch.float32, device=logits.device)
     tok = torch.empty(T * k, dtype=torch.int32, device=logits.device)
-    _run(logits, lib().inferno_moe_router_group_topk, _p(logits), _p(bias), T, E, k, score_fn,
-         int(norm), float(scale), n_group, topk_group, group_score, _p(ids), _p(w), _p(tok))
+    _run(logits, lib().inferno_moe_router_group_topk, _at(logits), _at(bias), T, E, k, score_fn,
+         int(norm), float(scale), n_group, topk_group, group_score, _at(ids), _at(w), _at(tok))
     return ids, w, tok
 
 
@@ -268,9 +276,9 @@ class W4:
         self.desc, self.ref = d, C.byref(d)
         d.packed_bytes = lib().inferno_w4_packed_bytes(self.ref)
         self.packed = torch.empty(d.packed_bytes, dtype=torch.uint8, device=codes.device)
-        _run(codes, lib().inferno_w4_pack, self.ref, _p(codes), codes.numel(), _p(scales),
-             scales.numel() * scales.element_size(), _p(zeros),
-             zeros.numel() if zeros is not None else 0, _p(self.packed))
+        _run(codes, lib().inferno_w4_pack, self.ref, _at(codes), codes.numel(), _at(scales),
+             scales.numel() * scales.element_size(), _at(zeros),
+             zeros.numel() if zeros is not None else 0, _at(self.packed))
         d.packed = self.packed.data_ptr()
 
 
@@ -292,7 +300,7 @@ def _w4_x(w, x, x_scales):
         raise ValueError("int8 activations need x_scales [tokens, groups], groups dividing "
                          f"{w.cols}")
     _like(x, "x_scales", x_scales, torch.float32, x.shape[0], x_scales.shape[1])
-    return I8, _p(x_scales), w.cols // x_scales.shape[1]
+    return I8, _at(x_scales), w.cols // x_scales.shape[1]
 
 
 def _w4_ws(x, n):
@@ -310,8 +318,8 @@ def w4_matvec_add2(w, x, residual_a=None, residual_b=None, x_scales=None):
     out = torch.empty(T, w.rows, dtype=torch.float32, device=x.device)
     n = lib().inferno_w4_workspace_bytes(T, w.cols)
     ws = _w4_ws(x, n)
-    _run(x, lib().inferno_w4_matvec_add2, w.ref, _p(x), dt, xs, xg, _p(residual_a),
-         _p(residual_b), T, _p(out), _p(ws), n)
+    _run(x, lib().inferno_w4_matvec_add2, w.ref, _at(x), dt, xs, xg, _at(residual_a),
+         _at(residual_b), T, _at(out), _at(ws), n)
     return out
 
 
@@ -324,8 +332,8 @@ def w4_gate_up_swiglu(gate, up, x, x_scales=None):
     out = torch.empty(T, gate.rows, dtype=torch.float32, device=x.device)
     n = lib().inferno_w4_workspace_bytes(T, gate.cols)
     ws = _w4_ws(x, n)
-    _run(x, lib().inferno_w4_gate_up_swiglu, gate.ref, up.ref, _p(x), dt, xs, xg, T, _p(out),
-         _p(ws), n)
+    _run(x, lib().inferno_w4_gate_up_swiglu, gate.ref, up.ref, _at(x), dt, xs, xg, T, _at(out),
+         _at(ws), n)
     return out
 
 
@@ -343,8 +351,8 @@ def w4_moe(gate, up, down, x, ids, weights, k, x_scales=None):
     out = torch.empty(T, H, dtype=torch.float32, device=x.device)
     n = lib().inferno_w4_moe_workspace_bytes(T, k, gate.experts, H, gate.rows)
     ws = _w4_ws(x, n)
-    _run(x, lib().inferno_w4_moe, gate.ref, up.ref, down.ref, _p(x), dt, xs, xg, _p(ids),
-         _p(weights), T, k, _p(out), _p(ws), n)
+    _run(x, lib().inferno_w4_moe, gate.ref, up.ref, down.ref, _at(x), dt, xs, xg, _at(ids),
+         _at(weights), T, k, _at(out), _at(ws), n)
     return out
 
 
