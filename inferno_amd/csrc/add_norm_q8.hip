@@ -7,6 +7,8 @@
 // values each, exact in 64 bits: q does not depend on how the squares are
 // summed, and is the same in every kernel. The squares are summed in 64 bits:
 // those of fp32 values pass fp32's range from 2^64 on.
+#include <type_traits>
+
 #include "kernels.hpp"
 
 namespace inferno {
@@ -29,6 +31,15 @@ __device__ __forceinline__ uint64_t magnitude(float s, float w) {
 __device__ __forceinline__ int8_t quantised(float s, float w, double largest) {
   if (!(largest > 0.0) || isinf(largest)) return 0;
   return int8_t(rint(127.0 * (double(s) * double(w)) / largest));
+}
+
+// A product of fp32 values as fp32 bits: at most 2^100 and at least 2^-100.
+__device__ __forceinline__ bool sound(uint32_t a) { return a - (27u << 23) <= (200u << 23); }
+
+// A group's scale, from the exact largest product or from its fp32 rounding.
+__device__ __forceinline__ float group_scale(double largest, double inv) {
+  const float f = float(largest);
+  return float((sound(f32_to_bits(f)) ? double(f) : largest) * inv / 127.0);
 }
 
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
@@ -68,9 +79,10 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   sq = 0.0;
   for (int i = 0; i < kThreads / kWave; ++i) sq += part[i];
-  const float root = float(sqrt(sq / double(H) + double(eps)));
+  const double inv = 1.0 / sqrt(sq / double(H) + double(eps));
+  const float f = float(inv);
   if (normed)
-    for (size_t i = tid; i < H; i += kThreads) store_act(normed + at + i, total(i) / root * w[i]);
+    for (size_t i = tid; i < H; i += kThreads) store_act(normed + at + i, total(i) * f * w[i]);
   if (!q) return;
   if (group == 0) {
     uint64_t a = 0;
@@ -81,7 +93,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int i = 0; i < kThreads / kWave; ++i) a = max(a, part64[i]);
     const double largest = __builtin_bit_cast(double, a);
     for (size_t i = tid; i < H; i += kThreads) q[at + i] = quantised(total(i), w[i], largest);
-    if (tid == 0) scales[row] = float(largest / double(root) / 127.0);
+    if (tid == 0) scales[row] = group_scale(largest, inv);
     return;
   }
   const size_t groups = H / group;
@@ -92,15 +104,238 @@ __global__ void __launch_bounds__(kThreads)
     const double largest = __builtin_bit_cast(double, wave_max64(a));
     for (size_t i = g * group + lane; i < (g + 1) * group; i += kWave)
       q[at + i] = quantised(total(i), w[i], largest);
-    if (lane == 0) scales[row * groups + g] = float(largest / double(root) / 127.0);
+    if (lane == 0) scales[row * groups + g] = group_scale(largest, inv);
+  }
+}
+
+// Largest of a value over 2^STEPS neighbouring lanes, in each of them.
+template <int STEPS>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if (STEPS >= 1) v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0xB1, 0xF, 0xF, false)));
+  if (STEPS >= 2) v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x4E, 0xF, 0xF, false)));
+  if (STEPS >= 3) v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x141, 0xF, 0xF, false)));
+  if (STEPS >= 4) v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x140, 0xF, 0xF, false)));
+  if (STEPS >= 5) {
+    const auto o = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(o[0], o[1]);
+  }
+  if (STEPS >= 6) {
+    const auto o = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(o[0], o[1]);
+  }
+  return v;
+}
+template <int STEPS>
+__device__ __forceinline__ uint64_t lanes_max64(uint64_t v) {
+#pragma unroll
+  for (int m = 1; m < (1 << STEPS); m <<= 1) {
+    const uint64_t o = __shfl_xor(v, m, kWave);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
+  const float4 f = *reinterpret_cast<const float4*>(p);
+  v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+}
+__device__ __forceinline__ void load4(const uint16_t* p, float (&v)[4]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  v[0] = bits_to_f32(u.x << 16); v[1] = bits_to_f32(u.x & 0xffff0000u);
+  v[2] = bits_to_f32(u.y << 16); v[3] = bits_to_f32(u.y & 0xffff0000u);
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(uint16_t* p, const float (&v)[4]) {
+  *reinterpret_cast<uint2*>(p) =
+      make_uint2(uint32_t(f32_to_bf16_bits(v[0])) | uint32_t(f32_to_bf16_bits(v[1])) << 16,
+                 uint32_t(f32_to_bf16_bits(v[2])) | uint32_t(f32_to_bf16_bits(v[3])) << 16);
+}
+
+// Widths of a multiple of 4 up to 1024 NV, rows on 16 bytes: one workgroup per
+// row, the row in registers (four neighbouring values per thread, NV times), so
+// that memory is read once. Quotients are formed in 32 bits, with an error below
+// 127 * 4 * 2^-24; one that lies nearer than 2^-14 to the border between two
+// values is formed again in 64 bits, as are those of groups whose largest value
+// is far from 1 (a product could leave fp32's range). STEPS: log2 of a group's
+// lanes, 0: the row is one group.
+template <typename XT, typename OT, int NV, int STEPS>
+__global__ void __launch_bounds__(kThreads)
+    add_norm_q8_kernel(const XT* __restrict__ x, const float* residual,
+                       const float* __restrict__ w, float eps, uint32_t H, float* sum,
+                       OT* __restrict__ normed, int8_t* __restrict__ q,
+                       float* __restrict__ scales) {
+  constexpr int kWaves = kThreads / kWave;
+  __shared__ double part[kWaves];
+  __shared__ uint32_t top[kWaves];
+  __shared__ uint64_t top64[kWaves];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const size_t at = size_t(blockIdx.x) * H;
+  float v[NV][4], g[NV][4];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const uint32_t i = min(uint32_t(j * kThreads + tid) * 4, H - 4);  // clamped: loads together
+    float r[4] = {0.f, 0.f, 0.f, 0.f};
+    load4(x + at + i, v[j]);
+    if (residual) load4(residual + at + i, r);
+    load4(w + i, g[j]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[j][e] += r[e];
+  }
+  double sq = 0.0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const uint32_t i = uint32_t(j * kThreads + tid) * 4;
+    if (i < H) {
+      if (sum) store4(sum + at + i, v[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sq = fma(double(v[j][e]), double(v[j][e]), sq);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = g[j][e] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) sq += __shfl_xor(sq, m, kWave);
+  if (lane == 0) part[wave] = sq;
+  uint32_t most = 0;
+  if (STEPS == 0 && q) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        most = max(most, f32_to_bits(v[j][e] * g[j][e]) & 0x7fffffffu);
+    most = lanes_max<6>(most);
+    if (lane == 0) top[wave] = most;
+  }
+  __syncthreads();
+  sq = part[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) sq += part[i];
+  const double inv = 1.0 / sqrt(sq / double(H) + double(eps));
+  if (normed) {
+    const float f = float(inv);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint32_t i = uint32_t(j * kThreads + tid) * 4;
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = v[j][e] * f * g[j][e];
+      if (i < H) store4(normed + at + i, y);
+    }
+  }
+  if (!q) return;
+  if (STEPS == 0) {
+    most = top[0];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) most = max(most, top[i]);
+  }
+  // four quotients in 32 bits; true where one has to be formed again
+  auto quotients = [&](int j, uint32_t a, uint32_t& packed) {
+    const float by = 127.f / bits_to_f32(a);
+    bool again = !sound(a);
+    packed = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float t = v[j][e] * g[j][e] * by, r = rintf(t);
+      again |= fabsf(fabsf(t - r) - 0.5f) < 6.1035e-5f;
+      packed |= (uint32_t(int(r)) & 255u) << (8 * e);
+    }
+    return again;
+  };
+  auto exactly = [&](int j, double a) {
+    uint32_t packed = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      packed |= (uint32_t(quantised(v[j][e], g[j][e], a)) & 255u) << (8 * e);
+    return packed;
+  };
+  auto magnitude4 = [&](int j) {
+    uint64_t a = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a = max(a, magnitude(v[j][e], g[j][e]));
+    return a;
+  };
+  if (STEPS == 0) {
+    uint32_t out[NV];
+    bool again = false;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) again |= quotients(j, most, out[j]);
+    double largest = double(bits_to_f32(most));
+    if (__syncthreads_or(again)) {
+      uint64_t a = 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) a = max(a, magnitude4(j));
+      a = lanes_max64<6>(a);
+      if (lane == 0) top64[wave] = a;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) a = max(a, top64[i]);
+      largest = __builtin_bit_cast(double, a);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) out[j] = exactly(j, largest);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint32_t i = uint32_t(j * kThreads + tid) * 4;
+      if (i < H) *reinterpret_cast<uint32_t*>(q + at + i) = out[j];
+    }
+    if (tid == 0) scales[blockIdx.x] = group_scale(largest, inv);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const uint32_t i = uint32_t(j * kThreads + tid) * 4;
+    uint32_t a = 0, out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a = max(a, f32_to_bits(v[j][e] * g[j][e]) & 0x7fffffffu);
+    a = lanes_max<STEPS>(a);
+    double largest = double(bits_to_f32(a));
+    if (__any(quotients(j, a, out))) {
+      largest = __builtin_bit_cast(double, lanes_max64<STEPS>(magnitude4(j)));
+      out = exactly(j, largest);
+    }
+    if (i < H) {
+      *reinterpret_cast<uint32_t*>(q + at + i) = out;
+      if (tid % (1u << STEPS) == 0)
+        scales[(at + i) >> (STEPS + 2)] = group_scale(largest, inv);
+    }
   }
 }
 
 template <typename XT, typename OT>
-void run(hipStream_t s, const AddNormQ8& p) {
+void run_rows(hipStream_t s, const AddNormQ8& p) {
   add_norm_q8_row_kernel<XT, OT><<<unsigned(p.rows), kThreads, 0, s>>>(
       static_cast<const XT*>(p.x), p.residual, p.w, p.eps, p.H, p.group, p.sum,
       static_cast<OT*>(p.normed), p.q, p.scales);
+}
+
+template <typename XT, typename OT, int NV>
+void run_registers(hipStream_t s, const AddNormQ8& p) {
+  auto go = [&](auto steps) {
+    add_norm_q8_kernel<XT, OT, NV, decltype(steps)::value><<<unsigned(p.rows), kThreads, 0, s>>>(
+        static_cast<const XT*>(p.x), p.residual, p.w, p.eps, uint32_t(p.H), p.sum,
+        static_cast<OT*>(p.normed), p.q, p.scales);
+  };
+  if (p.group == 32) go(std::integral_constant<int, 3>{});
+  else if (p.group == 64) go(std::integral_constant<int, 4>{});
+  else if (p.group == 128) go(std::integral_constant<int, 5>{});
+  else go(std::integral_constant<int, 0>{});
+}
+
+template <typename XT, typename OT>
+void run(hipStream_t s, const AddNormQ8& p) {
+  auto on = [](const void* q, size_t to) { return reinterpret_cast<uintptr_t>(q) % to == 0; };
+  const size_t n = (p.H + 4 * kThreads - 1) / (4 * kThreads);
+  if (p.H % 4 || n > 8 || !on(p.x, 4 * sizeof(XT)) || !on(p.residual, 16) || !on(p.w, 16) ||
+      !on(p.sum, 16) || !on(p.normed, 4 * sizeof(OT)) || !on(p.q, 4))
+    run_rows<XT, OT>(s, p);
+  else if (n <= 1) run_registers<XT, OT, 1>(s, p);
+  else if (n <= 2) run_registers<XT, OT, 2>(s, p);
+  else if (n <= 4) run_registers<XT, OT, 4>(s, p);
+  else if (n <= 6) run_registers<XT, OT, 6>(s, p);
+  else run_registers<XT, OT, 8>(s, p);
 }
 
 }  // namespace
