@@ -4,16 +4,50 @@
 // (as the router's top-k). A group's value is its largest v, or the sum of its
 // two largest; the topk_group best groups stay open (value descending, then
 // the lower group), and of their experts the k best win (v descending, then
-// the lower id). Values are formed in 64 bits: in 32 bits, values next to each
+// the lower id), by the values in 64 bits: in 32 bits, values next to each
 // other round to one or change places.
+//
+// Values are first formed in 32 bits. They decide wherever the values that they
+// order are further apart than their roundings, which is checked for the last
+// open group against the first closed one, for the last winner against the
+// best loser and for neighbouring winners; a token that fails (or holds a NaN)
+// is done again in 64 bits. 8192 tokens of 256 experts in 8 groups, all in 64
+// bits: 28 us.
 #include "kernels.hpp"
 #include "routing_dev.hpp"
 
 namespace inferno {
 namespace {
 
-constexpr int kPer = kMaxExperts / kWave;  // candidates per lane
-constexpr int kTokens = 4;                 // per workgroup, one wavefront each
+constexpr int kTokens = 4;  // per workgroup, one wavefront each
+
+struct GroupTopk {
+  const float* logits;
+  const float* bias;
+  size_t T;
+  int E, k, score_fn, norm;
+  float scale;
+  int groups, size, topk_group, rule;
+  int lanes;  // of one group: a power of two, groups * lanes <= 64 (0: more groups)
+  uint32_t* ids;
+  float* weights;
+  uint32_t* token_idx;
+};
+
+// One wavefront's scratch.
+union Scratch {
+  struct {
+    double value[kMaxExperts];
+    uint64_t group[kMaxExperts];
+  } exact;
+  struct {
+    float value[2 * kMaxExperts];  // a group's values one place apart from the next's
+    uint32_t key[kMaxTopK];
+    uint32_t id[kMaxTopK];
+    float score[kMaxTopK];
+    float by_rank[kMaxTopK];
+  } fast;
+};
 
 // Order-preserving map of a double onto u64; every NaN above +infinity.
 __device__ __forceinline__ uint64_t order_key(double v) {
@@ -23,64 +57,58 @@ __device__ __forceinline__ uint64_t order_key(double v) {
   return (b >> 63) ? ~b : (b | (1ull << 63));
 }
 
-__device__ __forceinline__ double wave_max_f64(double v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = fmax(v, __shfl_xor(v, m, kWave));
-  return v;
+// Weight of a winner: `sum` of the winners' scores, or of all.
+__device__ __forceinline__ float weight_of(const GroupTopk& p, float score, float sum) {
+  const bool divide =
+      (p.norm || p.score_fn == INFERNO_SCORE_SOFTMAX) && sum > 0.f && isfinite(sum);
+  return (divide ? score / sum : score) * p.scale;
 }
 
-__global__ void __launch_bounds__(kTokens* kWave)
-    group_topk_kernel(const float* __restrict__ logits, const float* __restrict__ bias, size_t T,
-                      int E, int k, int score_fn, int norm, float scale, int groups,
-                      int topk_group, int rule, uint32_t* __restrict__ ids,
-                      float* __restrict__ weights, uint32_t* __restrict__ token_idx) {
-  __shared__ double value_s[kTokens][kMaxExperts];
-  __shared__ uint64_t group_s[kTokens][kMaxExperts];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const size_t t = size_t(blockIdx.x) * kTokens + wave;
-  if (t >= T) return;  // no barrier of the workgroup below
-  double* value = value_s[wave];
-  uint64_t* gkey = group_s[wave];
-  const float* row = logits + t * size_t(E);
+__device__ __forceinline__ void exact_row(const GroupTopk& p, size_t t, Scratch& scratch) {
+  constexpr int kPer = kMaxExperts / kWave;
+  const int lane = threadIdx.x & 63;
+  double* value = scratch.exact.value;
+  uint64_t* gkey = scratch.exact.group;
+  const float* row = p.logits + t * size_t(p.E);
   float lg[kPer], score[kPer];
   float lmax = -INFINITY;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int e = lane + j * kWave;
-    lg[j] = e < E ? row[e] : -INFINITY;
+    lg[j] = e < p.E ? row[e] : -INFINITY;
     lmax = fmaxf(lmax, lg[j]);
   }
   lmax = wave_max(lmax);
+  float all = 0.f;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int e = lane + j * kWave;
     double v;
-    if (score_fn == INFERNO_SCORE_SIGMOID) {
+    if (p.score_fn == INFERNO_SCORE_SIGMOID) {
       v = 1.0 / (1.0 + exp(-double(lg[j])));
       score[j] = float(v);
     } else {
       v = lg[j];
-      score[j] = e < E && lmax != -INFINITY ? expf(lg[j] - lmax) : 0.f;
+      score[j] = e < p.E && lmax != -INFINITY ? expf(lg[j] - lmax) : 0.f;
     }
-    if (e < E) value[e] = v + (bias ? double(bias[e]) : 0.0);
+    if (e < p.E) {
+      value[e] = v + (p.bias ? double(p.bias[e]) : 0.0);
+      all += score[j];
+    }
   }
-  float all = 0.f;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) all += lane + j * kWave < E ? score[j] : 0.f;
   all = wave_sum(all);
   __builtin_amdgcn_wave_barrier();  // LDS is in order within a wavefront
-  const int size = E / groups;
-  for (int g = lane; g < groups; g += kWave) {
+  for (int g = lane; g < p.groups; g += kWave) {
     double a = -INFINITY, b = -INFINITY;
     bool nan = false;
-    for (int i = 0; i < size; ++i) {
-      const double v = value[g * size + i];
+    for (int i = 0; i < p.size; ++i) {
+      const double v = value[g * p.size + i];
       nan |= v != v;
       b = fmax(b, fmin(a, v));
       a = fmax(a, v);
     }
-    const double two = size > 1 ? a + b : a;
-    gkey[g] = nan ? ~0ull : order_key(rule == INFERNO_GROUP_TOP2 ? two : a);
+    const double two = p.size > 1 ? a + b : a;
+    gkey[g] = nan ? ~0ull : order_key(p.rule == INFERNO_GROUP_TOP2 ? two : a);
   }
   __builtin_amdgcn_wave_barrier();
   uint64_t key[kPer];
@@ -88,19 +116,19 @@ __global__ void __launch_bounds__(kTokens* kWave)
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int e = lane + j * kWave;
-    live[j] = e < E;
+    live[j] = e < p.E;
     key[j] = 0;
     if (!live[j]) continue;
-    const int g = e / size;
+    const int g = e / p.size;
     const uint64_t mine = gkey[g];
     int before = 0;
-    for (int o = 0; o < groups; ++o) before += gkey[o] > mine || (gkey[o] == mine && o < g);
-    live[j] = before < topk_group;
+    for (int o = 0; o < p.groups; ++o) before += gkey[o] > mine || (gkey[o] == mine && o < g);
+    live[j] = before < p.topk_group;
     key[j] = order_key(value[e]);
   }
   float sum = 0.f, mine_w = 0.f;
   uint32_t mine_id = 0;
-  for (int r = 0; r < k; ++r) {
+  for (int r = 0; r < p.k; ++r) {
     uint64_t best = 0;
     int id = INT32_MAX;
 #pragma unroll
@@ -133,13 +161,177 @@ __global__ void __launch_bounds__(kTokens* kWave)
       mine_id = uint32_t(id);
     }
   }
-  if (!norm) sum = all;
-  const bool divide = (norm || score_fn == INFERNO_SCORE_SOFTMAX) && sum > 0.f && isfinite(sum);
-  if (lane < k) {
-    const size_t a = t * size_t(k) + lane;
-    ids[a] = mine_id;
-    weights[a] = (divide ? mine_w / sum : mine_w) * scale;
-    if (token_idx) token_idx[a] = uint32_t(t);
+  if (lane < p.k) {
+    const size_t a = t * size_t(p.k) + lane;
+    p.ids[a] = mine_id;
+    p.weights[a] = weight_of(p, mine_w, p.norm ? sum : all);
+    if (p.token_idx) p.token_idx[a] = uint32_t(t);
+  }
+}
+
+// Whether a > b holds for the 64-bit values of two 32-bit ones. A sigmoid is
+// off by at most 2^-22, the addition of the bias by 2^-24 of the value; `times`
+// values were added. Infinities and NaN: no.
+__device__ __forceinline__ bool above(float a, float b, bool sigmoid, float times) {
+  const float off = (sigmoid ? 0x1p-20f : 0.f) + 0x1p-22f * fmaxf(fabsf(a), fabsf(b));
+  return a - b > times * off;
+}
+
+// The same in 32 bits; false if a value lies too near another one. PER: experts
+// per lane.
+template <int PER>
+__device__ __forceinline__ bool fast_row(const GroupTopk& p, size_t t, Scratch& scratch) {
+  auto& s = scratch.fast;
+  const int lane = threadIdx.x & 63;
+  const bool sigmoid = p.score_fn == INFERNO_SCORE_SIGMOID;
+  const float* row = p.logits + t * size_t(p.E);
+  float lg[PER], bs[PER], score[PER], v[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int e = min(lane + j * kWave, p.E - 1);
+    lg[j] = row[e];
+    bs[j] = p.bias ? p.bias[e] : 0.f;
+  }
+  float lmax = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    nan |= lg[j] + bs[j] != lg[j] + bs[j];  // +-infinity with the other as bias too
+    lmax = fmaxf(lmax, lg[j]);
+  }
+  if (__any(nan)) return false;
+  if (!sigmoid) {
+    lmax = bits_to_f32([](uint32_t k) { return (k >> 31) ? k ^ 0x80000000u : ~k; }(
+        wave_umax(total_order_key(lmax))));
+    if (lmax == -INFINITY) return false;
+  }
+  float all = 0.f;
+  const float magic = 1.f / float(p.size);
+  int group[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int e = lane + j * kWave;
+    score[j] = sigmoid ? 1.f / (1.f + expf(-lg[j])) : expf(lg[j] - lmax);
+    v[j] = (sigmoid ? score[j] : lg[j]) + bs[j];
+    // e / size for e < 256: the quotient's error is far below 1 / (2 size)
+    group[j] = int((float(e) + 0.5f) * magic);
+    if (e < p.E) {
+      all += score[j];
+      s.value[e + group[j]] = v[j];  // group g begins at g * (size + 1)
+    }
+  }
+  __builtin_amdgcn_wave_barrier();  // LDS is in order within a wavefront
+  uint64_t open = ~0ull;            // bit g * lanes: group g is
+  if (p.topk_group < p.groups) {
+    const int L = p.lanes, g = lane / L, sub = lane % L;
+    float a = -INFINITY, b = -INFINITY;  // the two largest of this lane's share
+    if (g < p.groups)
+      for (int i = sub; i < p.size; i += L) {
+        const float x = s.value[g * (p.size + 1) + i];
+        b = fmaxf(b, fminf(a, x));
+        a = fmaxf(a, x);
+      }
+    for (int m = 1; m < L; m <<= 1) {
+      const float oa = __shfl_xor(a, m, kWave), ob = __shfl_xor(b, m, kWave);
+      b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+      a = fmaxf(a, oa);
+    }
+    const bool two = p.rule == INFERNO_GROUP_TOP2 && p.size > 1;
+    const float gv = two ? a + b : a;
+    int before = 0;
+    float next = -INFINITY;  // the largest value at or below this group's, of another
+    for (int o = 0; o < p.groups; ++o) {
+      const float x = __shfl(gv, o * L, kWave);
+      before += x > gv || (x == gv && o < g);
+      if (x < gv || (x == gv && o > g)) next = fmaxf(next, x);
+    }
+    const bool mine = g < p.groups && sub == 0;
+    open = __ballot(mine && before < p.topk_group);
+    const bool last = mine && before == p.topk_group - 1;
+    if (__any(last && !above(gv, next, sigmoid, two ? 2.f : 1.f))) return false;
+  }
+  uint32_t key[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int e = lane + j * kWave;
+    const bool is = e < p.E &&
+                    (p.topk_group == p.groups || (open >> (min(group[j], 63 / p.lanes) * p.lanes) & 1));
+    key[j] = is ? max(total_order_key(v[j]), 1u) : 0u;
+  }
+  // the k-th largest key, bit by bit from the top; done as soon as exactly k
+  // keys are at or above the prefix
+  uint32_t kth = 0, n = 0;
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t c = kth | (1u << b);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) m += uint32_t(__popcll(__ballot(key[j] >= c)));
+    if (m >= uint32_t(p.k)) {
+      kth = c;
+      n = m;
+      if (m == uint32_t(p.k)) break;  // uniform
+    }
+  }
+  if (n != uint32_t(p.k)) return false;  // equal keys
+  uint32_t base = 0, loser = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const bool win = key[j] >= kth;
+    const uint64_t m = __ballot(win);
+    if (win) {
+      const uint32_t at = base + __builtin_amdgcn_mbcnt_hi(
+                                     uint32_t(m >> 32),
+                                     __builtin_amdgcn_mbcnt_lo(uint32_t(m), 0u));
+      s.key[at] = key[j];
+      s.id[at] = uint32_t(lane + j * kWave);
+      s.score[at] = score[j];
+    } else {
+      loser = max(loser, key[j]);
+    }
+    base += uint32_t(__popcll(m));
+  }
+  loser = wave_umax(loser);  // 0: none
+  __builtin_amdgcn_wave_barrier();
+  const uint32_t mine = s.key[min(lane, p.k - 1)];
+  const float my_score = s.score[min(lane, p.k - 1)];
+  uint32_t rank = 0, same = 0, below = loser;  // the best key below this winner's
+  for (int i = 0; i < p.k; ++i) {
+    const uint32_t o = s.key[i];
+    rank += o > mine ? 1u : 0u;
+    same += o == mine ? 1u : 0u;
+    if (o < mine) below = max(below, o);
+  }
+  auto value_of = [](uint32_t k) {
+    return bits_to_f32((k >> 31) ? k ^ 0x80000000u : ~k);
+  };
+  const bool clear =
+      same == 1 && (below == 0 || above(value_of(mine), value_of(below), sigmoid, 1.f));
+  if (__any(lane < p.k && !clear)) return false;
+  if (lane < p.k) s.by_rank[rank] = my_score;
+  __builtin_amdgcn_wave_barrier();
+  float sum = 0.f;
+  if (p.norm)
+    for (int r = 0; r < p.k; ++r) sum += s.by_rank[r];  // rank order
+  else
+    sum = wave_sum(all);
+  if (lane < p.k) {
+    const size_t a = t * size_t(p.k) + rank;
+    p.ids[a] = s.id[lane];
+    p.weights[a] = weight_of(p, my_score, sum);
+    if (p.token_idx) p.token_idx[a] = uint32_t(t);
+  }
+  return true;
+}
+
+template <int PER>
+__global__ void __launch_bounds__(kTokens* kWave) group_topk_kernel(GroupTopk p) {
+  __shared__ Scratch scratch[kTokens];
+  const int wave = threadIdx.x >> 6;
+  const size_t t = size_t(blockIdx.x) * kTokens + wave;
+  if (t >= p.T) return;  // no barrier of the workgroup below
+  if (p.lanes == 0 || !fast_row<PER>(p, t, scratch[wave])) {
+    __builtin_amdgcn_wave_barrier();
+    exact_row(p, t, scratch[wave]);
   }
 }
 
@@ -149,9 +341,14 @@ int launch_group_topk(hipStream_t s, const float* logits, const float* bias, siz
                       size_t k, int score_fn, int norm, float scale, size_t groups,
                       size_t topk_group, int rule, uint32_t* ids, float* weights,
                       uint32_t* token_idx) {
-  group_topk_kernel<<<unsigned((T + kTokens - 1) / kTokens), kTokens * kWave, 0, s>>>(
-      logits, bias, T, int(E), int(k), score_fn, norm, scale, int(groups), int(topk_group), rule,
-      ids, weights, token_idx);
+  int lanes = groups > 64 ? 0 : 1;
+  while (lanes && groups * lanes * 2 <= 64) lanes *= 2;
+  const GroupTopk p{logits, bias, T, int(E), int(k), score_fn, norm, scale, int(groups),
+                    int(E / groups), int(topk_group), rule, lanes, ids, weights, token_idx};
+  const unsigned grid = unsigned((T + kTokens - 1) / kTokens);
+  if (E <= 64) group_topk_kernel<1><<<grid, kTokens * kWave, 0, s>>>(p);
+  else if (E <= 128) group_topk_kernel<2><<<grid, kTokens * kWave, 0, s>>>(p);
+  else group_topk_kernel<4><<<grid, kTokens * kWave, 0, s>>>(p);
   INF_LAUNCHED();
   return INFERNO_OK;
 }
