@@ -109,6 +109,18 @@ W4Product product(const inferno_w4* w, const W4Acts& x, size_t T, float* out) {
   return p;
 }
 
+W4Token tokens(const inferno_w4* w, const void* x, int x_dtype, size_t T, float* out) {
+  W4Token q{};
+  q.m[0] = mat(w);
+  q.mats = 1;
+  q.x = x;
+  q.x_dtype = x_dtype;
+  q.T = T;
+  q.slots = q.segments = 1;
+  q.out = out;
+  return q;
+}
+
 struct W4MoeScratch {
   uint32_t* offsets;
   uint32_t* sorted;
@@ -191,6 +203,12 @@ int inferno_w4_matvec_add2(void* stream, const inferno_w4* w, const void* x, int
   if ((st = check_ws(workspace, workspace_bytes, inferno_w4_workspace_bytes(T, w->cols)))) return st;
   if (int st_ = require_device()) return st_;
   hipStream_t s = as_stream(stream);
+  if (x_dtype != INFERNO_I8) {
+    W4Token q = tokens(w, x, x_dtype, T, out);
+    q.res_a = residual_a;
+    q.res_b = residual_b;
+    if (w4_token_fits(q)) return launch_w4_token(s, q);
+  }
   Carver c{static_cast<char*>(workspace)};
   const W4Acts a = acts_for(carve_acts(c, T, w->cols), w, x_dtype);
   if ((st = launch_w4_stage(s, x, x_dtype, x_scales, x_group, T, w->cols, a))) return st;
@@ -215,6 +233,12 @@ int inferno_w4_gate_up_swiglu(void* stream, const inferno_w4* gate, const infern
     return st;
   if (int st_ = require_device()) return st_;
   hipStream_t s = as_stream(stream);
+  if (x_dtype != INFERNO_I8) {
+    W4Token q = tokens(gate, x, x_dtype, T, out);
+    q.m[1] = mat(up);
+    q.mats = 2;
+    if (w4_token_fits(q)) return launch_w4_token(s, q);
+  }
   Carver c{static_cast<char*>(workspace)};
   const W4Acts a = acts_for(carve_acts(c, T, gate->cols), gate, x_dtype);
   if ((st = launch_w4_stage(s, x, x_dtype, x_scales, x_group, T, gate->cols, a))) return st;
@@ -253,6 +277,22 @@ int inferno_w4_moe(void* stream, const inferno_w4* gate, const inferno_w4* up,
   hipStream_t s = as_stream(stream);
   Carver c{static_cast<char*>(workspace)};
   const W4MoeScratch m = carve_w4_moe(c, T, k, E, H, I);
+  if (T == 1 && x_dtype != INFERNO_I8) {
+    // gate and up of every rank, then the sum over the ranks (h rows of ids of
+    // no expert are not written, and count nothing)
+    W4Token g = tokens(gate, x, x_dtype, 1, m.h), d = tokens(down, m.h, INFERNO_F32, 1, out);
+    g.m[1] = mat(up);
+    g.mats = 2;
+    g.slots = k;
+    d.segments = k;
+    d.sum = true;
+    g.ids = d.ids = expert_ids;
+    g.route_w = expert_weights;
+    if (w4_token_fits(g) && w4_token_fits(d)) {
+      if ((st = launch_w4_token(s, g))) return st;
+      return launch_w4_token(s, d);
+    }
+  }
   if ((st = launch_dispatch(s, expert_ids, T, k, E, m.offsets, m.sorted, m.active))) return st;
   const W4Acts xa = acts_for(m.x, gate, x_dtype), ha = acts_for(m.h_acts, down, INFERNO_F32);
   if ((st = launch_w4_stage(s, x, x_dtype, x_scales, x_group, T, H, xa))) return st;

@@ -75,6 +75,21 @@ __device__ __forceinline__ uint32_t gather4(uint32_t a, uint32_t b, uint32_t c, 
   return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
+// The power of two (its exponent) that takes a chunk whose largest magnitude has
+// the bits `most` to three digits: the largest one that fits; chunks below 2^-96
+// share their step, 2^-118.
+__device__ __forceinline__ int digits_up(uint32_t most) {
+  const int up = 22 - max(int(most >> 23) - 127, -96);
+  return ldexpf(bits_to_f32(most), up) > float(kMaxDigits) ? up - 1 : up;
+}
+// A value's three digits in bytes 2, 1, 0, each offset by 128.
+__device__ __forceinline__ uint32_t digits_of(float v, int up, bool finite) {
+  return uint32_t((finite ? int(rintf(ldexpf(v, up))) : 0) + 0x808080);
+}
+__device__ __forceinline__ float digits_scale(int up, bool finite) {
+  return finite ? ldexpf(1.f, -up) : bits_to_f32(0x7fc00000u);
+}
+
 // One thread per 32 columns; the four threads of a chunk share its largest
 // value. Columns behind K are digits of 0. A plane's 128 bytes of a chunk are
 // two halves of four 16-byte pieces, a piece for each 16-lane row of the
@@ -110,15 +125,10 @@ __global__ void __launch_bounds__(256) w4_stage_kernel(Stage p) {
     most = max(most, uint32_t(__shfl_xor(int(most), 1, kWave)));
     most = max(most, uint32_t(__shfl_xor(int(most), 2, kWave)));
     const bool finite = most < 0x7f800000u;
-    // the largest power of two that keeps the value in three digits; chunks
-    // below 2^-96 share its step, 2^-118
-    const int e = max(int(most >> 23) - 127, -96);
-    int up = 22 - e;
-    if (ldexpf(bits_to_f32(most), up) > float(kMaxDigits)) --up;
+    const int up = digits_up(most);
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      X[j] = uint32_t((finite ? int(rintf(ldexpf(v[j], up))) : 0) + 0x808080);
-    xs = finite ? ldexpf(1.f, -up) : bits_to_f32(0x7fc00000u);
+    for (int j = 0; j < 32; ++j) X[j] = digits_of(v[j], up, finite);
+    xs = digits_scale(up, finite);
   }
   int8_t* out = p.a.planes + rc * (P * kW4Chunk);
 #pragma unroll
@@ -475,6 +485,165 @@ __global__ void __launch_bounds__(256) w4_rows_kernel(Product p, int split) {
   }
 }
 
+// One to four tokens, without other launches: a workgroup forms the digits of the
+// tokens by itself, in LDS, while its first weights are on their way, and takes
+// 16 rows of the matrices (the same rows of both). `segments` matrices follow
+// each other along the chunks (one token's experts for the sum over its ranks;
+// else one), which the workgroup's wavefronts share. Their sums are added in
+// order.
+struct Tokens {
+  Product p;
+  const void* x;      // [T or segments, K]
+  uint32_t K, segments;
+  bool sum;             // over the segments
+  const uint32_t* ids;  // experts: of blockIdx.y, or of the segments; null: one matrix
+  uint32_t E;
+};
+
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float4 f = reinterpret_cast<const float4*>(p)[i];
+    v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+  }
+}
+__device__ __forceinline__ void load8(const uint16_t* p, float (&v)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = bits_to_f32(w[j] << 16);
+    v[2 * j + 1] = bits_to_f32(w[j] & 0xffff0000u);
+  }
+}
+
+// Bytes of LDS: digits and scales of all chunks, and the wavefronts' sums.
+inline size_t token_lds(size_t rows, size_t chunks, int mats, int waves) {
+  return rows * chunks * (3 * kW4Chunk + 4) + size_t(waves) * mats * kWave * 4 + 16;
+}
+
+template <bool FINE, int MATS, bool ZEROS, typename ST, typename XT, int WAVES>
+__global__ void __launch_bounds__(WAVES* kWave) w4_token_kernel(Tokens a) {
+  constexpr int B = FINE ? 4 : 1;
+  extern __shared__ __align__(16) int8_t token_shared[];
+  const Product& p = a.p;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, quad = lane >> 4;
+  const bool sum = a.sum;
+  const uint32_t T = sum ? 1 : p.T, rows = sum ? a.segments : T;
+  const uint32_t total = a.segments * p.C;             // chunks
+  int8_t* digits = token_shared;                       // [total][T][3][128]
+  float* xs = reinterpret_cast<float*>(digits + size_t(total) * T * (3 * kW4Chunk));  // [total][T]
+  float* part = xs + size_t(total) * T;                // [WAVES][MATS][64]
+  uint32_t expert = 0;
+  if (a.ids && !sum) {
+    expert = __builtin_amdgcn_readfirstlane(a.ids[blockIdx.y]);
+    if (expert >= a.E) return;  // the same for the workgroup
+  }
+  const uint32_t pairs = (total + 1) / 2;
+  const uint32_t c0 = pairs * wave / WAVES * 2, c1 = pairs * (wave + 1) / WAVES * 2;
+  Codes<FINE, ZEROS, ST> w[2][MATS];
+  bool there[2];
+  auto load = [&](uint32_t chunk, int to) {
+    const uint32_t cc = min(chunk, total - 1);
+    uint32_t e = expert, c = cc;
+    there[to] = chunk < total;
+    if (sum) {
+      const uint32_t r = cc / p.C;
+      c = cc - r * p.C;
+      e = __builtin_amdgcn_readfirstlane(a.ids[r]);
+      there[to] = there[to] && e < a.E;
+      e = e < a.E ? e : 0;  // an id of no expert: any weights, with scales of 0
+    }
+    const size_t at = (size_t(e) * p.row_tiles + blockIdx.x) * p.C + c;
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) w[to][m].load(p.m[m], at, lane);
+  };
+  if (c0 < c1) {
+    load(c0, 0);
+    load(c0 + 1, 1);
+  }
+  // eight columns per thread; 16 neighbouring threads share a chunk's largest
+  // value. Columns behind K are digits of 0.
+  for (uint32_t i = threadIdx.x; i < rows * p.C * 16; i += WAVES * kWave) {
+    const uint32_t row = i / (p.C * 16), in_row = i - row * (p.C * 16), c = in_row / 16;
+    const uint32_t col = in_row * 8, b = in_row / 4 % 4, e = in_row % 4;  // block, eighth
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    // (no row was written for an id of no expert)
+    if (col < a.K && !(sum && a.ids[row] >= a.E))
+      load8(static_cast<const XT*>(a.x) + size_t(row) * a.K + col, v);
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = max(most, f32_to_bits(v[j]) & 0x7fffffffu);
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) most = max(most, uint32_t(__shfl_xor(int(most), m, kWave)));
+    const bool finite = most < 0x7f800000u;
+    const int up = digits_up(most);
+    uint32_t X[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) X[j] = digits_of(v[j], up, finite);
+    const uint32_t at = sum ? row * p.C + c : c * T + row;
+    int8_t* out = digits + size_t(at) * (3 * kW4Chunk);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      const uint32_t even = gather4(X[0], X[2], X[4], X[6], 2 - q) ^ 0x80808080u;
+      const uint32_t odd = gather4(X[1], X[3], X[5], X[7], 2 - q) ^ 0x80808080u;
+      int8_t* plane = out + q * kW4Chunk;
+      if (FINE) {
+        *reinterpret_cast<uint2*>(plane + (b / 2) * 64 + e * 16 + (b % 2) * 8) =
+            make_uint2(even, odd);
+      } else {
+        *reinterpret_cast<uint32_t*>(plane + b * 16 + e * 4) = even;
+        *reinterpret_cast<uint32_t*>(plane + 64 + b * 16 + e * 4) = odd;
+      }
+    }
+    if (in_row % 16 == 0) xs[at] = digits_scale(up, finite);
+  }
+  __syncthreads();
+  float acc[MATS];
+#pragma unroll
+  for (int m = 0; m < MATS; ++m) acc[m] = 0.f;
+  const uint32_t mine = min(uint32_t(n / 4), T - 1), his = min(uint32_t(quad), T - 1);
+  const int8_t* xp = digits + (mine * 3 + min(n & 3, 2)) * kW4Chunk + quad * 16;
+  auto step = [&](uint32_t chunk, int cur) {
+    const uint32_t cc = min(chunk, total - 1);
+    const v4u* at = reinterpret_cast<const v4u*>(xp + size_t(cc) * T * (3 * kW4Chunk));
+    const v4u x0 = at[0], x1 = at[4];
+    const float scale = xs[cc * T + his];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) {
+      v4i even, odd;
+      w[cur][m].widen(even, odd);
+      float value = 0.f;
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const v4i u = dot<FINE>(x0, x1, even, odd, b);
+        value = fmaf(w[cur][m].scale(b, there[cur]), join(u[0], u[1], u[2]), value);
+      }
+      acc[m] = fmaf(value, scale, acc[m]);
+    }
+    load(chunk + 2, cur);
+  };
+  for (uint32_t c = c0; c < c1; c += 2) {
+    step(c, 0);
+    step(c + 1, 1);
+  }
+#pragma unroll
+  for (int m = 0; m < MATS; ++m) part[(wave * MATS + m) * kWave + lane] = acc[m];
+  __syncthreads();
+  const uint32_t row = blockIdx.x * 16 + n;
+  if (wave || uint32_t(quad) >= T || row >= p.N) return;
+  float y[MATS];
+#pragma unroll
+  for (int m = 0; m < MATS; ++m) {
+    y[m] = part[m * kWave + lane];
+    for (int k = 1; k < WAVES; ++k) y[m] += part[(k * MATS + m) * kWave + lane];
+  }
+  const uint32_t j = a.ids && !sum ? blockIdx.y : uint32_t(quad);
+  store_result(p, j, row, y[0], MATS == 2 ? &y[MATS - 1] : nullptr);
+}
+
 // Many tokens. One workgroup: 64 tokens by 128 RT rows of the matrices; a
 // wavefront takes RT tiles of 16 rows of each matrix against all tokens. The
 // weights go from memory to the wavefront that owns them; the tokens' digits go
@@ -789,6 +958,58 @@ int launch_w4_product(hipStream_t s, const W4Product& q) {
       else go(std::integral_constant<int, 1>{});
     });
   }
+  INF_LAUNCHED();
+  return INFERNO_OK;
+}
+
+bool w4_token_fits(const W4Token& q) {
+  const size_t rows = q.sum ? q.segments : q.T;
+  // three workgroups per CU
+  return q.T <= 4 && rows * w4_chunks(q.m[0].cols) < 4096 &&
+         token_lds(rows, w4_chunks(q.m[0].cols), q.mats, 8) <= 53 * 1024;
+}
+
+int launch_w4_token(hipStream_t s, const W4Token& q) {
+  Tokens a{};
+  for (int m = 0; m < q.mats; ++m) {
+    const W4Layout l = w4_layout(q.m[m]);
+    const uint8_t* at = static_cast<const uint8_t*>(q.m[m].packed);
+    a.p.m[m] = Mat{at, at + l.scales, at + l.zeros};
+  }
+  a.p.N = uint32_t(q.m[0].rows);
+  a.p.C = uint32_t(w4_chunks(q.m[0].cols));
+  a.p.row_tiles = (a.p.N + 15) / 16;
+  a.p.T = uint32_t(q.T);
+  a.p.route_w = q.route_w;
+  a.p.res_a = q.res_a;
+  a.p.res_b = q.res_b;
+  a.p.out = q.out;
+  a.x = q.x;
+  a.K = uint32_t(q.m[0].cols);
+  a.segments = uint32_t(q.segments);
+  a.ids = q.ids;
+  a.E = uint32_t(q.m[0].experts);
+  a.sum = q.sum;
+  const bool bf16 = q.x_dtype == INFERNO_BF16;
+  const dim3 grid(a.p.row_tiles, unsigned(q.slots));
+  W4Product f{};
+  f.m[0] = q.m[0];
+  f.mats = q.mats;
+  by_format(f, [&](auto fine, auto mats, auto zeros, auto st) {
+    using ST = decltype(st);
+    constexpr int M = decltype(mats)::value;
+    auto go = [&](auto x, auto waves) {
+      constexpr int W = decltype(waves)::value;
+      const size_t rows = q.sum ? q.segments : q.T;
+      w4_token_kernel<fine.value, M, zeros.value, ST, decltype(x), W>
+          <<<grid, W * kWave, token_lds(rows, a.p.C, M, W), s>>>(a);
+    };
+    if constexpr (M == 1) {
+      if (q.sum) return go(0.f, std::integral_constant<int, 8>{});
+    }
+    if (bf16) go(uint16_t{}, std::integral_constant<int, 4>{});
+    else go(0.f, std::integral_constant<int, 4>{});
+  });
   INF_LAUNCHED();
   return INFERNO_OK;
 }

@@ -68,6 +68,26 @@ struct W4Product {
 };
 int launch_w4_product(hipStream_t s, const W4Product& p);
 
+// One to four fp32 or bf16 tokens of a matrix, or one token of its experts, in
+// one launch. ids: expert ids[y] of each slot y, result row y (none for an id of
+// no expert), or with `sum` the sum over the segments r of row r of x times
+// expert ids[r].
+struct W4Token {
+  W4Mat m[2];
+  int mats;
+  const void* x;
+  int x_dtype;
+  size_t T, slots, segments;
+  bool sum;
+  const uint32_t* ids;   // or null
+  const float* route_w;  // by slot, or null
+  const float* res_a;
+  const float* res_b;
+  float* out;
+};
+bool w4_token_fits(const W4Token& q);
+int launch_w4_token(hipStream_t s, const W4Token& q);
+
 // out[t] = sum over the ranks of token t, in rank order, of y[t*k + r]; ids of
 // no expert count nothing.
 int launch_w4_combine(hipStream_t s, const float* y, const uint32_t* ids, size_t T, size_t H,

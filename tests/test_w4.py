@@ -123,6 +123,8 @@ def test_moe_any_ids(cuda, T):
     _moe(mats, x, None, torch.full((T * k,), 3).int().cuda(), w, k)
     out = _moe(mats, x, None, torch.full((T * k,), E).int().cuda(), w, k)
     assert not out.any()
+    for e in (2, E):
+        _moe(mats, x, None, torch.full((T,), e).int().cuda(), w[:T].contiguous(), 1)
 
 
 @pytest.mark.gpu
