@@ -543,6 +543,7 @@ __global__ void __launch_bounds__(WAVES* kWave) w4_token_kernel(Tokens a) {
   }
   const uint32_t pairs = (total + 1) / 2;
   const uint32_t c0 = pairs * wave / WAVES * 2, c1 = pairs * (wave + 1) / WAVES * 2;
+  const uint32_t my_id = sum && uint32_t(lane) < a.segments ? a.ids[lane] : 0u;
   Codes<FINE, ZEROS, ST> w[2][MATS];
   bool there[2];
   auto load = [&](uint32_t chunk, int to) {
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(WAVES* kWave) w4_token_kernel(Tokens a) {
     if (sum) {
       const uint32_t r = cc / p.C;
       c = cc - r * p.C;
-      e = __builtin_amdgcn_readfirstlane(a.ids[r]);
+      e = __builtin_amdgcn_readlane(my_id, r);
       there[to] = there[to] && e < a.E;
       e = e < a.E ? e : 0;  // an id of no expert: any weights, with scales of 0
     }
@@ -964,9 +965,9 @@ int launch_w4_product(hipStream_t s, const W4Product& q) {
 
 bool w4_token_fits(const W4Token& q) {
   const size_t rows = q.sum ? q.segments : q.T;
-  // three workgroups per CU
-  return q.T <= 4 && rows * w4_chunks(q.m[0].cols) < 4096 &&
-         token_lds(rows, w4_chunks(q.m[0].cols), q.mats, 8) <= 53 * 1024;
+  // three workgroups of four wavefronts per CU, or two of sixteen
+  return q.T <= 4 && q.segments <= kWave && rows * w4_chunks(q.m[0].cols) < 4096 &&
+         token_lds(rows, w4_chunks(q.m[0].cols), q.mats, 16) <= size_t(q.sum ? 80 : 53) * 1024;
 }
 
 int launch_w4_token(hipStream_t s, const W4Token& q) {
@@ -1005,7 +1006,7 @@ int launch_w4_token(hipStream_t s, const W4Token& q) {
           <<<grid, W * kWave, token_lds(rows, a.p.C, M, W), s>>>(a);
     };
     if constexpr (M == 1) {
-      if (q.sum) return go(0.f, std::integral_constant<int, 8>{});
+      if (q.sum) return go(0.f, std::integral_constant<int, 16>{});
     }
     if (bf16) go(uint16_t{}, std::integral_constant<int, 4>{});
     else go(0.f, std::integral_constant<int, 4>{});
