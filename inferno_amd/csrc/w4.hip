@@ -263,6 +263,25 @@ __device__ __forceinline__ void store_result(const Product& p, uint32_t j, uint3
   p.out[at] = y;
 }
 
+// A lane's codes of a chunk as operands of the matrix instructions: for coarse
+// groups the even columns, then the odd ones; for fine groups both of each block
+// in one pair of registers.
+template <bool FINE>
+struct Wide {
+  v4i half[2];
+  __device__ __forceinline__ void put(int j, uint32_t even, uint32_t odd) {
+    half[0][j] = int(even);
+    half[1][j] = int(odd);
+  }
+};
+template <>
+struct Wide<true> {
+  long block[4];
+  __device__ __forceinline__ void put(int j, uint32_t even, uint32_t odd) {
+    block[j] = long(uint64_t(odd) << 32 | even);
+  }
+};
+
 // One chunk of one weight tile on its way: codes, and the scales and zero
 // points of this lane's row (of its four blocks for fine groups).
 template <bool FINE, bool ZEROS, typename ST>
@@ -284,17 +303,19 @@ struct Codes {
   }
   // Even and odd columns as int8: 16 (q - 8), or q - z with zero points (z is at
   // most 127: no byte borrows from the next).
-  __device__ __forceinline__ void widen(v4i& even, v4i& odd) const {
+  __device__ __forceinline__ void widen(Wide<FINE>& w) const {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      uint32_t even, odd;
       if (ZEROS) {
         const uint32_t zz = (FINE ? (z >> (8 * j)) & 255u : z) * 0x01010101u;
-        even[j] = int((((q[j] & 0x0f0f0f0fu) | 0x80808080u) - zz) ^ 0x80808080u);
-        odd[j] = int(((((q[j] >> 4) & 0x0f0f0f0fu) | 0x80808080u) - zz) ^ 0x80808080u);
+        even = (((q[j] & 0x0f0f0f0fu) | 0x80808080u) - zz) ^ 0x80808080u;
+        odd = ((((q[j] >> 4) & 0x0f0f0f0fu) | 0x80808080u) - zz) ^ 0x80808080u;
       } else {
-        even[j] = int((q[j] << 4) & 0xf0f0f0f0u);
-        odd[j] = int(q[j] & 0xf0f0f0f0u);
+        even = (q[j] << 4) & 0xf0f0f0f0u;
+        odd = q[j] & 0xf0f0f0f0u;
       }
+      w.put(j, even, odd);
     }
   }
   // Scale of block b for widen's values; 0 for a chunk that is not `there`.
@@ -306,24 +327,20 @@ struct Codes {
   }
 };
 
-__device__ __forceinline__ long two(uint32_t a, uint32_t b) {
-  return long((uint64_t(b) << 32) | a);
-}
-
 // Sums of one chunk's block b: 16 digit rows (the two halves x0, x1 of a plane)
 // by 16 weight rows.
 template <bool FINE>
-__device__ __forceinline__ v4i dot(const v4u& x0, const v4u& x1, const v4i& even, const v4i& odd,
-                                   int b) {
+__device__ __forceinline__ v4i dot(const v4u& x0, const v4u& x1, const Wide<FINE>& w, int b) {
   v4i s = {0, 0, 0, 0};
-  if (FINE) {
+  if constexpr (FINE) {
     const v4u& u = b < 2 ? x0 : x1;
-    return __builtin_amdgcn_mfma_i32_16x16x32_i8(two(u[2 * (b % 2)], u[2 * (b % 2) + 1]),
-                                                 two(uint32_t(even[b]), uint32_t(odd[b])), s, 0, 0,
+    const long x = long(uint64_t(u[2 * (b % 2) + 1]) << 32 | u[2 * (b % 2)]);
+    return __builtin_amdgcn_mfma_i32_16x16x32_i8(x, w.block[b], s, 0, 0, 0);
+  } else {
+    s = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, x0), w.half[0], s, 0, 0, 0);
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, x1), w.half[1], s, 0, 0,
                                                  0);
   }
-  s = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, x0), even, s, 0, 0, 0);
-  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, x1), odd, s, 0, 0, 0);
 }
 
 // Sum of a token's digits' sums as a float; a sum is at most 2^21.
@@ -401,15 +418,15 @@ __global__ void __launch_bounds__(256) w4_rows_kernel(Product p, int split) {
     auto step = [&](uint32_t c, int cur) {
 #pragma unroll
       for (int f = 0; f < F; ++f) {
-        v4i even, odd;
-        w[cur][f].widen(even, odd);
+        Wide<FINE> wide;
+        w[cur][f].widen(wide);
         float value[NV];
 #pragma unroll
         for (int b = 0; b < B; ++b) {
           v4i sum[NT];
 #pragma unroll
           for (int t = 0; t < NT; ++t)
-            sum[t] = dot<FINE>(x[cur][t][0], x[cur][t][1], even, odd, b);
+            sum[t] = dot<FINE>(x[cur][t][0], x[cur][t][1], wide, b);
           const float ws = w[cur][f].scale(b, c < p.C);
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
@@ -614,12 +631,12 @@ __global__ void __launch_bounds__(WAVES* kWave) w4_token_kernel(Tokens a) {
     const float scale = xs[cc * T + his];
 #pragma unroll
     for (int m = 0; m < MATS; ++m) {
-      v4i even, odd;
-      w[cur][m].widen(even, odd);
+      Wide<FINE> wide;
+      w[cur][m].widen(wide);
       float value = 0.f;
 #pragma unroll
       for (int b = 0; b < B; ++b) {
-        const v4i u = dot<FINE>(x0, x1, even, odd, b);
+        const v4i u = dot<FINE>(x0, x1, wide, b);
         value = fmaf(w[cur][m].scale(b, there[cur]), join(u[0], u[1], u[2]), value);
       }
       acc[m] = fmaf(value, scale, acc[m]);
@@ -645,8 +662,10 @@ __global__ void __launch_bounds__(WAVES* kWave) w4_token_kernel(Tokens a) {
   store_result(p, j, row, y[0], MATS == 2 ? &y[MATS - 1] : nullptr);
 }
 
-// Many tokens. One workgroup: 64 tokens by 128 RT rows of the matrices; a
-// wavefront takes RT tiles of 16 rows of each matrix against all tokens. The
+// Many tokens. One workgroup: 64 tokens by 128 RT / KS rows of the matrices; a
+// wavefront takes RT tiles of 16 rows of each matrix against all tokens, and one
+// of KS shares of the chunks (a chunk costs a workgroup 0.5 us at least, however
+// few there are of it). The
 // weights go from memory to the wavefront that owns them; the tokens' digits go
 // through LDS (two buffers of one chunk) in the order in which the matrix
 // instructions' lanes read them, so that a read is 1 KB without bank conflicts.
@@ -657,11 +676,22 @@ __global__ void __launch_bounds__(WAVES* kWave) w4_token_kernel(Tokens a) {
 constexpr int kTileTokens = 64;
 constexpr int kTileWaves = 8;
 
-template <bool FINE, int MATS, int P, bool ZEROS, typename ST, int RT>
+template <bool FINE, int MATS, int P, bool ZEROS, typename ST, int RT, int KS>
 __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p) {
   constexpr int F = MATS * RT, TT = kTileTokens / 16, B = FINE ? 4 : 1;
-  __shared__ __align__(16) int8_t xt[2][TT][2 * P][kWave * 16];
-  __shared__ __align__(16) float xst[2][kTileTokens];
+  constexpr int RW = kTileWaves / KS;  // wavefronts of a share
+  // chunks that loads are ahead: one where two would not fit the registers (64
+  // experts of 32 tokens, groups of 32: 792 us with two, in scratch memory, 222
+  // with one; coarse groups: 681 with two, 837 with one)
+  constexpr int LOOK = FINE && P == 3 ? 1 : 2;
+  struct Chunks {
+    int8_t x[2][TT][2 * P][kWave * 16];
+    float s[2][kTileTokens];
+  };
+  __shared__ __align__(16) union {
+    Chunks chunks[KS];
+    float part[kTileWaves][F * 4][kWave];  // sums of one token tile
+  } lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;
@@ -669,24 +699,37 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
   if (!slot_of(p, slot)) return;
   const uint32_t end = slot.end;
   // this wavefront's row tiles; those behind the last are the last one again
-  const uint32_t tile0 = (blockIdx.x * kTileWaves + wave) * RT;
+  const int share = wave / RW;
+  const uint32_t tile0 = (blockIdx.x * RW + wave % RW) * RT;
   size_t tile[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
     tile[r] = (size_t(slot.expert) * p.row_tiles + min(tile0 + r, p.row_tiles - 1)) * p.C;
+  auto& xt = lds.chunks[share].x;
+  auto& xst = lds.chunks[share].s;
+  // this share's chunks, in pairs; every share takes as many steps
+  const uint32_t pairs = (p.C + 1) / 2, steps = (pairs + KS - 1) / KS * 2;
+  const uint32_t c0 = pairs * share / KS * 2, c1 = min(pairs * (share + 1) / KS * 2, p.C);
   for (uint32_t t0 = slot.first + blockIdx.z * kTileTokens; t0 < end;
        t0 += gridDim.z * kTileTokens) {
     const uint32_t tokens = min(end - t0, uint32_t(kTileTokens));
     auto run = [&](auto token_tiles) __attribute__((always_inline)) {
       constexpr int NT = decltype(token_tiles)::value;
-      // kTileWaves / 4 wavefronts bring the digits of a token tile, the first of
-      // them its scales
-      constexpr int kPieces = 8 * P / kTileWaves;
-      const int ct = wave * 4 / kTileWaves, cp = wave * kPieces % (2 * P);
-      const bool brings = 16u * ct < tokens;
-      const size_t xr = x_row(p, slot, t0 + 16 * ct + n);
-      const int8_t* xp = p.planes + xr * p.C * (P * kW4Chunk) + cp * 64 + quad * 16;
-      const float* sp = p.xs + xr * p.xs_stride;
+      // a share's wavefronts bring the digits of its chunks: RW / 4 of them those
+      // of a token tile (or one those of 4 / RW tiles), the first its scales
+      constexpr int kPieces = RW >= 4 ? 8 * P / RW : 2 * P, kBring = RW >= 4 ? 1 : 4 / RW;
+      const int cw = wave % RW, ct0 = RW >= 4 ? cw * 4 / RW : cw * kBring;
+      const int cp = RW >= 4 ? cw * kPieces % (2 * P) : 0;
+      const int8_t* xp[kBring];
+      const float* sp[kBring];
+      bool brings[kBring];
+#pragma unroll
+      for (int i = 0; i < kBring; ++i) {
+        const size_t xr = x_row(p, slot, t0 + 16 * (ct0 + i) + n);
+        xp[i] = p.planes + xr * p.C * (P * kW4Chunk) + cp * 64 + quad * 16;
+        sp[i] = p.xs + xr * p.xs_stride;
+        brings[i] = 16u * (ct0 + i) < tokens;
+      }
       float acc[F][NT][4];
 #pragma unroll
       for (int f = 0; f < F; ++f)
@@ -696,26 +739,30 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
           for (int i = 0; i < 4; ++i) acc[f][t][i] = 0.f;
       // Loads on their way, of even and odd chunks. A chunk behind the end is the
       // last one again.
-      Codes<FINE, ZEROS, ST> w[2][F];
-      v4u digits[2][kPieces];
-      float digit_s[2];
+      Codes<FINE, ZEROS, ST> w[LOOK][F];
+      v4u digits[LOOK][kBring][kPieces];
+      float digit_s[LOOK][kBring];
       auto load_digits = [&](uint32_t chunk, int to) {
         const uint32_t c = min(chunk, p.C - 1);
-        if (brings) {
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i)
-            digits[to][i] =
-                *reinterpret_cast<const v4u*>(xp + size_t(c) * (P * kW4Chunk) + i * 64);
-          digit_s[to] = sp[c];
-        }
+        for (int k = 0; k < kBring; ++k)
+          if (brings[k]) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+              digits[to][k][i] =
+                  *reinterpret_cast<const v4u*>(xp[k] + size_t(c) * (P * kW4Chunk) + i * 64);
+            digit_s[to][k] = sp[k][c];
+          }
       };
       auto store_digits = [&](uint32_t c, int from) {
-        if (brings) {
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i)
-            *reinterpret_cast<v4u*>(&xt[c & 1][ct][cp + i][lane * 16]) = digits[from][i];
-          if (cp == 0 && lane < 16) xst[c & 1][16 * ct + n] = digit_s[from];
-        }
+        for (int k = 0; k < kBring; ++k)
+          if (brings[k]) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+              *reinterpret_cast<v4u*>(&xt[c & 1][ct0 + k][cp + i][lane * 16]) = digits[from][k][i];
+            if (cp == 0 && lane < 16) xst[c & 1][16 * (ct0 + k) + n] = digit_s[from][k];
+          }
       };
       auto load_codes = [&](uint32_t chunk, int to) {
         const uint32_t c = min(chunk, p.C - 1);
@@ -725,17 +772,18 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
       auto step = [&](uint32_t c, int cur) {
         // everybody has stored chunk c, and has read chunk c - 1
         __syncthreads();
-        store_digits(c + 1, cur ^ 1);
-        load_digits(c + 3, cur ^ 1);
-        v4i even[F], odd[F];
+        const int next = LOOK == 2 ? cur ^ 1 : 0;
+        store_digits(c + 1, next);
+        load_digits(c + 1 + LOOK, next);
+        Wide<FINE> wide[F];
         float ws[F][B];
 #pragma unroll
         for (int f = 0; f < F; ++f) {
-          w[cur][f].widen(even[f], odd[f]);
+          w[cur][f].widen(wide[f]);
 #pragma unroll
-          for (int b = 0; b < B; ++b) ws[f][b] = w[cur][f].scale(b, c < p.C);
+          for (int b = 0; b < B; ++b) ws[f][b] = w[cur][f].scale(b, c < c1);
         }
-        load_codes(c + 2, cur);
+        load_codes(c + LOOK, cur);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -753,7 +801,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
               v4i sum[P];
 #pragma unroll
               for (int q = 0; q < P; ++q)
-                sum[q] = dot<FINE>(x[2 * q], x[2 * q + 1], even[f], odd[f], b);
+                sum[q] = dot<FINE>(x[2 * q], x[2 * q + 1], wide[f], b);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const float v = P == 3 ? join(sum[0][i], sum[P / 2][i], sum[P - 1][i])
@@ -768,20 +816,41 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
           __builtin_amdgcn_sched_barrier(0);
         }
       };
-      load_digits(0, 0);
-      load_digits(1, 1);
-      load_codes(0, 0);
-      load_codes(1, 1);
-      store_digits(0, 0);
-      load_digits(2, 0);
+      // (c0 is even)
+      load_digits(c0, 0);
+      if (LOOK == 2) load_digits(c0 + 1, LOOK - 1);
+      load_codes(c0, 0);
+      if (LOOK == 2) load_codes(c0 + 1, LOOK - 1);
+      store_digits(c0, 0);
+      load_digits(c0 + LOOK, 0);
       // two at a time without a way past the second (a chunk behind the end has
       // scales of 0): the wait counts of a loop hold for its shortest path
-      for (uint32_t c = 0; c < p.C; c += 2) {
+#pragma unroll 1
+      for (uint32_t c = c0; c < c0 + steps; c += LOOK) {
         step(c, 0);
-        step(c + 1, 1);
+        if (LOOK == 2) step(c + 1, LOOK - 1);
       }
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        if (KS > 1) {
+          // the shares write the sums of the token tiles in turn
+          __syncthreads();
+#pragma unroll
+          for (int f = 0; f < F; ++f)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lds.part[wave][f * 4 + i][lane] = acc[f][t][i];
+          __syncthreads();
+          if (share != t % KS) continue;
+#pragma unroll
+          for (int f = 0; f < F; ++f)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float v = lds.part[wave % RW][f * 4 + i][lane];
+#pragma unroll
+              for (int k = 1; k < KS; ++k) v += lds.part[k * RW + wave % RW][f * 4 + i][lane];
+              acc[f][t][i] = v;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t j = t0 + 16 * t + 4 * quad + i;
@@ -793,6 +862,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
                            MATS == 2 ? &acc[(MATS - 1) * RT + r][t][i] : nullptr);
           }
         }
+      }
     };
     // a loop for each number of token tiles: a branch for each tile inside one
     // loop takes twice the registers
@@ -824,18 +894,33 @@ void by_format(const W4Product& q, Fn f) {
 
 // ----------------------------------------------------------------- combine
 
+// Rows of a token's assignments, added in the order of its ranks; those of no
+// expert are left out (they were never written). Each thread takes VEC columns
+// and has the rows of four ranks on their way: 512 tokens of 4096 columns and 10
+// ranks 16 us, one column and one row at a time 41 us (the 84 MB are still in the
+// last-level cache).
+template <int VEC>
 __global__ void __launch_bounds__(256)
-    w4_combine_kernel(const float* __restrict__ y, const uint32_t* __restrict__ ids, size_t n,
+    w4_combine_kernel(const float* __restrict__ y, const uint32_t* __restrict__ ids, size_t T,
                       uint32_t H, uint32_t k, uint32_t E, float* __restrict__ out) {
-  const size_t i = size_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n) return;
-  const size_t t = i / H, h = i % H;
-  float v = 0.f;
-  for (uint32_t r = 0; r < k; ++r) {
-    const size_t a = t * k + r;
-    if (ids[a] < E) v += y[a * H + h];
+  typedef float Vec __attribute__((ext_vector_type(VEC)));
+  const uint32_t h = (blockIdx.x * 256 + threadIdx.x) * VEC;
+  if (h >= H) return;
+  for (size_t t = blockIdx.y; t < T; t += gridDim.y) {
+    Vec sum = 0.f;
+    for (uint32_t r = 0; r < k; r += 4) {
+      Vec v[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const size_t a = t * k + r + i;
+        v[i] = 0.f;
+        if (r + i < k && ids[a] < E) v[i] = *reinterpret_cast<const Vec*>(y + a * H + h);
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) sum += v[i];
+    }
+    *reinterpret_cast<Vec*>(out + t * H + h) = sum;
   }
-  out[i] = v;
 }
 
 }  // namespace
@@ -913,23 +998,39 @@ int launch_w4_product(hipStream_t s, const W4Product& q) {
   const unsigned slots = q.offsets ? unsigned(std::min(q.m[0].experts, q.T * q.k)) : 1u;
   const size_t per_slot = q.T * (q.offsets ? q.k : 1) / slots;
   const bool one = q.x.P == 1;
-  if (per_slot > 16) {
+  // Measured: the tile kernel's step costs the same for 1 to 16 tokens. One expert
+  // of 16 tokens: rows 12.3 and 21.5 (one and three planes), tiles 14.3 and 32.5
+  // us. Routed, where the tile kernel reads an expert's weights once for all its
+  // tokens: 64 experts of 3 tokens each rows 92, tiles 96 us, of 4 rows 104, tiles
+  // 96; 128 of 3 rows 268, tiles 277, of 5 rows 294, tiles 282, of 15 rows 509,
+  // tiles 380.
+  if (per_slot > (q.offsets ? 3 : 16)) {
     // workgroups of a slot beyond its tokens end at once; a slot with more
     // tokens than they take goes round again
     const size_t blocks = q.offsets ? std::min<size_t>(2 * per_slot / kTileTokens + 1, 8)
                                     : (q.T + kTileTokens - 1) / kTileTokens;
     by_format(q, [&](auto fine, auto mats, auto zeros, auto st) {
       constexpr int M = decltype(mats)::value, RT = M == 2 ? 1 : 2;
-      constexpr unsigned tiles = RT * kTileWaves;
-      const dim3 grid((p.row_tiles + tiles - 1) / tiles, slots,
-                      unsigned(std::min<size_t>(blocks, 65535)));
       using ST = decltype(st);
-      if (one)
-        w4_tile_kernel<fine.value, M, 1, zeros.value, ST, RT>
+      auto go = [&](auto planes, auto shares) {
+        constexpr int P = decltype(planes)::value, KS = decltype(shares)::value;
+        constexpr unsigned tiles = RT * kTileWaves / KS;
+        const dim3 grid((p.row_tiles + tiles - 1) / tiles, slots,
+                        unsigned(std::min<size_t>(blocks, 65535)));
+        w4_tile_kernel<fine.value, M, P, zeros.value, ST, RT, KS>
             <<<grid, kTileWaves * kWave, 0, s>>>(p);
-      else
-        w4_tile_kernel<fine.value, M, 3, zeros.value, ST, RT>
-            <<<grid, kTileWaves * kWave, 0, s>>>(p);
+      };
+      // shares of the chunks until there is a workgroup for every CU
+      const size_t groups =
+          (p.row_tiles + RT * kTileWaves - 1) / (RT * kTileWaves) * slots * blocks;
+      auto three = std::integral_constant<int, 3>{};
+      auto single = std::integral_constant<int, 1>{};
+      auto twice = std::integral_constant<int, 2>{};
+      if (one && groups < 128) go(single, std::integral_constant<int, 4>{});
+      else if (one && groups < 256) go(single, twice);
+      else if (one) go(single, single);
+      else if (groups < 256) go(three, twice);
+      else go(three, single);
     });
   } else {
     // Measured over 81 to 32768 row tiles (whole passes, rt / split): enough
@@ -1017,9 +1118,15 @@ int launch_w4_token(hipStream_t s, const W4Token& q) {
 
 int launch_w4_combine(hipStream_t s, const float* y, const uint32_t* ids, size_t T, size_t H,
                       size_t k, size_t E, float* out) {
-  const size_t n = T * H;
-  w4_combine_kernel<<<unsigned((n + 255) / 256), 256, 0, s>>>(y, ids, n, uint32_t(H), uint32_t(k),
-                                                              uint32_t(E), out);
+  const bool wide = H % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const size_t threads = wide ? H / 4 : H;
+  const dim3 grid(unsigned((threads + 255) / 256), unsigned(std::min<size_t>(T, 65535)));
+  if (wide)
+    w4_combine_kernel<4>
+        <<<grid, 256, 0, s>>>(y, ids, T, uint32_t(H), uint32_t(k), uint32_t(E), out);
+  else
+    w4_combine_kernel<1>
+        <<<grid, 256, 0, s>>>(y, ids, T, uint32_t(H), uint32_t(k), uint32_t(E), out);
   INF_LAUNCHED();
   return INFERNO_OK;
 }
