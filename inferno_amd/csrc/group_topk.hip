@@ -10,9 +10,13 @@
 // Values are first formed in 32 bits. They decide wherever the values that they
 // order are further apart than their roundings, which is checked for the last
 // open group against the first closed one, for the last winner against the
-// best loser and for neighbouring winners; a token that fails (or holds a NaN)
-// is done again in 64 bits. 8192 tokens of 256 experts in 8 groups, all in 64
-// bits: 28 us.
+// best loser and for neighbouring winners. Where winners fail, the experts that
+// may be among the k best (one per lane) are formed and ranked in 64 bits; a
+// token whose groups fail, with more of them than lanes, or with a NaN is done
+// again in 64 bits as a whole. 8192 tokens of 256 experts in 8 groups: 15.7 us;
+// whole rows in 64 bits for every failure 20.3, for every token 28 us. All 8192
+// wavefronts are resident at once: what bounds it is their instructions and, for
+// few tokens, one chain of cross-lane steps (29 tokens: 5 us).
 #include "kernels.hpp"
 #include "routing_dev.hpp"
 
@@ -42,9 +46,8 @@ union Scratch {
   } exact;
   struct {
     float value[2 * kMaxExperts];  // a group's values one place apart from the next's
-    uint32_t key[kMaxTopK];
-    uint32_t id[kMaxTopK];
-    float score[kMaxTopK];
+    uint32_t key[kWave];
+    uint32_t id[kWave];
     float by_rank[kMaxTopK];
   } fast;
 };
@@ -169,6 +172,17 @@ __device__ __forceinline__ void exact_row(const GroupTopk& p, size_t t, Scratch&
   }
 }
 
+// The sigmoid but for 2^-22: the rounding of l log2(e) moves it by at most
+// max(|l| s (1 - s)) 2^-24 = 0.23 2^-24, that of the product with the constant's
+// as much; exponential, sum and reciprocal are off by a few 2^-24 of themselves.
+__device__ __forceinline__ float near_sigmoid(float l) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * l));
+}
+
+__device__ __forceinline__ float lane_of(float v, int lane) {  // lane: uniform
+  return bits_to_f32(__builtin_amdgcn_readlane(__builtin_bit_cast(uint32_t, v), lane));
+}
+
 // Whether a > b holds for the 64-bit values of two 32-bit ones. A sigmoid is
 // off by at most 2^-22, the addition of the bias by 2^-24 of the value; `times`
 // values were added. Infinities and NaN: no.
@@ -211,7 +225,7 @@ __device__ __forceinline__ bool fast_row(const GroupTopk& p, size_t t, Scratch& 
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int e = lane + j * kWave;
-    score[j] = sigmoid ? 1.f / (1.f + expf(-lg[j])) : expf(lg[j] - lmax);
+    score[j] = sigmoid ? near_sigmoid(lg[j]) : expf(lg[j] - lmax);
     v[j] = (sigmoid ? score[j] : lg[j]) + bs[j];
     // e / size for e < 256: the quotient's error is far below 1 / (2 size)
     group[j] = int((float(e) + 0.5f) * magic);
@@ -241,7 +255,7 @@ __device__ __forceinline__ bool fast_row(const GroupTopk& p, size_t t, Scratch& 
     int before = 0;
     float next = -INFINITY;  // the largest value at or below this group's, of another
     for (int o = 0; o < p.groups; ++o) {
-      const float x = __shfl(gv, o * L, kWave);
+      const float x = lane_of(gv, o * L);
       before += x > gv || (x == gv && o < g);
       if (x < gv || (x == gv && o > g)) next = fmaxf(next, x);
     }
@@ -272,51 +286,91 @@ __device__ __forceinline__ bool fast_row(const GroupTopk& p, size_t t, Scratch& 
       if (m == uint32_t(p.k)) break;  // uniform
     }
   }
-  if (n != uint32_t(p.k)) return false;  // equal keys
-  uint32_t base = 0, loser = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const bool win = key[j] >= kth;
-    const uint64_t m = __ballot(win);
-    if (win) {
-      const uint32_t at = base + __builtin_amdgcn_mbcnt_hi(
-                                     uint32_t(m >> 32),
-                                     __builtin_amdgcn_mbcnt_lo(uint32_t(m), 0u));
-      s.key[at] = key[j];
-      s.id[at] = uint32_t(lane + j * kWave);
-      s.score[at] = score[j];
-    } else {
-      loser = max(loser, key[j]);
-    }
-    base += uint32_t(__popcll(m));
-  }
-  loser = wave_umax(loser);  // 0: none
-  __builtin_amdgcn_wave_barrier();
-  const uint32_t mine = s.key[min(lane, p.k - 1)];
-  const float my_score = s.score[min(lane, p.k - 1)];
-  uint32_t rank = 0, same = 0, below = loser;  // the best key below this winner's
-  for (int i = 0; i < p.k; ++i) {
-    const uint32_t o = s.key[i];
-    rank += o > mine ? 1u : 0u;
-    same += o == mine ? 1u : 0u;
-    if (o < mine) below = max(below, o);
-  }
   auto value_of = [](uint32_t k) {
     return bits_to_f32((k >> 31) ? k ^ 0x80000000u : ~k);
   };
-  const bool clear =
-      same == 1 && (below == 0 || above(value_of(mine), value_of(below), sigmoid, 1.f));
-  if (__any(lane < p.k && !clear)) return false;
-  if (lane < p.k) s.by_rank[rank] = my_score;
-  __builtin_amdgcn_wave_barrier();
+  // puts the experts that `is` holds for next to each other, and returns how many
+  auto gather = [&](auto is) {
+    uint32_t base = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const bool win = is(key[j]);
+      const uint64_t m = __ballot(win);
+      const uint32_t at = base + __builtin_amdgcn_mbcnt_hi(
+                                     uint32_t(m >> 32),
+                                     __builtin_amdgcn_mbcnt_lo(uint32_t(m), 0u));
+      if (win && at < uint32_t(kWave)) {
+        s.key[at] = key[j];
+        s.id[at] = uint32_t(lane + j * kWave);
+      }
+      base += uint32_t(__popcll(m));
+    }
+    __builtin_amdgcn_wave_barrier();
+    return base;
+  };
+  bool clear = false;
+  uint32_t rank = 0, id = 0;  // of this lane's winner, if it has one
+  if (n == uint32_t(p.k)) {   // else keys are equal
+    gather([&](uint32_t k) { return k >= kth; });
+    uint32_t loser = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) loser = max(loser, key[j] < kth ? key[j] : 0u);
+    const uint32_t mine = s.key[min(lane, p.k - 1)];
+    id = s.id[min(lane, p.k - 1)];
+    uint32_t same = 0, below = wave_umax(loser);  // the best key below this winner's, 0: none
+    for (int i = 0; i < p.k; ++i) {
+      const uint32_t o = __builtin_amdgcn_readlane(mine, i);
+      rank += o > mine ? 1u : 0u;
+      same += o == mine ? 1u : 0u;
+      if (o < mine) below = max(below, o);
+    }
+    clear = same == 1 && (below == 0 || above(value_of(mine), value_of(below), sigmoid, 1.f));
+    if (lane >= p.k) rank = uint32_t(p.k);
+  }
+  if (__any(rank < uint32_t(p.k) && !clear)) {
+    // In 64 bits, but only the experts that may be among the k best: those not
+    // clearly below the k-th largest key.
+    kth = 0;
+    for (int b = 31; b >= 0; --b) {
+      const uint32_t c = kth | (1u << b);
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) m += uint32_t(__popcll(__ballot(key[j] >= c)));
+      if (m >= uint32_t(p.k)) kth = c;
+    }
+    const uint32_t many = gather([&](uint32_t k) {
+      return k >= kth || (k && !above(value_of(kth), value_of(k), sigmoid, 1.f));
+    });
+    if (many > uint32_t(kWave)) return false;
+    id = s.id[min(uint32_t(lane), many - 1)];
+    double exact = row[id];
+    if (sigmoid) exact = 1.0 / (1.0 + exp(-exact));
+    exact += p.bias ? double(p.bias[id]) : 0.0;
+    const uint64_t mine = order_key(exact);
+    rank = 0;
+    for (uint32_t i = 0; i < many; ++i) {
+      const uint32_t high = __builtin_amdgcn_readlane(uint32_t(mine >> 32), i);
+      const uint32_t low = __builtin_amdgcn_readlane(uint32_t(mine), i);
+      const uint64_t o = uint64_t(high) << 32 | low;
+      const uint32_t other = __builtin_amdgcn_readlane(id, i);
+      rank += o > mine || (o == mine && other < id) ? 1u : 0u;
+    }
+    if (uint32_t(lane) >= many) rank = uint32_t(p.k);
+  }
+  const bool won = rank < uint32_t(p.k);
+  const float my_score = sigmoid ? 1.f / (1.f + expf(-row[id])) : expf(row[id] - lmax);
   float sum = 0.f;
-  if (p.norm)
-    for (int r = 0; r < p.k; ++r) sum += s.by_rank[r];  // rank order
-  else
+  if (p.norm) {
+    if (won) s.by_rank[rank] = my_score;
+    __builtin_amdgcn_wave_barrier();
+    const float ranked = s.by_rank[min(lane, p.k - 1)];
+    for (int r = 0; r < p.k; ++r) sum += lane_of(ranked, r);  // rank order
+  } else {
     sum = wave_sum(all);
-  if (lane < p.k) {
+  }
+  if (won) {
     const size_t a = t * size_t(p.k) + rank;
-    p.ids[a] = s.id[lane];
+    p.ids[a] = id;
     p.weights[a] = weight_of(p, my_score, sum);
     if (p.token_idx) p.token_idx[a] = uint32_t(t);
   }

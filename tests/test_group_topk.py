@@ -102,6 +102,31 @@ def test_ties_and_neighbours(cuda, score_fn, rule):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("E", [24, 64, 70, 256])
+@pytest.mark.parametrize("score_fn", [SCORE_SIGMOID, SCORE_SOFTMAX])
+def test_few_and_many_near_ties(cuda, E, score_fn):
+    # a handful of values next to each other among many, up to all of them
+    g = torch.Generator().manual_seed(E)
+    for many in (2, 9, 30, 64, 65, E):
+        logits = torch.randn(50, E, generator=g) - 4.0
+        for t in range(50):
+            at = torch.randperm(E, generator=g)[:many]
+            logits[t, at] = 3.0 + torch.randint(0, 3, (len(at),), generator=g) * 2.0 ** -22
+        bias = torch.zeros(E)
+        bias[::3] = 2.0 ** -24
+        for b in (None, bias.to(cuda)):
+            _check(logits.to(cuda), b, min(8, E), score_fn, True, 1.0, 1, 1, GROUP_MAX)
+            _check(logits.to(cuda), b, 4, score_fn, False, 1.0, 2, 1, GROUP_TOP2)
+
+
+@pytest.mark.gpu
+def test_many_tokens(cuda):
+    g = torch.Generator().manual_seed(6)
+    _check(torch.randn(70001, 8, generator=g).to(cuda), None, 2, SCORE_SIGMOID, True, 1.0, 4, 2,
+           GROUP_MAX)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("score_fn", [SCORE_SIGMOID, SCORE_SOFTMAX])
 def test_closed_and_empty_rows(cuda, score_fn):
     g = torch.Generator().manual_seed(4)
