@@ -236,10 +236,11 @@ int inferno_w4_pack(void* stream, const inferno_w4* w, const void* codes, size_t
  * x_scales [T, cols / x_group] fp32 (x = value * scale; x_group a multiple of
  * 128 that divides cols, or 0: one scale per row; what
  * inferno_add_rms_norm_q8 writes). x lies at a multiple of 16 bytes; x_scales
- * and x_group are not read for F32 and BF16. The products of codes and
- * activations are summed exactly within a group: bf16 activations enter whole
- * (down to 2^-14 of the largest of their 128 columns), fp32 ones rounded to
- * 2^-23 of it. A NaN or an infinity in x makes its token's outputs NaN.
+ * and x_group are not read for F32 and BF16. bf16 activations enter whole (down
+ * to 2^-14 of the largest of their 128 columns), fp32 ones rounded to 2^-23 of
+ * it. The products of codes and activations are summed exactly within a group
+ * for I8 and for few tokens; for more (above 16, or above 3 per expert) in fp32,
+ * 128 columns at a time. A NaN or an infinity in x makes its token's outputs NaN.
  * T = 0 does nothing. */
 
 /* Workspace bytes of the two dense products over T tokens of `cols` columns. */

@@ -83,19 +83,27 @@ int check_tokens(size_t rows, size_t cols) {
   return INFERNO_OK;
 }
 
-// Room for three digits, which any call fits.
+// Room for two planes of fp16, which any call fits.
 W4Acts carve_acts(Carver& c, size_t rows, size_t cols) {
   const size_t n = rows * w4_chunks(cols);
   W4Acts a{};
-  a.planes = c.take<int8_t>(n * 3 * kW4Chunk);
+  a.planes = c.take<int8_t>(n * 4 * kW4Chunk);
   a.xs = c.take<float>(rows * w4_xs_stride(cols));
   return a;
 }
 
 // The same region for the matrices and activations of one call.
-W4Acts acts_for(W4Acts a, const inferno_w4* w, int x_dtype) {
+W4Acts acts_for(W4Acts a, const inferno_w4* w, int x_dtype, size_t T, size_t k) {
   a.P = x_dtype == INFERNO_I8 ? 1 : 3;
   a.fine = mat(w).fine();
+  // Two planes of fp16 are more to move than three of digits, but need no joins,
+  // of which fine groups have four in a chunk. fp32 tokens, two planes of fp16 and
+  // three digits: 128 experts' down, 512 tokens 335 and 250 us (groups of 128); 64
+  // experts, 256 tokens 178 and 222 us (groups of 32, whole pass).
+  if (w4_by_tiles(T, k, w->experts)) {
+    if (x_dtype == INFERNO_BF16) a.halves = 1;
+    else if (x_dtype == INFERNO_F32 && a.fine) a.halves = 2;
+  }
   return a;
 }
 
@@ -210,7 +218,7 @@ int inferno_w4_matvec_add2(void* stream, const inferno_w4* w, const void* x, int
     if (w4_token_fits(q)) return launch_w4_token(s, q);
   }
   Carver c{static_cast<char*>(workspace)};
-  const W4Acts a = acts_for(carve_acts(c, T, w->cols), w, x_dtype);
+  const W4Acts a = acts_for(carve_acts(c, T, w->cols), w, x_dtype, T, 0);
   if ((st = launch_w4_stage(s, x, x_dtype, x_scales, x_group, T, w->cols, a))) return st;
   W4Product p = product(w, a, T, out);
   p.res_a = residual_a;
@@ -240,7 +248,7 @@ int inferno_w4_gate_up_swiglu(void* stream, const inferno_w4* gate, const infern
     if (w4_token_fits(q)) return launch_w4_token(s, q);
   }
   Carver c{static_cast<char*>(workspace)};
-  const W4Acts a = acts_for(carve_acts(c, T, gate->cols), gate, x_dtype);
+  const W4Acts a = acts_for(carve_acts(c, T, gate->cols), gate, x_dtype, T, 0);
   if ((st = launch_w4_stage(s, x, x_dtype, x_scales, x_group, T, gate->cols, a))) return st;
   W4Product p = product(gate, a, T, out);
   p.m[1] = mat(up);
@@ -294,7 +302,8 @@ int inferno_w4_moe(void* stream, const inferno_w4* gate, const inferno_w4* up,
     }
   }
   if ((st = launch_dispatch(s, expert_ids, T, k, E, m.offsets, m.sorted, m.active))) return st;
-  const W4Acts xa = acts_for(m.x, gate, x_dtype), ha = acts_for(m.h_acts, down, INFERNO_F32);
+  const W4Acts xa = acts_for(m.x, gate, x_dtype, T, k),
+               ha = acts_for(m.h_acts, down, INFERNO_F32, T, k);
   if ((st = launch_w4_stage(s, x, x_dtype, x_scales, x_group, T, H, xa))) return st;
   W4Product g = product(gate, xa, T, m.h);
   g.m[1] = mat(up);

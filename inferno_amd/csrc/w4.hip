@@ -1,14 +1,18 @@
-// Products with 4-bit weights and group scales on the integer matrix cores.
+// Products with 4-bit weights and group scales on the matrix cores.
 //
 //   y[t, n] = sum_g s[n, g] sum_{c in g} (q[n, c] - z[n, g]) x[t, c]
 //
-// The inner sum is formed exactly. A code is widened to 16 (q - 8), an int8, by
+// int8 activations and few tokens: the inner sum is formed exactly. A code is widened to 16 (q - 8), an int8, by
 // one mask (its nibble stays in the high half of the byte), or to q - z with
 // four codes in one subtraction; an activation is one int8 digit (8-bit
 // activations) or three, a 24-bit fixed-point value relative to the largest of
 // its 128-column chunk: exact for every bf16 value down to 2^-14 of the
 // largest, and off by at most 2^-23 of it for fp32. The int32 sums of a group
-// are exact, the groups are added in fp32.
+// are exact, the groups are added in fp32. Joining three sums is six vector
+// instructions a result and chunk, more than their matrix instructions take, so
+// many bf16 tokens (and fp32 ones with groups of 32 or 64) go as fp16 instead,
+// one plane (two) of values scaled by a power of two for each chunk, against
+// codes widened to fp16, q - z whole; a chunk's sums are formed in fp32.
 //
 // Tile: 16 weight rows (the 16 columns of a 16x16 MFMA result) by 16 digit
 // rows. A lane holds 32 codes of its row per chunk (16 bytes: low nibbles are
@@ -25,6 +29,9 @@ namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxDigits = 127 * 65536 + 127 * 256 + 127;  // largest three-digit value
 
@@ -157,6 +164,56 @@ __global__ void __launch_bounds__(256) w4_stage_kernel(Stage p) {
   if (b == 1 && c + 1 == p.C && p.C < p.xs_stride) p.a.xs[r * p.xs_stride + p.C] = 0.f;
 }
 
+// The same as fp16 in PLANES planes: one holds a bf16 value whole (to 2^-31 of its
+// chunk's largest), two an fp32 value but for 2^-23 of itself. The chunk's largest
+// is taken to [2^14, 2^15). A plane's 256 bytes of a chunk are four pieces of 64,
+// one for each dword of a lane's codes; in a piece every 16-lane row of the
+// weights' tile has the 8 columns of its dword in the order in which
+// Halves::widen gives them.
+template <typename XT, int PLANES>
+__global__ void __launch_bounds__(256) w4_stage_halves_kernel(Stage p) {
+  const size_t i = size_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= p.R * p.C * 4) return;  // four threads of one chunk go together
+  const size_t rc = i / 4, r = rc / p.C, c = rc % p.C;
+  const int b = int(i % 4);
+  const size_t col = c * kW4Chunk + b * 32;
+  float v[32];
+  if (col < p.K) {
+    load32(static_cast<const XT*>(p.x) + r * p.K + col, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+  }
+  uint32_t most = 0;  // as integers: NaN lies above infinity
+#pragma unroll
+  for (int j = 0; j < 32; ++j) most = max(most, f32_to_bits(v[j]) & 0x7fffffffu);
+  most = max(most, uint32_t(__shfl_xor(int(most), 1, kWave)));
+  most = max(most, uint32_t(__shfl_xor(int(most), 2, kWave)));
+  const bool finite = most < 0x7f800000u;
+  const int up = 14 - max(int(most >> 23) - 127, -96);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = finite ? ldexpf(v[j], up) : 0.f;
+  int8_t* out = p.a.planes + rc * (PLANES * 2 * kW4Chunk);
+#pragma unroll
+  for (int q = 0; q < PLANES; ++q) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      v8h h;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float& value = v[8 * m + (j % 2) * 4 + j / 2];
+        h[j] = _Float16(value);
+        value -= float(h[j]);
+      }
+      // coarse groups: lane row b, dword m; fine ones: lane row m, dword b
+      const int piece = p.a.fine ? b : m, row = p.a.fine ? m : b;
+      *reinterpret_cast<v8h*>(out + q * 2 * kW4Chunk + piece * 64 + row * 16) = h;
+    }
+  }
+  if (b == 0) p.a.xs[r * p.xs_stride + c] = digits_scale(up, finite);
+  if (b == 1 && c + 1 == p.C && p.C < p.xs_stride) p.a.xs[r * p.xs_stride + p.C] = 0.f;
+}
+
 // -------------------------------------------------------------------- pack
 
 struct Pack {
@@ -229,16 +286,16 @@ struct Product {
   float* out;
 };
 
-// The expert of this workgroup (blockIdx.y) and its assignments, or all tokens;
-// false: none. Uniform values.
+// The expert of slot y and its assignments, or all tokens; false: none. Uniform
+// values.
 struct Slot {
   uint32_t expert, first, end;
 };
-__device__ __forceinline__ bool slot_of(const Product& p, Slot& s) {
+__device__ __forceinline__ bool slot_of(const Product& p, uint32_t y, Slot& s) {
   s = Slot{0, 0, p.T};
   if (!p.offsets) return true;
-  if (blockIdx.y >= p.active[0]) return false;
-  s.expert = __builtin_amdgcn_readfirstlane(p.active[1 + blockIdx.y]);
+  if (y >= p.active[0]) return false;
+  s.expert = __builtin_amdgcn_readfirstlane(p.active[1 + y]);
   s.first = __builtin_amdgcn_readfirstlane(p.offsets[s.expert]);
   s.end = __builtin_amdgcn_readfirstlane(p.offsets[s.expert + 1]);
   return true;
@@ -282,6 +339,37 @@ struct Wide<true> {
   }
 };
 
+// The same as fp16: q - 8 or q - z, one register quadruple for each dword of
+// codes, whose columns come in the order 0 4 1 5 2 6 3 7. 0x6400 with a code in
+// its low bits is 1024 + q, with a code four bits up 1024 + 16 q.
+struct Halves {
+  v4u dword[4];
+
+  template <bool FINE, bool ZEROS>
+  __device__ __forceinline__ void widen(const v4u& q, uint32_t z) {
+    const v2h sixteenth = {_Float16(0.0625f), _Float16(0.0625f)};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v2h low = {_Float16(-1032.f), _Float16(-1032.f)}, high = {_Float16(-72.f), _Float16(-72.f)};
+      if (ZEROS) {  // (1024 + z) with the sign bit, and 960 less
+        const uint32_t zz = FINE ? (z >> (8 * j)) & 255u : z;
+        low = __builtin_bit_cast(v2h, zz * 0x00010001u | 0xe400e400u);
+        high = low + v2h{_Float16(960.f), _Float16(960.f)};
+      }
+      uint32_t u = ZEROS ? q[j] : q[j] ^ 0x88888888u;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const v2h a = __builtin_bit_cast(v2h, (u & 0x000f000fu) | 0x64006400u);
+        const v2h b = __builtin_bit_cast(v2h, (u & 0x00f000f0u) | 0x64006400u);
+        dword[j][2 * i] = __builtin_bit_cast(uint32_t, a + low);
+        dword[j][2 * i + 1] =
+            __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, sixteenth, high));
+        u >>= 8;
+      }
+    }
+  }
+};
+
 // One chunk of one weight tile on its way: codes, and the scales and zero
 // points of this lane's row (of its four blocks for fine groups).
 template <bool FINE, bool ZEROS, typename ST>
@@ -318,12 +406,17 @@ struct Codes {
       w.put(j, even, odd);
     }
   }
-  // Scale of block b for widen's values; 0 for a chunk that is not `there`.
-  __device__ __forceinline__ float scale(int b, bool there) const {
+  __device__ __forceinline__ void widen(Halves& w) const { w.template widen<FINE, ZEROS>(q, z); }
+  // Scale of block b; 0 for a chunk that is not `there`.
+  __device__ __forceinline__ float plain_scale(int b, bool there) const {
     float v;
     if constexpr (sizeof(ST) == 2) v = bf16_bits_to_f32(s[b]);
     else v = s[b];
-    return there ? (ZEROS ? v : v * 0.0625f) : 0.f;
+    return there ? v : 0.f;
+  }
+  // The same for the int8 values of widen.
+  __device__ __forceinline__ float scale(int b, bool there) const {
+    return plain_scale(b, there) * (ZEROS ? 1.f : 0.0625f);
   }
 };
 
@@ -366,7 +459,7 @@ __global__ void __launch_bounds__(256) w4_rows_kernel(Product p, int split) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;
   Slot slot;
-  if (!slot_of(p, slot)) return;
+  if (!slot_of(p, blockIdx.y, slot)) return;
   const uint32_t end = slot.end;
   const uint32_t tile0 = (blockIdx.x * (4 / split) + wave / split) * RT;
   size_t tile[RT];
@@ -666,26 +759,34 @@ __global__ void __launch_bounds__(WAVES* kWave) w4_token_kernel(Tokens a) {
 // wavefront takes RT tiles of 16 rows of each matrix against all tokens, and one
 // of KS shares of the chunks (a chunk costs a workgroup 0.5 us at least, however
 // few there are of it). The
-// weights go from memory to the wavefront that owns them; the tokens' digits go
+// weights go from memory to the wavefront that owns them; the tokens' values go
 // through LDS (two buffers of one chunk) in the order in which the matrix
 // instructions' lanes read them, so that a read is 1 KB without bank conflicts.
 // Both are two chunks ahead in registers, since a chunk's loads take longer
 // than its arithmetic (copies to LDS that bypass registers would have to be
 // complete before any LDS read). Tiles of 16 tokens that an expert does not
-// have are left out.
+// have are left out; a tile's pieces are read while the one before is in use,
+// where they fit the registers.
+// What bounds it: one workgroup per CU (170 to 256 registers), whose loads,
+// reads from LDS and arithmetic overlap only in part. 512 bf16 tokens of 10 of
+// 128 experts, gate and up 1536 x 4096: 350 us for 0.82 GB of weights (2.3
+// TB/s), three digits 418; down, three digits: 246 us. 64 int8 tokens, gate and
+// up: 147 us (5.6 TB/s with the caches' help). One matrix pair 2048 x 6144, 256
+// tokens: int8 36, bf16 56 us, three digits 84.
 constexpr int kTileTokens = 64;
 constexpr int kTileWaves = 8;
 
-template <bool FINE, int MATS, int P, bool ZEROS, typename ST, int RT, int KS>
+template <bool FINE, int MATS, bool HALF, int P, bool ZEROS, typename ST, int RT, int KS>
 __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p) {
   constexpr int F = MATS * RT, TT = kTileTokens / 16, B = FINE ? 4 : 1;
   constexpr int RW = kTileWaves / KS;  // wavefronts of a share
-  // chunks that loads are ahead: one where two would not fit the registers (64
-  // experts of 32 tokens, groups of 32: 792 us with two, in scratch memory, 222
-  // with one; coarse groups: 681 with two, 837 with one)
-  constexpr int LOOK = FINE && P == 3 ? 1 : 2;
+  constexpr int PC = HALF ? 4 * P : 2 * P;  // pieces of 64 bytes of a token's chunk
+  // chunks that loads are ahead; with two, fine groups of fp16 go through scratch
+  // memory (64 tokens, groups of 32: 95 us, with one 74)
+  constexpr int LOOK = FINE && HALF ? 1 : 2;
+  constexpr int XB = PC <= 4 ? 2 : 1;  // token tiles whose pieces are in registers
   struct Chunks {
-    int8_t x[2][TT][2 * P][kWave * 16];
+    int8_t x[2][TT][PC][kWave * 16];
     float s[2][kTileTokens];
   };
   __shared__ __align__(16) union {
@@ -696,11 +797,16 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;
   Slot slot;
-  if (!slot_of(p, slot)) return;
+  // A routed product has eight slots in a row of workgroups, so that those of one
+  // expert (neighbours but seven) share the L2 of one XCD, which then takes the
+  // expert's tokens from memory once (gate and up of 512 tokens 380 -> 362 us
+  // with the next tile's reads ahead).
+  const uint32_t block = p.offsets ? blockIdx.x / 8 : blockIdx.x;
+  if (!slot_of(p, blockIdx.y * 8 + blockIdx.x % 8, slot)) return;
   const uint32_t end = slot.end;
   // this wavefront's row tiles; those behind the last are the last one again
   const int share = wave / RW;
-  const uint32_t tile0 = (blockIdx.x * RW + wave % RW) * RT;
+  const uint32_t tile0 = (block * RW + wave % RW) * RT;
   size_t tile[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
@@ -717,16 +823,16 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
       constexpr int NT = decltype(token_tiles)::value;
       // a share's wavefronts bring the digits of its chunks: RW / 4 of them those
       // of a token tile (or one those of 4 / RW tiles), the first its scales
-      constexpr int kPieces = RW >= 4 ? 8 * P / RW : 2 * P, kBring = RW >= 4 ? 1 : 4 / RW;
+      constexpr int kPieces = RW >= 4 ? 4 * PC / RW : PC, kBring = RW >= 4 ? 1 : 4 / RW;
       const int cw = wave % RW, ct0 = RW >= 4 ? cw * 4 / RW : cw * kBring;
-      const int cp = RW >= 4 ? cw * kPieces % (2 * P) : 0;
+      const int cp = RW >= 4 ? cw * kPieces % PC : 0;
       const int8_t* xp[kBring];
       const float* sp[kBring];
       bool brings[kBring];
 #pragma unroll
       for (int i = 0; i < kBring; ++i) {
         const size_t xr = x_row(p, slot, t0 + 16 * (ct0 + i) + n);
-        xp[i] = p.planes + xr * p.C * (P * kW4Chunk) + cp * 64 + quad * 16;
+        xp[i] = p.planes + xr * p.C * (PC * 64) + cp * 64 + quad * 16;
         sp[i] = p.xs + xr * p.xs_stride;
         brings[i] = 16u * (ct0 + i) < tokens;
       }
@@ -750,7 +856,7 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
               digits[to][k][i] =
-                  *reinterpret_cast<const v4u*>(xp[k] + size_t(c) * (P * kW4Chunk) + i * 64);
+                  *reinterpret_cast<const v4u*>(xp[k] + size_t(c) * (PC * 64) + i * 64);
             digit_s[to][k] = sp[k][c];
           }
       };
@@ -775,39 +881,59 @@ __global__ void __launch_bounds__(kTileWaves* kWave, 2) w4_tile_kernel(Product p
         const int next = LOOK == 2 ? cur ^ 1 : 0;
         store_digits(c + 1, next);
         load_digits(c + 1 + LOOK, next);
-        Wide<FINE> wide[F];
+        std::conditional_t<HALF, Halves, Wide<FINE>> wide[F];
         float ws[F][B];
 #pragma unroll
         for (int f = 0; f < F; ++f) {
           w[cur][f].widen(wide[f]);
 #pragma unroll
-          for (int b = 0; b < B; ++b) ws[f][b] = w[cur][f].scale(b, c < c1);
+          for (int b = 0; b < B; ++b) ws[f][b] = HALF ? w[cur][f].plain_scale(b, c < c1) : w[cur][f].scale(b, c < c1);
         }
         load_codes(c + LOOK, cur);
+        v4u x[XB][PC];
+        auto read = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+          for (int i = 0; i < PC; ++i)
+            x[t % XB][i] = *reinterpret_cast<const v4u*>(&xt[c & 1][t][i][lane * 16]);
+        };
+        if (XB == 2) read(0);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          v4u x[2 * P];
-#pragma unroll
-          for (int i = 0; i < 2 * P; ++i)
-            x[i] = *reinterpret_cast<const v4u*>(&xt[c & 1][t][i][lane * 16]);
+          if (XB == 1) read(t);
+          else if (t + 1 < NT) read(t + 1);
           const float4 s4 = *reinterpret_cast<const float4*>(&xst[c & 1][16 * t + 4 * quad]);
           const float xs[4] = {s4.x, s4.y, s4.z, s4.w};
+          const v4u(&held)[PC] = x[t % XB];
 #pragma unroll
           for (int f = 0; f < F; ++f) {
             float value[4];
 #pragma unroll
             for (int b = 0; b < B; ++b) {
-              v4i sum[P];
+              float sum[4];
+              if constexpr (HALF) {
+                v4f u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int q = 0; q < P; ++q)
-                sum[q] = dot<FINE>(x[2 * q], x[2 * q + 1], wide[f], b);
+                for (int d = FINE ? b : 0; d < (FINE ? b + 1 : 4); ++d)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float v = P == 3 ? join(sum[0][i], sum[P / 2][i], sum[P - 1][i])
-                                       : float(sum[0][i]);
-                value[i] = b == 0 ? ws[f][b] * v : fmaf(ws[f][b], v, value[i]);
+                  for (int q = 0; q < P; ++q)
+                    u = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        __builtin_bit_cast(v8h, held[4 * q + d]),
+                        __builtin_bit_cast(v8h, wide[f].dword[d]), u, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = u[i];
+              } else {
+                v4i u[P];
+#pragma unroll
+                for (int q = 0; q < P; ++q)
+                  u[q] = dot<FINE>(held[2 * q], held[2 * q + 1], wide[f], b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  sum[i] = P == 3 ? join(u[0][i], u[P / 2][i], u[P - 1][i]) : float(u[0][i]);
               }
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                value[i] = b == 0 ? ws[f][b] * sum[i] : fmaf(ws[f][b], sum[i], value[i]);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[f][t][i] = fmaf(value[i], xs[i], acc[f][t][i]);
@@ -929,7 +1055,9 @@ int launch_w4_stage(hipStream_t s, const void* x, int x_dtype, const float* x_sc
                     size_t x_group, size_t R, size_t K, const W4Acts& a) {
   const Stage p{x, x_scales, x_group ? x_group : K, R, K, w4_chunks(K), w4_xs_stride(K), a};
   const unsigned grid = unsigned((R * p.C * 4 + 255) / 256);
-  if (x_dtype == INFERNO_F32) w4_stage_kernel<float, 3><<<grid, 256, 0, s>>>(p);
+  if (a.halves == 2) w4_stage_halves_kernel<float, 2><<<grid, 256, 0, s>>>(p);
+  else if (a.halves == 1) w4_stage_halves_kernel<uint16_t, 1><<<grid, 256, 0, s>>>(p);
+  else if (x_dtype == INFERNO_F32) w4_stage_kernel<float, 3><<<grid, 256, 0, s>>>(p);
   else if (x_dtype == INFERNO_BF16) w4_stage_kernel<uint16_t, 3><<<grid, 256, 0, s>>>(p);
   else w4_stage_kernel<int8_t, 1><<<grid, 256, 0, s>>>(p);
   INF_LAUNCHED();
@@ -972,6 +1100,16 @@ int launch_w4_pack(hipStream_t s, const W4Mat& m, const void* codes, const void*
   return INFERNO_OK;
 }
 
+bool w4_by_tiles(size_t T, size_t k, size_t experts) {
+  // Measured: the tile kernel's step costs the same for 1 to 16 tokens. One expert
+  // of 16 tokens: rows 12.3 and 21.5 (one and three planes), tiles 14.3 and 32.5
+  // us. Routed, where the tile kernel reads an expert's weights once for all its
+  // tokens: 64 experts of 3 tokens each rows 92, tiles 96 us, of 4 rows 104, tiles
+  // 96; 128 of 3 rows 268, tiles 277, of 5 rows 294, tiles 282, of 15 rows 509,
+  // tiles 380.
+  return k ? T * k / std::min(experts, T * k) > 3 : T > 16;
+}
+
 int launch_w4_product(hipStream_t s, const W4Product& q) {
   Product p{};
   for (int m = 0; m < q.mats; ++m) {
@@ -998,13 +1136,8 @@ int launch_w4_product(hipStream_t s, const W4Product& q) {
   const unsigned slots = q.offsets ? unsigned(std::min(q.m[0].experts, q.T * q.k)) : 1u;
   const size_t per_slot = q.T * (q.offsets ? q.k : 1) / slots;
   const bool one = q.x.P == 1;
-  // Measured: the tile kernel's step costs the same for 1 to 16 tokens. One expert
-  // of 16 tokens: rows 12.3 and 21.5 (one and three planes), tiles 14.3 and 32.5
-  // us. Routed, where the tile kernel reads an expert's weights once for all its
-  // tokens: 64 experts of 3 tokens each rows 92, tiles 96 us, of 4 rows 104, tiles
-  // 96; 128 of 3 rows 268, tiles 277, of 5 rows 294, tiles 282, of 15 rows 509,
-  // tiles 380.
-  if (per_slot > (q.offsets ? 3 : 16)) {
+  const bool tile = w4_by_tiles(q.T, q.offsets ? q.k : 0, q.m[0].experts);
+  if (tile) {
     // workgroups of a slot beyond its tokens end at once; a slot with more
     // tokens than they take goes round again
     const size_t blocks = q.offsets ? std::min<size_t>(2 * per_slot / kTileTokens + 1, 8)
@@ -1012,25 +1145,37 @@ int launch_w4_product(hipStream_t s, const W4Product& q) {
     by_format(q, [&](auto fine, auto mats, auto zeros, auto st) {
       constexpr int M = decltype(mats)::value, RT = M == 2 ? 1 : 2;
       using ST = decltype(st);
-      auto go = [&](auto planes, auto shares) {
+      auto go = [&](auto half, auto planes, auto shares) {
         constexpr int P = decltype(planes)::value, KS = decltype(shares)::value;
         constexpr unsigned tiles = RT * kTileWaves / KS;
-        const dim3 grid((p.row_tiles + tiles - 1) / tiles, slots,
+        const unsigned row_blocks = (p.row_tiles + tiles - 1) / tiles;
+        const dim3 grid(q.offsets ? row_blocks * 8 : row_blocks, (slots + 7) / 8,
                         unsigned(std::min<size_t>(blocks, 65535)));
-        w4_tile_kernel<fine.value, M, P, zeros.value, ST, RT, KS>
+        w4_tile_kernel<fine.value, M, half.value, P, zeros.value, ST, RT, KS>
             <<<grid, kTileWaves * kWave, 0, s>>>(p);
       };
       // shares of the chunks until there is a workgroup for every CU
       const size_t groups =
           (p.row_tiles + RT * kTileWaves - 1) / (RT * kTileWaves) * slots * blocks;
-      auto three = std::integral_constant<int, 3>{};
-      auto single = std::integral_constant<int, 1>{};
-      auto twice = std::integral_constant<int, 2>{};
-      if (one && groups < 128) go(single, std::integral_constant<int, 4>{});
-      else if (one && groups < 256) go(single, twice);
-      else if (one) go(single, single);
-      else if (groups < 256) go(three, twice);
-      else go(three, single);
+      const std::false_type digits;
+      const std::true_type halves;
+      const std::integral_constant<int, 1> one;
+      const std::integral_constant<int, 2> two;
+      const std::integral_constant<int, 4> four;
+      if (q.x.halves == 1) {
+        groups < 256 ? go(halves, one, two) : go(halves, one, one);
+      } else if (q.x.P == 3 || q.x.halves) {
+        if constexpr (fine.value) {
+          groups < 256 ? go(halves, two, two) : go(halves, two, one);
+        } else {
+          const std::integral_constant<int, 3> three;
+          groups < 256 ? go(digits, three, two) : go(digits, three, one);
+        }
+      } else if (groups < 128) {
+        go(digits, one, four);
+      } else {
+        groups < 256 ? go(digits, one, two) : go(digits, one, one);
+      }
     });
   } else {
     // Measured over 81 to 32768 row tiles (whole passes, rt / split): enough

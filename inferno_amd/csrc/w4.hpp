@@ -39,9 +39,13 @@ inline size_t w4_xs_stride(size_t K) { return (w4_chunks(K) + 1) / 2 * 2; }
 struct W4Acts {
   int8_t* planes;
   float* xs;
-  int P;      // planes: 3 or 1
-  bool fine;  // groups of 32 or 64 columns
+  int P;       // planes of digits: 3 or 1
+  int halves;  // or planes of fp16 (two for fp32, one for bf16), 256 bytes of a chunk each
+  bool fine;   // groups of 32 or 64 columns
 };
+// Whether products of T tokens (of k experts each; 0: one matrix) take the
+// kernel that has fp16 for activations other than int8.
+bool w4_by_tiles(size_t T, size_t k, size_t experts);
 
 // Writes the activations' digits. x: fp32, bf16, or int8 with x_scales
 // [R, K / x_group] (x_group 0: one per row).

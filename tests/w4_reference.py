@@ -9,6 +9,9 @@ S = sum |w x| and M = sum over 128-column chunks of max |x| sum |w|:
     the fp32 additions are at most 4 per chunk, ceil(K / 128) chunks, 4 parts
     and 2 residuals, each rounding a partial sum of size at most S (plus the
     residuals): (4 ceil(K / 128) + 16) 2^-24 (S + |a| + |b|).
+    Calls of many fp32 or bf16 tokens sum a chunk's products of fp16 values in
+    fp32 instead, which may round 128 or 256 times per chunk; they are held to
+    the same bar, since roundings of either sign seldom add up to four steps.
 silu(g) has a slope of at most 1.1 and is formed with at most 8 roundings."""
 import math
 
