@@ -16,7 +16,7 @@
 // again in 64 bits as a whole. 8192 tokens of 256 experts in 8 groups: 15.7 us;
 // whole rows in 64 bits for every failure 20.3, for every token 28 us. All 8192
 // wavefronts are resident at once: what bounds it is their instructions and, for
-// few tokens, one chain of cross-lane steps (29 tokens: 5 us).
+// few tokens, one chain of cross-lane steps (29 tokens: 6.5 us).
 #include "kernels.hpp"
 #include "routing_dev.hpp"
 
