@@ -206,8 +206,8 @@ int inferno_q8_0_matvec_add2(void* stream, const void* w, size_t w_bytes, const 
  * another:
  *   W[r, c] = scales[r, c / group] * (code[r, c] - zeros[r, c / group])
  * without zero points 8 in their place. cols is a multiple of 32 and of group;
- * group is 32, 64 or a multiple of 128; one matrix has less than 2^33 codes,
- * experts <= 256. The products read a packed form, which inferno_w4_pack writes
+ * group is 32, 64 or a multiple of 128; one matrix has less than 2^33 codes and
+ * at most 2^25 rows, experts <= 256. The products read a packed form, which inferno_w4_pack writes
  * once; it takes inferno_w4_packed_bytes at a multiple of 16 bytes. */
 typedef struct inferno_w4 {
   size_t experts; /* 1: a plain matrix */
@@ -241,6 +241,7 @@ int inferno_w4_pack(void* stream, const inferno_w4* w, const void* codes, size_t
  * it. The products of codes and activations are summed exactly within a group
  * for I8 and for few tokens; for more (above 16, or above 3 per expert) in fp32,
  * 128 columns at a time. A NaN or an infinity in x makes its token's outputs NaN.
+ * Calls that may overlap need a workspace (a multiple of 16 bytes) each.
  * T = 0 does nothing. */
 
 /* Workspace bytes of the two dense products over T tokens of `cols` columns. */

@@ -26,7 +26,8 @@ W4Mat mat(const inferno_w4* w) {
 int check_shape(const char* what, const inferno_w4* w) {
   INF_CHECK_ARG(w != nullptr, "null 4-bit matrix");
   const size_t most = size_t(1) << 31;
-  if (w->experts == 0 || w->rows == 0 || w->cols == 0 || w->rows >= most || w->cols >= most ||
+  if (w->experts == 0 || w->rows == 0 || w->cols == 0 || w->cols >= most ||
+      w->rows > (size_t(1) << 25) ||  // a launch has less than 2^32 threads
       w->experts > size_t(kMaxExperts) || w->rows * w->cols >= 4 * most) {
     set_error(std::string("4-bit ") + what + " matrix: sizes out of range, experts=" +
               std::to_string(w->experts) + ", rows=" + std::to_string(w->rows) + ", cols=" +

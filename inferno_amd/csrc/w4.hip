@@ -227,12 +227,10 @@ struct Pack {
   bool fine;
 };
 
-// One wavefront per tile and chunk. Rows behind N and columns behind K get the
+// One tile's chunk, by one wavefront. Rows behind N and columns behind K get the
 // code, the scale and the zero point that count nothing.
 template <typename ST>
-__global__ void __launch_bounds__(256) w4_pack_kernel(Pack p) {
-  const size_t tc = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (tc >= size_t(p.tiles) * p.C) return;
+__device__ __forceinline__ void pack_chunk(const Pack& p, size_t tc) {
   const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
   const uint32_t tile = uint32_t(tc / p.C), c = uint32_t(tc % p.C);
   const uint32_t row = tile % p.row_tiles * 16 + n;
@@ -258,6 +256,13 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(Pack p) {
   const ST s = static_cast<const ST*>(p.scales)[from];
   reinterpret_cast<ST*>(p.to + p.scales_at)[at] = in ? s : ST(0);
   if (p.zeros) p.to[p.zeros_at + at] = in ? uint8_t(min(uint32_t(p.zeros[from]), 127u)) : 0;
+}
+
+template <typename ST>
+__global__ void __launch_bounds__(256) w4_pack_kernel(Pack p) {
+  for (size_t tc = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6); tc < size_t(p.tiles) * p.C;
+       tc += size_t(gridDim.x) * 4)
+    pack_chunk<ST>(p, tc);
 }
 
 // ----------------------------------------------------------------- product
@@ -1093,7 +1098,7 @@ int launch_w4_pack(hipStream_t s, const W4Mat& m, const void* codes, const void*
   p.group = uint32_t(m.group);
   p.groups = uint32_t(m.cols / m.group);
   p.fine = m.fine();
-  const unsigned grid = unsigned((size_t(p.tiles) * p.C + 3) / 4);
+  const unsigned grid = unsigned(std::min((size_t(p.tiles) * p.C + 3) / 4, size_t(1) << 22));
   if (m.scale_dtype == INFERNO_BF16) w4_pack_kernel<uint16_t><<<grid, 256, 0, s>>>(p);
   else w4_pack_kernel<float><<<grid, 256, 0, s>>>(p);
   INF_LAUNCHED();

@@ -349,7 +349,7 @@ def _desc(experts=1, rows=16, cols=64, group=32, p=16, **more):
 BAD_SIZES = [dict(rows=0), dict(cols=0), dict(experts=0), dict(group=0), dict(group=48),
              dict(group=128), dict(group=96, cols=96), dict(cols=48, group=16),
              dict(scale_dtype=2), dict(experts=257), dict(rows=1 << 20, cols=1 << 13, group=128),
-             dict(rows=1 << 31), dict(cols=1 << 31)]
+             dict(rows=1 << 31), dict(cols=1 << 31), dict(rows=(1 << 25) + 1)]
 
 
 def test_packed_bytes():
