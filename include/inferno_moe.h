@@ -207,8 +207,9 @@ int inferno_q8_0_matvec_add2(void* stream, const void* w, size_t w_bytes, const 
  *   W[r, c] = scales[r, c / group] * (code[r, c] - zeros[r, c / group])
  * without zero points 8 in their place. cols is a multiple of 32 and of group;
  * group is 32, 64 or a multiple of 128; one matrix has less than 2^33 codes and
- * at most 2^25 rows, experts <= 256. The products read a packed form, which inferno_w4_pack writes
- * once; it takes inferno_w4_packed_bytes at a multiple of 16 bytes. */
+ * at most 2^25 rows, experts <= 256. The products read a packed form, which
+ * inferno_w4_pack writes once; it takes inferno_w4_packed_bytes at a multiple of
+ * 16 bytes. */
 typedef struct inferno_w4 {
   size_t experts; /* 1: a plain matrix */
   size_t rows, cols, group;
@@ -239,8 +240,8 @@ int inferno_w4_pack(void* stream, const inferno_w4* w, const void* codes, size_t
  * and x_group are not read for F32 and BF16. bf16 activations enter whole (down
  * to 2^-14 of the largest of their 128 columns), fp32 ones rounded to 2^-23 of
  * it. The products of codes and activations are summed exactly within a group
- * for I8 and for few tokens; for more (above 16, or above 3 per expert) in fp32,
- * 128 columns at a time. A NaN or an infinity in x makes its token's outputs NaN.
+ * (of at most 128 columns); those of more than 16 tokens, or 3 per expert, in fp32
+ * if they are BF16, or F32 with a group of 32 or 64. A NaN or an infinity in x makes its token's outputs NaN.
  * Calls that may overlap need a workspace (a multiple of 16 bytes) each.
  * T = 0 does nothing. */
 
