@@ -29,10 +29,11 @@ inline size_t w4_chunks(size_t K) { return (K + kW4Chunk - 1) / kW4Chunk; }
 int launch_w4_pack(hipStream_t s, const W4Mat& m, const void* codes, const void* scales,
                    const void* zeros, void* packed);
 
-// Activations as int8 digits, the operands of the integer matrix cores.
+// Activations as operands of the matrix cores: int8 digits, or fp16 (halves).
 // A value of a 128-column chunk is (65536 d0 + 256 d1 + d2) xs (3 planes; d in
-// [-128, 127]), or d0 xs (1 plane, int8 activations).
-//   planes [rows][chunks][planes][128]: the digits of one chunk in the order
+// [-128, 127]), or d0 xs (1 plane, int8 activations); with halves the sum of its
+// planes' fp16 values times xs.
+//   planes [rows][chunks][planes][128 or 256 bytes]: one chunk in the order
 //     in which the lanes of the weights' tile hold its columns;
 //   xs [rows][chunks, to a multiple of 2 with 0].
 inline size_t w4_xs_stride(size_t K) { return (w4_chunks(K) + 1) / 2 * 2; }
