@@ -252,6 +252,9 @@ __device__ __forceinline__ bool fast_row(const GroupTopk& p, size_t t, Scratch& 
     }
     const bool two = p.rule == INFERNO_GROUP_TOP2 && p.size > 1;
     const float gv = two ? a + b : a;
+    // +infinity and -infinity: a NaN, which counts as the best group but compares as
+    // none
+    if (__any(gv != gv)) return false;
     int before = 0;
     float next = -INFINITY;  // the largest value at or below this group's, of another
     for (int o = 0; o < p.groups; ++o) {

@@ -169,6 +169,40 @@ def test_one_group_is_the_plain_top_k(cuda, score_fn):
     assert torch.allclose(a[1], b[1], rtol=32 * 2.0 ** -24, atol=0)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("score_fn", [SCORE_SIGMOID, SCORE_SOFTMAX])
+def test_groups_of_both_infinities(cuda, score_fn):
+    # the two largest values of a group are +infinity and -infinity: their sum is
+    # a NaN, which lies above every other group and does not open one more
+    inf = float("inf")
+
+    def route(v, k, n_group, kept):
+        # as logits, or as biases of equal scores
+        l, b = (v, None) if score_fn == SCORE_SOFTMAX else (torch.zeros_like(v), v[0].to(cuda))
+        ids, _, _ = ops.router_group_topk(l.to(cuda), b, k, score_fn, True, 1.0, n_group, kept,
+                                          GROUP_TOP2)
+        return ids.view(-1, k).tolist()
+
+    v = torch.tensor([[3.0, 2.0, inf, -inf, 2.9, 0.1, 0.5, 0.5]])
+    assert route(v, 3, 4, 2) == [[2, 0, 1]]
+    assert route(v, 2, 4, 1) == [[2, 3]]
+    g = torch.Generator().manual_seed(11)
+    for n_group in (16, 8):  # groups of 2, and of 4 with one value and -infinity
+        for _ in range(20):
+            v = torch.randn(1, 32, generator=g)
+            of = v.view(n_group, -1)
+            bad = int(torch.randint(0, n_group, (1,), generator=g))
+            of[bad] = -inf
+            of[bad, 0] = inf
+            best = of.topk(2, 1).values.double().sum(1)
+            best[bad] = inf
+            size = 32 // n_group
+            kept = torch.sort(best, descending=True, stable=True).indices[:3].tolist()
+            live = [e for e in range(32) if e // size in kept]
+            want = sorted(live, key=lambda e: (-v[0, e].item(), e))[:4]
+            assert route(v, 4, n_group, 3) == [want]
+
+
 def test_refusals():
     logits = torch.zeros(2, 32)
     ok = dict(bias=None, k=4, score_fn=0, norm=True, scale=1.0, n_group=4, topk_group=2,
