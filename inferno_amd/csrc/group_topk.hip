@@ -67,6 +67,13 @@ __device__ __forceinline__ float weight_of(const GroupTopk& p, float score, floa
   return (divide ? score / sum : score) * p.scale;
 }
 
+// What the winners' logits are taken relative to: normalised weights are ratios of
+// their scores alone, which vanish together if the row's largest logit is in a
+// closed group and more than 87 above them. top: the winners' largest logit.
+__device__ __forceinline__ float weights_from(const GroupTopk& p, float lmax, float top) {
+  return p.norm && fabsf(lmax) < INFINITY && top > -INFINITY ? top : lmax;
+}
+
 __device__ __forceinline__ void exact_row(const GroupTopk& p, size_t t, Scratch& scratch) {
   constexpr int kPer = kMaxExperts / kWave;
   const int lane = threadIdx.x & 63;
@@ -129,7 +136,7 @@ __device__ __forceinline__ void exact_row(const GroupTopk& p, size_t t, Scratch&
     live[j] = before < p.topk_group;
     key[j] = order_key(value[e]);
   }
-  float sum = 0.f, mine_w = 0.f;
+  float sum = 0.f, mine_w = 0.f, mine_l = -INFINITY;
   uint32_t mine_id = 0;
   for (int r = 0; r < p.k; ++r) {
     uint64_t best = 0;
@@ -149,19 +156,30 @@ __device__ __forceinline__ void exact_row(const GroupTopk& p, size_t t, Scratch&
       best = take ? ob : best;
       id = take ? oi : id;
     }
-    float s = 0.f;
+    float s = 0.f, l = 0.f;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       if (id == lane + j * kWave) {
         s = score[j];
+        l = lg[j];
         live[j] = false;
       }
     }
     s = __shfl(s, id & 63, kWave);
+    l = __shfl(l, id & 63, kWave);
     sum += s;  // rank order
     if (lane == r) {
       mine_w = s;
+      mine_l = l;
       mine_id = uint32_t(id);
+    }
+  }
+  if (p.score_fn == INFERNO_SCORE_SOFTMAX && !__any(mine_l != mine_l)) {
+    const float from = weights_from(p, lmax, wave_max(mine_l));
+    if (from != lmax) {  // uniform
+      mine_w = expf(mine_l - from);
+      sum = 0.f;
+      for (int r = 0; r < p.k; ++r) sum += __shfl(mine_w, r, kWave);  // rank order
     }
   }
   if (lane < p.k) {
@@ -361,7 +379,12 @@ __device__ __forceinline__ bool fast_row(const GroupTopk& p, size_t t, Scratch& 
     if (uint32_t(lane) >= many) rank = uint32_t(p.k);
   }
   const bool won = rank < uint32_t(p.k);
-  const float my_score = sigmoid ? 1.f / (1.f + expf(-row[id])) : expf(row[id] - lmax);
+  const float l = row[id];
+  if (!sigmoid && p.norm) {
+    const uint32_t top = wave_umax(won ? total_order_key(l) : 0u);
+    lmax = weights_from(p, lmax, bits_to_f32((top >> 31) ? top ^ 0x80000000u : ~top));
+  }
+  const float my_score = sigmoid ? 1.f / (1.f + expf(-l)) : expf(l - lmax);
   float sum = 0.f;
   if (p.norm) {
     if (won) s.by_rank[rank] = my_score;

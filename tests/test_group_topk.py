@@ -203,6 +203,45 @@ def test_groups_of_both_infinities(cuda, score_fn):
             assert route(v, 4, n_group, 3) == [want]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [20.0, 86.0, 95.0, 104.0, 1e4, 3e38])
+def test_weights_far_below_the_closed_groups(cuda, gap):
+    # the row's largest logit is in a closed group: the winners' softmax scores
+    # vanish in fp32, their normalised weights do not. Sums of two in 32 bits
+    # decide the second half's groups, ties send the first half's to 64 bits.
+    # Bar: two exponentials whose arguments are at most 3 (rounded to 3 2^-24,
+    # two roundings more), four additions, a quotient and the scale
+    g = torch.Generator().manual_seed(2)
+    l = torch.rand(20, 16, generator=g) * 3.0
+    l[:10, 5] = l[:10, 4]
+    l[:10, 8:10] = l[:10, 4:6]
+    l[:, 2], l[:, 3] = gap, -gap
+    ids, w, _ = ops.router_group_topk(l.to(cuda), None, 4, SCORE_SOFTMAX, True, 2.5, 8, 4,
+                                      GROUP_TOP2)
+    want, _ = _definition(l.numpy(), None, 4, SCORE_SOFTMAX, False, 2.5, 8, 4, GROUP_TOP2)
+    assert np.array_equal(ids.view(20, 4).cpu().numpy(), want) and (want // 2 != 1).all()
+    e = torch.exp(l.double().gather(1, torch.from_numpy(want)))
+    e = 2.5 * e / e.sum(1, keepdim=True)
+    assert ((w.view(20, 4).cpu().double() - e).abs() <= (2 * (3 + 2) + 4 + 2) * 2.0 ** -24 * e).all()
+
+
+@pytest.mark.gpu
+def test_weights_of_closed_and_infinite_logits(cuda):
+    # winners of -infinity alone, below a finite or an infinite closed logit
+    inf = float("inf")
+    l = torch.full((3, 8), -inf)
+    l[0, 0], l[1, 0], l[2, 0] = 5.0, inf, 5.0
+    l[2, 6] = 1.0
+    bias = torch.zeros(8)
+    bias[0] = -100.0
+    ids, w, _ = ops.router_group_topk(l[:, 2:].contiguous().to(cuda), None, 2, SCORE_SOFTMAX, True,
+                                      1.0, 3, 1, GROUP_MAX)
+    assert not w.view(3, 2)[:2].any() and w.view(3, 2)[2].tolist() == [1.0, 0.0]
+    ids, w, _ = ops.router_group_topk(l.to(cuda), bias.to(cuda), 1, SCORE_SOFTMAX, True, 1.0, 4, 1,
+                                      GROUP_MAX)
+    assert ids.tolist()[2] == 6 and w.tolist()[2] == 1.0
+
+
 def test_refusals():
     logits = torch.zeros(2, 32)
     ok = dict(bias=None, k=4, score_fn=0, norm=True, scale=1.0, n_group=4, topk_group=2,
