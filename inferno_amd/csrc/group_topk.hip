@@ -8,9 +8,10 @@
 // other round to one or change places.
 //
 // Values are first formed in 32 bits. They decide wherever the values that they
-// order are further apart than their roundings, which is checked for the last
-// open group against the first closed one, for the last winner against the
-// best loser and for neighbouring winners. Where winners fail, the experts that
+// order are further apart than their roundings, which is checked for every open
+// group against every closed one (a sum of two rounds by their magnitudes, which
+// it may be far below), for the last winner against the best loser and for
+// neighbouring winners. Where winners fail, the experts that
 // may be among the k best (one per lane) are formed and ranked in 64 bits; a
 // token whose groups fail, with more of them than lanes, or with a NaN is done
 // again in 64 bits as a whole. 8192 tokens of 256 experts in 8 groups: 15.7 us;
@@ -228,7 +229,10 @@ __device__ __forceinline__ bool fast_row(const GroupTopk& p, size_t t, Scratch& 
   bool nan = false;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    nan |= lg[j] + bs[j] != lg[j] + bs[j];  // +-infinity with the other as bias too
+    const float both = lg[j] + bs[j];
+    nan |= both != both;  // +-infinity with the other as bias too
+    // a sum behind fp32's range, so that infinite values below are infinite ones
+    nan |= fabsf(both) == INFINITY && fmaxf(fabsf(lg[j]), fabsf(bs[j])) < INFINITY;
     lmax = fmaxf(lmax, lg[j]);
   }
   if (__any(nan)) return false;
@@ -274,16 +278,23 @@ __device__ __forceinline__ bool fast_row(const GroupTopk& p, size_t t, Scratch& 
     // none
     if (__any(gv != gv)) return false;
     int before = 0;
-    float next = -INFINITY;  // the largest value at or below this group's, of another
     for (int o = 0; o < p.groups; ++o) {
       const float x = lane_of(gv, o * L);
       before += x > gv || (x == gv && o < g);
-      if (x < gv || (x == gv && o > g)) next = fmaxf(next, x);
     }
-    const bool mine = g < p.groups && sub == 0;
-    open = __ballot(mine && before < p.topk_group);
-    const bool last = mine && before == p.topk_group - 1;
-    if (__any(last && !above(gv, next, sigmoid, two ? 2.f : 1.f))) return false;
+    const bool mine = g < p.groups && sub == 0, in = before < p.topk_group;
+    open = __ballot(mine && in);
+    // How far gv may be off: each summand by 2^-24 of itself (and a sigmoid by
+    // 2^-22), their sum by 2^-24 of it, which is less than of both magnitudes; twice
+    // that, so that the roundings of these two borders are in it. An infinite value
+    // is one in 64 bits too.
+    const float size = two ? fabsf(a) + fabsf(b) : fabsf(a);
+    const bool infinite = fabsf(a) == INFINITY || (two && fabsf(b) == INFINITY);
+    const float off =
+        infinite ? 0.f : size * 0x1p-22f + (sigmoid ? (two ? 0x1p-20f : 0x1p-21f) : 0.f);
+    if (__any(mine && off == INFINITY)) return false;  // a sum behind fp32's range
+    const uint32_t lowest = ~wave_umax(mine && in ? ~total_order_key(gv - off) : 0u);
+    if (lowest <= wave_umax(mine && !in ? total_order_key(gv + off) : 0u)) return false;
   }
   uint32_t key[PER];
 #pragma unroll

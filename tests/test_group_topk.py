@@ -242,6 +242,70 @@ def test_weights_of_closed_and_infinite_logits(cuda):
     assert ids.tolist()[2] == 6 and w.tolist()[2] == 1.0
 
 
+def _check_ids(logits, bias, k, score_fn, n_group, topk_group, rule):
+    ids, _, _ = ops.router_group_topk(logits, bias, k, score_fn, True, 1.0, n_group, topk_group,
+                                      rule)
+    want, _ = _definition(logits.cpu().numpy(), bias.cpu().numpy(), k, score_fn, True, 1.0, n_group,
+                          topk_group, rule)
+    got = ids.view(-1, k).cpu().numpy()
+    assert np.array_equal(got, want), np.nonzero((got != want).any(1))[0][:5]
+    return got
+
+
+@pytest.mark.gpu
+def test_sums_of_two_that_nearly_cancel(cuda):
+    # logit + bias rounds relative to itself, which may be far more than the sum of
+    # a group's two largest values; the order has to be that of 64 bits
+    for l, b, best in (([1.7361599206924438, -1.7361599206924438, 17.175823211669922,
+                         -17.175823211669922], [0.07883994281292, -0.07883810251951,
+                                                -0.17062471807003, 0.17062482237816], 0),
+                       ([1000.0, -1000.0, 1.0, -0.99999], [1.5e-5, 0.0, 0.0, 0.0], 0)):
+        l, b = torch.tensor([l]).to(cuda), torch.tensor(b).to(cuda)
+        assert _check_ids(l, b, 2, SCORE_SOFTMAX, 2, 1, GROUP_TOP2).min() // 2 == best
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score_fn", [SCORE_SIGMOID, SCORE_SOFTMAX])
+@pytest.mark.parametrize("size", [2, 3, 8])
+@pytest.mark.parametrize("far", [1.0, 60.0, 1e4, 1e30])
+def test_many_sums_of_two_that_nearly_cancel(cuda, score_fn, size, far):
+    # groups of a value, nearly its negative, and for larger groups values far
+    # below both; their sums lie within a few roundings of each other
+    g = torch.Generator().manual_seed(int(size * 1000 + min(far, 1e6)))
+    T, groups = 60, 12
+    E = groups * size
+    big = far * (0.05 + torch.rand(groups, generator=g))
+    l = torch.randn(T, groups, size, generator=g)
+    bias = torch.full((groups, size), -4.0 * far)
+    if score_fn == SCORE_SIGMOID:  # the magnitudes are in the biases
+        bias[:, 0], bias[:, 1] = big, -big
+        bias[:, 1] -= 2.0 ** -24 * torch.randn(groups, generator=g) * far
+    else:
+        bias[:, 0] = 2.0 ** -20 * torch.randn(groups, generator=g) * far
+        bias[:, 1] = 2.0 ** -20 * torch.randn(groups, generator=g) * far
+        scale = big * (0.5 + torch.rand(T, groups, generator=g))
+        l[:, :, 0], l[:, :, 1] = scale, -scale
+    l, bias = l.view(T, E), bias.view(E)
+    for kept in (1, 4, 11):
+        _check_ids(l.to(cuda), bias.to(cuda), min(kept * size, 5), score_fn, groups, kept,
+                   GROUP_TOP2)
+
+
+@pytest.mark.gpu
+def test_group_values_behind_the_range(cuda):
+    # values and sums of two that leave fp32's range, next to true infinities
+    inf, big = float("inf"), 3e38
+    l = torch.tensor([[big, big, big, 2.5e38, -big, big, 1.0, -inf],
+                      [-big, -big, -inf, -inf, -big, -2e38, -big, big],
+                      [big, -big, 2e38, -big, -inf, big, -inf, 2.9e38],
+                      [-inf, -inf, -inf, -inf, 1.0, -inf, 2.0, -inf]])
+    for b in (torch.zeros(8), torch.tensor([big, 2e38, big, big, -big, -big, 0.0, 0.0]),
+              torch.tensor([-big, -big, big, -big, 1e38, -big, 1e38, 0.0])):
+        for kept in (1, 2, 3):
+            for rule in (GROUP_MAX, GROUP_TOP2):
+                _check_ids(l.to(cuda), b.to(cuda), 2, SCORE_SOFTMAX, 4, kept, rule)
+
+
 def test_refusals():
     logits = torch.zeros(2, 32)
     ok = dict(bias=None, k=4, score_fn=0, norm=True, scale=1.0, n_group=4, topk_group=2,
