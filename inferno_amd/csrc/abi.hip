@@ -273,7 +273,8 @@ int inferno_moe_router_group_topk(void* stream, const float* logits, const float
   INF_CHECK_ARG(group_score == INFERNO_GROUP_MAX || group_score == INFERNO_GROUP_TOP2,
                 "group_score must be GROUP_MAX or GROUP_TOP2");
   INF_CHECK_ARG(std::isfinite(routed_scaling_factor), "routed scaling factor must be finite");
-  INF_CHECK_ARG(T < (size_t(1) << 26), "too many tokens");
+  // a launch has less than 2^32 threads, four tokens take 256
+  INF_CHECK_ARG(T <= (size_t(1) << 26) - 4, "too many tokens");
   if (T == 0) return INFERNO_OK;
   INF_CHECK_ARG(logits && expert_ids && expert_weights, "null pointer");
   if (int st_ = require_device()) return st_;

@@ -331,3 +331,11 @@ def test_refusals():
         assert status(**bad) == -1, bad
     assert b"exceeds the 8 experts" in lib().inferno_last_error()
     assert status(T=0, p=None) == 0
+
+
+def test_refuses_more_tokens_than_a_launch_takes():
+    # four tokens a workgroup of 256 threads: 2^24 workgroups are 2^32 threads
+    f = lib().inferno_moe_router_group_topk
+    for T in ((1 << 26) - 3, (1 << 26) - 1, 1 << 40):
+        assert f(None, 16, None, T, 1, 1, 0, 1, 1.0, 1, 1, 0, 16, 16, None) == -1, T
+        assert b"too many tokens" in lib().inferno_last_error()
