@@ -6,7 +6,8 @@
 // The root cancels in q, so q is the quotient of two products of two fp32
 // values each, exact in 64 bits: q does not depend on how the squares are
 // summed, and is the same in every kernel. The squares are summed in 64 bits:
-// those of fp32 values pass fp32's range from 2^64 on.
+// those of fp32 values pass fp32's range from 2^64 on. A row of zeros has y = 0
+// and scale = 0 also with eps = 0, where the root is 0.
 #include <type_traits>
 
 #include "kernels.hpp"
@@ -40,6 +41,12 @@ __device__ __forceinline__ bool sound(uint32_t a) { return a - (27u << 23) <= (2
 __device__ __forceinline__ float group_scale(double largest, double inv) {
   const float f = float(largest);
   return float((sound(f32_to_bits(f)) ? double(f) : largest) * inv / 127.0);
+}
+
+// 1 / sqrt(mean(s^2) + eps) from the sum of squares; 0 for a row of zeros.
+__device__ __forceinline__ double inverse_root(double sq, double H, float eps) {
+  const double mean = sq / H + double(eps);
+  return mean == 0.0 ? 0.0 : 1.0 / sqrt(mean);
 }
 
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
@@ -79,7 +86,7 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   sq = 0.0;
   for (int i = 0; i < kThreads / kWave; ++i) sq += part[i];
-  const double inv = 1.0 / sqrt(sq / double(H) + double(eps));
+  const double inv = inverse_root(sq, double(H), eps);
   const float f = float(inv);
   if (normed)
     for (size_t i = tid; i < H; i += kThreads) store_act(normed + at + i, total(i) * f * w[i]);
@@ -213,7 +220,7 @@ __global__ void __launch_bounds__(kThreads)
   sq = part[0];
 #pragma unroll
   for (int i = 1; i < kWaves; ++i) sq += part[i];
-  const double inv = 1.0 / sqrt(sq / double(H) + double(eps));
+  const double inv = inverse_root(sq, double(H), eps);
   if (normed) {
     const float f = float(inv);
 #pragma unroll

@@ -112,6 +112,18 @@ def test_rows_of_zeros_and_not_finite(cuda, H, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,group", [(512, 0), (512, 64), (515, 0), (16384, 128)])
+def test_rows_of_zeros_without_eps(cuda, H, group):
+    x, r, w = _inputs(4, H, torch.float32, seed=6)
+    x[1], r[1] = 0.0, -0.0
+    x[2, :] = -r[2]  # a sum of zeros
+    s, y, q, sc = ops.add_rms_norm_q8(x, r, w, 0.0, group=group)
+    for t in (1, 2):
+        assert not s[t].any() and not y[t].any() and not q[t].any() and not sc[t].any()
+    _check(x[[0, 3]], r[[0, 3]], w, group, torch.float32, eps=0.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,group", [(2048, 128), (515, 0), (40000, 0)])
 def test_the_sum_in_place(cuda, H, group):
     x, r, w = _inputs(3, H, torch.float32, seed=7)
