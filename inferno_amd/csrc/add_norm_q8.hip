@@ -49,6 +49,14 @@ __device__ __forceinline__ double inverse_root(double sq, double H, float eps) {
   return mean == 0.0 ? 0.0 : 1.0 / sqrt(mean);
 }
 
+// s / sqrt(..) in 32 bits; in 64 where the factor is no normal fp32 value: with eps =
+// 0 rows below 2^-127 have one that passes fp32's range, rows from 2^126 on one that
+// fp32 holds in fewer bits. (the same for a row)
+__device__ __forceinline__ bool factor_fits(double inv) { return inv < 0x1p127 && inv > 0x1p-126; }
+__device__ __forceinline__ float scaled(float s, double inv, bool fits) {
+  return fits ? s * float(inv) : float(double(s) * inv);
+}
+
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) {
@@ -87,9 +95,10 @@ __global__ void __launch_bounds__(kThreads)
   sq = 0.0;
   for (int i = 0; i < kThreads / kWave; ++i) sq += part[i];
   const double inv = inverse_root(sq, double(H), eps);
-  const float f = float(inv);
+  const bool fits = factor_fits(inv);
   if (normed)
-    for (size_t i = tid; i < H; i += kThreads) store_act(normed + at + i, total(i) * f * w[i]);
+    for (size_t i = tid; i < H; i += kThreads)
+      store_act(normed + at + i, scaled(total(i), inv, fits) * w[i]);
   if (!q) return;
   if (group == 0) {
     uint64_t a = 0;
@@ -222,13 +231,13 @@ __global__ void __launch_bounds__(kThreads)
   for (int i = 1; i < kWaves; ++i) sq += part[i];
   const double inv = inverse_root(sq, double(H), eps);
   if (normed) {
-    const float f = float(inv);
+    const bool fits = factor_fits(inv);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const uint32_t i = uint32_t(j * kThreads + tid) * 4;
       float y[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = v[j][e] * f * g[j][e];
+      for (int e = 0; e < 4; ++e) y[e] = scaled(v[j][e], inv, fits) * g[j][e];
       if (i < H) store4(normed + at + i, y);
     }
   }

@@ -124,6 +124,19 @@ def test_rows_of_zeros_without_eps(cuda, H, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,group", [(512, 0), (512, 64), (515, 0), (16384, 128)])
+@pytest.mark.parametrize("size", [1e-44, 1e-42, 1e-40, 1e-38, 1e37, 9e37])
+def test_rows_whose_factor_leaves_the_range(cuda, H, group, size):
+    # 1 / sqrt(mean(s^2)) beyond fp32's largest value, or below its normal ones
+    g = torch.Generator(device="cuda").manual_seed(H)
+    x = size * (1.0 + torch.rand(3, H, generator=g, device="cuda"))
+    w = 1.0 + 0.2 * torch.randn(H, generator=g, device="cuda")
+    for act in (torch.float32, torch.bfloat16):
+        _check(x, None, w, group, act, eps=0.0)
+        _check(x, torch.full_like(x, -0.5 * size), w, group, act, eps=0.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,group", [(2048, 128), (515, 0), (40000, 0)])
 def test_the_sum_in_place(cuda, H, group):
     x, r, w = _inputs(3, H, torch.float32, seed=7)
