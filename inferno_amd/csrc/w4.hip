@@ -20,6 +20,7 @@
 // of a tile's chunk together in the lanes' order. Any order of the columns
 // inside a group gives the same sum, so no code moves inside its bytes, and the
 // digits are laid out to match.
+#include <atomic>
 #include <type_traits>
 
 #include "w4.hpp"
@@ -1214,12 +1215,32 @@ int launch_w4_product(hipStream_t s, const W4Product& q) {
   return INFERNO_OK;
 }
 
+// LDS of a launch of the token kernel: three workgroups of four wavefronts per CU,
+// or two of sixteen (sums).
+constexpr size_t kTokenLds = 53 * 1024, kTokenSumLds = 80 * 1024;
+
 bool w4_token_fits(const W4Token& q) {
   const size_t rows = q.sum ? q.segments : q.T;
-  // three workgroups of four wavefronts per CU, or two of sixteen
   return q.T <= 4 && q.segments <= kWave && rows * w4_chunks(q.m[0].cols) < 4096 &&
-         token_lds(rows, w4_chunks(q.m[0].cols), q.mats, 16) <= size_t(q.sum ? 80 : 53) * 1024;
+         token_lds(rows, w4_chunks(q.m[0].cols), q.mats, 16) <= (q.sum ? kTokenSumLds : kTokenLds);
 }
+
+namespace {
+
+// Raises a kernel's dynamic LDS limit (64 KB by default), once per device.
+template <typename K>
+int allow_lds(K kern, size_t bytes, std::atomic<uint64_t>& devices) {
+  int dev = 0;
+  INF_HIP(hipGetDevice(&dev));
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (devices.load() & bit) return INFERNO_OK;
+  INF_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+  devices.fetch_or(bit);
+  return INFERNO_OK;
+}
+
+}  // namespace
 
 int launch_w4_token(hipStream_t s, const W4Token& q) {
   Tokens a{};
@@ -1247,14 +1268,20 @@ int launch_w4_token(hipStream_t s, const W4Token& q) {
   W4Product f{};
   f.m[0] = q.m[0];
   f.mats = q.mats;
+  int status = INFERNO_OK;
   by_format(f, [&](auto fine, auto mats, auto zeros, auto st) {
     using ST = decltype(st);
     constexpr int M = decltype(mats)::value;
     auto go = [&](auto x, auto waves) {
       constexpr int W = decltype(waves)::value;
       const size_t rows = q.sum ? q.segments : q.T;
-      w4_token_kernel<fine.value, M, zeros.value, ST, decltype(x), W>
-          <<<grid, W * kWave, token_lds(rows, a.p.C, M, W), s>>>(a);
+      const size_t lds = token_lds(rows, a.p.C, M, W);
+      auto kern = w4_token_kernel<fine.value, M, zeros.value, ST, decltype(x), W>;
+      if constexpr (W == 16) {
+        static std::atomic<uint64_t> raised{0};
+        if (lds > 64 * 1024 && (status = allow_lds(kern, kTokenSumLds, raised))) return;
+      }
+      kern<<<grid, W * kWave, lds, s>>>(a);
     };
     if constexpr (M == 1) {
       if (q.sum) return go(0.f, std::integral_constant<int, 16>{});
@@ -1262,6 +1289,7 @@ int launch_w4_token(hipStream_t s, const W4Token& q) {
     if (bf16) go(uint16_t{}, std::integral_constant<int, 4>{});
     else go(0.f, std::integral_constant<int, 4>{});
   });
+  if (status) return status;
   INF_LAUNCHED();
   return INFERNO_OK;
 }

@@ -228,3 +228,32 @@ def test_many_tokens(cuda):
     d = [[ref.dense(v[0][e], v[1][e]) for e in range(2)] for v in mats]
     want, bar = ref.moe(*d, ref.values(x), ids, wt, 1)
     assert ((got.cpu().double() - want).abs() <= bar).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,k,I,group", [
+    # k rows of I digits in one workgroup's memory: 62312 bytes, 66192 twice (past the
+    # default limit of 65536), 78608, 80936 of the 81920 that it may take, then more
+    (12, 10, 1920, 128), (12, 10, 2016, 32), (12, 10, 2048, 128), (16, 16, 1536, 64),
+    (20, 11, 2304, 128), (20, 16, 1664, 32)])
+@pytest.mark.parametrize("dtype,zeros", [(BF16, False), (F32, True)])
+def test_one_token_of_large_sums(cuda, E, k, I, group, dtype, zeros):
+    g = torch.Generator().manual_seed(I + k)
+    H = 160 if group == 32 else 256
+    mats = [ref.make(g, I, H, group, E, zeros), ref.make(g, I, H, group, E, zeros),
+            ref.make(g, H, I, group, E, zeros, scales=F32 if zeros else BF16)]
+    x = torch.randn(1, H, generator=g).to(dtype).cuda()
+    ids = torch.randperm(E, generator=g)[:k].int().cuda()
+    w = torch.rand(k, generator=g).cuda()
+    handles = [ops.W4(*m) for m in mats]
+    got = ops.w4_moe(*handles, x, ids, w, k)
+    d = [[ref.dense(*(None if v is None else v[e] for v in m)) for e in range(E)] for m in mats]
+    want, bar = ref.moe(*d, ref.values(x), ids, w, k)
+    assert ((got.cpu().double() - want).abs() <= bar).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = ops.w4_moe(*handles, x, ids, w, k)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, ops.w4_moe(*handles, x, ids, w, k))
