@@ -239,7 +239,7 @@ int inferno_w4_pack(void* stream, const inferno_w4* w, const void* codes, size_t
  * inferno_add_rms_norm_q8 writes). x lies at a multiple of 16 bytes; x_scales
  * and x_group are not read for F32 and BF16. bf16 activations enter whole (down
  * to 2^-14 of the largest of their 128 columns), fp32 ones rounded to 2^-23 of
- * it. The products of codes and activations are summed exactly within a group
+ * it (both: of 2^-126 where it is smaller). The products of codes and activations are summed exactly within a group
  * (of at most 128 columns); those of more than 16 tokens, or 3 per expert, in fp32
  * if they are BF16, or F32 with a group of 32 or 64. A NaN or an infinity in x makes its token's outputs NaN.
  * Calls that may overlap need a workspace (a multiple of 16 bytes) each.

@@ -84,10 +84,10 @@ __device__ __forceinline__ uint32_t gather4(uint32_t a, uint32_t b, uint32_t c, 
 }
 
 // The power of two (its exponent) that takes a chunk whose largest magnitude has
-// the bits `most` to three digits: the largest one that fits; chunks below 2^-96
-// share their step, 2^-118.
+// the bits `most` to three digits: the largest one that fits; chunks below 2^-126,
+// fp32's smallest normal value, share their step, 2^-148.
 __device__ __forceinline__ int digits_up(uint32_t most) {
-  const int up = 22 - max(int(most >> 23) - 127, -96);
+  const int up = 22 - max(int(most >> 23) - 127, -126);
   return ldexpf(bits_to_f32(most), up) > float(kMaxDigits) ? up - 1 : up;
 }
 // A value's three digits in bytes 2, 1, 0, each offset by 128.
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(256) w4_stage_halves_kernel(Stage p) {
   most = max(most, uint32_t(__shfl_xor(int(most), 1, kWave)));
   most = max(most, uint32_t(__shfl_xor(int(most), 2, kWave)));
   const bool finite = most < 0x7f800000u;
-  const int up = 14 - max(int(most >> 23) - 127, -96);
+  const int up = 14 - max(int(most >> 23) - 127, -126);
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] = finite ? ldexpf(v[j], up) : 0.f;
   int8_t* out = p.a.planes + rc * (PLANES * 2 * kW4Chunk);

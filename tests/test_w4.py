@@ -144,6 +144,24 @@ def test_sizes_of_the_values(cuda, dtype, std):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 3, 9, 40, 300])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_vanishing_activations(cuda, T, group, dtype):
+    # down to fp32's smallest normal values a chunk's largest sets its step, as the
+    # header says; below, half of 2^-148. Results round to a multiple of 2^-149,
+    # (4 * 3 + 16) times
+    g = torch.Generator().manual_seed(T + group)
+    m = ref.make(g, 40, 384, group, scales=F32, scale=3.0)
+    w, handle = ref.dense(*m), ops.W4(*m)
+    for std in (1e-28, 1e-30, 1e-33, 1e-35, 1e-36, 1e-37, 1e-38, 1e-40, 1e-43):
+        x, _ = _x(g, T, 384, dtype, std=std)
+        want, bar = ref.linear(w, ref.values(x))
+        bar = bar + 2.0 ** -149 * (w.abs().sum(1) + 28)
+        _near(ops.w4_matvec_add2(handle, x), want, bar)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("group", [32, 128])
 def test_extreme_codes_and_zero_points(cuda, group):
     # the largest sums: every code 0 or 15, zero points of any byte, digits of
