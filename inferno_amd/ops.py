@@ -252,8 +252,9 @@ class W4:
     cols], or one per expert [E, rows, cols]. ``codes`` holds two columns a byte
     (uint8 [..., cols / 2], the even column in the low nibble), ``scales`` one
     factor per cols / scales.shape[-1] columns (fp32 or bf16), ``zeros`` a zero
-    point for each scale (uint8; None: 8). Packed once, here, on the current stream
-    (inferno_w4_pack); the tensors are not kept."""
+    point for each scale (uint8; None: 8), of which one above 127 counts as 127.
+    Packed once, here, on the current stream (inferno_w4_pack); the tensors are not
+    kept."""
 
     def __init__(self, codes, scales, zeros=None):
         if codes.dtype != torch.uint8 or codes.dim() not in (2, 3) or not codes.is_contiguous():

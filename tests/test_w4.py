@@ -183,6 +183,30 @@ def test_extreme_codes_and_zero_points(cuda, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 128])
+def test_zero_points_above_127_count_as_127(cuda, group):
+    g = torch.Generator().manual_seed(group)
+    codes, s, z = ref.make(g, 40, 256, group, zeros=True)
+    z[::2] += 100
+    z[1::4] = 127
+    z[::3, 0] = 255
+    plain = ops.W4(codes, s, z.clamp(max=127))
+    w = ops.W4(codes, s, z)
+    assert int(z.max()) == 255
+    for T in (1, 8, 40):
+        for dtype in (F32, BF16, I8):
+            x, xs = _x(g, T, 256, dtype)
+            got = ops.w4_matvec_add2(w, x, x_scales=xs)
+            assert torch.equal(got, ops.w4_matvec_add2(plain, x, x_scales=xs))
+            # the definition's matrix, of the zero points that count
+            q = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).cpu().double()
+            zz = z.cpu().double().clamp(max=127).repeat_interleave(group, 1)
+            d = (q - zz) * s.cpu().double().repeat_interleave(group, 1)
+            want, bar = ref.linear(d, ref.values(x, xs), dtype != I8)
+            _near(got, want, bar)
+
+
+@pytest.mark.gpu
 def test_digits_hold_bf16_whole(cuda):
     # one column at a time through a matrix of ones: values down to 2^-14 of
     # their chunk's largest come back as they are
