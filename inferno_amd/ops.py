@@ -253,8 +253,10 @@ class W4:
     (uint8 [..., cols / 2], the even column in the low nibble), ``scales`` one
     factor per cols / scales.shape[-1] columns (fp32 or bf16), ``zeros`` a zero
     point for each scale (uint8; None: 8), of which one above 127 counts as 127.
-    Packed once, here, on the current stream (inferno_w4_pack); the tensors are not
-    kept."""
+    Packed once, here, on the current stream (inferno_w4_pack), which is waited for:
+    the handle may be used on any stream at once, and the tensors are not kept. While
+    the stream is being captured nothing is waited for; such a handle holds its matrix
+    after the graph's first replay."""
 
     def __init__(self, codes, scales, zeros=None):
         if codes.dtype != torch.uint8 or codes.dim() not in (2, 3) or not codes.is_contiguous():
@@ -281,6 +283,10 @@ class W4:
              scales.numel() * scales.element_size(), _at(zeros),
              zeros.numel() if zeros is not None else 0, _at(self.packed))
         d.packed = self.packed.data_ptr()
+        stream = torch.cuda.current_stream(self.device)
+        with torch.cuda.device(self.device):
+            if not torch.cuda.is_current_stream_capturing():
+                stream.synchronize()
 
 
 _ACT = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: I8}

@@ -257,3 +257,46 @@ def test_one_token_of_large_sums(cuda, E, k, I, group, dtype, zeros):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(again, ops.w4_moe(*handles, x, ids, w, k))
+
+
+@pytest.mark.gpu
+def test_a_handle_packed_behind_other_work_is_used_on_another_stream(cuda):
+    # packing waits behind some milliseconds of products on its stream; the caller's
+    # tensors are overwritten and the handle is used elsewhere right afterwards
+    g = torch.Generator().manual_seed(4)
+    m = ref.make(g, 300, 1024, 64, zeros=True)
+    x = torch.randn(6, 1024, generator=g).to(BF16).cuda()
+    want, bar = ref.linear(ref.dense(*m), ref.values(x))
+    a = torch.randn(4096, 4096, device=cuda)
+    b = a @ a
+    torch.cuda.synchronize()
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(10):
+            torch.mm(a, a, out=b)
+        w = ops.W4(*m)
+    with torch.cuda.stream(other):
+        for t in m:
+            t.zero_()
+        got = ops.w4_matvec_add2(w, x)
+    torch.cuda.synchronize()
+    assert ((got.cpu().double() - want).abs() <= bar).all()
+
+
+@pytest.mark.gpu
+def test_a_handle_packed_in_a_graph(cuda):
+    g = torch.Generator().manual_seed(5)
+    first, second = (ref.make(g, 40, 256, 128) for _ in range(2))
+    x = torch.randn(3, 256, generator=g).cuda()
+    held = [t.clone() if t is not None else None for t in first]
+    ops.w4_matvec_add2(ops.W4(*first), x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.w4_matvec_add2(ops.W4(*held), x)
+    for m in (first, second, first):
+        for t, v in zip(held, m):
+            if t is not None:
+                t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, ops.w4_matvec_add2(ops.W4(*m), x))
