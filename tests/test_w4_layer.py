@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import w4_reference as ref
-from inferno_amd import GROUP_TOP2, SCORE_SIGMOID, ops
+from inferno_amd import GROUP_TOP2, SCORE_SIGMOID, lib, ops
 from test_group_topk import _definition as routing
 
 F32, BF16, I8 = torch.float32, torch.bfloat16, torch.int8
@@ -300,3 +300,32 @@ def test_a_handle_packed_in_a_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, ops.w4_matvec_add2(ops.W4(*m), x))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,mats,one", [
+    # bytes of a workgroup: T ceil(K / 128) 388 + 1024 mats + 16, of 54272
+    (4, 4096, 2, True), (4, 4352, 2, False), (4, 4352, 1, True), (3, 5632, 2, True),
+    (3, 5888, 2, False), (2, 8704, 1, True), (1, 17536, 1, True), (1, 17664, 1, False)])
+def test_few_tokens_that_fit_take_one_launch(cuda, T, K, mats, one):
+    # the launch that stages its tokens by itself leaves the workspace as it was
+    g = torch.Generator().manual_seed(K)
+    m = ref.make(g, 24, K, 128)
+    w = ops.W4(*m)
+    x = torch.randn(T, K, generator=g).cuda()
+    n = lib().inferno_w4_workspace_bytes(T, K)
+    ws = torch.full((n,), 171, dtype=torch.uint8, device=cuda)
+    out = torch.empty(T, 24, device=cuda)
+    s = torch.cuda.current_stream().cuda_stream
+    tail = (x.data_ptr(), 0, None, 0)
+    if mats == 2:
+        st = lib().inferno_w4_gate_up_swiglu(s, w.ref, w.ref, *tail, T, out.data_ptr(),
+                                             ws.data_ptr(), n)
+        want, bar = ref.swiglu(ref.dense(*m), ref.dense(*m), ref.values(x))
+    else:
+        st = lib().inferno_w4_matvec_add2(s, w.ref, *tail, None, None, T, out.data_ptr(),
+                                          ws.data_ptr(), n)
+        want, bar = ref.linear(ref.dense(*m), ref.values(x))
+    assert st == 0
+    assert bool((ws == 171).all()) == one
+    assert ((out.cpu().double() - want).abs() <= bar).all()
