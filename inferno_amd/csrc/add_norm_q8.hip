@@ -67,10 +67,11 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
 }
 
 // Any width and alignment: one workgroup per row, the row read again from
-// memory (or the cache) for each of the three steps.
+// memory (or the cache) for each of the three steps. sum may be x or residual,
+// which are therefore not __restrict__ (in either kernel).
 template <typename XT, typename OT>
 __global__ void __launch_bounds__(kThreads)
-    add_norm_q8_row_kernel(const XT* __restrict__ x, const float* residual,
+    add_norm_q8_row_kernel(const XT* x, const float* residual,
                            const float* __restrict__ w, float eps, size_t H, size_t group,
                            float* sum, OT* __restrict__ normed, int8_t* __restrict__ q,
                            float* __restrict__ scales) {
@@ -178,7 +179,7 @@ __device__ __forceinline__ void store4(uint16_t* p, const float (&v)[4]) {
 // lanes, 0: the row is one group.
 template <typename XT, typename OT, int NV, int STEPS>
 __global__ void __launch_bounds__(kThreads)
-    add_norm_q8_kernel(const XT* __restrict__ x, const float* residual,
+    add_norm_q8_kernel(const XT* x, const float* residual,
                        const float* __restrict__ w, float eps, uint32_t H, float* sum,
                        OT* __restrict__ normed, int8_t* __restrict__ q,
                        float* __restrict__ scales) {

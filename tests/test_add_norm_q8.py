@@ -149,6 +149,21 @@ def test_the_sum_in_place(cuda, H, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,group", [(2048, 128), (515, 0), (1028, 0), (6144, 32), (40000, 0)])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_the_sum_over_x(cuda, H, group, with_residual):
+    x, r, w = _inputs(7, H, torch.float32, seed=8)
+    r = r if with_residual else None
+    want = ops.add_rms_norm_q8(x, r, w, EPS, group=group)
+    for _ in range(3):
+        stream = x.clone()
+        got = ops.add_rms_norm_q8(stream, r, w, EPS, group=group, out=stream)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        assert torch.equal(stream, want[0])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,group", [(256, 64), (259, 0)])
 def test_outputs_left_out_and_pointers_off_alignment(cuda, H, group):
     # every output but one left out; inputs and outputs one element past an
