@@ -266,6 +266,68 @@ def test_same_bits_again_and_rows_by_themselves(cuda, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("few,many", [(1, 4), (2, 3), (5, 16), (7, 13), (17, 64), (65, 200)])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("dtype", [F32, BF16, I8])
+def test_a_row_does_not_depend_on_the_others(cuda, few, many, group, dtype):
+    # between sizes that take one kernel, in another order, and among other tokens
+    g = torch.Generator().manual_seed(few)
+    w, u = (ops.W4(*ref.make(g, 200, 1152, group)) for _ in range(2))
+    x, xs = _x(g, many, 1152, dtype)
+    y, ys = _x(g, many, 1152, dtype)
+    y[:few] = x[:few]
+    if xs is not None:
+        ys[:few] = xs[:few]
+    order = torch.randperm(many, generator=g).cuda()
+    for f in (lambda a, s: ops.w4_matvec_add2(w, a, x_scales=s),
+              lambda a, s: ops.w4_gate_up_swiglu(w, u, a, x_scales=s)):
+        whole = f(x, xs)
+        part = f(x[:few].contiguous(), None if xs is None else xs[:few].contiguous())
+        assert torch.equal(whole[:few], part)
+        assert torch.equal(f(y, ys)[:few], part)
+        moved = f(x[order].contiguous(), None if xs is None else xs[order].contiguous())
+        assert torch.equal(moved, whole[order])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [2, 6, 40, 150])
+@pytest.mark.parametrize("dtype", [F32, BF16, I8])
+def test_a_routed_token_does_not_depend_on_the_others(cuda, T, dtype):
+    g = torch.Generator().manual_seed(T)
+    mats = _experts(g, 8, 256, 192, 64)
+    ws = [ops.W4(*m) for m in mats]
+    x, xs = _x(g, T, 256, dtype)
+    ids, w = _routing(g, T, 8, 3)
+    whole = ops.w4_moe(*ws, x, ids, w, 3, x_scales=xs)
+    order = torch.randperm(T, generator=g).cuda()
+    moved = ops.w4_moe(*ws, x[order].contiguous(), ids.view(T, 3)[order].flatten(),
+                       w.view(T, 3)[order].flatten(), 3,
+                       x_scales=None if xs is None else xs[order].contiguous())
+    assert torch.equal(moved, whole[order])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [17, 70, 300])
+@pytest.mark.parametrize("K", [32, 128, 1152])
+@pytest.mark.parametrize("dtype,group,planes", [(BF16, 32, 1), (BF16, 128, 1), (F32, 32, 2)])
+def test_fp16_sums_of_one_sign(cuda, T, K, dtype, group, planes):
+    # Many tokens sum a chunk's products of fp16 values in fp32. Whatever the order
+    # inside a matrix instruction, a chunk has at most 128 additions a plane, each off
+    # by at most 2^-23 (were it cut off) of a partial sum of one sign; the rest as in
+    # w4_reference.py
+    group = min(group, K) if K % 128 else group
+    g = torch.Generator().manual_seed(K)
+    codes = torch.randint(9, 16, (50, K), generator=g, dtype=torch.uint8)
+    packed = (codes[:, 0::2] | codes[:, 1::2] << 4).contiguous()
+    s = 0.01 * (1.0 + torch.rand(50, K // group, generator=g))
+    x = (0.5 + torch.rand(T, K, generator=g)).to(dtype)
+    w = ref.dense(packed, s)
+    want, bar = ref.linear(w, x.double())
+    bar = bar + 256 * planes * ref.U * want
+    _near(ops.w4_matvec_add2(ops.W4(packed.cuda(), s.cuda()), x.cuda()), want, bar)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 5, 33])
 def test_only_the_outputs_are_written(cuda, T):
     # the library's call with outputs inside a larger buffer and a workspace of
