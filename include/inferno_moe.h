@@ -110,12 +110,14 @@ int inferno_moe_router_topk(void* stream, const float* logits, const float* bias
 /* The same top-k over the best groups of experts: expert e is in group
  * e / (E / n_group); the topk_group groups of the highest group_score stay open
  * (ties go to the lower group), the others' experts are not selected.
- * Selection values are sigmoid(l) + bias, or l + bias (softmax), compared in 64
- * bits; -0 equals +0 and a NaN lies above +infinity, for its group too. Weights
- * as above; softmax scores are normalised over all E experts, open or not, and
- * a row of -infinity has weights 0. bias and token_indices may be NULL.
- * n_group divides E, E <= 256, k <= min(16, topk_group * E / n_group).
- * T = 0 does nothing. */
+ * Selection values are sigmoid(l) + bias, or l + bias (softmax: of logits as above,
+ * not of scores, which a bias or a sum of two may order otherwise), compared in 64
+ * bits, as are the sums of two; -0 equals +0 and a NaN lies above +infinity, for its
+ * group too. Weights as above: with norm_topk_prob ratios of the winners' scores,
+ * however far a closed group's logit lies above them; softmax scores without it are
+ * normalised over all E experts, open or not. A row of -infinity has weights 0. bias
+ * and token_indices may be NULL. n_group divides E, E <= 256,
+ * k <= min(16, topk_group * E / n_group), T <= 2^26 - 4. T = 0 does nothing. */
 int inferno_moe_router_group_topk(void* stream, const float* logits, const float* bias, size_t T,
                                   size_t E, size_t k, int score_fn, int norm_topk_prob,
                                   float routed_scaling_factor, size_t n_group, size_t topk_group,
@@ -205,7 +207,8 @@ int inferno_q8_0_matvec_add2(void* stream, const void* w, size_t w_bytes, const 
  * `group` consecutive columns of a row, or `experts` such matrices one after
  * another:
  *   W[r, c] = scales[r, c / group] * (code[r, c] - zeros[r, c / group])
- * without zero points 8 in their place. cols is a multiple of 32 and of group;
+ * without zero points 8 in their place. Scales are 0 or lie between 2^-100 and 2^90
+ * in magnitude (fp32 partial sums are formed before the activations' scale). cols is a multiple of 32 and of group;
  * group is 32, 64 or a multiple of 128; one matrix has less than 2^33 codes and
  * at most 2^25 rows, experts <= 256. The products read a packed form, which
  * inferno_w4_pack writes once; it takes inferno_w4_packed_bytes at a multiple of
@@ -237,11 +240,16 @@ int inferno_w4_pack(void* stream, const inferno_w4* w, const void* codes, size_t
  * x_scales [T, cols / x_group] fp32 (x = value * scale; x_group a multiple of
  * 128 that divides cols, or 0: one scale per row; what
  * inferno_add_rms_norm_q8 writes). x lies at a multiple of 16 bytes; x_scales
- * and x_group are not read for F32 and BF16. bf16 activations enter whole (down
- * to 2^-14 of the largest of their 128 columns), fp32 ones rounded to 2^-23 of
- * it (both: of 2^-126 where it is smaller). The products of codes and activations are summed exactly within a group
- * (of at most 128 columns); those of more than 16 tokens, or 3 per expert, in fp32
- * if they are BF16, or F32 with a group of 32 or 64. A NaN or an infinity in x makes its token's outputs NaN.
+ * and x_group are not read for F32 and BF16.
+ * Up to 16 tokens, or 3 per expert on average: activations are fixed-point values
+ * relative to the largest of their 128 columns (or to 2^-126 if that is larger), bf16
+ * whole down to 2^-14 of it, fp32 rounded to 2^-23 of it, so that a value a
+ * thousandth of the largest keeps 13 bits; products with codes are summed exactly in
+ * a group (of at most 128 columns). More tokens: the same for F32 with groups of 128
+ * and more; BF16 ones are whole down to 2^-31 of the largest, and F32 ones with groups
+ * of 32 or 64 rounded to 2^-23 of themselves, their products summed in fp32. The
+ * routed experts' h is F32. I8 is exact for any number of tokens.
+ * A NaN or an infinity in x makes its token's outputs NaN.
  * Calls that may overlap need a workspace (a multiple of 16 bytes) each.
  * T = 0 does nothing. */
 
@@ -308,12 +316,13 @@ int inferno_rms_norm(void* stream, const float* x, const float* w, size_t rows, 
  *   y = s / sqrt(mean(s^2) + eps) * w, rounded to act_dtype (F32 or BF16);
  *   q = rint(127 y / A), scale = A / 127, A = max |y| over each `group` columns
  *     (32, 64 or 128, which divides H; 0: the row), so that y ~ q * scale. q is
- *     the rounding of the exact quotient, ties to even.
+ *     the rounding of the quotient in 64 bits, ties to even.
  * x is [rows,H] f32 or bf16. sum_out receives s, normed_out y, q_out [rows,H]
  * int8 and scales_out [rows, H/group]; each may be NULL, q_out and scales_out
  * together. sum_out may be residual, or an fp32 x; no other overlap. A group
  * with a NaN or an infinity has q = 0 and a scale that is not finite. A group
- * of zeros has q = 0, scale = 0. rows = 0 does nothing. */
+ * of zeros has q = 0, scale = 0, and a row of zeros y = 0, also with eps = 0. The
+ * 4-bit products take scales per row or per 128 columns. rows = 0 does nothing. */
 int inferno_add_rms_norm_q8(void* stream, const void* x, int x_dtype, const float* residual,
                             const float* w, float eps, size_t rows, size_t H, size_t group,
                             int act_dtype, float* sum_out, void* normed_out, int8_t* q_out,

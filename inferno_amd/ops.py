@@ -207,7 +207,8 @@ def _run(x, fn, *args):
 def add_rms_norm_q8(x, residual, w, eps, group=0, act_dtype=torch.float32, out=None):
     """Residual addition, RMSNorm and 8-bit activations (inferno_add_rms_norm_q8):
     s = x + residual (None: x), y = s / sqrt(mean(s^2) + eps) * w, and y in int8
-    with one fp32 scale per ``group`` columns (32, 64, 128; 0: the row). Returns
+    with one fp32 scale per ``group`` columns (32, 64, 128; 0: the row; the 4-bit
+    products take those of 128 and of the row). Returns
     (s, y in act_dtype, q, scales); ``out`` (fp32, may be ``residual``) receives s."""
     _rows_of(x, "x", tuple(_DT))
     T, H = x.shape
@@ -232,7 +233,8 @@ def add_rms_norm_q8(x, residual, w, eps, group=0, act_dtype=torch.float32, out=N
 
 def router_group_topk(logits, bias, k, score_fn, norm, scale, n_group, topk_group, group_score):
     """``router_topk`` over the ``topk_group`` best of ``n_group`` groups of
-    experts (inferno_moe_router_group_topk)."""
+    experts (inferno_moe_router_group_topk). With softmax, experts and groups are
+    ranked by logit + bias, as ``router_topk`` does, not by their scores."""
     _rows_of(logits, "logits", (torch.float32,))
     T, E = logits.shape
     if bias is not None:
