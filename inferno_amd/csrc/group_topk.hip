@@ -11,13 +11,14 @@
 // order are further apart than their roundings, which is checked for every open
 // group against every closed one (a sum of two rounds by their magnitudes, which
 // it may be far below), for the last winner against the best loser and for
-// neighbouring winners. Where winners fail, the experts that
-// may be among the k best (one per lane) are formed and ranked in 64 bits; a
-// token whose groups fail, with more of them than lanes, or with a NaN is done
-// again in 64 bits as a whole. 8192 tokens of 256 experts in 8 groups: 15.7 us;
-// whole rows in 64 bits for every failure 20.3, for every token 28 us. All 8192
-// wavefronts are resident at once: what bounds it is their instructions and, for
-// few tokens, one chain of cross-lane steps (29 tokens: 6.5 us).
+// neighbouring winners. Where winners fail, the experts that may be among the k
+// best (one per lane) are formed and ranked in 64 bits; a token whose groups fail,
+// with more of them than lanes, or with a NaN is done again in 64 bits as a whole.
+// 8192 tokens of 256 experts in 8 groups: 15.5 us (15.2 with the last open and the
+// first closed group alone compared); whole rows in 64 bits for every failure 20.3,
+// for every token 28 us. All 8192 wavefronts are resident at once: what bounds it is
+// their instructions and, for few tokens, one chain of cross-lane steps (29 tokens:
+// 6.4 us).
 #include "kernels.hpp"
 #include "routing_dev.hpp"
 

@@ -2,17 +2,22 @@
 //
 //   y[t, n] = sum_g s[n, g] sum_{c in g} (q[n, c] - z[n, g]) x[t, c]
 //
-// int8 activations and few tokens: the inner sum is formed exactly. A code is widened to 16 (q - 8), an int8, by
-// one mask (its nibble stays in the high half of the byte), or to q - z with
-// four codes in one subtraction; an activation is one int8 digit (8-bit
-// activations) or three, a 24-bit fixed-point value relative to the largest of
-// its 128-column chunk: exact for every bf16 value down to 2^-14 of the
-// largest, and off by at most 2^-23 of it for fp32. The int32 sums of a group
+// int8 activations and few tokens: the inner sum is formed exactly. A code is
+// widened to 16 (q - 8), an int8, by one mask (its nibble stays in the high half of
+// the byte), or to q - z with four codes in one subtraction; an activation is one
+// int8 digit (8-bit activations) or three, a 24-bit fixed-point value relative to
+// the largest of its 128-column chunk: exact for every bf16 value down to 2^-14 of
+// the largest, and off by at most 2^-23 of it for fp32. The int32 sums of a group
 // are exact, the groups are added in fp32. Joining three sums is six vector
 // instructions a result and chunk, more than their matrix instructions take, so
 // many bf16 tokens (and fp32 ones with groups of 32 or 64) go as fp16 instead,
 // one plane (two) of values scaled by a power of two for each chunk, against
 // codes widened to fp16, q - z whole; a chunk's sums are formed in fp32.
+//
+// Why fp32 has three digits: with four (off by 2^-31 of the largest) one to four
+// tokens take as long, but 16 tokens of 8 of 64 experts with groups of 32 130
+// instead of 78 us, 512 of 10 of 128 experts (whose h is fp32) 767 instead of 605,
+// and 256 of one matrix 2048 x 6144 181 instead of 94.
 //
 // Tile: 16 weight rows (the 16 columns of a 16x16 MFMA result) by 16 digit
 // rows. A lane holds 32 codes of its row per chunk (16 bytes: low nibbles are
@@ -346,8 +351,9 @@ struct Wide<true> {
 };
 
 // The same as fp16: q - 8 or q - z, one register quadruple for each dword of
-// codes, whose columns come in the order 0 4 1 5 2 6 3 7. 0x6400 with a code in
-// its low bits is 1024 + q, with a code four bits up 1024 + 16 q.
+// codes, whose columns come in the order 0 4 1 5 2 6 3 7. The widening is the
+// well-known one by the exponent: 0x6400 with a code in its low bits is 1024 + q,
+// with a code four bits up 1024 + 16 q.
 struct Halves {
   v4u dword[4];
 
@@ -763,8 +769,9 @@ __global__ void __launch_bounds__(WAVES* kWave) w4_token_kernel(Tokens a) {
 
 // Many tokens. One workgroup: 64 tokens by 128 RT / KS rows of the matrices; a
 // wavefront takes RT tiles of 16 rows of each matrix against all tokens, and one
-// of KS shares of the chunks (a chunk costs a workgroup 0.5 us at least, however
-// few there are of it). The
+// of KS shares of the chunks (a step of one chunk costs a workgroup 0.5 us or more
+// whatever it holds; one of four shares at once, 256 int8 tokens of a pair 2048 x
+// 6144, 2.7 us). The
 // weights go from memory to the wavefront that owns them; the tokens' values go
 // through LDS (two buffers of one chunk) in the order in which the matrix
 // instructions' lanes read them, so that a read is 1 KB without bank conflicts.
@@ -775,10 +782,10 @@ __global__ void __launch_bounds__(WAVES* kWave) w4_token_kernel(Tokens a) {
 // where they fit the registers.
 // What bounds it: one workgroup per CU (170 to 256 registers), whose loads,
 // reads from LDS and arithmetic overlap only in part. 512 bf16 tokens of 10 of
-// 128 experts, gate and up 1536 x 4096: 350 us for 0.82 GB of weights (2.3
-// TB/s), three digits 418; down, three digits: 246 us. 64 int8 tokens, gate and
-// up: 147 us (5.6 TB/s with the caches' help). One matrix pair 2048 x 6144, 256
-// tokens: int8 36, bf16 56 us, three digits 84.
+// 128 experts, gate and up 1536 x 4096: 344 to 352 us (by card) for 0.82 GB of
+// weights (2.3 TB/s), three digits 418; down, three digits: 246 to 261 us. 64 int8
+// tokens, gate and up: 147 to 150 us (5.6 TB/s with the caches' help). One matrix
+// pair 2048 x 6144, 256 tokens: int8 36, bf16 56 us, three digits 84.
 constexpr int kTileTokens = 64;
 constexpr int kTileWaves = 8;
 
