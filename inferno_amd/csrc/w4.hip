@@ -15,9 +15,10 @@
 // codes widened to fp16, q - z whole; a chunk's sums are formed in fp32.
 //
 // Why fp32 has three digits: with four (off by 2^-31 of the largest) one to four
-// tokens take as long, but 16 tokens of 8 of 64 experts with groups of 32 130
-// instead of 78 us, 512 of 10 of 128 experts (whose h is fp32) 767 instead of 605,
-// and 256 of one matrix 2048 x 6144 181 instead of 94.
+// tokens take as long, but 16 tokens of 8 of 64 experts with groups of 32 97
+// instead of 78 us, 128 and 512 of 10 of 128 experts 454 and 701 instead of 318 and
+// 605 (h is fp32), 256 of one matrix 2048 x 6144 115 instead of 94; with two chunks
+// ahead as three digits have, the registers do not suffice and it is more.
 //
 // Tile: 16 weight rows (the 16 columns of a 16x16 MFMA result) by 16 digit
 // rows. A lane holds 32 codes of its row per chunk (16 bytes: low nibbles are
