@@ -114,7 +114,7 @@ int inferno_moe_router_topk(void* stream, const float* logits, const float* bias
  * not of scores, which a bias or a sum of two may order otherwise), compared in 64
  * bits, as are the sums of two; -0 equals +0 and a NaN lies above +infinity, for its
  * group too. Weights as above: with norm_topk_prob ratios of the winners' scores,
- * however far a closed group's logit lies above them; softmax scores without it are
+ * however small these are; softmax scores without it are
  * normalised over all E experts, open or not. A row of -infinity has weights 0. bias
  * and token_indices may be NULL. n_group divides E, E <= 256,
  * k <= min(16, topk_group * E / n_group), T <= 2^26 - 4. T = 0 does nothing. */

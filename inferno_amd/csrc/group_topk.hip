@@ -76,6 +76,12 @@ __device__ __forceinline__ float weights_from(const GroupTopk& p, float lmax, fl
   return p.norm && fabsf(lmax) < INFINITY && top > -INFINITY ? top : lmax;
 }
 
+// The same for sigmoids, which are exp(l) in 32 bits from -17 down: whether the
+// winners' are so small that they vanish. sum: of their scores.
+__device__ __forceinline__ bool vanishing(const GroupTopk& p, float sum, float top) {
+  return p.norm && sum < 0x1p-80f && top > -INFINITY;
+}
+
 __device__ __forceinline__ void exact_row(const GroupTopk& p, size_t t, Scratch& scratch) {
   constexpr int kPer = kMaxExperts / kWave;
   const int lane = threadIdx.x & 63;
@@ -176,9 +182,11 @@ __device__ __forceinline__ void exact_row(const GroupTopk& p, size_t t, Scratch&
       mine_id = uint32_t(id);
     }
   }
-  if (p.score_fn == INFERNO_SCORE_SOFTMAX && !__any(mine_l != mine_l)) {
-    const float from = weights_from(p, lmax, wave_max(mine_l));
-    if (from != lmax) {  // uniform
+  if (!__any(mine_l != mine_l)) {
+    const float top = wave_max(mine_l);
+    const bool softmax = p.score_fn == INFERNO_SCORE_SOFTMAX;
+    const float from = softmax ? weights_from(p, lmax, top) : top;
+    if (softmax ? from != lmax : vanishing(p, sum, top)) {  // uniform
       mine_w = expf(mine_l - from);
       sum = 0.f;
       for (int r = 0; r < p.k; ++r) sum += __shfl(mine_w, r, kWave);  // rank order
@@ -394,15 +402,28 @@ __device__ __forceinline__ bool fast_row(const GroupTopk& p, size_t t, Scratch& 
   const float l = row[id];
   if (!sigmoid && p.norm) {
     const uint32_t top = wave_umax(won ? total_order_key(l) : 0u);
-    lmax = weights_from(p, lmax, bits_to_f32((top >> 31) ? top ^ 0x80000000u : ~top));
+    lmax = weights_from(p, lmax, value_of(top));
   }
-  const float my_score = sigmoid ? 1.f / (1.f + expf(-l)) : expf(l - lmax);
+  float my_score = sigmoid ? 1.f / (1.f + expf(-l)) : expf(l - lmax);
   float sum = 0.f;
-  if (p.norm) {
+  auto add_up = [&] {
     if (won) s.by_rank[rank] = my_score;
     __builtin_amdgcn_wave_barrier();
     const float ranked = s.by_rank[min(lane, p.k - 1)];
+    sum = 0.f;
     for (int r = 0; r < p.k; ++r) sum += lane_of(ranked, r);  // rank order
+  };
+  if (p.norm) {
+    add_up();
+    if (sigmoid && sum < 0x1p-80f) {  // uniform
+      const uint32_t key = wave_umax(won ? total_order_key(l) : 0u);
+      const float top = value_of(key);
+      if (vanishing(p, sum, top)) {
+        my_score = expf(l - top);
+        __builtin_amdgcn_wave_barrier();
+        add_up();
+      }
+    }
   } else {
     sum = wave_sum(all);
   }

@@ -226,6 +226,30 @@ def test_weights_far_below_the_closed_groups(cuda, gap):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("far", [-20.0, -60.0, -86.0, -95.0, -104.0, -1e4])
+@pytest.mark.parametrize("ties", [False, True])
+def test_normalised_weights_of_vanishing_sigmoids(cuda, far, ties):
+    # the winners' scores vanish in fp32 (biases decide), their ratios do not. Bar:
+    # exponentials of arguments of at most 3 and far's rounding, which is the input's;
+    # four additions, a quotient and the scale; above -17 the sigmoid's own roundings
+    g = torch.Generator().manual_seed(9)
+    l = far + 3.0 * torch.rand(20, 16, generator=g)
+    bias = torch.rand(16, generator=g)
+    if ties:  # whole rows in 64 bits
+        bias[:] = 0.25
+        l[:, 4:8] = l[:, 0:4]
+    ids, w, _ = ops.router_group_topk(l.to(cuda), bias.to(cuda), 4, SCORE_SIGMOID, True, 2.5, 4, 2,
+                                      GROUP_TOP2)
+    ids = ids.view(20, 4).cpu().long()
+    assert all(len(set(r)) == 4 for r in ids.tolist())
+    won = l.double().gather(1, ids)
+    e = torch.exp(won - won.amax(1, keepdim=True)) / (1.0 + torch.exp(won))
+    e = 2.5 * e / e.sum(1, keepdim=True)
+    bar = (2 * (3 + 2) + 4 + 2 + 2 * (abs(far) if far > -56.0 else 0)) * 2.0 ** -24
+    assert ((w.view(20, 4).cpu().double() - e).abs() <= bar * e).all()
+
+
+@pytest.mark.gpu
 def test_weights_of_closed_and_infinite_logits(cuda):
     # winners of -infinity alone, below a finite or an infinite closed logit
     inf = float("inf")
