@@ -14,7 +14,7 @@
 // neighbouring winners. Where winners fail, the experts that may be among the k
 // best (one per lane) are formed and ranked in 64 bits; a token whose groups fail,
 // with more of them than lanes, or with a NaN is done again in 64 bits as a whole.
-// 8192 tokens of 256 experts in 8 groups: 15.5 us (15.2 with the last open and the
+// 8192 tokens of 256 experts in 8 groups: 15.6 us (15.3 with the last open and the
 // first closed group alone compared); whole rows in 64 bits for every failure 20.3,
 // for every token 28 us. All 8192 wavefronts are resident at once: what bounds it is
 // their instructions and, for few tokens, one chain of cross-lane steps (29 tokens:
