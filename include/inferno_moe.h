@@ -114,10 +114,10 @@ int inferno_moe_router_topk(void* stream, const float* logits, const float* bias
  * not of scores, which a bias or a sum of two may order otherwise), compared in 64
  * bits, as are the sums of two; -0 equals +0 and a NaN lies above +infinity, for its
  * group too. Weights as above: with norm_topk_prob ratios of the winners' scores,
- * however small these are; softmax scores without it are
- * normalised over all E experts, open or not. A row of -infinity has weights 0. bias
- * and token_indices may be NULL. n_group divides E, E <= 256,
- * k <= min(16, topk_group * E / n_group), T <= 2^26 - 4. T = 0 does nothing. */
+ * however small these are; softmax scores without it are normalised over all E
+ * experts, open or not. A row of -infinity has weights 0. bias and token_indices may
+ * be NULL. n_group divides E, E <= 256, k <= min(16, topk_group * E / n_group),
+ * T <= 2^26 - 4. T = 0 does nothing. */
 int inferno_moe_router_group_topk(void* stream, const float* logits, const float* bias, size_t T,
                                   size_t E, size_t k, int score_fn, int norm_topk_prob,
                                   float routed_scaling_factor, size_t n_group, size_t topk_group,
@@ -208,11 +208,11 @@ int inferno_q8_0_matvec_add2(void* stream, const void* w, size_t w_bytes, const 
  * another:
  *   W[r, c] = scales[r, c / group] * (code[r, c] - zeros[r, c / group])
  * without zero points 8 in their place. Scales are 0 or lie between 2^-100 and 2^90
- * in magnitude (fp32 partial sums are formed before the activations' scale). cols is a multiple of 32 and of group;
- * group is 32, 64 or a multiple of 128; one matrix has less than 2^33 codes and
- * at most 2^25 rows, experts <= 256. The products read a packed form, which
- * inferno_w4_pack writes once; it takes inferno_w4_packed_bytes at a multiple of
- * 16 bytes. */
+ * in magnitude (fp32 partial sums are formed before the activations' scale). cols is
+ * a multiple of 32 and of group; group is 32, 64 or a multiple of 128; one matrix has
+ * less than 2^33 codes and at most 2^25 rows, experts <= 256. The products read a
+ * packed form, which inferno_w4_pack writes once; it takes inferno_w4_packed_bytes at
+ * a multiple of 16 bytes. */
 typedef struct inferno_w4 {
   size_t experts; /* 1: a plain matrix */
   size_t rows, cols, group;

@@ -49,9 +49,9 @@ __device__ __forceinline__ double inverse_root(double sq, double H, float eps) {
   return mean == 0.0 ? 0.0 : 1.0 / sqrt(mean);
 }
 
-// s / sqrt(..) in 32 bits; in 64 where the factor is no normal fp32 value: with eps =
-// 0 rows below 2^-127 have one that passes fp32's range, rows from 2^126 on one that
-// fp32 holds in fewer bits. (the same for a row)
+// s / sqrt(..) in 32 bits; in 64 for a row whose factor is no normal fp32 value: with
+// eps = 0 rows below 2^-127 have one that passes fp32's range, rows from 2^126 on one
+// that fp32 holds in fewer bits.
 __device__ __forceinline__ bool factor_fits(double inv) { return inv < 0x1p127 && inv > 0x1p-126; }
 __device__ __forceinline__ float scaled(float s, double inv, bool fits) {
   return fits ? s * float(inv) : float(double(s) * inv);

@@ -772,9 +772,8 @@ __global__ void __launch_bounds__(WAVES* kWave) w4_token_kernel(Tokens a) {
 // wavefront takes RT tiles of 16 rows of each matrix against all tokens, and one
 // of KS shares of the chunks (a step of one chunk costs a workgroup 0.5 us or more
 // whatever it holds; one of four shares at once, 256 int8 tokens of a pair 2048 x
-// 6144, 2.7 us). The
-// weights go from memory to the wavefront that owns them; the tokens' values go
-// through LDS (two buffers of one chunk) in the order in which the matrix
+// 6144, 2.7 us). The weights go from memory to the wavefront that owns them; the
+// tokens' values go through LDS (two buffers of one chunk) in the order in which the matrix
 // instructions' lanes read them, so that a read is 1 KB without bank conflicts.
 // Both are two chunks ahead in registers, since a chunk's loads take longer
 // than its arithmetic (copies to LDS that bypass registers would have to be

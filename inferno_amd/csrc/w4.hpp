@@ -75,8 +75,8 @@ int launch_w4_product(hipStream_t s, const W4Product& p);
 
 // One to four fp32 or bf16 tokens of a matrix, or one token of its experts, in
 // one launch, as far as the tokens' digits fit a workgroup's LDS (4 tokens of 4096
-// columns, 1 of 17536). ids: expert ids[y] of each slot y, result row y (none for an id of
-// no expert), or with `sum` the sum over the segments r of row r of x times
+// columns, 1 of 17536). ids: expert ids[y] of each slot y, result row y (none for an
+// id of no expert), or with `sum` the sum over the segments r of row r of x times
 // expert ids[r].
 struct W4Token {
   W4Mat m[2];
