@@ -52,8 +52,9 @@ enum inferno_quant {
   INFERNO_Q6_K = 14
 };
 
-/* INFERNO_I8: activations of the 4-bit products only. */
-enum inferno_dtype { INFERNO_F32 = 0, INFERNO_BF16 = 1, INFERNO_I8 = 2 };
+/* INFERNO_I8: activations of the 4-bit products only. INFERNO_MXFP4: weights and
+ * rows of the products grouped by expert only. */
+enum inferno_dtype { INFERNO_F32 = 0, INFERNO_BF16 = 1, INFERNO_I8 = 2, INFERNO_MXFP4 = 3 };
 
 enum inferno_score_fn { INFERNO_SCORE_SIGMOID = 0, INFERNO_SCORE_SOFTMAX = 1 };
 
@@ -280,6 +281,71 @@ int inferno_w4_moe(void* stream, const inferno_w4* gate, const inferno_w4* up,
                    const inferno_w4* down, const void* x, int x_dtype, const float* x_scales,
                    size_t x_group, const uint32_t* expert_ids, const float* expert_weights,
                    size_t T, size_t k, float* out, void* workspace, size_t workspace_bytes);
+
+/* ----------------------------------- experts in bf16 or 4-bit floating point */
+
+/* MXFP4: one code per value, two a byte (the even column in the low nibble), and
+ * one scale byte s per 32 columns of a row. Code c stands for (-1)^(c >> 3) times
+ * 0, 0.5, 1, 1.5, 2, 3, 4 or 6 (c & 7), times 2^(s - 127); s = 255 is NaN.
+ *
+ * Rows to MXFP4. For each 32 columns, m their largest magnitude: s - 127 =
+ * floor(log2(m)) - 2, at least -127 (m = 0 too); each code is the nearest one to
+ * x / 2^(s - 127), halfway values go to the code whose last bit is 0, magnitudes
+ * above 6 to 6, and the sign of a zero is kept. 32 columns with a NaN or an
+ * infinity have s = 255 and codes 0. x is [rows,cols] f32 or bf16, codes
+ * [rows, cols / 2], scales [rows, cols / 32]; values, which may be NULL, receives
+ * what the codes stand for in x's type (exactly). cols is a multiple of 32; x,
+ * codes and values lie at multiples of 16 bytes. rows = 0 does nothing. */
+int inferno_mxfp4_quantize(void* stream, const void* x, int x_dtype, size_t rows, size_t cols,
+                           void* codes, uint8_t* scales, void* values);
+
+/* One matrix [rows,cols], or one per expert. BF16: data is [experts][rows][cols]
+ * as it is, cols a multiple of 8. MXFP4: data is the packed form that
+ * inferno_mxfp4_pack writes once, cols a multiple of 32; scales (but for 255) lie
+ * between 2^-100 and 2^100. data lies at a multiple of 16 bytes. experts <= 256,
+ * rows and cols <= 2^24, one matrix at most 2^33 values. */
+typedef struct inferno_experts {
+  size_t experts;
+  size_t rows;       /* outputs */
+  size_t cols;       /* inputs */
+  int format;        /* INFERNO_BF16 or INFERNO_MXFP4 */
+  const void* data;
+  size_t data_bytes; /* 2 experts rows cols, or inferno_mxfp4_packed_bytes */
+} inferno_experts;
+
+/* Bytes of the packed form (of w, only sizes and format are read; 0: refused). */
+size_t inferno_mxfp4_packed_bytes(const inferno_experts* w);
+
+/* Packs codes [experts, rows, cols / 2] and scales [experts, rows, cols / 32]
+ * (w->data is not read, w->data_bytes is the size of packed). */
+int inferno_mxfp4_pack(void* stream, const inferno_experts* w, const void* codes,
+                       size_t codes_bytes, const uint8_t* scales, size_t scales_bytes,
+                       void* packed);
+
+/* Products of rows that are grouped by expert, groups of any size, empty ones too:
+ * for every expert e and c in [offsets[e], offsets[e + 1]), with a = sorted[c],
+ *   out[a] = x[a / k] W[e]^T                                      (grouped_matmul)
+ *   out[a] = silu(x[a / k] gate[e]^T) * (x[a / k] up[e]^T)  (grouped_gate_up_swiglu)
+ * offsets and sorted are inferno_moe_dispatch's: k results of each token's row
+ * for gate and up; for down, k = 1 and one row per assignment. sorted = NULL: a =
+ * c, rows that lie in the order of the experts (k = 1). offsets = NULL: one
+ * matrix and all rows (sorted = NULL).
+ *   x       [x_rows, cols] bf16, or with weights in MXFP4 also MXFP4: codes
+ *           [x_rows, cols / 2] with x_scales [x_rows, cols / 32] (else NULL)
+ *   offsets [experts + 1] ascending, at most x_rows k
+ *   sorted  [x_rows k]; of an index out of range, or of a row in no group, no
+ *           result is written
+ *   out     [x_rows k, rows] F32 or BF16, which may not overlap an input
+ * Sums are held in fp32, products are exact. A row that holds a NaN, an infinity or
+ * a scale of 255 changes its own results alone. x and out lie at multiples of 16
+ * bytes; x_rows k <= 2^22. x_rows = 0 does nothing. */
+int inferno_grouped_matmul(void* stream, const inferno_experts* w, const void* x, int x_dtype,
+                           const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
+                           const uint32_t* sorted, size_t k, int out_dtype, void* out);
+int inferno_grouped_gate_up_swiglu(void* stream, const inferno_experts* gate,
+                                   const inferno_experts* up, const void* x, int x_dtype,
+                                   const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
+                                   const uint32_t* sorted, size_t k, int out_dtype, void* out);
 
 /* --------------------------------------------------------------- combine */
 

@@ -4,7 +4,7 @@ from pathlib import Path
 
 lib_path = Path(__file__).resolve().parent / "libinferno_moe.so"
 
-F32, BF16, I8 = 0, 1, 2
+F32, BF16, I8, MXFP4 = 0, 1, 2, 3
 Q8_0, Q2_K, Q3_K, Q4_K, Q6_K = 8, 10, 11, 12, 14
 SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
 GROUP_MAX, GROUP_TOP2 = 0, 1
@@ -37,6 +37,14 @@ class W4Desc(C.Structure):
     _fields_ = [
         ("experts", _sz), ("rows", _sz), ("cols", _sz), ("group", _sz), ("scale_dtype", _i),
         ("has_zeros", _i), ("packed", _vp), ("packed_bytes", _sz),
+    ]
+
+
+class ExpertsDesc(C.Structure):
+    """Mirror of `struct inferno_experts`."""
+    _fields_ = [
+        ("experts", _sz), ("rows", _sz), ("cols", _sz), ("format", _i), ("data", _vp),
+        ("data_bytes", _sz),
     ]
 
 
@@ -86,6 +94,13 @@ SIGNATURES = {
     "inferno_w4_moe_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz]),
     "inferno_w4_moe": (_i, [_vp, C.POINTER(W4Desc), C.POINTER(W4Desc), C.POINTER(W4Desc), _vp, _i,
                             _vp, _sz, _vp, _vp, _sz, _sz, _vp, _vp, _sz]),
+    "inferno_mxfp4_quantize": (_i, [_vp, _vp, _i, _sz, _sz, _vp, _vp, _vp]),
+    "inferno_mxfp4_packed_bytes": (_sz, [C.POINTER(ExpertsDesc)]),
+    "inferno_mxfp4_pack": (_i, [_vp, C.POINTER(ExpertsDesc), _vp, _sz, _vp, _sz, _vp]),
+    "inferno_grouped_matmul": (_i, [_vp, C.POINTER(ExpertsDesc), _vp, _i, _vp, _sz, _vp, _vp, _sz,
+                                    _i, _vp]),
+    "inferno_grouped_gate_up_swiglu": (_i, [_vp, C.POINTER(ExpertsDesc), C.POINTER(ExpertsDesc),
+                                            _vp, _i, _vp, _sz, _vp, _vp, _sz, _i, _vp]),
     "inferno_moe_layer_workspace_bytes": (_sz, [C.POINTER(LayerDesc), _sz]),
     "inferno_moe_layer_forward": (_i, [_vp, C.POINTER(LayerDesc), _vp, _i, _vp, _sz, _vp, _vp,
                                        _vp, _vp, _sz]),

@@ -1,0 +1,164 @@
+// extern "C" entry points of MXFP4 and of the products of rows grouped by
+// expert: argument validation and kernel sequencing. No function allocates
+// device memory or synchronises.
+#include "abi_common.hpp"
+#include "experts.hpp"
+
+namespace inferno {
+namespace {
+
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+int check_bytes(const char* what, const char* part, size_t got, size_t want) {
+  if (got == want) return INFERNO_OK;
+  set_error(std::string(what) + " matrix: its " + part + " must take " + std::to_string(want) +
+            " bytes, got " + std::to_string(got));
+  return INFERNO_ERR_SIZE;
+}
+
+ExpertMat mat(const inferno_experts* w) {
+  return ExpertMat{w->experts, w->rows, w->cols, w->format == INFERNO_MXFP4, w->data};
+}
+
+int check_shape(const char* what, const inferno_experts* w) {
+  INF_CHECK_ARG(w != nullptr, "null expert matrices");
+  INF_CHECK_ARG(w->format == INFERNO_BF16 || w->format == INFERNO_MXFP4,
+                "the format of expert matrices must be BF16 or MXFP4");
+  if (w->experts == 0 || w->rows == 0 || w->cols == 0 || w->rows > (size_t(1) << 24) ||
+      w->cols > (size_t(1) << 24) || w->experts > size_t(kMaxExperts) ||
+      w->rows * w->cols > (size_t(1) << 33)) {
+    set_error(std::string(what) + " matrix: sizes out of range, experts=" +
+              std::to_string(w->experts) + ", rows=" + std::to_string(w->rows) + ", cols=" +
+              std::to_string(w->cols));
+    return INFERNO_ERR_INVALID;
+  }
+  if (w->format == INFERNO_MXFP4)
+    INF_CHECK_ARG(w->cols % kMxBlock == 0, "the columns of an MXFP4 matrix must be a multiple of 32");
+  else
+    INF_CHECK_ARG(w->cols % 8 == 0, "the columns of a bf16 matrix must be a multiple of 8");
+  return INFERNO_OK;
+}
+
+int check_mat(const char* what, const inferno_experts* w) {
+  int st;
+  if ((st = check_shape(what, w))) return st;
+  const size_t want = w->format == INFERNO_MXFP4 ? mx_layout(mat(w)).bytes
+                                                 : w->experts * w->rows * w->cols * 2;
+  if ((st = check_bytes(what, "data", w->data_bytes, want))) return st;
+  INF_CHECK_ARG(w->data != nullptr, "null pointer in an expert matrix");
+  INF_CHECK_ARG(aligned(w->data, 16), "an expert matrix must lie at a multiple of 16 bytes");
+  return INFERNO_OK;
+}
+
+int run_product(void* stream, const inferno_experts* w0, const inferno_experts* w1, const void* x,
+                int x_dtype, const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
+                const uint32_t* sorted, size_t k, int out_dtype, void* out) {
+  INF_CHECK_ARG(out_dtype == INFERNO_F32 || out_dtype == INFERNO_BF16,
+                "out dtype must be F32 or BF16");
+  INF_CHECK_ARG(x_dtype == INFERNO_BF16 || (x_dtype == INFERNO_MXFP4 && w0->format == INFERNO_MXFP4),
+                "x dtype must be BF16, or MXFP4 with weights in MXFP4");
+  INF_CHECK_ARG(k > 0, "k must be positive");
+  INF_CHECK_ARG(k == 1 || sorted, "several result rows per input row need sorted");
+  INF_CHECK_ARG(!sorted || offsets, "sorted rows need the experts' offsets");
+  INF_CHECK_ARG(offsets || w0->experts == 1, "several experts need offsets");
+  if (x_rows == 0) return INFERNO_OK;
+  const size_t most = size_t(1) << 22;
+  INF_CHECK_ARG(x_rows <= most && k <= most && x_rows * k <= most, "too many rows");
+  INF_CHECK_ARG(x && out, "null pointer");
+  INF_CHECK_ARG((x_dtype == INFERNO_MXFP4) == (x_scales != nullptr),
+                "x_scales belong to MXFP4 rows, which need them");
+  INF_CHECK_ARG(aligned(x, 16) && aligned(out, 16), "x and out must lie at multiples of 16 bytes");
+  INF_CHECK_ARG(aligned(offsets, 4) && aligned(sorted, 4),
+                "offsets and sorted must lie at multiples of 4 bytes");
+  if (int st_ = require_device()) return st_;
+  ExpertProduct p{};
+  p.m[0] = mat(w0);
+  p.mats = w1 ? 2 : 1;
+  if (w1) p.m[1] = mat(w1);
+  p.x = x;
+  p.x_scales = x_scales;
+  p.A = x_rows * k;
+  p.k = k;
+  p.offsets = offsets;
+  p.sorted = sorted;
+  p.out_dtype = out_dtype;
+  p.out = out;
+  return launch_expert_product(as_stream(stream), p);
+}
+
+}  // namespace
+}  // namespace inferno
+
+using namespace inferno;
+
+extern "C" {
+
+int inferno_mxfp4_quantize(void* stream, const void* x, int x_dtype, size_t rows, size_t cols,
+                           void* codes, uint8_t* scales, void* values) {
+  clear_error();
+  INF_CHECK_ARG(x_dtype == INFERNO_F32 || x_dtype == INFERNO_BF16, "x dtype must be F32 or BF16");
+  INF_CHECK_ARG(cols > 0 && cols % kMxBlock == 0, "the columns must be a multiple of 32");
+  if (rows == 0) return INFERNO_OK;
+  INF_CHECK_ARG(cols < (size_t(1) << 32) && rows < (size_t(1) << 32) &&
+                    rows * cols <= (size_t(1) << 34),
+                "too many values");
+  INF_CHECK_ARG(x && codes && scales, "null pointer");
+  INF_CHECK_ARG(aligned(x, 16) && aligned(codes, 16) && aligned(values, 16),
+                "x, codes and values must lie at multiples of 16 bytes");
+  if (int st_ = require_device()) return st_;
+  return launch_mxfp4_quantize(as_stream(stream), x, x_dtype, rows * cols, codes, scales, values);
+}
+
+size_t inferno_mxfp4_packed_bytes(const inferno_experts* w) {
+  clear_error();
+  if (check_shape("given", w)) return 0;
+  if (w->format != INFERNO_MXFP4) {
+    set_error("matrices in bf16 are not packed");
+    return 0;
+  }
+  return mx_layout(mat(w)).bytes;
+}
+
+int inferno_mxfp4_pack(void* stream, const inferno_experts* w, const void* codes,
+                       size_t codes_bytes, const uint8_t* scales, size_t scales_bytes,
+                       void* packed) {
+  clear_error();
+  int st;
+  if ((st = check_shape("given", w))) return st;
+  INF_CHECK_ARG(w->format == INFERNO_MXFP4, "matrices in bf16 are not packed");
+  const size_t rows = w->experts * w->rows;
+  if ((st = check_bytes("given", "codes", codes_bytes, rows * (w->cols / 2)))) return st;
+  if ((st = check_bytes("given", "scales", scales_bytes, rows * (w->cols / kMxBlock)))) return st;
+  if ((st = check_bytes("given", "data", w->data_bytes, mx_layout(mat(w)).bytes))) return st;
+  INF_CHECK_ARG(codes && scales && packed, "null pointer");
+  INF_CHECK_ARG(aligned(codes, 16) && aligned(packed, 16),
+                "codes and the packed matrix must lie at multiples of 16 bytes");
+  if (int st_ = require_device()) return st_;
+  return launch_mxfp4_pack(as_stream(stream), mat(w), codes, scales, packed);
+}
+
+int inferno_grouped_matmul(void* stream, const inferno_experts* w, const void* x, int x_dtype,
+                           const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
+                           const uint32_t* sorted, size_t k, int out_dtype, void* out) {
+  clear_error();
+  if (int st = check_mat("weight", w)) return st;
+  return run_product(stream, w, nullptr, x, x_dtype, x_scales, x_rows, offsets, sorted, k,
+                     out_dtype, out);
+}
+
+int inferno_grouped_gate_up_swiglu(void* stream, const inferno_experts* gate,
+                                   const inferno_experts* up, const void* x, int x_dtype,
+                                   const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
+                                   const uint32_t* sorted, size_t k, int out_dtype, void* out) {
+  clear_error();
+  int st;
+  if ((st = check_mat("gate", gate))) return st;
+  if ((st = check_mat("up", up))) return st;
+  INF_CHECK_ARG(gate->experts == up->experts && gate->rows == up->rows && gate->cols == up->cols &&
+                    gate->format == up->format,
+                "the gate and up matrices must have the same sizes and format");
+  return run_product(stream, gate, up, x, x_dtype, x_scales, x_rows, offsets, sorted, k, out_dtype,
+                     out);
+}
+
+}  // extern "C"

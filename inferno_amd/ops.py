@@ -7,7 +7,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import BF16, F32, I8, Q8_0, LayerDesc, W4Desc, check, lib
+from ._lib import BF16, F32, I8, MXFP4, Q8_0, ExpertsDesc, LayerDesc, W4Desc, check, lib
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
 
@@ -363,6 +363,117 @@ def w4_moe(gate, up, down, x, ids, weights, k, x_scales=None):
     _run(x, lib().inferno_w4_moe, gate.ref, up.ref, down.ref, _at(x), dt, xs, xg, _at(ids),
          _at(weights), T, k, _at(out), _at(ws), n)
     return out
+
+
+def mxfp4_quantize(x, values=False):
+    """Rows to 4-bit floating point with a scale per 32 columns
+    (inferno_mxfp4_quantize): (codes uint8 [rows, cols / 2], scales uint8 [rows,
+    cols / 32]) of x, fp32 or bf16 [rows, cols]; with ``values`` also what the codes
+    stand for, in x's type."""
+    _rows_of(x, "x", tuple(_DT))
+    T, H = x.shape
+    if H == 0 or H % 32:
+        raise ValueError(f"the columns must be a multiple of 32, got {H}")
+    codes = torch.empty(T, H // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(T, H // 32, dtype=torch.uint8, device=x.device)
+    held = torch.empty_like(x) if values else None
+    _run(x, lib().inferno_mxfp4_quantize, _at(x), _DT[x.dtype], T, H, _at(codes), _at(scales),
+         _at(held))
+    return (codes, scales, held) if values else (codes, scales)
+
+
+class Experts:
+    """Weights of the products grouped by expert (struct inferno_experts): one
+    matrix [rows, cols], or one per expert [E, rows, cols]. A bf16 tensor is used
+    as it lies and kept. MXFP4 is ``codes`` (uint8 [..., cols / 2], the even column
+    in the low nibble) and ``scales`` (uint8 [..., cols / 32]), packed once, here, on
+    the current stream (inferno_mxfp4_pack), which is waited for: the handle may be
+    used on any stream at once, and the tensors are not kept. While the stream is
+    being captured nothing is waited for; such a handle holds its matrices after the
+    graph's first replay."""
+
+    def __init__(self, weights, scales=None):
+        dtype = torch.bfloat16 if scales is None else torch.uint8
+        if weights.dtype != dtype or weights.dim() not in (2, 3) or not weights.is_contiguous():
+            raise ValueError(f"{'weights' if scales is None else 'codes'} must be a contiguous 2-D "
+                             f"or 3-D {dtype} tensor, got {weights.dtype} {tuple(weights.shape)}")
+        self.device = _dev(weights).device
+        self.experts = weights.shape[0] if weights.dim() == 3 else 1
+        self.rows = weights.shape[-2]
+        self.cols = weights.shape[-1] * (1 if scales is None else 2)
+        self.mxfp4 = scales is not None
+        if self.cols % (32 if self.mxfp4 else 8):
+            raise ValueError(f"the columns must be a multiple of {32 if self.mxfp4 else 8}, got "
+                             f"{self.cols}")
+        d = ExpertsDesc(self.experts, self.rows, self.cols, MXFP4 if self.mxfp4 else BF16, None, 0)
+        self.desc, self.ref = d, C.byref(d)
+        if not self.mxfp4:
+            self.data = weights
+            d.data, d.data_bytes = weights.data_ptr(), weights.numel() * 2
+            return
+        _like(weights, "scales", scales, torch.uint8, *weights.shape[:-1], self.cols // 32)
+        d.data_bytes = lib().inferno_mxfp4_packed_bytes(self.ref)
+        self.data = torch.empty(d.data_bytes, dtype=torch.uint8, device=self.device)
+        _run(weights, lib().inferno_mxfp4_pack, self.ref, _at(weights), weights.numel(), _at(scales),
+             scales.numel(), _at(self.data))
+        d.data = self.data.data_ptr()
+        stream = torch.cuda.current_stream(self.device)
+        with torch.cuda.device(self.device):
+            if not torch.cuda.is_current_stream_capturing():
+                stream.synchronize()
+
+
+def _grouped(fn, mats, x, x_scales, offsets, sorted_, k, out_dtype, out):
+    w = mats[0]
+    fp4 = x.dtype == torch.uint8
+    _rows_of(x, "x", (torch.bfloat16, torch.uint8) if w.mxfp4 else (torch.bfloat16,))
+    T = x.shape[0]
+    if x.shape[1] != (w.cols // 2 if fp4 else w.cols) or any(m.device != x.device for m in mats):
+        raise ValueError(f"x must be [rows, {w.cols}] in bf16{' or MXFP4' if w.mxfp4 else ''} on the "
+                         f"weights' device {w.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    if fp4 != (x_scales is not None):
+        raise ValueError("x_scales belong to MXFP4 rows, which need them")
+    if fp4:
+        _like(x, "x_scales", x_scales, torch.uint8, T, w.cols // 32)
+    if k < 1 or (sorted_ is None and k != 1):
+        raise ValueError(f"k must be positive, and 1 without sorted_, got {k}")
+    if offsets is not None:
+        _like(x, "offsets", offsets, torch.int32, w.experts + 1)
+    if sorted_ is not None:
+        _like(x, "sorted_", sorted_, torch.int32, T * k)
+    if out is None:
+        if out_dtype not in _DT:
+            raise ValueError(f"out_dtype must be one of {tuple(_DT)}, got {out_dtype}")
+        out = torch.empty(T * k, w.rows, dtype=out_dtype, device=x.device)
+    else:
+        if out.dtype not in _DT:
+            raise ValueError(f"out must be one of {tuple(_DT)}, got {out.dtype}")
+        _like(x, "out", out, out.dtype, T * k, w.rows)
+    _run(x, fn, *(m.ref for m in mats), _at(x), MXFP4 if fp4 else BF16, _at(x_scales), T,
+         _at(offsets), _at(sorted_), k, _DT[out.dtype], _at(out))
+    return out
+
+
+def grouped_matmul(w, x, x_scales=None, *, offsets=None, sorted_=None, k=1,
+                   out_dtype=torch.float32, out=None):
+    """x[a / k] W[e]^T for the rows a = sorted_[offsets[e] : offsets[e + 1]] of every
+    expert e (inferno_grouped_matmul), groups of any size. ``w``: Experts. ``x``: bf16
+    [rows, cols], or with weights in MXFP4 also mxfp4_quantize's codes and scales.
+    ``offsets`` and ``sorted_`` are ``dispatch``'s; without sorted_ the rows lie in the
+    order of the experts, without offsets all rows go through one matrix. The result
+    has rows * k rows; those of no group are left as ``out`` holds them (without
+    ``out``: undefined)."""
+    return _grouped(lib().inferno_grouped_matmul, (w,), x, x_scales, offsets, sorted_, k, out_dtype,
+                    out)
+
+
+def grouped_gate_up_swiglu(gate, up, x, x_scales=None, *, offsets=None, sorted_=None, k=1,
+                           out_dtype=torch.bfloat16, out=None):
+    """silu(x gate[e]^T) * (x up[e]^T) of rows grouped by expert
+    (inferno_grouped_gate_up_swiglu); arguments as in ``grouped_matmul``. In bf16 the
+    result is grouped_matmul's x for the down matrices, with k = 1."""
+    return _grouped(lib().inferno_grouped_gate_up_swiglu, (gate, up), x, x_scales, offsets, sorted_,
+                    k, out_dtype, out)
 
 
 class NormRouter:
