@@ -338,14 +338,20 @@ int inferno_mxfp4_pack(void* stream, const inferno_experts* w, const void* codes
  *   out     [x_rows k, rows] F32 or BF16, which may not overlap an input
  * Sums are held in fp32, products are exact. A row that holds a NaN, an infinity or
  * a scale of 255 changes its own results alone. x and out lie at multiples of 16
- * bytes; x_rows k <= 2^22. x_rows = 0 does nothing. */
+ * bytes; x_rows k <= 2^22. x_rows = 0 does nothing. The workspace takes
+ * inferno_grouped_workspace_bytes at a multiple of 16 bytes (NULL where that is 0,
+ * as it is for most products); calls that overlap need one each. */
+size_t inferno_grouped_workspace_bytes(const inferno_experts* w, int matrices, int x_dtype,
+                                       size_t x_rows, size_t k, int grouped);
 int inferno_grouped_matmul(void* stream, const inferno_experts* w, const void* x, int x_dtype,
                            const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
-                           const uint32_t* sorted, size_t k, int out_dtype, void* out);
+                           const uint32_t* sorted, size_t k, int out_dtype, void* out,
+                           void* workspace, size_t workspace_bytes);
 int inferno_grouped_gate_up_swiglu(void* stream, const inferno_experts* gate,
                                    const inferno_experts* up, const void* x, int x_dtype,
                                    const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
-                                   const uint32_t* sorted, size_t k, int out_dtype, void* out);
+                                   const uint32_t* sorted, size_t k, int out_dtype, void* out,
+                                   void* workspace, size_t workspace_bytes);
 
 /* --------------------------------------------------------------- combine */
 

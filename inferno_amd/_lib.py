@@ -97,10 +97,11 @@ SIGNATURES = {
     "inferno_mxfp4_quantize": (_i, [_vp, _vp, _i, _sz, _sz, _vp, _vp, _vp]),
     "inferno_mxfp4_packed_bytes": (_sz, [C.POINTER(ExpertsDesc)]),
     "inferno_mxfp4_pack": (_i, [_vp, C.POINTER(ExpertsDesc), _vp, _sz, _vp, _sz, _vp]),
+    "inferno_grouped_workspace_bytes": (_sz, [C.POINTER(ExpertsDesc), _i, _i, _sz, _sz, _i]),
     "inferno_grouped_matmul": (_i, [_vp, C.POINTER(ExpertsDesc), _vp, _i, _vp, _sz, _vp, _vp, _sz,
-                                    _i, _vp]),
+                                    _i, _vp, _vp, _sz]),
     "inferno_grouped_gate_up_swiglu": (_i, [_vp, C.POINTER(ExpertsDesc), C.POINTER(ExpertsDesc),
-                                            _vp, _i, _vp, _sz, _vp, _vp, _sz, _i, _vp]),
+                                            _vp, _i, _vp, _sz, _vp, _vp, _sz, _i, _vp, _vp, _sz]),
     "inferno_moe_layer_workspace_bytes": (_sz, [C.POINTER(LayerDesc), _sz]),
     "inferno_moe_layer_forward": (_i, [_vp, C.POINTER(LayerDesc), _vp, _i, _vp, _sz, _vp, _vp,
                                        _vp, _vp, _sz]),

@@ -50,9 +50,25 @@ int check_mat(const char* what, const inferno_experts* w) {
   return INFERNO_OK;
 }
 
+constexpr size_t kMostRows = size_t(1) << 22;
+
+ExpertProduct product(const inferno_experts* w0, const inferno_experts* w1, const uint8_t* x_scales,
+                      size_t rows, size_t k, const uint32_t* offsets) {
+  ExpertProduct p{};
+  p.m[0] = mat(w0);
+  p.mats = w1 ? 2 : 1;
+  if (w1) p.m[1] = mat(w1);
+  p.x_scales = x_scales;
+  p.A = rows;
+  p.k = k;
+  p.offsets = offsets;
+  return p;
+}
+
 int run_product(void* stream, const inferno_experts* w0, const inferno_experts* w1, const void* x,
                 int x_dtype, const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
-                const uint32_t* sorted, size_t k, int out_dtype, void* out) {
+                const uint32_t* sorted, size_t k, int out_dtype, void* out, void* workspace,
+                size_t workspace_bytes) {
   INF_CHECK_ARG(out_dtype == INFERNO_F32 || out_dtype == INFERNO_BF16,
                 "out dtype must be F32 or BF16");
   INF_CHECK_ARG(x_dtype == INFERNO_BF16 || (x_dtype == INFERNO_MXFP4 && w0->format == INFERNO_MXFP4),
@@ -62,27 +78,22 @@ int run_product(void* stream, const inferno_experts* w0, const inferno_experts* 
   INF_CHECK_ARG(!sorted || offsets, "sorted rows need the experts' offsets");
   INF_CHECK_ARG(offsets || w0->experts == 1, "several experts need offsets");
   if (x_rows == 0) return INFERNO_OK;
-  const size_t most = size_t(1) << 22;
-  INF_CHECK_ARG(x_rows <= most && k <= most && x_rows * k <= most, "too many rows");
+  INF_CHECK_ARG(x_rows <= kMostRows && k <= kMostRows && x_rows * k <= kMostRows, "too many rows");
   INF_CHECK_ARG(x && out, "null pointer");
   INF_CHECK_ARG((x_dtype == INFERNO_MXFP4) == (x_scales != nullptr),
                 "x_scales belong to MXFP4 rows, which need them");
   INF_CHECK_ARG(aligned(x, 16) && aligned(out, 16), "x and out must lie at multiples of 16 bytes");
   INF_CHECK_ARG(aligned(offsets, 4) && aligned(sorted, 4),
                 "offsets and sorted must lie at multiples of 4 bytes");
+  ExpertProduct p = product(w0, w1, x_scales, x_rows * k, k, offsets);
+  if (int st = need_ws(workspace, workspace_bytes, product_workspace(p))) return st;
+  INF_CHECK_ARG(aligned(workspace, 16), "the workspace must lie at a multiple of 16 bytes");
   if (int st_ = require_device()) return st_;
-  ExpertProduct p{};
-  p.m[0] = mat(w0);
-  p.mats = w1 ? 2 : 1;
-  if (w1) p.m[1] = mat(w1);
   p.x = x;
-  p.x_scales = x_scales;
-  p.A = x_rows * k;
-  p.k = k;
-  p.offsets = offsets;
   p.sorted = sorted;
   p.out_dtype = out_dtype;
   p.out = out;
+  p.workspace = workspace;
   return launch_expert_product(as_stream(stream), p);
 }
 
@@ -137,19 +148,34 @@ int inferno_mxfp4_pack(void* stream, const inferno_experts* w, const void* codes
   return launch_mxfp4_pack(as_stream(stream), mat(w), codes, scales, packed);
 }
 
+size_t inferno_grouped_workspace_bytes(const inferno_experts* w, int matrices, int x_dtype,
+                                       size_t x_rows, size_t k, int grouped) {
+  clear_error();
+  if (check_shape("given", w) || x_rows > kMostRows || k > kMostRows || x_rows * k > kMostRows ||
+      x_rows * k == 0)
+    return 0;
+  static const uint8_t scale = 127;  // (only whether there are scales and offsets counts)
+  static const uint32_t offset = 0;
+  return product_workspace(product(w, matrices == 2 ? w : nullptr,
+                                   x_dtype == INFERNO_MXFP4 ? &scale : nullptr, x_rows * k, k,
+                                   grouped ? &offset : nullptr));
+}
+
 int inferno_grouped_matmul(void* stream, const inferno_experts* w, const void* x, int x_dtype,
                            const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
-                           const uint32_t* sorted, size_t k, int out_dtype, void* out) {
+                           const uint32_t* sorted, size_t k, int out_dtype, void* out, void* workspace,
+                           size_t workspace_bytes) {
   clear_error();
   if (int st = check_mat("weight", w)) return st;
   return run_product(stream, w, nullptr, x, x_dtype, x_scales, x_rows, offsets, sorted, k,
-                     out_dtype, out);
+                     out_dtype, out, workspace, workspace_bytes);
 }
 
 int inferno_grouped_gate_up_swiglu(void* stream, const inferno_experts* gate,
                                    const inferno_experts* up, const void* x, int x_dtype,
                                    const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
-                                   const uint32_t* sorted, size_t k, int out_dtype, void* out) {
+                                   const uint32_t* sorted, size_t k, int out_dtype, void* out, void* workspace,
+                           size_t workspace_bytes) {
   clear_error();
   int st;
   if ((st = check_mat("gate", gate))) return st;
@@ -158,7 +184,7 @@ int inferno_grouped_gate_up_swiglu(void* stream, const inferno_experts* gate,
                     gate->format == up->format,
                 "the gate and up matrices must have the same sizes and format");
   return run_product(stream, gate, up, x, x_dtype, x_scales, x_rows, offsets, sorted, k, out_dtype,
-                     out);
+                     out, workspace, workspace_bytes);
 }
 
 }  // extern "C"

@@ -50,7 +50,19 @@ struct ExpertProduct {
   const uint32_t* sorted;  // [A], or null
   int out_dtype;
   void* out;               // [A, rows]
+  void* workspace;         // product_workspace bytes
 };
+
+// Which kernel takes a product: tiles (experts_tiles.hip) of 64 * width weight rows,
+// the columns shared by `splits` workgroups; or 16 * width grouped rows
+// (experts_rows.hip), the columns shared by `shares` wavefronts.
+struct ExpertPlan {
+  bool tiles;
+  int width, shares;
+  size_t splits;
+};
+ExpertPlan plan_product(const ExpertProduct& p);
+size_t product_workspace(const ExpertProduct& p);
 int launch_expert_product(hipStream_t s, const ExpertProduct& p);
 
 }  // namespace inferno

@@ -16,6 +16,7 @@ struct Product {
   const uint32_t* ws[2];    // packed scales
   const uint8_t* x;
   const uint8_t* xs;        // scales of codes
+  uint32_t x_bytes;         // of x; below 2^32 where rows go through LDS
   const uint32_t* offsets;  // or null
   const uint32_t* sorted;   // or null
   uint32_t E, A, k;
@@ -23,6 +24,8 @@ struct Product {
   uint32_t tiles, chunks, quads;  // packed weights of an expert: 16-row tiles, chunks, four chunks
   void* out;
   bool out_f32;
+  uint32_t splits;          // shares of the columns in launches of their own workgroups
+  float* partial;           // [splits][matrices][A][N, to a multiple of 4]: their sums
 };
 
 // Tile `t` of at most TM rows of one expert, tiles counted expert by expert:
@@ -77,6 +80,12 @@ __device__ __forceinline__ uint32_t find_tile(const Product& p, uint32_t t, uint
 // Result row of grouped row c < A; A or more: none (an index out of range).
 __device__ __forceinline__ uint32_t result_row(const Product& p, uint32_t c) {
   return p.sorted ? p.sorted[c] : c;
+}
+
+// Where the sums of a share, matrix and grouped row begin in `partial`.
+__device__ __forceinline__ size_t partial_row(const Product& p, uint32_t mats, uint32_t split,
+                                              uint32_t m, uint32_t c) {
+  return ((size_t(split) * mats + m) * p.A + c) * ((p.N + 3) & ~3u);
 }
 
 // 2^(byte - 127) where only the exponent is read (v_cvt_scalef32_*: 255 is NaN).
@@ -134,4 +143,10 @@ __device__ __forceinline__ void store4(const Product& p, uint32_t row, uint32_t 
 }
 
 }  // namespace experts
+
+// Tiles of up to 128 rows by 16 * 4 * width weight rows of both matrices; `tiles`:
+// at least as many as there are.
+int launch_experts_tiles(hipStream_t s, const experts::Product& p, int mats, bool wfp4, bool xfp4,
+                         size_t tiles, int width);
+
 }  // namespace inferno

@@ -1,10 +1,15 @@
-// Products of rows grouped by expert: 16 weight rows by 16 grouped rows, the
-// operands straight from memory in the order of the matrix instructions.
+// Products of rows grouped by expert, few rows: one or two tiles of 16 weight rows
+// (of both matrices) by 16 or 32 grouped rows, the operands straight from memory to registers in the
+// order of the matrix instructions.
 //
 // The weights are the first operand (lane l: row l % 16, quarter l / 16 of the
 // columns of a step), the grouped rows the second, so that a lane's four sums
-// are four neighbouring values of one result row. A workgroup's wavefronts share
-// the columns, 128 at a time, and add their sums in order through LDS.
+// are four neighbouring values of one result row. Of a workgroup's four wavefronts
+// SHARES take the same weight rows and share the columns; they add their sums in
+// order through LDS. What bounds it is how many bytes are on their way: every
+// wavefront loads kAhead chunks of 128 columns before it uses the first.
+#include <cmath>
+
 #include "experts_dev.hpp"
 
 namespace inferno {
@@ -14,85 +19,247 @@ using namespace experts;
 
 constexpr int kWaves = 4;
 
-template <bool WFP4, bool XFP4, int MATS>
-__global__ void __launch_bounds__(kWaves* kWave) experts_rows_kernel(Product p) {
-  __shared__ floatx4 part[kWaves][MATS][kWave];
+// One chunk's operands of a wavefront, 128 columns.
+template <bool WFP4, bool XFP4, int RT, int NB>
+struct Chunk {
+  uint4 w[RT][WFP4 ? 1 : 4], x[NB][XFP4 ? 1 : 4];
+  uint32_t ws[RT], xs[NB];
+};
+
+template <bool WFP4, bool XFP4, int MATS, int RT, int NB, int SHARES>
+__global__ void __launch_bounds__(kWaves* kWave) experts_rows_kernel(Product p, uint32_t blocks) {
+  using C = Chunk<WFP4, XFP4, RT, NB>;
+  constexpr int kAhead = WFP4 && XFP4 ? 4 : 2;
+  constexpr int kPerMat = RT / MATS;
+  __shared__ floatx4 part[SHARES > 1 ? kWaves : 1][RT][NB][kWave];
   uint32_t e, c0, c1;
-  const uint32_t slot = blockIdx.x / p.tiles;
-  if (slot >= find_tile<16>(p, slot, e, c0, c1)) return;
+  const uint32_t slot = blockIdx.x / blocks;
+  if (slot >= find_tile<16 * NB>(p, slot, e, c0, c1)) return;
   const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t tile = blockIdx.x - slot * p.tiles;  // of weight rows
-  const uint32_t c = c0 + n;
-  const uint32_t a = c < c1 ? result_row(p, c) : p.A;
-  const bool on = a < p.A;
-  const size_t xrow = on ? a / p.k : 0;
-  const uint32_t wrow = min(tile * 16 + n, p.N - 1);
-  floatx4 acc[MATS];
+  const uint32_t share = wave % SHARES;
+  // the wavefront's first weight tile of each matrix
+  const uint32_t first_tile =
+      ((blockIdx.x - slot * blocks) * (kWaves / SHARES) + wave / SHARES) * kPerMat;
+  const uint32_t pitch = XFP4 ? p.K / 2 : p.K * 2;
+  // rows behind the tile's last are computed as it is, and not stored
+  uint32_t a[NB];
+  const uint8_t* x[NB];
+  const uint8_t* xs[NB];
 #pragma unroll
-  for (int m = 0; m < MATS; ++m) acc[m] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const uint4 none = make_uint4(0, 0, 0, 0);
-  for (uint32_t ch = wave; ch < p.chunks; ch += kWaves) {
+  for (int b = 0; b < NB; ++b) {
+    a[b] = result_row(p, min(c0 + 16 * b + n, c1 - 1));
+    const size_t row = a[b] < p.A ? a[b] / p.k : 0;
+    x[b] = p.x + row * pitch;
+    xs[b] = p.xs + row * (p.K / kMxBlock);
+  }
+  const uint8_t* w[RT];
+  const uint32_t* ws[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const uint32_t tile = min(first_tile + r % kPerMat, p.tiles - 1);
+    const size_t at = size_t(e) * p.tiles + tile;
     if constexpr (WFP4) {
-      const uint32_t col = ch * kMxChunk + 32 * g;
-      const bool in = on && col < p.K;  // whole blocks of 32
-      const size_t wt = (size_t(e) * p.tiles + tile);
-      uint4 w[MATS];
-      uint32_t ws[MATS];
+      w[r] = p.w[r / kPerMat] + at * p.chunks * 1024 + lane * 16;
+      ws[r] = p.ws[r / kPerMat] + at * p.quads * 64 + lane;
+    } else {
+      w[r] = p.w[r / kPerMat] + (size_t(e) * p.N + min(tile * 16 + n, p.N - 1)) * pitch;
+    }
+  }
+  // column of the lane's 16 bytes number j of a chunk
+  auto column = [&](uint32_t ch, int j) {
+    return ch * kMxChunk + (WFP4 ? 32 * g + 8 * j : 32 * j + 8 * g);
+  };
+  auto load = [&](uint32_t ch, C& v) {
 #pragma unroll
-      for (int m = 0; m < MATS; ++m) {
-        w[m] = reinterpret_cast<const uint4*>(p.w[m])[(wt * p.chunks + ch) * 64 + lane];
-        ws[m] = p.ws[m][(wt * p.quads + ch / 4) * 64 + lane] >> (8 * (ch % 4)) & 255u;
-      }
-      if constexpr (XFP4) {
-        const size_t at = xrow * (p.K / 32) + col / 32;
-        const uint4 xv = in ? reinterpret_cast<const uint4*>(p.x)[at] : none;
-        const uint32_t xs = in ? p.xs[at] : 127u;
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) acc[m] = mfma_fp4(w[m], xv, acc[m], ws[m], xs);
+    for (int m = 0; m < RT; ++m) {
+      if constexpr (WFP4) {
+        v.w[m][0] = *reinterpret_cast<const uint4*>(w[m] + size_t(ch) * 1024);
+        v.ws[m] = ws[m][size_t(ch / 4) * 64] >> (8 * (ch % 4));
       } else {
-        const uint4* at = reinterpret_cast<const uint4*>(p.x + (xrow * p.K + (in ? col : 0)) * 2);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint4 xv = in ? at[j] : none;
-#pragma unroll
-          for (int m = 0; m < MATS; ++m) {
-            const uint32_t cw = j == 0 ? w[m].x : j == 1 ? w[m].y : j == 2 ? w[m].z : w[m].w;
-            acc[m] = mfma_bf16(widen(cw, scale_of(ws[m])), __builtin_bit_cast(bf16x8, xv), acc[m]);
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t col = ch * kMxChunk + 32 * j + 8 * g;
-        const bool in = col < p.K;
-        const uint4 xv =
-            on && in ? *reinterpret_cast<const uint4*>(p.x + (xrow * p.K + col) * 2) : none;
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-          const size_t at = ((size_t(e) * p.N + wrow) * p.K + col) * 2;
-          const uint4 w = in ? *reinterpret_cast<const uint4*>(p.w[m] + at) : none;
-          acc[m] = mfma_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, xv), acc[m]);
+          const uint32_t col = column(ch, j);
+          v.w[m][j] = *reinterpret_cast<const uint4*>(w[m] + (col < p.K ? col * 2 : 0));
         }
       }
     }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      if constexpr (XFP4) {
+        const uint32_t col = column(ch, 0);
+        v.x[b][0] = *reinterpret_cast<const uint4*>(x[b] + (col < p.K ? col / 2 : 0));
+        v.xs[b] = xs[b][col < p.K ? col / kMxBlock : 0];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t col = column(ch, j);
+          v.x[b][j] = *reinterpret_cast<const uint4*>(x[b] + (col < p.K ? col * 2 : 0));
+        }
+      }
+    }
+  };
+  floatx4 acc[RT][NB];
+#pragma unroll
+  for (int m = 0; m < RT; ++m)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[m][b] = floatx4{0.f, 0.f, 0.f, 0.f};
+  auto use = [&](uint32_t ch, C& v) {
+    if ((ch + 1) * kMxChunk > p.K) {  // the last chunk: nothing behind the last column
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t keep = column(ch, j) < p.K ? ~0u : 0u;
+        auto cut = [&](uint4& u) { u = make_uint4(u.x & keep, u.y & keep, u.z & keep, u.w & keep); };
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          if (j == 0 || !XFP4) cut(v.x[b][XFP4 ? 0 : j]);
+        if constexpr (!WFP4) {
+#pragma unroll
+          for (int m = 0; m < RT; ++m) cut(v.w[m][j]);
+        }
+      }
+    }
+    if constexpr (WFP4 && XFP4) {
+#pragma unroll
+      for (int m = 0; m < RT; ++m)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          acc[m][b] = mfma_fp4(v.w[m][0], v.x[b][0], acc[m][b], v.ws[m], v.xs[b]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int m = 0; m < RT; ++m) {
+          bf16x8 f;
+          if constexpr (WFP4) {
+            const uint4 c = v.w[m][0];
+            f = widen(j == 0 ? c.x : j == 1 ? c.y : j == 2 ? c.z : c.w, scale_of(v.ws[m] & 255u));
+          } else {
+            f = __builtin_bit_cast(bf16x8, v.w[m][j]);
+          }
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            acc[m][b] = mfma_bf16(f, __builtin_bit_cast(bf16x8, v.x[b][j]), acc[m][b]);
+        }
+    }
+  };
+  // this wavefront's chunks
+  const uint32_t first = p.chunks * share / SHARES, last = p.chunks * (share + 1) / SHARES;
+  if (first < last) {
+    C v[kAhead];
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) load(min(first + d, last - 1), v[d]);
+    for (uint32_t ch = first; ch < last; ch += kAhead) {
+#pragma unroll
+      for (int d = 0; d < kAhead; ++d) {
+        if (ch + d < last) use(ch + d, v[d]);
+        load(min(ch + d + kAhead, last - 1), v[d]);
+      }
+    }
   }
+  if constexpr (SHARES > 1) {
 #pragma unroll
-  for (int m = 0; m < MATS; ++m) part[wave][m][lane] = acc[m];
-  __syncthreads();
-  if (wave) return;
+    for (int m = 0; m < RT; ++m)
 #pragma unroll
-  for (int m = 0; m < MATS; ++m)
-    for (int v = 1; v < kWaves; ++v) acc[m] += part[v][m][lane];
-  if (!on) return;
-  float y[4];
+      for (int b = 0; b < NB; ++b) part[wave][m][b][lane] = acc[m][b];
+    __syncthreads();
+  }
+  // the wavefronts of a share write the 16 rows number b in turn
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = MATS == 2 ? silu_mul(acc[0][i], acc[MATS - 1][i]) : acc[0][i];
-  store4(p, a, tile * 16 + 4 * g, y);
+  for (int b = 0; b < NB; ++b) {
+    if (share != uint32_t(b % SHARES)) continue;
+    if constexpr (SHARES > 1) {
+#pragma unroll
+      for (int m = 0; m < RT; ++m) {
+        acc[m][b] = part[wave - share][m][b][lane];
+        for (int v = 1; v < SHARES; ++v) acc[m][b] += part[wave - share + v][m][b][lane];
+      }
+    }
+    if (c0 + 16 * b + n >= c1 || a[b] >= p.A) continue;
+#pragma unroll
+    for (int r = 0; r < kPerMat; ++r) {
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        y[i] = MATS == 2 ? silu_mul(acc[r][b][i], acc[r + RT - kPerMat][b][i]) : acc[r][b][i];
+      store4(p, a[b], (first_tile + r) * 16 + 4 * g, y);
+    }
+  }
+}
+
+template <int RT, int NB, int SHARES>
+int launch(hipStream_t s, const Product& p, int mats, bool wfp4, bool xfp4, size_t tiles) {
+  const size_t per = kWaves / SHARES * RT / mats;  // weight tiles of a workgroup
+  const size_t blocks = (p.tiles + per - 1) / per;
+  if (tiles * blocks * (kWaves * kWave) >= size_t(1) << 32) {
+    set_error("too many rows for one launch");
+    return INFERNO_ERR_INVALID;
+  }
+  auto go = [&](auto wf, auto xf) {
+    constexpr bool W = decltype(wf)::value, X = decltype(xf)::value;
+    const unsigned grid = unsigned(tiles * blocks), threads = kWaves * kWave;
+    if (mats == 1)
+      experts_rows_kernel<W, X, 1, RT, NB, SHARES><<<grid, threads, 0, s>>>(p, unsigned(blocks));
+    else if constexpr (RT > 1)
+      experts_rows_kernel<W, X, 2, RT, NB, SHARES><<<grid, threads, 0, s>>>(p, unsigned(blocks));
+  };
+  if (!wfp4) go(std::false_type{}, std::false_type{});
+  else if (xfp4) go(std::true_type{}, std::true_type{});
+  else go(std::true_type{}, std::false_type{});
+  INF_LAUNCHED();
+  return INFERNO_OK;
 }
 
 }  // namespace
+
+// The rules below compare sizes that decide: how many rows an expert has, how many
+// workgroups a form makes, and how much each of them has to do.
+ExpertPlan plan_product(const ExpertProduct& q) {
+  const ExpertMat& m = q.m[0];
+  const bool xfp4 = q.x_scales != nullptr;
+  ExpertPlan r{};
+  r.splits = 1;
+  // experts that the rows reach if each picks one by chance, and rows of one
+  const double E = double(m.experts), A = double(q.A), N = double(m.rows) * q.mats;
+  const double used = q.offsets ? E * (1.0 - std::pow(1.0 - 1.0 / E, A)) : 1.0;
+  const double rows = A / used;
+  // workgroups of the tile kernel, and of this one's narrow form with all wavefronts
+  // on one pair of weight tiles
+  const double tiles = q.offsets ? used * std::max(1.0, rows / 128 + 0.5) : std::ceil(A / 128);
+  auto blocks = [&](size_t width) { return tiles * std::ceil(N / double(64 * width)); };
+  const double groups = std::ceil(rows / 16) * used * std::ceil(N / 32);
+  const size_t pitch = xfp4 ? m.cols / 2 : m.cols * 2, stages = (pitch + 255) / 256;
+  // Enough workgroups of the wide tiles for all CUs: they win from a few rows an expert
+  // on, earlier the more a weight costs to load or widen. Fewer: their latency counts,
+  // and the rows kernel wins as long as its workgroups, which read every row again
+  // for 32 weight rows, have little to do.
+  const bool many = blocks(4) >= (m.fp4 ? 320 : 384);
+  const double least = m.fp4 ? (xfp4 ? 3 : 1.25) : m.cols < 1024 ? 4 : 6;
+  r.tiles = many ? rows > least
+                 : rows > 8 && groups * double(m.cols) > (m.fp4 ? 3.2e6 : 1.3e6);
+  if (switch_on("INFERNO_EXPERTS_TILES")) r.tiles = true;
+  if (switch_off("INFERNO_EXPERTS_TILES") || q.A / q.k * pitch >= size_t(1) << 32) r.tiles = false;
+  if (r.tiles) {
+    r.width = many && (m.fp4 || rows > 64) ? 4 : 2;
+    // shares of at least four stages, until they make a workgroup for every CU; of
+    // weights that are widened two for every CU
+    const bool widened = m.fp4 && !xfp4;
+    if (!many)
+      while (r.splits < 8 && r.splits * 8 <= stages &&
+             double(r.splits) * blocks(2) <= (widened && r.splits == 1 ? 256 : 128))
+        r.splits *= 2;
+  } else {
+    r.width = rows > 32 ? 2 : 1;
+    const double mine = groups / r.width;
+    r.shares = mine < 256 || (mine < 1024 && m.cols >= 4096) ? 4 : m.cols >= 1536 ? 2 : 1;
+  }
+  return r;
+}
+
+size_t product_workspace(const ExpertProduct& q) {
+  const ExpertPlan r = plan_product(q);
+  return r.splits > 1 ? r.splits * q.mats * q.A * ((q.m[0].rows + 3) / 4 * 16) : 0;
+}
 
 int launch_expert_product(hipStream_t s, const ExpertProduct& q) {
   Product p{};
@@ -116,22 +283,25 @@ int launch_expert_product(hipStream_t s, const ExpertProduct& q) {
   p.quads = uint32_t(l.quads);
   p.out = q.out;
   p.out_f32 = q.out_dtype == INFERNO_F32;
-  const size_t most = q.offsets ? q.A / 16 + std::min(m.experts, q.A) : (q.A + 15) / 16;
-  if (most * l.tiles * (kWaves * kWave) >= size_t(1) << 32) {
-    set_error("too many rows for one launch");
-    return INFERNO_ERR_INVALID;
-  }
-  const unsigned grid = unsigned(l.tiles * most);
-  auto go = [&](auto wf, auto xf) {
-    constexpr bool W = decltype(wf)::value, X = decltype(xf)::value;
-    if (q.mats == 2) experts_rows_kernel<W, X, 2><<<grid, kWaves * kWave, 0, s>>>(p);
-    else experts_rows_kernel<W, X, 1><<<grid, kWaves * kWave, 0, s>>>(p);
+  auto tiles_of = [&](size_t rows) {
+    return q.offsets ? q.A / rows + std::min(m.experts, q.A) : (q.A + rows - 1) / rows;
   };
-  if (!m.fp4) go(std::false_type{}, std::false_type{});
-  else if (q.x_scales) go(std::true_type{}, std::true_type{});
-  else go(std::true_type{}, std::false_type{});
-  INF_LAUNCHED();
-  return INFERNO_OK;
+  const bool xfp4 = q.x_scales != nullptr;
+  const size_t x_bytes = q.A / q.k * (xfp4 ? m.cols / 2 : m.cols * 2);
+  p.x_bytes = uint32_t(x_bytes);
+  const ExpertPlan plan = plan_product(q);
+  p.splits = uint32_t(plan.splits);
+  p.partial = static_cast<float*>(q.workspace);
+  if (plan.tiles) return launch_experts_tiles(s, p, q.mats, m.fp4, xfp4, tiles_of(128), plan.width);
+  const size_t tiles = tiles_of(16 * plan.width);
+  auto pick = [&](auto width) -> int {
+    constexpr int NB = decltype(width)::value;
+    if (plan.shares == 1) return launch<2, NB, 1>(s, p, q.mats, m.fp4, xfp4, tiles);
+    if (plan.shares == 2) return launch<2, NB, 2>(s, p, q.mats, m.fp4, xfp4, tiles);
+    return launch<2, NB, 4>(s, p, q.mats, m.fp4, xfp4, tiles);
+  };
+  if (plan.width == 1) return pick(std::integral_constant<int, 1>{});
+  return pick(std::integral_constant<int, 2>{});
 }
 
 }  // namespace inferno

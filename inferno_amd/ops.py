@@ -449,8 +449,11 @@ def _grouped(fn, mats, x, x_scales, offsets, sorted_, k, out_dtype, out):
         if out.dtype not in _DT:
             raise ValueError(f"out must be one of {tuple(_DT)}, got {out.dtype}")
         _like(x, "out", out, out.dtype, T * k, w.rows)
-    _run(x, fn, *(m.ref for m in mats), _at(x), MXFP4 if fp4 else BF16, _at(x_scales), T,
-         _at(offsets), _at(sorted_), k, _DT[out.dtype], _at(out))
+    dt = MXFP4 if fp4 else BF16
+    n = lib().inferno_grouped_workspace_bytes(w.ref, len(mats), dt, T, k, offsets is not None)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    _run(x, fn, *(m.ref for m in mats), _at(x), dt, _at(x_scales), T, _at(offsets), _at(sorted_), k,
+         _DT[out.dtype], _at(out), _at(ws), n)
     return out
 
 

@@ -11,6 +11,13 @@ FORMATS = [(False, False), (True, False), (True, True)]  # weights, rows in MXFP
 IDS = ["bf16", "mxfp4", "mxfp4-mxfp4"]
 
 
+@pytest.fixture(params=["rule", "tiles", "rows"])
+def kernels(request, monkeypatch):
+    """The kernel that the rule takes, and either one for all sizes."""
+    if request.param != "rule":
+        monkeypatch.setenv("INFERNO_EXPERTS_TILES", "1" if request.param == "tiles" else "0")
+
+
 def _call(mats, x, **kw):
     w = [ops.Experts(*m.parts) for m in mats]
     return (ops.grouped_matmul if len(w) == 1 else ops.grouped_gate_up_swiglu)(*w, *x, **kw)
@@ -33,7 +40,7 @@ SHAPES = [  # T, k, E, N, K, empty experts
 @pytest.mark.parametrize("w4,x4", FORMATS, ids=IDS)
 @pytest.mark.parametrize("mats", [1, 2])
 @pytest.mark.parametrize("T,k,E,N,K,empty", SHAPES)
-def test_grouped(cuda, T, k, E, N, K, empty, mats, w4, x4):
+def test_grouped(cuda, kernels, T, k, E, N, K, empty, mats, w4, x4):
     """Tokens that serve k experts, rows of their own, and rows in the experts' order."""
     g = torch.Generator().manual_seed(T + N + K)
     m = [ref.Mats(g, N, K, E, w4) for _ in range(mats)]
@@ -53,7 +60,7 @@ def test_grouped(cuda, T, k, E, N, K, empty, mats, w4, x4):
 @pytest.mark.parametrize("mats", [1, 2])
 @pytest.mark.parametrize("T,N,K", [(1, 48, 2048), (1, 1285, 96), (2, 16, 32), (9, 40, 1056), (16, 70, 4096),
                                    (33, 96, 224), (65, 33, 512), (129, 260, 192), (520, 300, 160)])
-def test_one_matrix(cuda, T, N, K, mats, w4, x4):
+def test_one_matrix(cuda, kernels, T, N, K, mats, w4, x4):
     g = torch.Generator().manual_seed(T + N + K)
     m = [ref.Mats(g, N, K, 0, w4) for _ in range(mats)]
     x, xv = ref.rows(g, T, K, x4)
@@ -66,7 +73,7 @@ def test_one_matrix(cuda, T, N, K, mats, w4, x4):
 @pytest.mark.gpu
 @pytest.mark.parametrize("mats", [1, 2])
 @pytest.mark.parametrize("T,N,K", [(1, 5, 8), (3, 16, 24), (20, 33, 136), (150, 130, 72), (260, 24, 1032)])
-def test_bf16_columns_of_eight(cuda, T, N, K, mats):
+def test_bf16_columns_of_eight(cuda, kernels, T, N, K, mats):
     g = torch.Generator().manual_seed(T + N + K)
     m = [ref.Mats(g, N, K, 3) for _ in range(mats)]
     offsets, sorted_ = ref.groups(g, T, 2, 3)
@@ -80,7 +87,7 @@ def test_bf16_columns_of_eight(cuda, T, N, K, mats):
 @pytest.mark.parametrize("w4,x4", FORMATS, ids=IDS)
 @pytest.mark.parametrize("counts", [[0, 0, 0, 200], [200, 0, 0, 0], [1, 198, 1, 0], [0, 0, 0, 0],
                                     [16, 16, 16, 16], [17, 15, 33, 31], [128, 1, 129, 127]])
-def test_uneven_groups(cuda, counts, w4, x4):
+def test_uneven_groups(cuda, kernels, counts, w4, x4):
     g = torch.Generator().manual_seed(sum(counts))
     m = [ref.Mats(g, 80, 192, 4, w4)]
     A = 400  # rows behind the last group stay as they are
@@ -98,7 +105,7 @@ def test_uneven_groups(cuda, counts, w4, x4):
 @pytest.mark.gpu
 @pytest.mark.parametrize("w4,x4", FORMATS, ids=IDS)
 @pytest.mark.parametrize("A", [40, 900])
-def test_offsets_and_indices_out_of_range(cuda, A, w4, x4):
+def test_offsets_and_indices_out_of_range(cuda, kernels, A, w4, x4):
     """Offsets that no dispatch gives (behind the last row, running back, so that two
     experts' ranges overlap) and indices behind the last row: nothing is read or written
     out of range, and a value is one of its experts' results or left as it was."""
@@ -124,7 +131,7 @@ def test_offsets_and_indices_out_of_range(cuda, A, w4, x4):
 @pytest.mark.gpu
 @pytest.mark.parametrize("w4,x4", FORMATS, ids=IDS)
 @pytest.mark.parametrize("T", [3, 40, 500])
-def test_not_finite_rows_change_their_own_results(cuda, T, w4, x4):
+def test_not_finite_rows_change_their_own_results(cuda, kernels, T, w4, x4):
     g = torch.Generator().manual_seed(T)
     m = [ref.Mats(g, 40, 160, 2, w4)]
     x, _ = ref.rows(g, T, 160, x4)
@@ -146,7 +153,7 @@ def test_not_finite_rows_change_their_own_results(cuda, T, w4, x4):
 @pytest.mark.gpu
 @pytest.mark.parametrize("x4", [False, True])
 @pytest.mark.parametrize("T", [2, 40, 300])
-def test_weights_of_scale_255_are_nan(cuda, T, x4):
+def test_weights_of_scale_255_are_nan(cuda, kernels, T, x4):
     g = torch.Generator().manual_seed(T)
     m = ref.Mats(g, 50, 256, 2, True)
     x, _ = ref.rows(g, T, 256, x4)
@@ -162,7 +169,7 @@ def test_weights_of_scale_255_are_nan(cuda, T, x4):
 @pytest.mark.gpu
 @pytest.mark.parametrize("x4", [False, True])
 @pytest.mark.parametrize("T", [1, 30, 300])
-def test_scales_over_the_stated_range(cuda, T, x4):
+def test_scales_over_the_stated_range(cuda, kernels, T, x4):
     """Weights of scales from 2^-100 to 2^100, one size a row."""
     g = torch.Generator().manual_seed(T)
     m = ref.Mats(g, 201, 96, 0, True)
@@ -176,7 +183,7 @@ def test_scales_over_the_stated_range(cuda, T, x4):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("w4,x4", FORMATS, ids=IDS)
-def test_swiglu_of_large_gates(cuda, w4, x4):
+def test_swiglu_of_large_gates(cuda, kernels, w4, x4):
     """Gates far from zero on both sides: no overflow of the exponential."""
     g = torch.Generator().manual_seed(5)
     m = [ref.Mats(g, 64, 128, 0, w4) for _ in range(2)]
@@ -196,7 +203,7 @@ def test_swiglu_of_large_gates(cuda, w4, x4):
 @pytest.mark.gpu
 @pytest.mark.parametrize("w4,x4", FORMATS, ids=IDS)
 @pytest.mark.parametrize("T", [1, 8, 200, 1500])
-def test_same_bits_again_and_in_a_graph(cuda, T, w4, x4):
+def test_same_bits_again_and_in_a_graph(cuda, kernels, T, w4, x4):
     """Replayed with other inputs in the same buffers, eager work between."""
     g = torch.Generator().manual_seed(T)
     up = [ref.Mats(g, 96, 160, 6, w4) for _ in range(2)]
@@ -314,11 +321,11 @@ def test_refusals_of_the_library():
             2 * E * N * K if fmt == 1 else L.inferno_mxfp4_packed_bytes(d)
         return d
 
-    def call(w, x=at, dt=1, xs=None, rows=4, offsets=at, sorted_=None, k=1, od=0, out=at, up=None):
+    def call(w, x=at, dt=1, xs=None, rows=4, offsets=at, sorted_=None, k=1, od=0, out=at, up=None, ws=None, n=0):
         if up is not None:
             return L.inferno_grouped_gate_up_swiglu(None, w, up, x, dt, xs, rows, offsets, sorted_, k,
-                                                    od, out)
-        return L.inferno_grouped_matmul(None, w, x, dt, xs, rows, offsets, sorted_, k, od, out)
+                                                    od, out, ws, n)
+        return L.inferno_grouped_matmul(None, w, x, dt, xs, rows, offsets, sorted_, k, od, out, ws, n)
 
     ok = desc()
     for w in (None, desc(fmt=0), desc(fmt=2), desc(E=0), desc(E=257), desc(N=0), desc(K=0), desc(K=60),
@@ -334,7 +341,8 @@ def test_refusals_of_the_library():
         assert call(ok, **bad) == -1 and L.inferno_last_error(), bad
     assert call(desc(fmt=3), dt=3) == -1  # codes without scales
     for up in (None, desc(N=32), desc(K=128), desc(E=3), desc(fmt=3)):
-        assert L.inferno_grouped_gate_up_swiglu(None, ok, up, at, 1, None, 4, at, None, 1, 0, at) == -1
+        assert L.inferno_grouped_gate_up_swiglu(None, ok, up, at, 1, None, 4, at, None, 1, 0, at, None,
+                                                0) == -1
     assert call(ok, rows=0, x=None, out=None) == 0 and call(ok, up=desc(), rows=0) == 0
     pack = L.inferno_mxfp4_pack
     w = desc(fmt=3)
