@@ -53,12 +53,13 @@ struct ExpertProduct {
   void* workspace;         // product_workspace bytes
 };
 
-// Which kernel takes a product: tiles (experts_tiles.hip) of 64 * width weight rows,
-// the columns shared by `splits` workgroups; or 16 * width grouped rows
-// (experts_rows.hip), the columns shared by `shares` wavefronts.
+// Which kernel takes a product: tiles (experts_tiles.hip) of `rows` grouped rows by
+// 64 * width weight rows, the columns shared by `splits` workgroups; or
+// (experts_rows.hip) 16 * width grouped rows, the columns shared by `shares`
+// wavefronts.
 struct ExpertPlan {
   bool tiles;
-  int width, shares;
+  int width, rows, shares;
   size_t splits;
 };
 ExpertPlan plan_product(const ExpertProduct& p);

@@ -28,25 +28,28 @@ struct Product {
   float* partial;           // [splits][matrices][A][N, to a multiple of 4]: their sums
 };
 
-// Tile `t` of at most TM rows of one expert, tiles counted expert by expert:
-// rows [c0, c1) of the grouped order. Returns the number of all tiles; t is one
-// of them if it is below. Every wavefront finds its own (257 words at most, which
-// L2 holds, and one scan over the lanes): a launch before the product would
-// cost more. Ranges that are not ascending, or end behind the last row, are cut,
-// so that whatever lies in offsets no row index is A or more.
-template <uint32_t TM>
-__device__ __forceinline__ uint32_t find_tile(const Product& p, uint32_t t, uint32_t& e,
-                                              uint32_t& c0, uint32_t& c1) {
-  if (!p.offsets) {
-    e = 0;
-    c0 = min(t * TM, p.A);
-    c1 = min(c0 + TM, p.A);
-    return (p.A + TM - 1) / TM;
-  }
+// The work of workgroup b of a launch of tiles of at most TM rows by `units`
+// workgroups each (blocks of weight rows, shares of the columns).
+struct Work {
+  uint32_t e, c0, c1;  // expert, rows [c0, c1) of the grouped order
+  uint32_t unit;
+};
+
+// Finds it, or says that there is none (launches have as many workgroups as the
+// rows can need at most). Every wavefront finds its own (257 words, which L2 holds,
+// and one scan over the lanes): a launch before the product would cost more. Ranges
+// that are not ascending, or end behind the last row, are cut, so that whatever lies
+// in offsets no row index is A or more.
+// With XCD, each of the eight XCDs, to which workgroups go in turn, has one run of
+// the work, in which an expert's tiles of one unit follow each other: what they
+// share comes to the XCD's L2 once.
+template <uint32_t TM, bool XCD>
+__device__ __forceinline__ bool find_work(const Product& p, uint32_t b, uint32_t units, Work& w) {
   const uint32_t lane = threadIdx.x & 63;
-  uint32_t o[5], sum = 0, n[4];
+  uint32_t o[5], n[4], sum = 0;
 #pragma unroll
-  for (uint32_t j = 0; j < 5; ++j) o[j] = min(p.offsets[min(4 * lane + j, p.E)], p.A);
+  for (uint32_t j = 0; j < 5; ++j)
+    o[j] = min(p.offsets ? p.offsets[min(4 * lane + j, p.E)] : 4 * lane + j ? p.A : 0u, p.A);
 #pragma unroll
   for (uint32_t j = 0; j < 4; ++j) {
     n[j] = o[j + 1] > o[j] ? (o[j + 1] - o[j] + TM - 1) / TM : 0;
@@ -58,23 +61,33 @@ __device__ __forceinline__ uint32_t find_tile(const Product& p, uint32_t t, uint
     const uint32_t v = uint32_t(__shfl_up(int(upto), d, kWave));
     if (int(lane) >= d) upto += v;
   }
-  const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
-  const uint64_t behind = __ballot(upto > t);
-  if (behind == 0) return all;
-  const int at = __ffsll((unsigned long long)behind) - 1;
-  uint32_t rest = t - (upto - sum), j = 0;  // of the lane `at` alone
+  const uint32_t all = __builtin_amdgcn_readlane(upto, 63) * units;
+  if constexpr (XCD) {
+    const uint32_t run = (all + 7) / 8;
+    if (b / 8 >= run) return false;
+    b = b % 8 * run + b / 8;
+  }
+  if (b >= all) return false;
+  const uint32_t t = b / units;
+  const int at = __ffsll((unsigned long long)__ballot(upto > t)) - 1;
+  // of the lane `at` alone: its expert j, which has tiles before .. before + n[j]
+  uint32_t before = upto - sum, j = 0;
 #pragma unroll
   for (uint32_t i = 0; i < 3; ++i)
-    if (j == i && rest >= n[i]) {
-      rest -= n[i];
+    if (j == i && t >= before + n[i]) {
+      before += n[i];
       j = i + 1;
     }
-  const uint32_t first = j == 0 ? o[0] : j == 1 ? o[1] : j == 2 ? o[2] : o[3];
-  const uint32_t last = j == 0 ? o[1] : j == 1 ? o[2] : j == 2 ? o[3] : o[4];
-  e = __builtin_amdgcn_readlane(4 * lane + j, at);
-  c0 = __builtin_amdgcn_readlane(first + rest * TM, at);
-  c1 = min(c0 + TM, __builtin_amdgcn_readlane(last, at));
-  return all;
+  const uint32_t begin = __builtin_amdgcn_readlane(j == 0 ? o[0] : j == 1 ? o[1] : j == 2 ? o[2] : o[3], at);
+  const uint32_t end = __builtin_amdgcn_readlane(j == 0 ? o[1] : j == 1 ? o[2] : j == 2 ? o[3] : o[4], at);
+  const uint32_t tiles = __builtin_amdgcn_readlane(j == 0 ? n[0] : j == 1 ? n[1] : j == 2 ? n[2] : n[3], at);
+  const uint32_t inside = b - __builtin_amdgcn_readlane(before, at) * units;
+  w.e = __builtin_amdgcn_readlane(4 * lane + j, at);
+  w.unit = XCD ? inside / tiles : inside % units;
+  const uint32_t tile = XCD ? inside - w.unit * tiles : inside / units;
+  w.c0 = begin + tile * TM;
+  w.c1 = min(w.c0 + TM, end);
+  return true;
 }
 
 // Result row of grouped row c < A; A or more: none (an index out of range).
@@ -144,9 +157,9 @@ __device__ __forceinline__ void store4(const Product& p, uint32_t row, uint32_t 
 
 }  // namespace experts
 
-// Tiles of up to 128 rows by 16 * 4 * width weight rows of both matrices; `tiles`:
+// Tiles of up to `rows` (32 or 128) by 16 * 4 * width weight rows of both matrices; `tiles`:
 // at least as many as there are.
 int launch_experts_tiles(hipStream_t s, const experts::Product& p, int mats, bool wfp4, bool xfp4,
-                         size_t tiles, int width);
+                         size_t tiles, int width, int rows);
 
 }  // namespace inferno

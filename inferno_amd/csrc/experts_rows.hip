@@ -32,15 +32,14 @@ __global__ void __launch_bounds__(kWaves* kWave) experts_rows_kernel(Product p, 
   constexpr int kAhead = WFP4 && XFP4 ? 4 : 2;
   constexpr int kPerMat = RT / MATS;
   __shared__ floatx4 part[SHARES > 1 ? kWaves : 1][RT][NB][kWave];
-  uint32_t e, c0, c1;
-  const uint32_t slot = blockIdx.x / blocks;
-  if (slot >= find_tile<16 * NB>(p, slot, e, c0, c1)) return;
+  Work work;
+  if (!find_work<16 * NB, false>(p, blockIdx.x, blocks, work)) return;
+  const uint32_t e = work.e, c0 = work.c0, c1 = work.c1;
   const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t share = wave % SHARES;
   // the wavefront's first weight tile of each matrix
-  const uint32_t first_tile =
-      ((blockIdx.x - slot * blocks) * (kWaves / SHARES) + wave / SHARES) * kPerMat;
+  const uint32_t first_tile = (work.unit * (kWaves / SHARES) + wave / SHARES) * kPerMat;
   const uint32_t pitch = XFP4 ? p.K / 2 : p.K * 2;
   // rows behind the tile's last are computed as it is, and not stored
   uint32_t a[NB];
@@ -212,47 +211,70 @@ int launch(hipStream_t s, const Product& p, int mats, bool wfp4, bool xfp4, size
 
 }  // namespace
 
-// The rules below compare sizes that decide: how many rows an expert has, how many
-// workgroups a form makes, and how much each of them has to do.
+// The rules compare sizes that decide: how many rows an expert has, how many
+// workgroups a form makes, and how much each of them has to do. Times are
+// microseconds of one call, this kernel against the other or one form of tiles
+// against another.
 ExpertPlan plan_product(const ExpertProduct& q) {
   const ExpertMat& m = q.m[0];
-  const bool xfp4 = q.x_scales != nullptr;
+  const bool xfp4 = q.x_scales != nullptr, widened = m.fp4 && !xfp4;
   ExpertPlan r{};
   r.splits = 1;
   // experts that the rows reach if each picks one by chance, and rows of one
   const double E = double(m.experts), A = double(q.A), N = double(m.rows) * q.mats;
+  const double K = double(m.cols);
   const double used = q.offsets ? E * (1.0 - std::pow(1.0 - 1.0 / E, A)) : 1.0;
   const double rows = A / used;
-  // workgroups of the tile kernel, and of this one's narrow form with all wavefronts
-  // on one pair of weight tiles
-  const double tiles = q.offsets ? used * std::max(1.0, rows / 128 + 0.5) : std::ceil(A / 128);
-  auto blocks = [&](size_t width) { return tiles * std::ceil(N / double(64 * width)); };
+  // workgroups of tiles of so many rows by 64 * width weight rows, and of this
+  // kernel's narrow form with all wavefronts on one pair of weight tiles
+  auto tiles = [&](int width, double height) {
+    const double n = q.offsets ? used * std::max(1.0, rows / height + (rows > height / 2 ? 0.5 : 0.0))
+                               : std::ceil(A / height);
+    return n * std::ceil(N / (64.0 * width));
+  };
   const double groups = std::ceil(rows / 16) * used * std::ceil(N / 32);
   const size_t pitch = xfp4 ? m.cols / 2 : m.cols * 2, stages = (pitch + 255) / 256;
-  // Enough workgroups of the wide tiles for all CUs: they win from a few rows an expert
-  // on, earlier the more a weight costs to load or widen. Fewer: their latency counts,
-  // and the rows kernel wins as long as its workgroups, which read every row again
-  // for 32 weight rows, have little to do.
-  const bool many = blocks(4) >= (m.fp4 ? 320 : 384);
-  const double least = m.fp4 ? (xfp4 ? 3 : 1.25) : m.cols < 1024 ? 4 : 6;
-  r.tiles = many ? rows > least
-                 : rows > 8 && groups * double(m.cols) > (m.fp4 ? 3.2e6 : 1.3e6);
+
+  // This kernel reads every row again for 32 weight rows, tiles have four wavefronts
+  // wait for each other. With many workgroups of tiles these win from a few rows an
+  // expert on; with few as soon as this kernel's workgroups have much to do.
+  const bool many = m.fp4 ? tiles(2, 32) >= 384 : tiles(2, 128) >= 192;
+  if (many) {
+    const double least = widened ? 1.1 : xfp4 ? 1.5 : tiles(2, 128) < 1024 ? 6 : K < 1024 ? 1.25 : 2;
+    r.tiles = rows > least;
+  } else {
+    r.tiles = rows > 8 && groups * K > (m.fp4 ? 1.5e6 : 1.3e6);
+  }
   if (switch_on("INFERNO_EXPERTS_TILES")) r.tiles = true;
   if (switch_off("INFERNO_EXPERTS_TILES") || q.A / q.k * pitch >= size_t(1) << 32) r.tiles = false;
-  if (r.tiles) {
-    r.width = many && (m.fp4 || rows > 64) ? 4 : 2;
-    // shares of at least four stages, until they make a workgroup for every CU; of
-    // weights that are widened two for every CU
-    const bool widened = m.fp4 && !xfp4;
-    if (!many)
-      while (r.splits < 8 && r.splits * 8 <= stages &&
-             double(r.splits) * blocks(2) <= (widened && r.splits == 1 ? 256 : 128))
-        r.splits *= 2;
-  } else {
+  if (!r.tiles) {
     r.width = rows > 32 ? 2 : 1;
     const double mine = groups / r.width;
-    r.shares = mine < 256 || (mine < 1024 && m.cols >= 4096) ? 4 : m.cols >= 1536 ? 2 : 1;
+    r.shares = mine < 256 || (mine < 1024 && K >= 4096) ? 4 : K >= 1536 ? 2 : 1;
+    return r;
   }
+  // Wide tiles where there are enough of them; lower tiles, and then shares of the
+  // columns, where there are few.
+  double most = 0, each = 4;  // workgroups up to which shares are doubled, stages of a share
+  if (!m.fp4) {
+    r.width = rows > 64 && tiles(4, 128) >= 384 ? 4 : 2;
+    r.rows = 128;
+    most = 128;
+  } else if (widened) {
+    r.width = rows >= 16 && tiles(4, 64) >= 512 ? 4 : 2;
+    r.rows = r.width == 4 || (rows >= 16 && tiles(2, 64) >= 512) ? 64 : 32;
+    most = 256;
+    each = 12;
+  } else {
+    r.width = rows >= 64 && tiles(4, 128) >= 500 ? 4 : 2;
+    r.rows = r.width == 4 || (K >= 4096 && rows >= 64 && tiles(2, 128) >= 512) ? 128
+             : tiles(2, 64) >= 192                                             ? 64
+                                                                               : 32;
+  }
+  if (r.width == 2)
+    while (r.splits < 8 && double(2 * r.splits) * each <= double(stages) &&
+           double(r.splits) * tiles(2, r.rows) <= most)
+      r.splits *= 2;
   return r;
 }
 
@@ -292,7 +314,7 @@ int launch_expert_product(hipStream_t s, const ExpertProduct& q) {
   const ExpertPlan plan = plan_product(q);
   p.splits = uint32_t(plan.splits);
   p.partial = static_cast<float*>(q.workspace);
-  if (plan.tiles) return launch_experts_tiles(s, p, q.mats, m.fp4, xfp4, tiles_of(128), plan.width);
+  if (plan.tiles) return launch_experts_tiles(s, p, q.mats, m.fp4, xfp4, tiles_of(plan.rows), plan.width, plan.rows);
   const size_t tiles = tiles_of(16 * plan.width);
   auto pick = [&](auto width) -> int {
     constexpr int NB = decltype(width)::value;

@@ -19,7 +19,6 @@ namespace {
 using namespace experts;
 
 constexpr int kWaves = 4;
-constexpr uint32_t kRows = 128;      // grouped rows of a tile
 constexpr uint32_t kStageBytes = 256;  // of a row in LDS: four steps
 
 typedef __attribute__((address_space(3))) void* lptr_t;
@@ -32,23 +31,21 @@ __device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t from, uint32_t off
   __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lptr_t)l, 16, int(off), int(soff), 0, 0);
 }
 
-struct Tile {
-  uint32_t e, c0, c1;  // expert, grouped rows
-  uint32_t first;      // of the workgroup's 16-row weight tiles
-  uint32_t split;      // which share of the columns
-};
-
 template <bool WFP4, bool XFP4, int MATS, int RT, int NB>
 struct Run {
+  // 4-bit weights against bf16 rows: a lane's 16 bytes of step j are number 4 g + j of
+  // a row's stage, else 4 j + g
+  static constexpr bool kWiden = WFP4 && !XFP4;
   static constexpr uint32_t kBuf = NB * 16 * kStageBytes;
   static constexpr int kPerMat = RT / MATS;
-  // steps that weights are ahead: what the registers beside 128 rows' sums hold
-  static constexpr int kAhead = WFP4 && !XFP4 ? 1 : NB * RT == 32 ? 2 : 4;
+  static constexpr int kAhead = kWiden ? 1 : 4;   // steps of weights in registers
+  static constexpr int kHalf = NB == 8 ? 4 : NB;  // 16-row groups read from LDS at once
   // loads of weights that a stage issues behind its copies
-  static constexpr int kBehind = WFP4 && !XFP4 ? 2 * RT : 4 * RT;
+  static constexpr int kBehind = kWiden ? 2 * RT : 4 * RT;
 
   const Product& p;
-  const Tile& t;
+  const Work& t;
+  uint32_t first_tile, split;  // weight tiles of a matrix from here; share of the columns
   uint32_t lane, wave, n, g;
   uint32_t steps;            // of 64 bytes of a weight row (or a chunk)
   uint32_t pitch;            // bytes of a grouped row
@@ -61,7 +58,7 @@ struct Run {
   uint32_t piece;            // of the lane's 16 bytes of a row's stage (in the first copy)
   floatx4 acc[RT][NB];
 
-  __device__ __forceinline__ Run(const Product& p_, const Tile& t_) : p(p_), t(t_) {}
+  __device__ __forceinline__ Run(const Product& p_, const Work& t_) : p(p_), t(t_) {}
 
   // weights of step s (from 0; the last again behind it)
   __device__ __forceinline__ uint4 weight(int r, uint32_t s) const {
@@ -84,27 +81,32 @@ struct Run {
     const uint32_t most = min(pitch - s * kStageBytes, kStageBytes) - 16;
 #pragma unroll
     for (int u = 0; u < NB; ++u)
-      copy16(xbuf, xrow[u] + min(piece ^ (64 * ((wave * NB + u) & 3)), most), s * kStageBytes,
+      copy16(xbuf, xrow[u] + min(piece ^ ((kWiden ? 16 : 64) * ((wave * NB + u) & 3)), most),
+             s * kStageBytes,
              to + (wave * NB + u) * 1024);
   }
 
   // Scales of MXFP4 rows: the thread's row's sixteen of stage s (0 behind the
-  // last, where the codes are zeros). Rows of scales lie at any byte.
+  // last, where the codes are zeros). Rows of scales lie at any byte; the last
+  // stage takes the last sixteen and moves them.
   __device__ __forceinline__ void load_scales(uint32_t s, const uint8_t* row, uint32_t (&v)[4]) const {
+    const uint32_t blocks = p.K / kMxBlock, at = min(s * 16, blocks - 16), by = s * 16 - at;
+    __builtin_memcpy(v, row + at, 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = __builtin_amdgcn_alignbyte(j < 3 ? v[j + 1] : 0u, v[j], by & 3);
+    if (by & 4) v[0] = v[1], v[1] = v[2], v[2] = v[3], v[3] = 0;
+    if (by & 8) v[0] = v[2], v[1] = v[3], v[2] = v[3] = 0;
+  }
+  // The same of the only stage of a row of fewer.
+  __device__ __forceinline__ void load_few_scales(const uint8_t* row, uint32_t (&v)[4]) const {
     const uint32_t blocks = p.K / kMxBlock;
-    if (blocks < 4) {
-      v[0] = row[0];
-      if (blocks > 1) v[0] |= uint32_t(row[1]) << 8;
-      if (blocks > 2) v[0] |= uint32_t(row[2]) << 16;
-      v[1] = v[2] = v[3] = 0;
-      return;
-    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t b = s * 16 + 4 * j, at = min(b, blocks - 4), shift = 8 * (b - at);
-      uint32_t u;
-      __builtin_memcpy(&u, row + at, 4);
-      v[j] = shift < 32 ? u >> shift : 0;
+      v[j] = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        if (4 * j + i < blocks) v[j] |= uint32_t(row[4 * j + i]) << (8 * i);
     }
   }
   // From four words of four blocks, one a step, to one word per block of a step.
@@ -128,7 +130,7 @@ struct Run {
     if constexpr (!LAST) {
       copy_rows(s + 1, next);
       asm volatile("" ::: "memory");  // the loads below are younger
-      if constexpr (WFP4 && !XFP4) {
+      if constexpr (kWiden) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           w_next[r] = weight(r, s + 1);
@@ -142,64 +144,77 @@ struct Run {
       for (int b = 0; b < NB; ++b)
         xs[b] = *reinterpret_cast<const uint32_t*>(cur_scales + (b * 16 + n) * 16 + g * 4);
     }
-    const uint32_t x0 = n * kStageBytes + 16 * ((WFP4 && !XFP4 ? 4 * g : g) ^ n);
+    const uint32_t x0 =
+        n * kStageBytes + 16 * (kWiden ? (4 * g) ^ (n >> 2 | (n & 3) << 2) : g ^ n);
     auto step = [&](auto jc) __attribute__((always_inline)) {
       constexpr int j = decltype(jc)::value;
       __builtin_amdgcn_sched_barrier(0);  // (registers)
-      const uint32_t at = x0 ^ (WFP4 && !XFP4 ? 16 * j : 64 * j);
-      uint4 xv[NB];
+      const uint32_t at = x0 ^ (kWiden ? 16 * j : 64 * j);
+      bf16x8 wide[kWiden ? RT : 1];
+      if constexpr (kWiden) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-        xv[b] = *reinterpret_cast<const uint4*>(cur + b * 4096 + at);
-      if constexpr (LAST) {  // nothing behind the last column
-        const uint32_t col = s * kStageBytes + 16 * (WFP4 && !XFP4 ? 4 * g + j : 4 * j + g);
-        const uint32_t keep = col < pitch ? ~0u : 0u;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-          xv[b] = make_uint4(xv[b].x & keep, xv[b].y & keep, xv[b].z & keep, xv[b].w & keep);
-      }
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        if constexpr (WFP4 && XFP4) {
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            const intx8 av = {int(w[j % kAhead][r].x), int(w[j % kAhead][r].y), int(w[j % kAhead][r].z), int(w[j % kAhead][r].w), 0, 0, 0, 0};
-            const intx8 bv = {int(xv[b].x), int(xv[b].y), int(xv[b].z), int(xv[b].w), 0, 0, 0, 0};
-            acc[r][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                av, bv, acc[r][b], 4, 4, j, int(ws[r]), j, int(xs[b]));
-          }
-        } else {
-          bf16x8 a;
-          if constexpr (WFP4) {
-            const uint4 c = w[0][r];
-            a = widen(j == 0 ? c.x : j == 1 ? c.y : j == 2 ? c.z : c.w,
-                      scale_of((ws[r] >> (8 * (s & 3))) & 255u));
-          } else {
-            uint4 v = w[j % kAhead][r];
-            if constexpr (LAST) {  // nothing behind the last column
-              const uint32_t keep = (4 * s + j) * 32 + 8 * g < p.K ? ~0u : 0u;
-              v = make_uint4(v.x & keep, v.y & keep, v.z & keep, v.w & keep);
-            }
-            a = __builtin_bit_cast(bf16x8, v);
-          }
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-            acc[r][b] = mfma_bf16(a, __builtin_bit_cast(bf16x8, xv[b]), acc[r][b]);
+        for (int r = 0; r < RT; ++r) {
+          const uint4 c = w[0][r];
+          wide[r] = widen(j == 0 ? c.x : j == 1 ? c.y : j == 2 ? c.z : c.w,
+                          scale_of((ws[r] >> (8 * (s & 3))) & 255u));
         }
       }
-      if constexpr (!(WFP4 && !XFP4) && (!LAST || j + kAhead < 4)) {
+      const uint32_t col = s * kStageBytes + 16 * (kWiden ? 4 * g + j : 4 * j + g);
+      const uint32_t keep_x = col < pitch ? ~0u : 0u;  // nothing behind the last column
+      const uint32_t keep_w = (4 * s + j) * 32 + 8 * g < p.K ? ~0u : 0u;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) w[j % kAhead][r] = weight(r, 4 * s + j + kAhead);
+      for (int h = 0; h < NB; h += kHalf) {
+        if (h) __builtin_amdgcn_sched_barrier(0);  // (registers)
+        uint4 xv[kHalf];
+#pragma unroll
+        for (int b = 0; b < kHalf; ++b) {
+          xv[b] = *reinterpret_cast<const uint4*>(cur + (h + b) * 4096 + at);
+          if constexpr (LAST)
+            xv[b] = make_uint4(xv[b].x & keep_x, xv[b].y & keep_x, xv[b].z & keep_x, xv[b].w & keep_x);
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          if constexpr (WFP4 && XFP4) {
+            const uint4 v = w[j][r];
+            const intx8 av = {int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < kHalf; ++b) {
+              const intx8 bv = {int(xv[b].x), int(xv[b].y), int(xv[b].z), int(xv[b].w), 0, 0, 0, 0};
+              acc[r][h + b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                  av, bv, acc[r][h + b], 4, 4, j, int(ws[r]), j, int(xs[h + b]));
+            }
+          } else {
+            bf16x8 a;
+            if constexpr (kWiden) {
+              a = wide[r];
+            } else {
+              uint4 v = w[j][r];
+              if constexpr (LAST) v = make_uint4(v.x & keep_w, v.y & keep_w, v.z & keep_w, v.w & keep_w);
+              a = __builtin_bit_cast(bf16x8, v);
+            }
+#pragma unroll
+            for (int b = 0; b < kHalf; ++b)
+              acc[r][h + b] = mfma_bf16(a, __builtin_bit_cast(bf16x8, xv[b]), acc[r][h + b]);
+          }
+        }
+      }
+      // The next weights: in bf16 two steps at once, which share the 128-byte lines
+      // (one by one, L1 has lost a line before its second half is asked for).
+      if constexpr (!kWiden && !LAST && (WFP4 || j % 2 == 1)) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = WFP4 ? j : j - 1; i <= j; ++i) w[i][r] = weight(r, 4 * s + 4 + i);
       }
     };
     step(std::integral_constant<int, 0>{});
-    if (LAST && !(WFP4 && !XFP4) && 4 * s + 1 >= steps) return;
+    if (LAST && !kWiden && 4 * s + 1 >= steps) return;
     step(std::integral_constant<int, 1>{});
-    if (LAST && !(WFP4 && !XFP4) && 4 * s + 2 >= steps) return;
+    if (LAST && !kWiden && 4 * s + 2 >= steps) return;
     step(std::integral_constant<int, 2>{});
-    if (LAST && !(WFP4 && !XFP4) && 4 * s + 3 >= steps) return;
+    if (LAST && !kWiden && 4 * s + 3 >= steps) return;
     step(std::integral_constant<int, 3>{});
-    if constexpr (!LAST && WFP4 && !XFP4) {
+    if constexpr (!LAST && kWiden) {
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         w[0][r] = w_next[r];
@@ -213,16 +228,18 @@ struct Run {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     n = lane & 15;
     g = lane >> 4;
+    first_tile = t.unit / p.splits * (kWaves * kPerMat);
+    split = t.unit % p.splits;
     pitch = XFP4 ? p.K / 2 : p.K * 2;
     steps = WFP4 ? p.chunks : (p.K + 31) / 32;
     const uint32_t stages = (pitch + kStageBytes - 1) / kStageBytes;
-    const uint32_t first = stages * t.split / p.splits, last = stages * (t.split + 1) / p.splits;
+    const uint32_t first = stages * split / p.splits, last = stages * (split + 1) / p.splits;
     const uint32_t all_tiles = (p.N + 15) / 16;
     glast = (steps - 1) * 32 + 8 * g < p.K ? 16 * g : 0;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int m = r / kPerMat;
-      const uint32_t tile = min(t.first + wave * kPerMat + r % kPerMat, all_tiles - 1);
+      const uint32_t tile = min(first_tile + wave * kPerMat + r % kPerMat, all_tiles - 1);
       if constexpr (WFP4) {
         const size_t at = size_t(t.e) * p.tiles + tile;
         wbase[r] = p.w[m] + at * p.chunks * 1024;
@@ -238,11 +255,13 @@ struct Run {
     };
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
-      // four rows a copy; the pieces of a row exclusive-or'ed with it, so that 16
-      // rows' reads of one column touch all banks
+      // four rows a copy
       xrow[u] = input_row(4 * (wave * NB + u) + g) * pitch;
     }
-    piece = 16 * (n ^ g);
+    // the 16 pieces of a row lie exclusive-or'ed with its number (kWiden: with the
+    // number's halves exchanged), so that the 16 lanes that LDS serves at once,
+    // eight of quarter g and eight of the next, touch all banks
+    piece = 16 * (n ^ (kWiden ? 4 * g : g));
     xbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.x), 0, int(p.x_bytes), 0x00020000);
 #pragma unroll
     for (int r = 0; r < RT; ++r)
@@ -257,7 +276,8 @@ struct Run {
     uint32_t sv[4];
     if constexpr (XFP4) {
       scale_row = p.xs + size_t(input_row(srow)) * (p.K / kMxBlock);
-      load_scales(first, scale_row, sv);
+      if (p.K >= 16 * kMxBlock) load_scales(first, scale_row, sv);
+      else load_few_scales(scale_row, sv);
     }
     uint4 w[kAhead][RT];
     uint32_t ws[RT], ws_next[RT];
@@ -265,7 +285,7 @@ struct Run {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) w[j][r] = weight(r, (WFP4 && !XFP4 ? 1 : 4) * first + j);
+      for (int r = 0; r < RT; ++r) w[j][r] = weight(r, (kWiden ? 1 : 4) * first + j);
     if constexpr (WFP4) {
 #pragma unroll
       for (int r = 0; r < RT; ++r) ws[r] = weight_scale(r, XFP4 ? first : first / 4);
@@ -305,10 +325,10 @@ struct Run {
       if (p.splits > 1) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const uint32_t at = (t.first + wave * kPerMat + r % kPerMat) * 16 + 4 * g;
+          const uint32_t at = (first_tile + wave * kPerMat + r % kPerMat) * 16 + 4 * g;
           if (at < p.N)
             *reinterpret_cast<floatx4*>(
-                p.partial + partial_row(p, MATS, t.split, r / kPerMat, c) + at) = acc[r][b];
+                p.partial + partial_row(p, MATS, split, r / kPerMat, c) + at) = acc[r][b];
         }
         continue;
       }
@@ -320,26 +340,24 @@ struct Run {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           y[i] = MATS == 2 ? silu_mul(acc[r][b][i], acc[r + RT - kPerMat][b][i]) : acc[r][b][i];
-        store4(p, a, (t.first + wave * kPerMat + r) * 16 + 4 * g, y);
+        store4(p, a, (first_tile + wave * kPerMat + r) * 16 + 4 * g, y);
       }
     }
   }
 };
 
-template <bool WFP4, bool XFP4, int MATS, int RT>
-__global__ void __launch_bounds__(kWaves* kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <bool WFP4, bool XFP4, int MATS, int RT, int NB>
+__global__ void __launch_bounds__(kWaves* kWave) __attribute__((amdgpu_waves_per_eu(NB == 8 ? 2 : NB == 4 ? 3 : 4)))
     experts_tiles_kernel(Product p, uint32_t blocks) {
   extern __shared__ __attribute__((aligned(16))) uint8_t tile_shared[];
-  Tile t;
-  const uint32_t block = blockIdx.x / p.splits, slot = block / blocks;
-  if (slot >= find_tile<kRows>(p, slot, t.e, t.c0, t.c1)) return;
-  t.first = (block - slot * blocks) * (kWaves * RT / MATS);
-  t.split = blockIdx.x - block * p.splits;
+  Work t;
+  if (!find_work<NB * 16, true>(p, blockIdx.x, blocks * p.splits, t)) return;
   const uint32_t rows = t.c1 - t.c0;
-  if (rows <= 16) Run<WFP4, XFP4, MATS, RT, 1>(p, t)(tile_shared);
-  else if (rows <= 32) Run<WFP4, XFP4, MATS, RT, 2>(p, t)(tile_shared);
-  else if (rows <= 64) Run<WFP4, XFP4, MATS, RT, 4>(p, t)(tile_shared);
-  else Run<WFP4, XFP4, MATS, RT, 8>(p, t)(tile_shared);
+  if (rows <= 16) return Run<WFP4, XFP4, MATS, RT, 1>(p, t)(tile_shared);
+  if (rows <= 32) return Run<WFP4, XFP4, MATS, RT, 2>(p, t)(tile_shared);
+  if constexpr (NB > 2)
+    if (rows <= 64) return Run<WFP4, XFP4, MATS, RT, 4>(p, t)(tile_shared);
+  if constexpr (NB > 4) Run<WFP4, XFP4, MATS, RT, 8>(p, t)(tile_shared);
 }
 
 // The sums of the shares in order, and what follows a product: one thread per four
@@ -365,12 +383,12 @@ __global__ void __launch_bounds__(256) experts_join_kernel(Product p, uint32_t q
   store4(p, a, n, y);
 }
 
-template <int RT>
-int launch(hipStream_t s, const Product& p, int mats, bool wfp4, bool xfp4, size_t tiles) {
+template <bool WFP4, bool XFP4, int RT, int NB>
+int launch(hipStream_t s, const Product& p, int mats, size_t tiles) {
   const size_t per = kWaves * RT / mats;  // weight tiles of a workgroup
   const size_t blocks = ((p.N + 15) / 16 + per - 1) / per;
-  const size_t lds = 2 * kRows * kStageBytes + (xfp4 ? 2 * kRows * 16 : 0);
-  const size_t grid = tiles * blocks * p.splits;
+  const size_t lds = 2 * NB * 16 * (kStageBytes + (XFP4 ? 16 : 0));
+  const size_t grid = (tiles * blocks * p.splits + 7) / 8 * 8;  // each XCD the same number
   if (grid * (kWaves * kWave) >= size_t(1) << 32) {
     set_error("too many rows for one launch");
     return INFERNO_ERR_INVALID;
@@ -381,29 +399,37 @@ int launch(hipStream_t s, const Product& p, int mats, bool wfp4, bool xfp4, size
                                   hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
     kernel<<<unsigned(grid), kWaves * kWave, lds, s>>>(p, uint32_t(blocks));
     INF_LAUNCHED();
-    if (p.splits > 1) {
-      const uint32_t quarter = (p.N + 3) / 4;
-      const unsigned n = unsigned((size_t(p.A) * quarter + 255) / 256);
-      if (mats == 2) experts_join_kernel<2><<<n, 256, 0, s>>>(p, quarter);
-      else experts_join_kernel<1><<<n, 256, 0, s>>>(p, quarter);
-      INF_LAUNCHED();
-    }
     return INFERNO_OK;
   };
-  auto with = [&](auto wf, auto xf) -> int {
-    constexpr bool W = decltype(wf)::value, X = decltype(xf)::value;
-    return mats == 2 ? go(experts_tiles_kernel<W, X, 2, RT>) : go(experts_tiles_kernel<W, X, 1, RT>);
-  };
-  if (!wfp4) return with(std::false_type{}, std::false_type{});
-  return xfp4 ? with(std::true_type{}, std::true_type{}) : with(std::true_type{}, std::false_type{});
+  return mats == 2 ? go(experts_tiles_kernel<WFP4, XFP4, 2, RT, NB>)
+                   : go(experts_tiles_kernel<WFP4, XFP4, 1, RT, NB>);
 }
 
 }  // namespace
 
 int launch_experts_tiles(hipStream_t s, const Product& p, int mats, bool wfp4, bool xfp4,
-                         size_t tiles, int width) {
-  return width == 4 ? launch<4>(s, p, mats, wfp4, xfp4, tiles)
-                    : launch<2>(s, p, mats, wfp4, xfp4, tiles);
+                         size_t tiles, int width, int rows) {
+  int st;
+  if (!wfp4) {
+    st = width == 4 ? launch<false, false, 4, 8>(s, p, mats, tiles)
+                    : launch<false, false, 2, 8>(s, p, mats, tiles);
+  } else if (!xfp4) {
+    st = width == 4   ? launch<true, false, 4, 4>(s, p, mats, tiles)
+         : rows == 64 ? launch<true, false, 2, 4>(s, p, mats, tiles)
+                      : launch<true, false, 2, 2>(s, p, mats, tiles);
+  } else {
+    st = width == 4    ? launch<true, true, 4, 8>(s, p, mats, tiles)
+         : rows == 128 ? launch<true, true, 2, 8>(s, p, mats, tiles)
+         : rows == 64  ? launch<true, true, 2, 4>(s, p, mats, tiles)
+                       : launch<true, true, 2, 2>(s, p, mats, tiles);
+  }
+  if (st || p.splits == 1) return st;
+  const uint32_t quarter = (p.N + 3) / 4;
+  const unsigned n = unsigned((size_t(p.A) * quarter + 255) / 256);
+  if (mats == 2) experts_join_kernel<2><<<n, 256, 0, s>>>(p, quarter);
+  else experts_join_kernel<1><<<n, 256, 0, s>>>(p, quarter);
+  INF_LAUNCHED();
+  return INFERNO_OK;
 }
 
 }  // namespace inferno
