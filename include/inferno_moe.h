@@ -299,28 +299,28 @@ int inferno_w4_moe(void* stream, const inferno_w4* gate, const inferno_w4* up,
 int inferno_mxfp4_quantize(void* stream, const void* x, int x_dtype, size_t rows, size_t cols,
                            void* codes, uint8_t* scales, void* values);
 
-/* One matrix [rows,cols], or one per expert. BF16: data is [experts][rows][cols]
- * as it is, cols a multiple of 8. MXFP4: data is the packed form that
- * inferno_mxfp4_pack writes once, cols a multiple of 32; scales (but for 255) lie
- * between 2^-100 and 2^100. data lies at a multiple of 16 bytes. experts <= 256,
- * rows and cols <= 2^24, one matrix at most 2^33 values. */
+/* One matrix [rows,cols], or one per expert, in the packed form that
+ * inferno_experts_pack writes once, at a multiple of 16 bytes. BF16: cols a multiple of
+ * 8. MXFP4: cols a multiple of 32; scales (but for 255) lie between 2^-100 and 2^100.
+ * experts <= 256, rows and cols <= 2^24, one matrix at most 2^33 values. */
 typedef struct inferno_experts {
   size_t experts;
   size_t rows;       /* outputs */
   size_t cols;       /* inputs */
   int format;        /* INFERNO_BF16 or INFERNO_MXFP4 */
-  const void* data;
-  size_t data_bytes; /* 2 experts rows cols, or inferno_mxfp4_packed_bytes */
+  const void* data;  /* packed */
+  size_t data_bytes; /* inferno_experts_packed_bytes */
 } inferno_experts;
 
 /* Bytes of the packed form (of w, only sizes and format are read; 0: refused). */
-size_t inferno_mxfp4_packed_bytes(const inferno_experts* w);
+size_t inferno_experts_packed_bytes(const inferno_experts* w);
 
-/* Packs codes [experts, rows, cols / 2] and scales [experts, rows, cols / 32]
- * (w->data is not read, w->data_bytes is the size of packed). */
-int inferno_mxfp4_pack(void* stream, const inferno_experts* w, const void* codes,
-                       size_t codes_bytes, const uint8_t* scales, size_t scales_bytes,
-                       void* packed);
+/* Packs weights [experts, rows, cols] in bf16 (scales NULL, 0 bytes), or codes
+ * [experts, rows, cols / 2] with scales [experts, rows, cols / 32]. w->data is not
+ * read, w->data_bytes is the size of packed. */
+int inferno_experts_pack(void* stream, const inferno_experts* w, const void* weights,
+                         size_t weights_bytes, const uint8_t* scales, size_t scales_bytes,
+                         void* packed);
 
 /* Products of rows that are grouped by expert, groups of any size, empty ones too:
  * for every expert e and c in [offsets[e], offsets[e + 1]), with a = sorted[c],

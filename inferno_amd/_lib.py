@@ -95,8 +95,8 @@ SIGNATURES = {
     "inferno_w4_moe": (_i, [_vp, C.POINTER(W4Desc), C.POINTER(W4Desc), C.POINTER(W4Desc), _vp, _i,
                             _vp, _sz, _vp, _vp, _sz, _sz, _vp, _vp, _sz]),
     "inferno_mxfp4_quantize": (_i, [_vp, _vp, _i, _sz, _sz, _vp, _vp, _vp]),
-    "inferno_mxfp4_packed_bytes": (_sz, [C.POINTER(ExpertsDesc)]),
-    "inferno_mxfp4_pack": (_i, [_vp, C.POINTER(ExpertsDesc), _vp, _sz, _vp, _sz, _vp]),
+    "inferno_experts_packed_bytes": (_sz, [C.POINTER(ExpertsDesc)]),
+    "inferno_experts_pack": (_i, [_vp, C.POINTER(ExpertsDesc), _vp, _sz, _vp, _sz, _vp]),
     "inferno_grouped_workspace_bytes": (_sz, [C.POINTER(ExpertsDesc), _i, _i, _sz, _sz, _i]),
     "inferno_grouped_matmul": (_i, [_vp, C.POINTER(ExpertsDesc), _vp, _i, _vp, _sz, _vp, _vp, _sz,
                                     _i, _vp, _vp, _sz]),

@@ -42,9 +42,7 @@ int check_shape(const char* what, const inferno_experts* w) {
 int check_mat(const char* what, const inferno_experts* w) {
   int st;
   if ((st = check_shape(what, w))) return st;
-  const size_t want = w->format == INFERNO_MXFP4 ? mx_layout(mat(w)).bytes
-                                                 : w->experts * w->rows * w->cols * 2;
-  if ((st = check_bytes(what, "data", w->data_bytes, want))) return st;
+  if ((st = check_bytes(what, "packed form", w->data_bytes, expert_layout(mat(w)).bytes))) return st;
   INF_CHECK_ARG(w->data != nullptr, "null pointer in an expert matrix");
   INF_CHECK_ARG(aligned(w->data, 16), "an expert matrix must lie at a multiple of 16 bytes");
   return INFERNO_OK;
@@ -120,32 +118,31 @@ int inferno_mxfp4_quantize(void* stream, const void* x, int x_dtype, size_t rows
   return launch_mxfp4_quantize(as_stream(stream), x, x_dtype, rows * cols, codes, scales, values);
 }
 
-size_t inferno_mxfp4_packed_bytes(const inferno_experts* w) {
+size_t inferno_experts_packed_bytes(const inferno_experts* w) {
   clear_error();
-  if (check_shape("given", w)) return 0;
-  if (w->format != INFERNO_MXFP4) {
-    set_error("matrices in bf16 are not packed");
-    return 0;
-  }
-  return mx_layout(mat(w)).bytes;
+  return check_shape("given", w) ? 0 : expert_layout(mat(w)).bytes;
 }
 
-int inferno_mxfp4_pack(void* stream, const inferno_experts* w, const void* codes,
-                       size_t codes_bytes, const uint8_t* scales, size_t scales_bytes,
-                       void* packed) {
+int inferno_experts_pack(void* stream, const inferno_experts* w, const void* weights,
+                         size_t weights_bytes, const uint8_t* scales, size_t scales_bytes,
+                         void* packed) {
   clear_error();
   int st;
   if ((st = check_shape("given", w))) return st;
-  INF_CHECK_ARG(w->format == INFERNO_MXFP4, "matrices in bf16 are not packed");
-  const size_t rows = w->experts * w->rows;
-  if ((st = check_bytes("given", "codes", codes_bytes, rows * (w->cols / 2)))) return st;
-  if ((st = check_bytes("given", "scales", scales_bytes, rows * (w->cols / kMxBlock)))) return st;
-  if ((st = check_bytes("given", "data", w->data_bytes, mx_layout(mat(w)).bytes))) return st;
-  INF_CHECK_ARG(codes && scales && packed, "null pointer");
-  INF_CHECK_ARG(aligned(codes, 16) && aligned(packed, 16),
-                "codes and the packed matrix must lie at multiples of 16 bytes");
+  const bool fp4 = w->format == INFERNO_MXFP4;
+  const size_t values = w->experts * w->rows * w->cols;
+  if ((st = check_bytes("given", fp4 ? "codes" : "weights", weights_bytes,
+                        fp4 ? values / 2 : values * 2)))
+    return st;
+  if ((st = check_bytes("given", "scales", scales_bytes, fp4 ? values / kMxBlock : 0))) return st;
+  if ((st = check_bytes("given", "packed form", w->data_bytes, expert_layout(mat(w)).bytes)))
+    return st;
+  INF_CHECK_ARG(weights && packed && fp4 == (scales != nullptr),
+                "null pointer, or scales of matrices in bf16");
+  INF_CHECK_ARG(aligned(weights, 16) && aligned(packed, 16),
+                "the weights and their packed form must lie at multiples of 16 bytes");
   if (int st_ = require_device()) return st_;
-  return launch_mxfp4_pack(as_stream(stream), mat(w), codes, scales, packed);
+  return launch_experts_pack(as_stream(stream), mat(w), weights, scales, packed);
 }
 
 size_t inferno_grouped_workspace_bytes(const inferno_experts* w, int matrices, int x_dtype,

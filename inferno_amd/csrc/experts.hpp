@@ -5,38 +5,42 @@
 
 namespace inferno {
 
-constexpr int kMxBlock = 32;    // columns of one scale
-constexpr int kMxChunk = 128;   // columns of one packed chunk: 64 bytes of codes per row
+constexpr int kMxBlock = 32;    // columns of one MXFP4 scale
 
-// One matrix, or one per expert. bf16: [experts][rows][cols] as they are. MXFP4,
-// packed: for every tile of 16 rows and chunk of 128 columns the 1024 bytes of
-// codes that a wavefront takes in one load, lane l the 32 columns l / 16 of row
-// l % 16; after all of them, for every tile and four chunks, one word per lane:
-// the scales of its row's 32 columns in the four chunks. Rows behind the last
-// and columns behind cols are zeros of scale 1.
+// One matrix, or one per expert, packed: for every tile of 16 rows and step of 64
+// bytes of a row (32 columns in bf16, 128 in MXFP4) the 1024 bytes that a wavefront
+// takes in one load, lane l 16 bytes of row l % 16, number l / 16. (As rows lie,
+// four neighbouring lanes ask for four rows, and the address unit, which joins
+// neighbours, takes 16 bytes a cycle instead of 64: with them it was busy for nine
+// cycles of ten.) After all of them, for MXFP4, one word per lane for every tile and
+// four steps: the scales of its row's 32 columns in the four. Rows behind the last
+// and columns behind cols are zeros, of scale 1.
 struct ExpertMat {
   size_t experts, rows, cols;
   bool fp4;
   const void* data;
 };
-struct MxLayout {
-  size_t tiles, chunks, quads;  // of one expert
-  size_t scales, bytes;         // byte offset of the scales, and the size
+struct ExpertLayout {
+  size_t tiles, steps, quads;  // of one expert
+  size_t scales, bytes;        // byte offset of the scales, and the size
 };
-inline MxLayout mx_layout(const ExpertMat& m) {
-  MxLayout l{};
+inline ExpertLayout expert_layout(const ExpertMat& m) {
+  const size_t step = m.fp4 ? 128 : 32;
+  ExpertLayout l{};
   l.tiles = (m.rows + 15) / 16;
-  l.chunks = (m.cols + kMxChunk - 1) / kMxChunk;
-  l.quads = (l.chunks + 3) / 4;
-  l.scales = m.experts * l.tiles * l.chunks * 1024;
+  l.steps = (m.cols + step - 1) / step;
+  l.quads = m.fp4 ? (l.steps + 3) / 4 : 0;
+  l.scales = m.experts * l.tiles * l.steps * 1024;
   l.bytes = l.scales + m.experts * l.tiles * l.quads * 256;
   return l;
 }
 
 int launch_mxfp4_quantize(hipStream_t s, const void* x, int x_dtype, size_t n, void* codes,
                           void* scales, void* values);
-int launch_mxfp4_pack(hipStream_t s, const ExpertMat& m, const void* codes, const void* scales,
-                      void* packed);
+// weights: bf16 [experts, rows, cols], or codes [experts, rows, cols / 2] with
+// scales [experts, rows, cols / 32].
+int launch_experts_pack(hipStream_t s, const ExpertMat& m, const void* weights, const void* scales,
+                        void* packed);
 
 // One product launch. Row c of expert e's range [offsets[e], offsets[e+1]) is
 // result row a = sorted[c] (c itself without sorted), of input row a / k.

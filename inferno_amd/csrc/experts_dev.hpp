@@ -12,8 +12,8 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef int intx8 __attribute__((ext_vector_type(8)));
 
 struct Product {
-  const uint8_t* w[2];      // codes, or bf16
-  const uint32_t* ws[2];    // packed scales
+  const uint8_t* w[2];      // packed weights
+  const uint32_t* ws[2];    // and their scales
   const uint8_t* x;
   const uint8_t* xs;        // scales of codes
   uint32_t x_bytes;         // of x; below 2^32 where rows go through LDS
@@ -21,7 +21,7 @@ struct Product {
   const uint32_t* sorted;   // or null
   uint32_t E, A, k;
   uint32_t N, K;
-  uint32_t tiles, chunks, quads;  // packed weights of an expert: 16-row tiles, chunks, four chunks
+  uint32_t tiles, steps, quads;  // of an expert's packed weights
   void* out;
   bool out_f32;
   uint32_t splits;          // shares of the columns in launches of their own workgroups
@@ -127,17 +127,21 @@ __device__ __forceinline__ floatx4 mfma_fp4(uint4 a, uint4 b, floatx4 c, uint32_
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
 
-// Four neighbouring values of one result row.
+// Four neighbouring values of one result row. Rows of a length that is no multiple
+// of four lie at any multiple of a value's size.
 __device__ __forceinline__ void store4(const Product& p, uint32_t row, uint32_t n, const float (&y)[4]) {
   if (n >= p.N) return;
   const size_t at = size_t(row) * p.N + n;
+  const bool whole = p.N % 4 == 0;
   if (p.out_f32) {
     float* to = static_cast<float*>(p.out) + at;
-    if (p.N % 4 == 0) {
+    if (whole) {
       *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+    } else if (n + 4 <= p.N) {
+      __builtin_memcpy(to, y, 16);
     } else {
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i)
+      for (uint32_t i = 0; i < 3; ++i)
         if (n + i < p.N) to[i] = y[i];
     }
     return;
@@ -146,11 +150,14 @@ __device__ __forceinline__ void store4(const Product& p, uint32_t row, uint32_t 
   uint32_t h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = __builtin_bit_cast(uint16_t, (__bf16)y[i]);
-  if (p.N % 4 == 0) {
-    *reinterpret_cast<uint2*>(to) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+  const uint2 two = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+  if (whole) {
+    *reinterpret_cast<uint2*>(to) = two;
+  } else if (n + 4 <= p.N) {
+    __builtin_memcpy(to, &two, 8);
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
+    for (uint32_t i = 0; i < 3; ++i)
       if (n + i < p.N) to[i] = uint16_t(h[i]);
   }
 }

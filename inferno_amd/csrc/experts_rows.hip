@@ -18,6 +18,7 @@ namespace {
 using namespace experts;
 
 constexpr int kWaves = 4;
+constexpr uint32_t kChunk = 128;  // columns
 
 // One chunk's operands of a wavefront, 128 columns.
 template <bool WFP4, bool XFP4, int RT, int NB>
@@ -58,16 +59,12 @@ __global__ void __launch_bounds__(kWaves* kWave) experts_rows_kernel(Product p, 
   for (int r = 0; r < RT; ++r) {
     const uint32_t tile = min(first_tile + r % kPerMat, p.tiles - 1);
     const size_t at = size_t(e) * p.tiles + tile;
-    if constexpr (WFP4) {
-      w[r] = p.w[r / kPerMat] + at * p.chunks * 1024 + lane * 16;
-      ws[r] = p.ws[r / kPerMat] + at * p.quads * 64 + lane;
-    } else {
-      w[r] = p.w[r / kPerMat] + (size_t(e) * p.N + min(tile * 16 + n, p.N - 1)) * pitch;
-    }
+    w[r] = p.w[r / kPerMat] + at * p.steps * 1024 + lane * 16;
+    if constexpr (WFP4) ws[r] = p.ws[r / kPerMat] + at * p.quads * 64 + lane;
   }
   // column of the lane's 16 bytes number j of a chunk
   auto column = [&](uint32_t ch, int j) {
-    return ch * kMxChunk + (WFP4 ? 32 * g + 8 * j : 32 * j + 8 * g);
+    return ch * kChunk + (WFP4 ? 32 * g + 8 * j : 32 * j + 8 * g);
   };
   auto load = [&](uint32_t ch, C& v) {
 #pragma unroll
@@ -77,10 +74,9 @@ __global__ void __launch_bounds__(kWaves* kWave) experts_rows_kernel(Product p, 
         v.ws[m] = ws[m][size_t(ch / 4) * 64] >> (8 * (ch % 4));
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t col = column(ch, j);
-          v.w[m][j] = *reinterpret_cast<const uint4*>(w[m] + (col < p.K ? col * 2 : 0));
-        }
+        for (int j = 0; j < 4; ++j)
+          v.w[m][j] =
+              *reinterpret_cast<const uint4*>(w[m] + size_t(min(4 * ch + j, p.steps - 1)) * 1024);
       }
     }
 #pragma unroll
@@ -104,7 +100,7 @@ __global__ void __launch_bounds__(kWaves* kWave) experts_rows_kernel(Product p, 
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[m][b] = floatx4{0.f, 0.f, 0.f, 0.f};
   auto use = [&](uint32_t ch, C& v) {
-    if ((ch + 1) * kMxChunk > p.K) {  // the last chunk: nothing behind the last column
+    if ((ch + 1) * kChunk > p.K) {  // the last chunk: nothing behind the last column
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t keep = column(ch, j) < p.K ? ~0u : 0u;
@@ -143,7 +139,8 @@ __global__ void __launch_bounds__(kWaves* kWave) experts_rows_kernel(Product p, 
     }
   };
   // this wavefront's chunks
-  const uint32_t first = p.chunks * share / SHARES, last = p.chunks * (share + 1) / SHARES;
+  const uint32_t chunks = (p.K + kChunk - 1) / kChunk;
+  const uint32_t first = chunks * share / SHARES, last = chunks * (share + 1) / SHARES;
   if (first < last) {
     C v[kAhead];
 #pragma unroll
@@ -236,35 +233,42 @@ ExpertPlan plan_product(const ExpertProduct& q) {
   const size_t pitch = xfp4 ? m.cols / 2 : m.cols * 2, stages = (pitch + 255) / 256;
 
   // This kernel reads every row again for 32 weight rows, tiles have four wavefronts
-  // wait for each other. With many workgroups of tiles these win from a few rows an
-  // expert on; with few as soon as this kernel's workgroups have much to do.
-  const bool many = m.fp4 ? tiles(2, 32) >= 384 : tiles(2, 128) >= 192;
-  if (many) {
-    const double least = widened ? 1.1 : xfp4 ? 1.5 : tiles(2, 128) < 1024 ? 6 : K < 1024 ? 1.25 : 2;
-    r.tiles = rows > least;
-  } else {
-    r.tiles = rows > 8 && groups * K > (m.fp4 ? 1.5e6 : 1.3e6);
-  }
+  // wait for each other. With enough workgroups of the lowest tiles these win (8 tokens
+  // of 8 of 64 experts, gate and up 768 x 2048 in bf16: 44 against 53 us); with fewer
+  // as soon as this kernel's have much to do (64 tokens by 6144 x 2048 in bf16: 15
+  // against 13 us, two such matrices 19 against 21).
+  const bool many = tiles(2, 32) >= 384;
+  r.tiles = many || (rows > 8 && groups * K > (q.offsets || rows > 32 ? 1.5e6 : 2e6));
   if (switch_on("INFERNO_EXPERTS_TILES")) r.tiles = true;
   if (switch_off("INFERNO_EXPERTS_TILES") || q.A / q.k * pitch >= size_t(1) << 32) r.tiles = false;
   if (!r.tiles) {
-    r.width = rows > 32 ? 2 : 1;
+    r.width = rows > 64 ? 2 : 1;
     const double mine = groups / r.width;
-    r.shares = mine < 256 || (mine < 1024 && K >= 4096) ? 4 : K >= 1536 ? 2 : 1;
+    r.shares = mine < 256 || (mine < 1024 && K >= 2048) ? 4 : K >= 1536 ? 2 : 1;
     return r;
   }
-  // Wide tiles where there are enough of them; lower tiles, and then shares of the
-  // columns, where there are few.
-  double most = 0, each = 4;  // workgroups up to which shares are doubled, stages of a share
+  // The largest tiles of which there are enough; then, where a workgroup's columns are
+  // long, shares of them. Experts have uneven numbers of rows, so that a tile holds
+  // twice their mean, or fills the CUs with workgroups.
+  double most = 0;  // workgroups up to which shares are doubled
   if (!m.fp4) {
-    r.width = rows > 64 && tiles(4, 128) >= 384 ? 4 : 2;
-    r.rows = 128;
-    most = 128;
+    most = 192;
+    if (q.offsets) {
+      r.width = rows > 64 && tiles(4, 128) >= 384 ? 4 : 2;
+      r.rows = r.width == 4                                                  ? 128
+               : rows <= 12                                                  ? 32
+               : rows <= 28 || (rows > 80 && tiles(2, 128) < 384)            ? 64
+                                                                             : 128;
+    } else {
+      // (short columns: more workgroups, which start and end while others run)
+      const bool brief = m.cols <= 2048;
+      r.width = tiles(4, 128) >= (brief ? 512 : 192) ? 4 : 2;
+      r.rows = r.width == 4 || (!brief && tiles(2, 128) >= 192) ? 128 : tiles(2, 64) >= 192 ? 64 : 32;
+    }
   } else if (widened) {
-    r.width = rows >= 16 && tiles(4, 64) >= 512 ? 4 : 2;
-    r.rows = r.width == 4 || (rows >= 16 && tiles(2, 64) >= 512) ? 64 : 32;
     most = 256;
-    each = 12;
+    r.width = rows >= 16 && tiles(4, 64) >= 512 ? 4 : 2;
+    r.rows = r.width == 4 || (rows >= 32 && tiles(2, 64) >= 512) ? 64 : 32;
   } else {
     r.width = rows >= 64 && tiles(4, 128) >= 500 ? 4 : 2;
     r.rows = r.width == 4 || (K >= 4096 && rows >= 64 && tiles(2, 128) >= 512) ? 128
@@ -272,8 +276,7 @@ ExpertPlan plan_product(const ExpertProduct& q) {
                                                                                : 32;
   }
   if (r.width == 2)
-    while (r.splits < 8 && double(2 * r.splits) * each <= double(stages) &&
-           double(r.splits) * tiles(2, r.rows) <= most)
+    while (r.splits < 8 && r.splits * 24 <= stages && double(r.splits) * tiles(2, r.rows) <= most)
       r.splits *= 2;
   return r;
 }
@@ -286,7 +289,7 @@ size_t product_workspace(const ExpertProduct& q) {
 int launch_expert_product(hipStream_t s, const ExpertProduct& q) {
   Product p{};
   const ExpertMat& m = q.m[0];
-  const MxLayout l = mx_layout(m);
+  const ExpertLayout l = expert_layout(m);
   for (int i = 0; i < q.mats; ++i) {
     p.w[i] = static_cast<const uint8_t*>(q.m[i].data);
     p.ws[i] = reinterpret_cast<const uint32_t*>(p.w[i] + l.scales);
@@ -301,7 +304,7 @@ int launch_expert_product(hipStream_t s, const ExpertProduct& q) {
   p.N = uint32_t(m.rows);
   p.K = uint32_t(m.cols);
   p.tiles = uint32_t(l.tiles);
-  p.chunks = uint32_t(l.chunks);
+  p.steps = uint32_t(l.steps);
   p.quads = uint32_t(l.quads);
   p.out = q.out;
   p.out_f32 = q.out_dtype == INFERNO_F32;

@@ -47,12 +47,9 @@ struct Run {
   const Work& t;
   uint32_t first_tile, split;  // weight tiles of a matrix from here; share of the columns
   uint32_t lane, wave, n, g;
-  uint32_t steps;            // of 64 bytes of a weight row (or a chunk)
   uint32_t pitch;            // bytes of a grouped row
   const uint8_t* wbase[RT];   // of the wavefront's weight tiles
   const uint8_t* sbase[RT];   // of their scales
-  uint32_t woff[RT];          // bf16: of the lane's row
-  uint32_t glast;            // bf16: of its columns in the last step, the first ones if it has none
   uint32_t xrow[NB];         // byte offsets of the rows that this wavefront copies
   __amdgpu_buffer_rsrc_t xbuf;
   uint32_t piece;            // of the lane's 16 bytes of a row's stage (in the first copy)
@@ -62,13 +59,7 @@ struct Run {
 
   // weights of step s (from 0; the last again behind it)
   __device__ __forceinline__ uint4 weight(int r, uint32_t s) const {
-    const uint32_t at = min(s, steps - 1);
-    if constexpr (WFP4) {
-      return *reinterpret_cast<const uint4*>(wbase[r] + size_t(at) * 1024 + lane * 16);
-    } else {
-      const uint32_t off = woff[r] + (at == steps - 1 ? glast : 16 * g);
-      return *reinterpret_cast<const uint4*>(wbase[r] + size_t(at) * 64 + off);
-    }
+    return *reinterpret_cast<const uint4*>(wbase[r] + size_t(min(s, p.steps - 1)) * 1024 + lane * 16);
   }
   __device__ __forceinline__ uint32_t weight_scale(int r, uint32_t quad) const {
     return reinterpret_cast<const uint32_t*>(sbase[r] + size_t(min(quad, p.quads - 1)) * 256)[lane];
@@ -161,7 +152,6 @@ struct Run {
       }
       const uint32_t col = s * kStageBytes + 16 * (kWiden ? 4 * g + j : 4 * j + g);
       const uint32_t keep_x = col < pitch ? ~0u : 0u;  // nothing behind the last column
-      const uint32_t keep_w = (4 * s + j) * 32 + 8 * g < p.K ? ~0u : 0u;
 #pragma unroll
       for (int h = 0; h < NB; h += kHalf) {
         if (h) __builtin_amdgcn_sched_barrier(0);  // (registers)
@@ -188,9 +178,7 @@ struct Run {
             if constexpr (kWiden) {
               a = wide[r];
             } else {
-              uint4 v = w[j][r];
-              if constexpr (LAST) v = make_uint4(v.x & keep_w, v.y & keep_w, v.z & keep_w, v.w & keep_w);
-              a = __builtin_bit_cast(bf16x8, v);
+              a = __builtin_bit_cast(bf16x8, w[j][r]);
             }
 #pragma unroll
             for (int b = 0; b < kHalf; ++b)
@@ -198,21 +186,17 @@ struct Run {
           }
         }
       }
-      // The next weights: in bf16 two steps at once, which share the 128-byte lines
-      // (one by one, L1 has lost a line before its second half is asked for).
-      if constexpr (!kWiden && !LAST && (WFP4 || j % 2 == 1)) {
+      if constexpr (!kWiden && !LAST) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int i = WFP4 ? j : j - 1; i <= j; ++i) w[i][r] = weight(r, 4 * s + 4 + i);
+        for (int r = 0; r < RT; ++r) w[j][r] = weight(r, 4 * s + 4 + j);
       }
     };
     step(std::integral_constant<int, 0>{});
-    if (LAST && !kWiden && 4 * s + 1 >= steps) return;
+    if (LAST && !kWiden && 4 * s + 1 >= p.steps) return;
     step(std::integral_constant<int, 1>{});
-    if (LAST && !kWiden && 4 * s + 2 >= steps) return;
+    if (LAST && !kWiden && 4 * s + 2 >= p.steps) return;
     step(std::integral_constant<int, 2>{});
-    if (LAST && !kWiden && 4 * s + 3 >= steps) return;
+    if (LAST && !kWiden && 4 * s + 3 >= p.steps) return;
     step(std::integral_constant<int, 3>{});
     if constexpr (!LAST && kWiden) {
 #pragma unroll
@@ -231,23 +215,15 @@ struct Run {
     first_tile = t.unit / p.splits * (kWaves * kPerMat);
     split = t.unit % p.splits;
     pitch = XFP4 ? p.K / 2 : p.K * 2;
-    steps = WFP4 ? p.chunks : (p.K + 31) / 32;
     const uint32_t stages = (pitch + kStageBytes - 1) / kStageBytes;
     const uint32_t first = stages * split / p.splits, last = stages * (split + 1) / p.splits;
-    const uint32_t all_tiles = (p.N + 15) / 16;
-    glast = (steps - 1) * 32 + 8 * g < p.K ? 16 * g : 0;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int m = r / kPerMat;
-      const uint32_t tile = min(first_tile + wave * kPerMat + r % kPerMat, all_tiles - 1);
-      if constexpr (WFP4) {
-        const size_t at = size_t(t.e) * p.tiles + tile;
-        wbase[r] = p.w[m] + at * p.chunks * 1024;
-        sbase[r] = reinterpret_cast<const uint8_t*>(p.ws[m]) + at * p.quads * 256;
-      } else {
-        wbase[r] = p.w[m] + (size_t(t.e) * p.N + tile * 16) * p.K * 2;
-        woff[r] = min(n, p.N - 1 - tile * 16) * p.K * 2;
-      }
+      const uint32_t tile = min(first_tile + wave * kPerMat + r % kPerMat, p.tiles - 1);
+      const size_t at = size_t(t.e) * p.tiles + tile;
+      wbase[r] = p.w[m] + at * p.steps * 1024;
+      sbase[r] = reinterpret_cast<const uint8_t*>(p.ws[m]) + at * p.quads * 256;
     }
     auto input_row = [&](uint32_t row) {
       const uint32_t a = result_row(p, min(t.c0 + row, t.c1 - 1));
@@ -411,8 +387,10 @@ int launch_experts_tiles(hipStream_t s, const Product& p, int mats, bool wfp4, b
                          size_t tiles, int width, int rows) {
   int st;
   if (!wfp4) {
-    st = width == 4 ? launch<false, false, 4, 8>(s, p, mats, tiles)
-                    : launch<false, false, 2, 8>(s, p, mats, tiles);
+    st = width == 4    ? launch<false, false, 4, 8>(s, p, mats, tiles)
+         : rows == 128 ? launch<false, false, 2, 8>(s, p, mats, tiles)
+         : rows == 64  ? launch<false, false, 2, 4>(s, p, mats, tiles)
+                       : launch<false, false, 2, 2>(s, p, mats, tiles);
   } else if (!xfp4) {
     st = width == 4   ? launch<true, false, 4, 4>(s, p, mats, tiles)
          : rows == 64 ? launch<true, false, 2, 4>(s, p, mats, tiles)

@@ -1,5 +1,5 @@
 // MXFP4: rows to 4-bit floating point with one power-of-two scale per 32
-// columns, and the packing of weights.
+// columns, and the packing of experts' weights, in bf16 too.
 //
 // A block's scale is 2^(floor(log2 m) - 2), m its largest magnitude: 4 <= m /
 // scale < 8, and the largest code stands for 6, so that quotients above 6
@@ -77,28 +77,25 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// One thread per 16 bytes of codes; those of a tile's first chunk of four bring
-// the scales.
+// One thread per 16 bytes, of `pieces` a row; those of a tile's first step of four
+// bring the scales.
 __global__ void __launch_bounds__(kThreads)
-    mxfp4_pack_kernel(const uint4* __restrict__ codes, const uint8_t* __restrict__ scales, size_t N,
-                      size_t K, size_t tiles, size_t chunks, size_t quads, size_t n,
-                      uint4* __restrict__ to, uint32_t* __restrict__ to_scales) {
+    experts_pack_kernel(const uint4* __restrict__ weights, const uint8_t* __restrict__ scales,
+                        size_t N, size_t pieces, size_t tiles, size_t steps, size_t quads, size_t n,
+                        uint4* __restrict__ to, uint32_t* __restrict__ to_scales) {
   for (size_t i = size_t(blockIdx.x) * kThreads + threadIdx.x; i < n;
        i += size_t(gridDim.x) * kThreads) {
     const uint32_t lane = uint32_t(i % 64);
-    const size_t at = i / 64, c = at % chunks, tile = at / chunks;  // of all experts
+    const size_t at = i / 64, c = at % steps, tile = at / steps;  // of all experts
     const size_t e = tile / tiles, row = (tile - e * tiles) * 16 + lane % 16;
-    const size_t blocks = K / kMxBlock, block = c * 4 + lane / 16;
+    const size_t piece = c * 4 + lane / 16, src = (e * N + row) * pieces;
     const bool there = row < N;
-    const size_t src = (e * N + row) * blocks;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (there && block < blocks) u = codes[src + block];
-    to[i] = u;
-    if (c % 4 == 0) {
+    to[i] = there && piece < pieces ? weights[src + piece] : make_uint4(0, 0, 0, 0);
+    if (scales && c % 4 == 0) {
       uint32_t w = 0;
       for (uint32_t j = 0; j < 4; ++j) {
-        const size_t b = block + 4 * j;
-        w |= (there && b < blocks ? uint32_t(scales[src + b]) : 127u) << (8 * j);
+        const size_t b = piece + 4 * j;
+        w |= (there && b < pieces ? uint32_t(scales[src + b]) : 127u) << (8 * j);
       }
       to_scales[(tile * quads + c / 4) * 64 + lane] = w;
     }
@@ -129,15 +126,15 @@ int launch_mxfp4_quantize(hipStream_t s, const void* x, int x_dtype, size_t n, v
   return INFERNO_OK;
 }
 
-int launch_mxfp4_pack(hipStream_t s, const ExpertMat& m, const void* codes, const void* scales,
-                      void* packed) {
-  const MxLayout l = mx_layout(m);
-  const size_t n = m.experts * l.tiles * l.chunks * 64;
+int launch_experts_pack(hipStream_t s, const ExpertMat& m, const void* weights, const void* scales,
+                        void* packed) {
+  const ExpertLayout l = expert_layout(m);
+  const size_t n = m.experts * l.tiles * l.steps * 64;
   const size_t most = size_t(1) << 20;  // workgroups
   const unsigned grid = unsigned(std::min((n + kThreads - 1) / kThreads, most));
-  mxfp4_pack_kernel<<<grid, kThreads, 0, s>>>(
-      static_cast<const uint4*>(codes), static_cast<const uint8_t*>(scales), m.rows, m.cols,
-      l.tiles, l.chunks, l.quads, n, static_cast<uint4*>(packed),
+  experts_pack_kernel<<<grid, kThreads, 0, s>>>(
+      static_cast<const uint4*>(weights), static_cast<const uint8_t*>(scales), m.rows,
+      m.cols / (m.fp4 ? 32 : 8), l.tiles, l.steps, l.quads, n, static_cast<uint4*>(packed),
       reinterpret_cast<uint32_t*>(static_cast<char*>(packed) + l.scales));
   INF_LAUNCHED();
   return INFERNO_OK;

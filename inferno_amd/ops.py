@@ -384,13 +384,12 @@ def mxfp4_quantize(x, values=False):
 
 class Experts:
     """Weights of the products grouped by expert (struct inferno_experts): one
-    matrix [rows, cols], or one per expert [E, rows, cols]. A bf16 tensor is used
-    as it lies and kept. MXFP4 is ``codes`` (uint8 [..., cols / 2], the even column
-    in the low nibble) and ``scales`` (uint8 [..., cols / 32]), packed once, here, on
-    the current stream (inferno_mxfp4_pack), which is waited for: the handle may be
-    used on any stream at once, and the tensors are not kept. While the stream is
-    being captured nothing is waited for; such a handle holds its matrices after the
-    graph's first replay."""
+    matrix [rows, cols], or one per expert [E, rows, cols], as a bf16 tensor, or in
+    MXFP4 as ``codes`` (uint8 [..., cols / 2], the even column in the low nibble) and
+    ``scales`` (uint8 [..., cols / 32]). Packed once, here, on the current stream
+    (inferno_experts_pack), which is waited for: the handle may be used on any stream
+    at once, and the tensors are not kept. While the stream is being captured nothing is
+    waited for; such a handle holds its matrices after the graph's first replay."""
 
     def __init__(self, weights, scales=None):
         dtype = torch.bfloat16 if scales is None else torch.uint8
@@ -407,15 +406,13 @@ class Experts:
                              f"{self.cols}")
         d = ExpertsDesc(self.experts, self.rows, self.cols, MXFP4 if self.mxfp4 else BF16, None, 0)
         self.desc, self.ref = d, C.byref(d)
-        if not self.mxfp4:
-            self.data = weights
-            d.data, d.data_bytes = weights.data_ptr(), weights.numel() * 2
-            return
-        _like(weights, "scales", scales, torch.uint8, *weights.shape[:-1], self.cols // 32)
-        d.data_bytes = lib().inferno_mxfp4_packed_bytes(self.ref)
+        if self.mxfp4:
+            _like(weights, "scales", scales, torch.uint8, *weights.shape[:-1], self.cols // 32)
+        d.data_bytes = lib().inferno_experts_packed_bytes(self.ref)
         self.data = torch.empty(d.data_bytes, dtype=torch.uint8, device=self.device)
-        _run(weights, lib().inferno_mxfp4_pack, self.ref, _at(weights), weights.numel(), _at(scales),
-             scales.numel(), _at(self.data))
+        _run(weights, lib().inferno_experts_pack, self.ref, _at(weights),
+             weights.numel() * weights.element_size(), _at(scales),
+             scales.numel() if self.mxfp4 else 0, _at(self.data))
         d.data = self.data.data_ptr()
         stream = torch.cuda.current_stream(self.device)
         with torch.cuda.device(self.device):

@@ -298,8 +298,7 @@ def test_refusals_of_the_wrappers(cuda):
     with pytest.raises(InfernoError, match="16 bytes"):
         ops.grouped_matmul(one, torch.zeros(4 * 64 + 1, dtype=BF16, device="cuda")[1:].view(4, 64))
     with pytest.raises(InfernoError, match="16 bytes"):
-        v = ops.Experts(torch.zeros(16 * 64 + 1, dtype=BF16, device="cuda")[1:].view(16, 64))
-        ops.grouped_matmul(v, x)
+        ops.Experts(torch.zeros(16 * 64 + 1, dtype=BF16, device="cuda")[1:].view(16, 64))
     for bad in [(torch.zeros(16, 60, dtype=BF16), None), (torch.zeros(16, 64), None),
                 (torch.zeros(16, dtype=BF16), None), (torch.zeros(16, 128, dtype=BF16)[:, ::2], None),
                 (torch.zeros(16, 24, dtype=U8), torch.zeros(16, 1, dtype=U8)),
@@ -317,8 +316,7 @@ def test_refusals_of_the_library():
 
     def desc(E=2, N=16, K=64, fmt=1, data=at, nbytes=None):
         d = ExpertsDesc(E, N, K, fmt, data, 0)
-        d.data_bytes = nbytes if nbytes is not None else \
-            2 * E * N * K if fmt == 1 else L.inferno_mxfp4_packed_bytes(d)
+        d.data_bytes = nbytes if nbytes is not None else L.inferno_experts_packed_bytes(d)
         return d
 
     def call(w, x=at, dt=1, xs=None, rows=4, offsets=at, sorted_=None, k=1, od=0, out=at, up=None, ws=None, n=0):
@@ -344,13 +342,14 @@ def test_refusals_of_the_library():
         assert L.inferno_grouped_gate_up_swiglu(None, ok, up, at, 1, None, 4, at, None, 1, 0, at, None,
                                                 0) == -1
     assert call(ok, rows=0, x=None, out=None) == 0 and call(ok, up=desc(), rows=0) == 0
-    pack = L.inferno_mxfp4_pack
+    pack, size = L.inferno_experts_pack, L.inferno_experts_packed_bytes
     w = desc(fmt=3)
-    assert L.inferno_mxfp4_packed_bytes(ok) == 0 and L.inferno_last_error()
-    assert L.inferno_mxfp4_packed_bytes(desc(fmt=3, K=48, nbytes=0)) == 0
-    # two experts of one tile and one chunk: codes, and the scales of four chunks
-    assert L.inferno_mxfp4_packed_bytes(w) == 2 * (1024 + 256)
-    assert pack(None, ok, at, 1024, at, 64, at) == -1
+    assert size(desc(fmt=3, K=48, nbytes=0)) == 0 and L.inferno_last_error()
+    # two experts of one tile: one step of codes and the scales of four, two steps of bf16
+    assert size(w) == 2 * (1024 + 256) and size(ok) == 2 * 2 * 1024
+    assert size(desc(N=17, K=40)) == 2 * 2 * 2 * 1024
+    assert pack(None, ok, at, 4096, at, 0, at) == -1  # scales of bf16
+    assert pack(None, ok, at, 4095, None, 0, at) == -2 and pack(None, ok, at, 4096, None, 8, at) == -2
     assert pack(None, w, at, 1023, at, 64, at) == -2 and pack(None, w, at, 1024, at, 63, at) == -2
     assert pack(None, desc(fmt=3, nbytes=7), at, 1024, at, 64, at) == -2
     for a, b, c in ((None, at, at), (at, None, at), (at, at, None), (at + 4, at, at), (at, at, at + 8)):
