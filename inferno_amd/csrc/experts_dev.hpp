@@ -20,6 +20,7 @@ struct Product {
   const uint32_t* offsets;  // or null
   const uint32_t* sorted;   // or null
   uint32_t E, A, k;
+  uint32_t per_k;           // 2^32 / k + 1, of k above 1
   uint32_t N, K;
   uint32_t tiles, steps, quads;  // of an expert's packed weights
   void* out;
@@ -47,9 +48,15 @@ template <uint32_t TM, bool XCD>
 __device__ __forceinline__ bool find_work(const Product& p, uint32_t b, uint32_t units, Work& w) {
   const uint32_t lane = threadIdx.x & 63;
   uint32_t o[5], n[4], sum = 0;
+  if (p.offsets) {
 #pragma unroll
-  for (uint32_t j = 0; j < 5; ++j)
-    o[j] = min(p.offsets ? p.offsets[min(4 * lane + j, p.E)] : 4 * lane + j ? p.A : 0u, p.A);
+    for (uint32_t j = 0; j < 5; ++j) o[j] = p.offsets[min(4 * lane + j, p.E)];
+#pragma unroll
+    for (uint32_t j = 0; j < 5; ++j) o[j] = min(o[j], p.A);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 5; ++j) o[j] = 4 * lane + j ? p.A : 0;
+  }
 #pragma unroll
   for (uint32_t j = 0; j < 4; ++j) {
     n[j] = o[j + 1] > o[j] ? (o[j + 1] - o[j] + TM - 1) / TM : 0;
@@ -90,9 +97,24 @@ __device__ __forceinline__ bool find_work(const Product& p, uint32_t b, uint32_t
   return true;
 }
 
-// Result row of grouped row c < A; A or more: none (an index out of range).
-__device__ __forceinline__ uint32_t result_row(const Product& p, uint32_t c) {
-  return p.sorted ? p.sorted[c] : c;
+// Result rows of grouped rows c < A, in place; A or more: none (an index out of
+// range). All loads at once, since each takes as long as all.
+template <int N>
+__device__ __forceinline__ void result_rows(const Product& p, uint32_t (&c)[N]) {
+  if (!p.sorted) return;
+  uint32_t a[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = p.sorted[c[i]];
+#pragma unroll
+  for (int i = 0; i < N; ++i) c[i] = a[i];
+}
+
+// Input row of a result row (0 where there is none). With a < 2^22 and k <= 1024, a
+// (2^32 / k + 1) / 2^32 is a / k but for less than 1 / k.
+__device__ __forceinline__ uint32_t input_row(const Product& p, uint32_t a) {
+  if (a >= p.A) return 0;
+  if (p.k == 1) return a;
+  return p.k <= 1024 ? __umulhi(a, p.per_k) : a / p.k;
 }
 
 // Where the sums of a share, matrix and grouped row begin in `partial`.

@@ -47,9 +47,11 @@ __global__ void __launch_bounds__(kWaves* kWave) experts_rows_kernel(Product p, 
   const uint8_t* x[NB];
   const uint8_t* xs[NB];
 #pragma unroll
+  for (int b = 0; b < NB; ++b) a[b] = min(c0 + 16 * b + n, c1 - 1);
+  result_rows(p, a);
+#pragma unroll
   for (int b = 0; b < NB; ++b) {
-    a[b] = result_row(p, min(c0 + 16 * b + n, c1 - 1));
-    const size_t row = a[b] < p.A ? a[b] / p.k : 0;
+    const size_t row = input_row(p, a[b]);
     x[b] = p.x + row * pitch;
     xs[b] = p.xs + row * (p.K / kMxBlock);
   }
@@ -301,6 +303,7 @@ int launch_expert_product(hipStream_t s, const ExpertProduct& q) {
   p.E = uint32_t(m.experts);
   p.A = uint32_t(q.A);
   p.k = uint32_t(q.k);
+  p.per_k = q.k > 1 ? uint32_t((size_t(1) << 32) / q.k + 1) : 0;
   p.N = uint32_t(m.rows);
   p.K = uint32_t(m.cols);
   p.tiles = uint32_t(l.tiles);

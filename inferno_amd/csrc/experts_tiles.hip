@@ -225,15 +225,15 @@ struct Run {
       wbase[r] = p.w[m] + at * p.steps * 1024;
       sbase[r] = reinterpret_cast<const uint8_t*>(p.ws[m]) + at * p.quads * 256;
     }
-    auto input_row = [&](uint32_t row) {
-      const uint32_t a = result_row(p, min(t.c0 + row, t.c1 - 1));
-      return a < p.A ? a / p.k : 0;  // (of an index out of range no result is written)
-    };
+    // rows behind the tile's last are copied as it is, and not stored
+    uint32_t a[NB + 1];
 #pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      // four rows a copy
-      xrow[u] = input_row(4 * (wave * NB + u) + g) * pitch;
-    }
+    for (int u = 0; u < NB; ++u) a[u] = min(t.c0 + 4 * (wave * NB + u) + g, t.c1 - 1);
+    const uint32_t srow = threadIdx.x % (NB * 16);
+    a[NB] = min(t.c0 + srow, t.c1 - 1);
+    result_rows(p, a);
+#pragma unroll
+    for (int u = 0; u < NB; ++u) xrow[u] = input_row(p, a[u]) * pitch;  // four rows a copy
     // the 16 pieces of a row lie exclusive-or'ed with its number (kWiden: with the
     // number's halves exchanged), so that the 16 lanes that LDS serves at once,
     // eight of quarter g and eight of the next, touch all banks
@@ -247,11 +247,10 @@ struct Run {
     uint8_t* const scales = smem + 2 * kBuf;
     // every thread brings a row's scales, the same row several times if there are
     // fewer rows than threads
-    const uint32_t srow = threadIdx.x % (NB * 16);
     const uint8_t* scale_row = nullptr;
     uint32_t sv[4];
     if constexpr (XFP4) {
-      scale_row = p.xs + size_t(input_row(srow)) * (p.K / kMxBlock);
+      scale_row = p.xs + size_t(input_row(p, a[NB])) * (p.K / kMxBlock);
       if (p.K >= 16 * kMxBlock) load_scales(first, scale_row, sv);
       else load_few_scales(scale_row, sv);
     }
@@ -294,6 +293,10 @@ struct Run {
       const uint32_t s = last - 1;
       stage<true>(s, nullptr, smem + (s & 1) * kBuf, scales + (s & 1) * (NB * 256), w, ws);
     }
+    uint32_t to[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) to[b] = min(t.c0 + 16 * b + n, t.c1 - 1);
+    if (p.splits == 1) result_rows(p, to);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const uint32_t c = t.c0 + 16 * b + n;
@@ -308,15 +311,14 @@ struct Run {
         }
         continue;
       }
-      const uint32_t a = result_row(p, c);
-      if (a >= p.A) continue;
+      if (to[b] >= p.A) continue;
 #pragma unroll
       for (int r = 0; r < kPerMat; ++r) {
         float y[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           y[i] = MATS == 2 ? silu_mul(acc[r][b][i], acc[r + RT - kPerMat][b][i]) : acc[r][b][i];
-        store4(p, a, (first_tile + wave * kPerMat + r) * 16 + 4 * g, y);
+        store4(p, to[b], (first_tile + wave * kPerMat + r) * 16 + 4 * g, y);
       }
     }
   }
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(256) experts_join_kernel(Product p, uint32_t q
   const uint32_t i = blockIdx.x * 256 + threadIdx.x, c = i / quarter, n = (i - c * quarter) * 4;
   if (c >= p.A) return;
   if (p.offsets && (c < p.offsets[0] || c >= p.offsets[p.E])) return;
-  const uint32_t a = result_row(p, c);
+  const uint32_t a = p.sorted ? p.sorted[c] : c;
   if (a >= p.A) return;
   floatx4 sum[MATS];
 #pragma unroll
