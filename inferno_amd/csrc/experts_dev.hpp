@@ -186,8 +186,8 @@ __device__ __forceinline__ void store4(const Product& p, uint32_t row, uint32_t 
 
 }  // namespace experts
 
-// Tiles of up to `rows` (32 or 128) by 16 * 4 * width weight rows of both matrices; `tiles`:
-// at least as many as there are.
+// Tiles of up to `rows` (32, 64 or 128) by 64 * width weight rows of all matrices;
+// `tiles`: at least as many as there are.
 int launch_experts_tiles(hipStream_t s, const experts::Product& p, int mats, bool wfp4, bool xfp4,
                          size_t tiles, int width, int rows);
 

@@ -1,13 +1,20 @@
-// Products of rows grouped by expert, few rows: one or two tiles of 16 weight rows
-// (of both matrices) by 16 or 32 grouped rows, the operands straight from memory to registers in the
-// order of the matrix instructions.
+// Products of rows grouped by expert, few rows: two tiles of 16 weight rows (one of
+// each matrix, if there are two) by 16 or 32 grouped rows, the operands straight from
+// memory to registers in the order of the matrix instructions. And which kernel takes
+// a product.
 //
 // The weights are the first operand (lane l: row l % 16, quarter l / 16 of the
 // columns of a step), the grouped rows the second, so that a lane's four sums
 // are four neighbouring values of one result row. Of a workgroup's four wavefronts
 // SHARES take the same weight rows and share the columns; they add their sums in
 // order through LDS. What bounds it is how many bytes are on their way: every
-// wavefront loads kAhead chunks of 128 columns before it uses the first.
+// wavefront loads kAhead chunks of 128 columns before it uses the first (twice as
+// many, and workgroups of 8 or 16 wavefronts, were slower).
+//
+// One token, microseconds of a call among others: down of 8 of 256 experts, 6144 x
+// 2048 in MXFP4, 12.2 (4.4 TB/s); gate and up of 8 of 64 experts, 768 x 2048 in bf16,
+// 11.2 (4.5 TB/s); gate and up of a shared expert, 1536 x 4096 in MXFP4, 8.2, where a
+// launch of nothing takes 6.2.
 #include <cmath>
 
 #include "experts_dev.hpp"
@@ -18,7 +25,9 @@ namespace {
 using namespace experts;
 
 constexpr int kWaves = 4;
+constexpr int kTiles = 2;         // of 16 weight rows, of a wavefront
 constexpr uint32_t kChunk = 128;  // columns
+constexpr double kCUs = 256;
 
 // One chunk's operands of a wavefront, 128 columns.
 template <bool WFP4, bool XFP4, int RT, int NB>
@@ -27,8 +36,9 @@ struct Chunk {
   uint32_t ws[RT], xs[NB];
 };
 
-template <bool WFP4, bool XFP4, int MATS, int RT, int NB, int SHARES>
+template <bool WFP4, bool XFP4, int MATS, int NB, int SHARES>
 __global__ void __launch_bounds__(kWaves* kWave) experts_rows_kernel(Product p, uint32_t blocks) {
+  constexpr int RT = kTiles;
   using C = Chunk<WFP4, XFP4, RT, NB>;
   constexpr int kAhead = WFP4 && XFP4 ? 4 : 2;
   constexpr int kPerMat = RT / MATS;
@@ -185,9 +195,9 @@ __global__ void __launch_bounds__(kWaves* kWave) experts_rows_kernel(Product p, 
   }
 }
 
-template <int RT, int NB, int SHARES>
+template <int NB, int SHARES>
 int launch(hipStream_t s, const Product& p, int mats, bool wfp4, bool xfp4, size_t tiles) {
-  const size_t per = kWaves / SHARES * RT / mats;  // weight tiles of a workgroup
+  const size_t per = kWaves / SHARES * kTiles / mats;  // weight tiles of a workgroup
   const size_t blocks = (p.tiles + per - 1) / per;
   if (tiles * blocks * (kWaves * kWave) >= size_t(1) << 32) {
     set_error("too many rows for one launch");
@@ -197,9 +207,9 @@ int launch(hipStream_t s, const Product& p, int mats, bool wfp4, bool xfp4, size
     constexpr bool W = decltype(wf)::value, X = decltype(xf)::value;
     const unsigned grid = unsigned(tiles * blocks), threads = kWaves * kWave;
     if (mats == 1)
-      experts_rows_kernel<W, X, 1, RT, NB, SHARES><<<grid, threads, 0, s>>>(p, unsigned(blocks));
-    else if constexpr (RT > 1)
-      experts_rows_kernel<W, X, 2, RT, NB, SHARES><<<grid, threads, 0, s>>>(p, unsigned(blocks));
+      experts_rows_kernel<W, X, 1, NB, SHARES><<<grid, threads, 0, s>>>(p, unsigned(blocks));
+    else
+      experts_rows_kernel<W, X, 2, NB, SHARES><<<grid, threads, 0, s>>>(p, unsigned(blocks));
   };
   if (!wfp4) go(std::false_type{}, std::false_type{});
   else if (xfp4) go(std::true_type{}, std::true_type{});
@@ -210,13 +220,43 @@ int launch(hipStream_t s, const Product& p, int mats, bool wfp4, bool xfp4, size
 
 }  // namespace
 
-// The rules compare sizes that decide: how many rows an expert has, how many
-// workgroups a form makes, and how much each of them has to do. Times are
-// microseconds of one call, this kernel against the other or one form of tiles
-// against another.
+// What a form of tiles costs a CU: every workgroup `tile` and for each 256 bytes of a
+// row `stage`, and the first one `first` a stage that nothing overlaps with. The unit
+// is a tenth of the stage of a tile of 64 rows by 128 weight rows, 0.037 us in bf16.
+struct TileCost {
+  int width, rows;
+  double first, stage, tile;
+};
+constexpr TileCost kTileCosts[3][4] = {
+    {{4, 128, 7, 25, 44}, {2, 128, 6.7, 14, 47}, {2, 64, 2.7, 10, 7}, {2, 32, 0.9, 10.4, 10}},
+    {{4, 64, 12.7, 10.4, 49}, {2, 64, 3.3, 10, 12}, {2, 32, 2.9, 5.1, 6.6}, {}},
+    {{4, 128, 9.6, 29.6, 62}, {2, 128, 7.1, 16.6, 34}, {2, 64, 4.2, 10, 13}, {2, 32, 3.4, 10.2, 16}}};
+// What this kernel costs with 16 or 32 rows a workgroup: `chunk` for each chunk of a
+// wavefront, and for each turn of workgroups over the CUs `turn` and for each chunk
+// `turn_chunk`; of all that `start`.
+struct RowsCost {
+  double chunk, turn_chunk, turn;
+};
+constexpr RowsCost kRowsCosts[3][2] = {
+    {{4.6, 9.4, 57}, {4.2, 27, 16}}, {{4.7, 6.5, 26}, {9.9, 12, 12}}, {{1.3, 2.6, 36}, {2.2, 6.6, 16}}};
+constexpr double kRowsStart[3] = {-13, -24, -27};
+// The launch that joins shares of the columns, and a value of them.
+constexpr double kJoin[2] = {135, 92}, kJoinValue[2] = {5e-5, 2e-5};
+
+// The costs were fitted to 1600 products (1 to 256 experts or one matrix, 1 to 8192
+// tokens) timed in every form that the kernels have. Of 760 others the form that is
+// taken was 2.5% slower than the best on the mean, 28% at most. Some of both sides,
+// microseconds, tokens x columns x weight rows of one matrix in bf16: 4096 x 2048 x
+// 2048 by tiles of 128 x 256 37, by 64 x 128 46; 1536 x 2048 x 2048 31 and 22; 768 x
+// 1024 x 1024 by 64 x 128 10, by 32 x 128 9; 384 x 4096 x 512 by 32 x 128 17, with the
+// columns in four shares 13; 100 x 6144 x 1024 in eight shares 14, by this kernel 12.
+// Down of 640 tokens of 8 of 64 experts, 2048 x 768, MXFP4 by MXFP4, by 128 x 256 30,
+// by 64 x 128 23; gate and up of 1024 tokens of 10 of 128 experts, 1536 x 4096, MXFP4
+// by bf16, by 32 x 128 324, by 64 x 256 275.
 ExpertPlan plan_product(const ExpertProduct& q) {
   const ExpertMat& m = q.m[0];
-  const bool xfp4 = q.x_scales != nullptr, widened = m.fp4 && !xfp4;
+  const bool xfp4 = q.x_scales != nullptr;
+  const int form = !m.fp4 ? 0 : !xfp4 ? 1 : 2;
   ExpertPlan r{};
   r.splits = 1;
   // experts that the rows reach if each picks one by chance, and rows of one
@@ -224,62 +264,63 @@ ExpertPlan plan_product(const ExpertProduct& q) {
   const double K = double(m.cols);
   const double used = q.offsets ? E * (1.0 - std::pow(1.0 - 1.0 / E, A)) : 1.0;
   const double rows = A / used;
-  // workgroups of tiles of so many rows by 64 * width weight rows, and of this
-  // kernel's narrow form with all wavefronts on one pair of weight tiles
-  auto tiles = [&](int width, double height) {
-    const double n = q.offsets ? used * std::max(1.0, rows / height + (rows > height / 2 ? 0.5 : 0.0))
+  // workgroups of tiles of so many rows by 64 * width weight rows, the last tile of an
+  // expert counted as `part` of one
+  auto tiles = [&](int width, double height, double part) {
+    const double n = q.offsets ? used * std::max(1.0, rows / height + (rows > height / 2 ? part : 0.0))
                                : std::ceil(A / height);
     return n * std::ceil(N / (64.0 * width));
   };
-  const double groups = std::ceil(rows / 16) * used * std::ceil(N / 32);
   const size_t pitch = xfp4 ? m.cols / 2 : m.cols * 2, stages = (pitch + 255) / 256;
+  const bool only_tiles = switch_on("INFERNO_EXPERTS_TILES");
+  const bool only_rows = switch_off("INFERNO_EXPERTS_TILES") || q.A / q.k * pitch >= size_t(1) << 32;
+  double least = 0;
+  auto offer = [&](double time, bool by_tiles, int width, int height, int shares, size_t splits) {
+    if (r.width && time >= least) return;
+    least = time;
+    r = ExpertPlan{by_tiles, width, height, shares, splits};
+  };
 
-  // This kernel reads every row again for 32 weight rows, tiles have four wavefronts
-  // wait for each other. With enough workgroups of the lowest tiles these win (8 tokens
-  // of 8 of 64 experts, gate and up 768 x 2048 in bf16: 44 against 53 us); with fewer
-  // as soon as this kernel's have much to do (64 tokens by 6144 x 2048 in bf16: 15
-  // against 13 us, two such matrices 19 against 21).
-  const bool many = tiles(2, 32) >= 384;
-  r.tiles = many || (rows > 8 && groups * K > (q.offsets || rows > 32 ? 1.5e6 : 2e6));
-  if (switch_on("INFERNO_EXPERTS_TILES")) r.tiles = true;
-  if (switch_off("INFERNO_EXPERTS_TILES") || q.A / q.k * pitch >= size_t(1) << 32) r.tiles = false;
-  if (!r.tiles) {
-    r.width = rows > 64 ? 2 : 1;
-    const double mine = groups / r.width;
-    r.shares = mine < 256 || (mine < 1024 && K >= 2048) ? 4 : K >= 1536 ? 2 : 1;
-    return r;
-  }
-  // The largest tiles of which there are enough; then, where a workgroup's columns are
-  // long, shares of them. Experts have uneven numbers of rows, so that a tile holds
-  // twice their mean, or fills the CUs with workgroups.
-  double most = 0;  // workgroups up to which shares are doubled
-  if (!m.fp4) {
-    most = 192;
-    if (q.offsets) {
-      r.width = rows > 64 && tiles(4, 128) >= 384 ? 4 : 2;
-      r.rows = r.width == 4                                                  ? 128
-               : rows <= 12                                                  ? 32
-               : rows <= 28 || (rows > 80 && tiles(2, 128) < 384)            ? 64
-                                                                             : 128;
-    } else {
-      // (short columns: more workgroups, which start and end while others run)
-      const bool brief = m.cols <= 2048;
-      r.width = tiles(4, 128) >= (brief ? 512 : 192) ? 4 : 2;
-      r.rows = r.width == 4 || (!brief && tiles(2, 128) >= 192) ? 128 : tiles(2, 64) >= 192 ? 64 : 32;
+  if (q.offsets && rows <= 8 && !only_tiles) {
+    // The weights' bytes bound it, the kernels differ by what each CU has on its way.
+    // With enough workgroups of the lowest tiles these win (8 tokens of 8 of 64 experts,
+    // gate and up 768 x 2048 in MXFP4 by bf16: 18 against 20 us; 64 tokens: 22
+    // against 33), with fewer this kernel, which needs no barrier between stages (4
+    // tokens in bf16: 28 against 33).
+    if (only_rows || tiles(2, 32, 0.5) < 384) {
+      // wavefronts on the same weights where that makes workgroups enough, or shortens
+      // long rows (one token of 8 of 64 experts, gate and up 768 x 2048 in bf16: 16
+      // with one, 12 with two, 13 with four; of one matrix, 1536 x 4096, 9.3 with four
+      // and 10.2 with two)
+      const double mine = used * std::ceil(N / 32);
+      r.width = 1;
+      r.shares = mine < 256 || (mine < 1024 && K >= 2048) ? 4 : K >= 1536 ? 2 : 1;
+      return r;
     }
-  } else if (widened) {
-    most = 256;
-    r.width = rows >= 16 && tiles(4, 64) >= 512 ? 4 : 2;
-    r.rows = r.width == 4 || (rows >= 32 && tiles(2, 64) >= 512) ? 64 : 32;
-  } else {
-    r.width = rows >= 64 && tiles(4, 128) >= 500 ? 4 : 2;
-    r.rows = r.width == 4 || (K >= 4096 && rows >= 64 && tiles(2, 128) >= 512) ? 128
-             : tiles(2, 64) >= 192                                             ? 64
-                                                                               : 32;
+  } else if (!only_tiles) {
+    for (int width = 1; width <= 2; ++width)
+      for (int shares = 1; shares <= 4; shares *= 2) {
+        const RowsCost& c = kRowsCosts[form][width - 1];
+        const double chunks = std::ceil(K / (128.0 * shares));
+        const double turns =
+            std::ceil(used * std::ceil(rows / (16.0 * width)) * std::ceil(N * shares / 128) / kCUs);
+        offer(kRowsStart[form] + c.chunk * chunks + turns * (c.turn_chunk * chunks + c.turn), false, width,
+              16 * width, shares, 1);
+      }
+    if (only_rows) return r;
   }
-  if (r.width == 2)
-    while (r.splits < 8 && r.splits * 24 <= stages && double(r.splits) * tiles(2, r.rows) <= most)
-      r.splits *= 2;
+  // Shares of the columns, of twelve stages or more, where the workgroups are few. (Rows
+  // in MXFP4 have four times the columns in a stage: 12288 for two shares.)
+  for (const TileCost& c : kTileCosts[form]) {
+    for (size_t splits = 1; c.width && splits <= 8; splits *= 2) {
+      if (splits > 1 && (xfp4 || c.width > 2 || splits * 12 > stages)) break;
+      const double n = tiles(c.width, c.rows, xfp4 ? 0.3 : 0.7) * double(splits) / kCUs;
+      const double turns = q.offsets ? std::max(1.0, n) : std::ceil(n);
+      const double mine = std::ceil(double(stages) / double(splits));
+      const double join = splits > 1 ? kJoin[m.fp4] + kJoinValue[m.fp4] * double(splits) * A * N : 0;
+      offer(c.first * mine + turns * (c.stage * mine + c.tile) + join, true, c.width, c.rows, 0, splits);
+    }
+  }
   return r;
 }
 
@@ -324,9 +365,9 @@ int launch_expert_product(hipStream_t s, const ExpertProduct& q) {
   const size_t tiles = tiles_of(16 * plan.width);
   auto pick = [&](auto width) -> int {
     constexpr int NB = decltype(width)::value;
-    if (plan.shares == 1) return launch<2, NB, 1>(s, p, q.mats, m.fp4, xfp4, tiles);
-    if (plan.shares == 2) return launch<2, NB, 2>(s, p, q.mats, m.fp4, xfp4, tiles);
-    return launch<2, NB, 4>(s, p, q.mats, m.fp4, xfp4, tiles);
+    if (plan.shares == 1) return launch<NB, 1>(s, p, q.mats, m.fp4, xfp4, tiles);
+    if (plan.shares == 2) return launch<NB, 2>(s, p, q.mats, m.fp4, xfp4, tiles);
+    return launch<NB, 4>(s, p, q.mats, m.fp4, xfp4, tiles);
   };
   if (plan.width == 1) return pick(std::integral_constant<int, 1>{});
   return pick(std::integral_constant<int, 2>{});

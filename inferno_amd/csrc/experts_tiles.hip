@@ -1,16 +1,28 @@
-// Products of rows grouped by expert, many rows: tiles of up to 128 grouped rows
-// by 256 weight rows (128 gate and 128 up) on 16x16 matrix instructions.
+// Products of rows grouped by expert, many rows: tiles of up to 32, 64 or 128 grouped
+// rows by 128 or 256 weight rows (of two matrices half each) on 16x16 matrix
+// instructions.
 //
-// A wavefront owns four tiles of 16 weight rows against all rows of the tile, so
-// that the weights go from memory to registers once per workgroup, four steps
-// ahead, and only the grouped rows, which all four wavefronts read, go through
-// LDS (copied there directly, two buffers of 256 bytes a row). Of every 32
-// matrix instructions of a step (512 cycles) a wavefront reads 8 KB from LDS: half
-// of what LDS delivers. A step is 64 bytes of a row for either operand in bf16 (32
-// columns) and in 4 bits (128 columns); 4-bit weights against bf16 rows are
-// widened in registers, four steps from one load.
-// Tiles are cut at 128 rows, what is left takes the narrowest form of 16, 32, 64
-// or 128 rows that holds it.
+// Each of four wavefronts owns two or four tiles of 16 weight rows against all rows of
+// the tile, so that the weights, packed in the order of the lanes, go from memory to
+// registers once per workgroup, four steps ahead, and only the grouped rows, which all
+// wavefronts read, go through LDS (copied there directly, two buffers of 256 bytes a
+// row). Of the 32 matrix instructions of a step of the largest tile (512 cycles) a
+// wavefront reads 8 KB from LDS: half of what LDS delivers. A step is 64 bytes of a row
+// for either operand in bf16 (32 columns) and in 4 bits (128 columns); 4-bit weights
+// against bf16 rows are widened in registers, four steps from one load. What is left of
+// an expert's rows takes the narrowest code of 16, 32, 64 or 128 rows that holds it.
+// Where the columns are long and the workgroups few, several share a tile's columns;
+// a second launch adds their sums in order.
+//
+// Measured (a large copy moves 5.0 TB/s here, a large bf16 library product reaches 1.39
+// PFLOP/s): gate and up, 1536 x 4096, of 4096 tokens of 10 of 128 experts, MXFP4 by
+// bf16, 854 us: 1.21 PFLOP/s, the matrix cores. Down, 4096 x 1536, of 2048 such tokens
+// in bf16 441 us: 1.6 GB of weights and 336 MB of fp32 results, 4.6 TB/s. Down of 4096
+// tokens of 8 of 256 experts, 6144 x 2048, MXFP4 by MXFP4, 568 us: 1.7 GB and 805 MB, 4.5
+// TB/s. Where rows are few it is the weights' bytes: 512 tokens of those experts' gate
+// and up 581 us, 5.9 TB/s; 64 tokens of 10 of 128 in bf16 508 us, 6.1 TB/s.
+// Tiles of 256 rows by eight wavefronts were slower, as were results stored past the
+// caches.
 #include "experts_dev.hpp"
 
 namespace inferno {
