@@ -332,13 +332,15 @@ int inferno_experts_pack(void* stream, const inferno_experts* w, const void* wei
  * matrix and all rows (sorted = NULL).
  *   x       [x_rows, cols] bf16, or with weights in MXFP4 also MXFP4: codes
  *           [x_rows, cols / 2] with x_scales [x_rows, cols / 32] (else NULL)
- *   offsets [experts + 1] ascending, at most x_rows k
+ *   offsets [experts + 1] ascending, at most x_rows k (others write nothing out of
+ *           range, but results of their rows may be of anything)
  *   sorted  [x_rows k]; of an index out of range, or of a row in no group, no
  *           result is written
  *   out     [x_rows k, rows] F32 or BF16, which may not overlap an input
  * Sums are held in fp32, products are exact. A row that holds a NaN, an infinity or
  * a scale of 255 changes its own results alone. x and out lie at multiples of 16
- * bytes; x_rows k <= 2^22. x_rows = 0 does nothing. The workspace takes
+ * bytes; x_rows k <= 2^22, and with more than 2^24 workgroups, which needs some 10^10
+ * results, a call is refused. x_rows = 0 does nothing. The workspace takes
  * inferno_grouped_workspace_bytes at a multiple of 16 bytes (NULL where that is 0,
  * as it is for most products); calls that overlap need one each. */
 size_t inferno_grouped_workspace_bytes(const inferno_experts* w, int matrices, int x_dtype,

@@ -272,8 +272,9 @@ ExpertPlan plan_product(const ExpertProduct& q) {
     return n * std::ceil(N / (64.0 * width));
   };
   const size_t pitch = xfp4 ? m.cols / 2 : m.cols * 2, stages = (pitch + 255) / 256;
-  const bool only_tiles = switch_on("INFERNO_EXPERTS_TILES");
+  // (tiles copy rows by offsets of 32 bits)
   const bool only_rows = switch_off("INFERNO_EXPERTS_TILES") || q.A / q.k * pitch >= size_t(1) << 32;
+  const bool only_tiles = !only_rows && switch_on("INFERNO_EXPERTS_TILES");
   double least = 0;
   auto offer = [&](double time, bool by_tiles, int width, int height, int shares, size_t splits) {
     if (r.width && time >= least) return;

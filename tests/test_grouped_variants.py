@@ -149,6 +149,61 @@ def test_the_rule_shares_long_columns(cuda, w4):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tiles", [None, "1"])
+@pytest.mark.parametrize("form,K", [("bf16", 488), ("bf16", 520), ("mxfp4", 480), ("mxfp4-mxfp4", 1984),
+                                    ("mxfp4-mxfp4", 2080)])
+def test_rows_far_behind_the_first(cuda, monkeypatch, form, K, tiles):
+    """Rows of 4.1e9 bytes in all, and of more than 2^32, which tiles do not take."""
+    if tiles:
+        monkeypatch.setenv("INFERNO_EXPERTS_TILES", tiles)
+    w4, x4 = FORMS[form]
+    g = torch.Generator().manual_seed(K)
+    m = ref.Mats(g, 24, K, 0, w4)
+    A = (1 << 22) - 5
+    on_gpu = torch.Generator(device="cuda").manual_seed(K)
+    if x4:
+        x = (torch.randint(0, 256, (A, K // 2), generator=on_gpu, device="cuda", dtype=torch.uint8),
+             torch.randint(120, 124, (A, K // 32), generator=on_gpu, device="cuda", dtype=torch.uint8))
+    else:
+        x = (torch.empty(A, K, dtype=BF16, device="cuda").normal_(generator=on_gpu),)
+    got = _call([m], x)
+    at = torch.cat([torch.arange(40), torch.arange(A // 2, A // 2 + 40), torch.arange(A - 200, A)])
+    part = [t[at.cuda()].cpu() for t in x]
+    xv = ref.values(*part) if x4 else part[0].double()
+    want, bar = ref.product(m, xv, 0, torch.arange(len(at)))
+    ref.near(got[at.cuda()], want, bar + 2.0 ** -24 * want.abs() + 1e-38)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 300])
+def test_weights_far_behind_the_first(cuda, rows):
+    """The last of experts of 5e9 bytes."""
+    E, N, K = 200, 2040, 6144
+    w = torch.empty(E, N, K, dtype=BF16, device="cuda")
+    w.normal_(0.0, 0.05, generator=torch.Generator(device="cuda").manual_seed(rows))
+    handle = ops.Experts(w)
+    last = w[E - 1].cpu().double()
+    del w
+    x, xv = ref.rows(torch.Generator().manual_seed(rows), rows, K)
+    offsets = torch.zeros(E + 1, dtype=torch.int32)
+    offsets[E] = rows
+    got = ops.grouped_matmul(handle, *x, offsets=offsets.cuda())
+    want, bar = xv @ last.T, K * 2.0 ** -23 * (xv.abs() @ last.abs().T)
+    ref.near(got, want, bar + 2.0 ** -24 * want.abs())
+
+
+@pytest.mark.gpu
+def test_quantised_rows_far_behind_the_first(cuda):
+    x = torch.empty((1 << 21) + 3, 2048, dtype=BF16, device="cuda")
+    x.normal_(generator=torch.Generator(device="cuda").manual_seed(4))
+    codes, scales, held = ops.mxfp4_quantize(x, values=True)
+    for at in (slice(0, 3), slice((1 << 20) - 2, (1 << 20) + 2), slice((1 << 21) - 1, None)):
+        c, s, v = ref.quantize(x[at])
+        assert torch.equal(codes[at].cpu(), c) and torch.equal(scales[at].cpu(), s)
+        assert torch.equal(held[at].cpu().double(), v)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("form,T,E,N,K,tiles", [("mxfp4-mxfp4", 2240, 64, 2000, 96, None),
                                                 ("mxfp4-mxfp4", 2240, 64, 1000, 4096, None),
                                                 ("bf16", 2240, 64, 1500, 72, None),
