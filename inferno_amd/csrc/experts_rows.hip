@@ -284,10 +284,10 @@ ExpertPlan plan_product(const ExpertProduct& q) {
 
   if (q.offsets && rows <= 8 && !only_tiles) {
     // The weights' bytes bound it, the kernels differ by what each CU has on its way.
-    // With enough workgroups of the lowest tiles these win (8 tokens of 8 of 64 experts,
-    // gate and up 768 x 2048 in MXFP4 by bf16: 18 against 20 us; 64 tokens: 22
-    // against 33), with fewer this kernel, which needs no barrier between stages (4
-    // tokens in bf16: 28 against 33).
+    // With enough workgroups of the lowest tiles these win (64 tokens of 8 of 64 experts,
+    // gate and up 768 x 2048 in MXFP4 by bf16: 22 against 33 us; 8 tokens: both 18),
+    // with fewer this kernel, which needs no barrier between stages (4 tokens in bf16:
+    // 28 against 33).
     if (only_rows || tiles(2, 32, 0.5) < 384) {
       // wavefronts on the same weights where that makes workgroups enough, or shortens
       // long rows (one token of 8 of 64 experts, gate and up 768 x 2048 in bf16: 16
