@@ -177,3 +177,53 @@ def test_handles_outlive_their_tensors(cuda):
     got = ops.grouped_matmul(w, *x, offsets=offsets.cuda(), sorted_=sorted_.cuda())
     want, bar, _ = ref.expected([m], xv, 30, 1, offsets, sorted_, F32)
     ref.near(got, want, bar)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("w4", [False, True])
+def test_packed_inside_a_graph(cuda, w4):
+    """A handle that a graph packs holds its matrices after the first replay, and those
+    that the tensors hold at a later one."""
+    g = torch.Generator().manual_seed(1)
+    m, other = (ref.Mats(g, 70, 160, 3, w4) for _ in range(2))
+    x, xv = ref.rows(g, 33, 160)
+    offsets, sorted_ = ref.groups(g, 33, 1, 3)
+    offsets_, sorted__ = offsets.cuda(), sorted_.cuda()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w = ops.Experts(*m.parts)
+        y = ops.grouped_matmul(w, *x, offsets=offsets_, sorted_=sorted__)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        got = ops.grouped_matmul(w, *x, offsets=offsets_, sorted_=sorted__)
+        want, bar, _ = ref.expected([m], xv, 33, 1, offsets, sorted_, F32)
+        ref.near(got, want, bar)
+        assert torch.equal(got, y)
+        for to, new in zip(m.parts, other.parts):
+            to.copy_(new)
+        m.values = other.values
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("w4,x4", FORMS, ids=IDS)
+def test_the_same_assignment_twice(cuda, w4, x4):
+    """An index that comes twice: its row is one of its two experts' results, value by
+    value, and all others are as ever."""
+    g = torch.Generator().manual_seed(6)
+    m = [ref.Mats(g, 48, 192, 2, w4)]
+    x, xv = ref.rows(g, 40, 192, x4)
+    offsets = torch.tensor([0, 20, 40], dtype=torch.int32)
+    order = torch.randperm(40, generator=g).to(torch.int32)
+    order[30] = order[3]
+    w = ops.Experts(*m[0].parts)
+    out = torch.full((40, 48), 7.0, device="cuda")
+    got = ops.grouped_matmul(w, *x, offsets=offsets.cuda(), sorted_=order.cuda(), out=out).cpu().double()
+    fine = got == 7.0
+    for e in range(2):
+        a = order[20 * e: 20 * e + 20].long()
+        y, d = ref.product(m[0], xv, e, a)
+        near = (got[a] - y).abs() <= d + 2.0 ** -24 * y.abs()
+        fine[a] |= near
+    assert fine.all() and (got[torch.tensor([i for i in range(40) if i not in order.tolist()])] == 7.0).all()
