@@ -244,8 +244,8 @@ constexpr double kRowsStart[3] = {-13, -24, -27};
 constexpr double kJoin[2] = {135, 92}, kJoinValue[2] = {5e-5, 2e-5};
 
 // The costs were fitted to 1600 products (1 to 256 experts or one matrix, 1 to 8192
-// tokens) timed in every form that the kernels have. Of 760 others the form that is
-// taken was 2.5% slower than the best on the mean, 28% at most. Some of both sides,
+// tokens) timed in every form that the kernels have. Of 400 others the form that is
+// taken was 2.5% slower than the best on the mean, 22% at most. Some of both sides,
 // microseconds, tokens x columns x weight rows of one matrix in bf16: 4096 x 2048 x
 // 2048 by tiles of 128 x 256 37, by 64 x 128 46; 1536 x 2048 x 2048 31 and 22; 768 x
 // 1024 x 1024 by 64 x 128 10, by 32 x 128 9; 384 x 4096 x 512 by 32 x 128 17, with the
