@@ -249,16 +249,42 @@ def router_group_topk(logits, bias, k, score_fn, norm, scale, n_group, topk_grou
     return ids, w, tok
 
 
-class W4:
+class _Packed:
+    """Weights that were packed on one stream and may be used on any."""
+
+    def _hold(self, data):
+        """Waits for the packing into ``data``, but for a stream that is being captured."""
+        self._data, self._streams = data, {_raw_stream(self.device.index)}
+        stream = torch.cuda.current_stream(self.device)
+        with torch.cuda.device(self.device):
+            if not torch.cuda.is_current_stream_capturing():
+                stream.synchronize()
+
+    def _on(self, x):
+        """``ref``, for a call on x's current stream. When the handle goes, the
+        allocator gives the packed bytes to the stream that they were packed on; of each
+        other stream it is told once, and then waits for what is queued there. (Of a
+        graph's replays it cannot know: the handle has to outlive the graph.)"""
+        stream = _raw_stream(self.device.index)
+        if stream not in self._streams:
+            with torch.cuda.device(self.device):
+                if not torch.cuda.is_current_stream_capturing():
+                    self._data.record_stream(torch.cuda.current_stream(self.device))
+                    self._streams.add(stream)
+        return self.ref
+
+
+class W4(_Packed):
     """4-bit weights with group scales (struct inferno_w4): one matrix [rows,
     cols], or one per expert [E, rows, cols]. ``codes`` holds two columns a byte
     (uint8 [..., cols / 2], the even column in the low nibble), ``scales`` one
     factor per cols / scales.shape[-1] columns (fp32 or bf16), ``zeros`` a zero
     point for each scale (uint8; None: 8), of which one above 127 counts as 127.
     Packed once, here, on the current stream (inferno_w4_pack), which is waited for:
-    the handle may be used on any stream at once, and the tensors are not kept. While
-    the stream is being captured nothing is waited for; such a handle holds its matrix
-    after the graph's first replay."""
+    the handle may be used on any stream at once, and may go while calls are queued
+    there; a graph that captured a call needs it as long as it is replayed. The tensors
+    are not kept. While the stream is being captured nothing is waited for; such a
+    handle holds its matrix after the graph's first replay."""
 
     def __init__(self, codes, scales, zeros=None):
         if codes.dtype != torch.uint8 or codes.dim() not in (2, 3) or not codes.is_contiguous():
@@ -285,10 +311,7 @@ class W4:
              scales.numel() * scales.element_size(), _at(zeros),
              zeros.numel() if zeros is not None else 0, _at(self.packed))
         d.packed = self.packed.data_ptr()
-        stream = torch.cuda.current_stream(self.device)
-        with torch.cuda.device(self.device):
-            if not torch.cuda.is_current_stream_capturing():
-                stream.synchronize()
+        self._hold(self.packed)
 
 
 _ACT = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: I8}
@@ -327,7 +350,7 @@ def w4_matvec_add2(w, x, residual_a=None, residual_b=None, x_scales=None):
     out = torch.empty(T, w.rows, dtype=torch.float32, device=x.device)
     n = lib().inferno_w4_workspace_bytes(T, w.cols)
     ws = _w4_ws(x, n)
-    _run(x, lib().inferno_w4_matvec_add2, w.ref, _at(x), dt, xs, xg, _at(residual_a),
+    _run(x, lib().inferno_w4_matvec_add2, w._on(x), _at(x), dt, xs, xg, _at(residual_a),
          _at(residual_b), T, _at(out), _at(ws), n)
     return out
 
@@ -341,8 +364,8 @@ def w4_gate_up_swiglu(gate, up, x, x_scales=None):
     out = torch.empty(T, gate.rows, dtype=torch.float32, device=x.device)
     n = lib().inferno_w4_workspace_bytes(T, gate.cols)
     ws = _w4_ws(x, n)
-    _run(x, lib().inferno_w4_gate_up_swiglu, gate.ref, up.ref, _at(x), dt, xs, xg, T, _at(out),
-         _at(ws), n)
+    _run(x, lib().inferno_w4_gate_up_swiglu, gate._on(x), up._on(x), _at(x), dt, xs, xg, T,
+         _at(out), _at(ws), n)
     return out
 
 
@@ -360,8 +383,8 @@ def w4_moe(gate, up, down, x, ids, weights, k, x_scales=None):
     out = torch.empty(T, H, dtype=torch.float32, device=x.device)
     n = lib().inferno_w4_moe_workspace_bytes(T, k, gate.experts, H, gate.rows)
     ws = _w4_ws(x, n)
-    _run(x, lib().inferno_w4_moe, gate.ref, up.ref, down.ref, _at(x), dt, xs, xg, _at(ids),
-         _at(weights), T, k, _at(out), _at(ws), n)
+    _run(x, lib().inferno_w4_moe, gate._on(x), up._on(x), down._on(x), _at(x), dt, xs, xg,
+         _at(ids), _at(weights), T, k, _at(out), _at(ws), n)
     return out
 
 
@@ -382,14 +405,16 @@ def mxfp4_quantize(x, values=False):
     return (codes, scales, held) if values else (codes, scales)
 
 
-class Experts:
+class Experts(_Packed):
     """Weights of the products grouped by expert (struct inferno_experts): one
     matrix [rows, cols], or one per expert [E, rows, cols], as a bf16 tensor, or in
     MXFP4 as ``codes`` (uint8 [..., cols / 2], the even column in the low nibble) and
     ``scales`` (uint8 [..., cols / 32]). Packed once, here, on the current stream
     (inferno_experts_pack), which is waited for: the handle may be used on any stream
-    at once, and the tensors are not kept. While the stream is being captured nothing is
-    waited for; such a handle holds its matrices after the graph's first replay."""
+    at once, and may go while calls are queued there; a graph that captured a call needs
+    it as long as it is replayed. The tensors are not kept. While the stream is being
+    captured nothing is waited for; such a handle holds its matrices after the graph's
+    first replay."""
 
     def __init__(self, weights, scales=None):
         dtype = torch.bfloat16 if scales is None else torch.uint8
@@ -414,10 +439,7 @@ class Experts:
              weights.numel() * weights.element_size(), _at(scales),
              scales.numel() if self.mxfp4 else 0, _at(self.data))
         d.data = self.data.data_ptr()
-        stream = torch.cuda.current_stream(self.device)
-        with torch.cuda.device(self.device):
-            if not torch.cuda.is_current_stream_capturing():
-                stream.synchronize()
+        self._hold(self.data)
 
 
 def _grouped(fn, mats, x, x_scales, offsets, sorted_, k, out_dtype, out):
@@ -449,8 +471,8 @@ def _grouped(fn, mats, x, x_scales, offsets, sorted_, k, out_dtype, out):
     dt = MXFP4 if fp4 else BF16
     n = lib().inferno_grouped_workspace_bytes(w.ref, len(mats), dt, T, k, offsets is not None)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    _run(x, fn, *(m.ref for m in mats), _at(x), dt, _at(x_scales), T, _at(offsets), _at(sorted_), k,
-         _DT[out.dtype], _at(out), _at(ws), n)
+    _run(x, fn, *(m._on(x) for m in mats), _at(x), dt, _at(x_scales), T, _at(offsets), _at(sorted_),
+         k, _DT[out.dtype], _at(out), _at(ws), n)
     return out
 
 

@@ -1,0 +1,110 @@
+"""Packed weights (Experts, W4) and the streams that use them: a handle may go while a
+call on another stream is queued."""
+import contextlib
+
+import pytest
+import torch
+
+import experts_reference as ref
+from inferno_amd import ops
+
+F32, BF16, U8 = torch.float32, torch.bfloat16, torch.uint8
+
+
+class _Bytes:
+    """Stands for packed bytes; notes the streams that it is told of."""
+
+    def __init__(self):
+        self.told = []
+
+    def record_stream(self, stream):
+        self.told.append(stream)
+
+
+@pytest.mark.parametrize("kind", [ops.Experts, ops.W4])
+def test_each_other_stream_is_told_of_once(monkeypatch, kind):
+    now = {"stream": 5, "capturing": False}
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: now["stream"])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: now["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: contextlib.nullcontext())
+    h = kind.__new__(kind)
+    h.device, h.ref, data = torch.device("cuda:0"), object(), _Bytes()
+    now["capturing"] = True  # (nothing to wait for here)
+    h._hold(data)
+    for stream, capturing, told in [(5, False, []), (7, True, []), (7, False, [7]), (7, False, [7]),
+                                    (5, False, [7]), (9, False, [7, 9]), (7, True, [7, 9])]:
+        now.update(stream=stream, capturing=capturing)
+        assert h._on(None) is h.ref and data.told == told
+
+
+def _experts(g, fp4):
+    m = ref.Mats(g, 2080, 2048, 8, fp4)
+    x, xv = ref.rows(g, 24, 2048)
+    offsets, sorted_ = ref.groups(g, 24, 2, 8)
+    o, s = offsets.cuda(), sorted_.cuda()
+    want, bar, _ = ref.expected([m], xv, 48, 2, offsets, sorted_, F32)
+    return lambda: ops.Experts(*m.parts), \
+        lambda w: ops.grouped_matmul(w, *x, offsets=o, sorted_=s, k=2), want, bar
+
+
+def _w4(g):
+    codes = torch.randint(0, 256, (8192, 1024), generator=g, dtype=U8)
+    scales = 0.01 * (1.0 + torch.rand(8192, 16, generator=g))
+    x = torch.randn(1, 2048, generator=g).to(BF16)
+    q = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).double() - 8.0
+    w = q * scales.double().repeat_interleave(128, -1)
+    # x is exact in bf16: sums of 128 exact products, times a scale, in fp32
+    bar = 2048 * 2.0 ** -23 * (x.double().abs() @ w.abs().T) + 1e-30
+    codes, scales, xs = codes.cuda(), scales.cuda(), x.cuda()
+    return lambda: ops.W4(codes, scales), lambda w: ops.w4_matvec_add2(w, xs), x.double() @ w.T, bar
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "mxfp4", "w4"])
+def test_a_handle_goes_while_its_call_is_queued(cuda, kind):
+    """Its bytes are given to nobody before the other stream has read them."""
+    g = torch.Generator().manual_seed(11)
+    make, call, want, bar = _w4(g) if kind == "w4" else _experts(g, kind == "mxfp4")
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        long = torch.zeros(8192, 8192, dtype=BF16, device="cuda")
+        warm = make()
+        call(warm)
+        long @ long
+    del warm
+    torch.cuda.synchronize()
+    w = make()
+    data = w.packed if kind == "w4" else w.data
+    size, at = data.numel(), data.data_ptr()
+    del data
+    with torch.cuda.stream(side):
+        for _ in range(60):
+            long @ long
+        got = call(w)
+        busy = torch.cuda.Event()
+        busy.record()
+    del w
+    other = torch.full((size,), 255, dtype=U8, device="cuda")
+    assert not busy.query()  # the call was queued all that while
+    assert other.data_ptr() != at
+    side.synchronize()
+    ref.near(got, want, bar)
+
+
+@pytest.mark.gpu
+def test_captured_on_another_stream(cuda):
+    """A graph's call tells the allocator nothing; the handle outlives the graph."""
+    g = torch.Generator().manual_seed(12)
+    make, call, want, bar = _experts(g, True)
+    w = make()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call(w)
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        ref.near(y, want, bar)
+        ref.near(call(w), want, bar)
