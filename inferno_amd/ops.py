@@ -252,12 +252,16 @@ def router_group_topk(logits, bias, k, score_fn, norm, scale, n_group, topk_grou
 class _Packed:
     """Weights that were packed on one stream and may be used on any."""
 
-    def _hold(self, data):
-        """Waits for the packing into ``data``, but for a stream that is being captured."""
+    def _hold(self, data, *tensors):
+        """Waits for the packing of ``tensors`` into ``data``. While the stream is being
+        captured there is nothing to wait for, but each replay packs again: it keeps
+        them."""
         self._data, self._streams = data, {_raw_stream(self.device.index)}
         stream = torch.cuda.current_stream(self.device)
         with torch.cuda.device(self.device):
-            if not torch.cuda.is_current_stream_capturing():
+            capturing = torch.cuda.is_current_stream_capturing()
+            self._tensors = tensors if capturing else ()
+            if not capturing:
                 stream.synchronize()
 
     def _on(self, x):
@@ -284,7 +288,8 @@ class W4(_Packed):
     the handle may be used on any stream at once, and may go while calls are queued
     there; a graph that captured a call needs it as long as it is replayed. The tensors
     are not kept. While the stream is being captured nothing is waited for; such a
-    handle holds its matrix after the graph's first replay."""
+    handle holds its matrix after the graph's first replay, and keeps the tensors, which
+    every replay packs again."""
 
     def __init__(self, codes, scales, zeros=None):
         if codes.dtype != torch.uint8 or codes.dim() not in (2, 3) or not codes.is_contiguous():
@@ -311,7 +316,7 @@ class W4(_Packed):
              scales.numel() * scales.element_size(), _at(zeros),
              zeros.numel() if zeros is not None else 0, _at(self.packed))
         d.packed = self.packed.data_ptr()
-        self._hold(self.packed)
+        self._hold(self.packed, codes, scales, zeros)
 
 
 _ACT = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: I8}
@@ -414,7 +419,7 @@ class Experts(_Packed):
     at once, and may go while calls are queued there; a graph that captured a call needs
     it as long as it is replayed. The tensors are not kept. While the stream is being
     captured nothing is waited for; such a handle holds its matrices after the graph's
-    first replay."""
+    first replay, and keeps the tensors, which every replay packs again."""
 
     def __init__(self, weights, scales=None):
         dtype = torch.bfloat16 if scales is None else torch.uint8
@@ -439,7 +444,7 @@ class Experts(_Packed):
              weights.numel() * weights.element_size(), _at(scales),
              scales.numel() if self.mxfp4 else 0, _at(self.data))
         d.data = self.data.data_ptr()
-        self._hold(self.data)
+        self._hold(self.data, weights, scales)
 
 
 def _grouped(fn, mats, x, x_scales, offsets, sorted_, k, out_dtype, out):
