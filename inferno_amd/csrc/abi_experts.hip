@@ -63,6 +63,11 @@ ExpertProduct product(const inferno_experts* w0, const inferno_experts* w1, cons
   return p;
 }
 
+int check_form(const ExpertPlan& plan) {
+  INF_CHECK_ARG(plan.width > 0, "INFERNO_EXPERTS_FORM names no form of this product");
+  return INFERNO_OK;
+}
+
 int run_product(void* stream, const inferno_experts* w0, const inferno_experts* w1, const void* x,
                 int x_dtype, const uint8_t* x_scales, size_t x_rows, const uint32_t* offsets,
                 const uint32_t* sorted, size_t k, int out_dtype, void* out, void* workspace,
@@ -84,7 +89,9 @@ int run_product(void* stream, const inferno_experts* w0, const inferno_experts* 
   INF_CHECK_ARG(aligned(offsets, 4) && aligned(sorted, 4),
                 "offsets and sorted must lie at multiples of 4 bytes");
   ExpertProduct p = product(w0, w1, x_scales, x_rows * k, k, offsets);
-  if (int st = need_ws(workspace, workspace_bytes, product_workspace(p))) return st;
+  const ExpertPlan plan = plan_product(p);
+  if (int st = check_form(plan)) return st;
+  if (int st = need_ws(workspace, workspace_bytes, product_workspace(p, plan))) return st;
   INF_CHECK_ARG(aligned(workspace, 16), "the workspace must lie at a multiple of 16 bytes");
   if (int st_ = require_device()) return st_;
   p.x = x;
@@ -92,7 +99,7 @@ int run_product(void* stream, const inferno_experts* w0, const inferno_experts* 
   p.out_dtype = out_dtype;
   p.out = out;
   p.workspace = workspace;
-  return launch_expert_product(as_stream(stream), p);
+  return launch_expert_product(as_stream(stream), p, plan);
 }
 
 }  // namespace
@@ -153,9 +160,11 @@ size_t inferno_grouped_workspace_bytes(const inferno_experts* w, int matrices, i
     return 0;
   static const uint8_t scale = 127;  // (only whether there are scales and offsets counts)
   static const uint32_t offset = 0;
-  return product_workspace(product(w, matrices == 2 ? w : nullptr,
-                                   x_dtype == INFERNO_MXFP4 ? &scale : nullptr, x_rows * k, k,
-                                   grouped ? &offset : nullptr));
+  const ExpertProduct p = product(w, matrices == 2 ? w : nullptr,
+                                  x_dtype == INFERNO_MXFP4 ? &scale : nullptr, x_rows * k, k,
+                                  grouped ? &offset : nullptr);
+  const ExpertPlan plan = plan_product(p);
+  return check_form(plan) ? 0 : product_workspace(p, plan);
 }
 
 int inferno_grouped_matmul(void* stream, const inferno_experts* w, const void* x, int x_dtype,

@@ -63,11 +63,11 @@ struct ExpertProduct {
 // wavefronts.
 struct ExpertPlan {
   bool tiles;
-  int width, rows, shares;
+  int width, rows, shares;  // width 0: the environment names a form that there is not
   size_t splits;
 };
 ExpertPlan plan_product(const ExpertProduct& p);
-size_t product_workspace(const ExpertProduct& p);
-int launch_expert_product(hipStream_t s, const ExpertProduct& p);
+size_t product_workspace(const ExpertProduct& p, const ExpertPlan& plan);
+int launch_expert_product(hipStream_t s, const ExpertProduct& p, const ExpertPlan& plan);
 
 }  // namespace inferno

@@ -16,6 +16,7 @@
 // 11.2 (4.5 TB/s); gate and up of a shared expert, 1536 x 4096 in MXFP4, 8.2, where a
 // launch of nothing takes 6.2.
 #include <cmath>
+#include <cstdio>
 
 #include "experts_dev.hpp"
 
@@ -243,6 +244,18 @@ constexpr double kRowsStart[3] = {-13, -24, -27};
 // The launch that joins shares of the columns, and a value of them.
 constexpr double kJoin[2] = {135, 92}, kJoinValue[2] = {5e-5, 2e-5};
 
+// "t4-128/1": tiles of 128 rows by 64 * 4 weight rows, the columns in one share;
+// "r2/4": this kernel with 16 * 2 rows, the columns shared by four wavefronts.
+ExpertPlan named_form(const char* name) {
+  ExpertPlan r{};
+  r.tiles = std::sscanf(name, "t%d-%d/%zu", &r.width, &r.rows, &r.splits) == 3;
+  if (r.tiles) return r;
+  if (std::sscanf(name, "r%d/%d", &r.width, &r.shares) != 2) return ExpertPlan{};
+  r.rows = 16 * r.width;
+  r.splits = 1;
+  return r;
+}
+
 // The costs were fitted to 1600 products (1 to 256 experts or one matrix, 1 to 8192
 // tokens) timed in every form that the kernels have. Of 400 others the form that is
 // taken was 2.5% slower than the best on the mean, 22% at most. Some of both sides,
@@ -275,14 +288,19 @@ ExpertPlan plan_product(const ExpertProduct& q) {
   // (tiles copy rows by offsets of 32 bits)
   const bool only_rows = switch_off("INFERNO_EXPERTS_TILES") || q.A / q.k * pitch >= size_t(1) << 32;
   const bool only_tiles = !only_rows && switch_on("INFERNO_EXPERTS_TILES");
+  const char* name = std::getenv("INFERNO_EXPERTS_FORM");
+  const ExpertPlan named = name ? named_form(name) : ExpertPlan{};
   double least = 0;
   auto offer = [&](double time, bool by_tiles, int width, int height, int shares, size_t splits) {
+    if (name && (named.tiles != by_tiles || named.width != width || named.rows != height ||
+                 named.shares != shares || named.splits != splits))
+      return;
     if (r.width && time >= least) return;
     least = time;
     r = ExpertPlan{by_tiles, width, height, shares, splits};
   };
 
-  if (q.offsets && rows <= 8 && !only_tiles) {
+  if (q.offsets && rows <= 8 && !only_tiles && !name) {
     // The weights' bytes bound it, the kernels differ by what each CU has on its way.
     // With enough workgroups of the lowest tiles these win (64 tokens of 8 of 64 experts,
     // gate and up 768 x 2048 in MXFP4 by bf16: 22 against 33 us; 8 tokens: both 18),
@@ -325,12 +343,11 @@ ExpertPlan plan_product(const ExpertProduct& q) {
   return r;
 }
 
-size_t product_workspace(const ExpertProduct& q) {
-  const ExpertPlan r = plan_product(q);
+size_t product_workspace(const ExpertProduct& q, const ExpertPlan& r) {
   return r.splits > 1 ? r.splits * q.mats * q.A * ((q.m[0].rows + 3) / 4 * 16) : 0;
 }
 
-int launch_expert_product(hipStream_t s, const ExpertProduct& q) {
+int launch_expert_product(hipStream_t s, const ExpertProduct& q, const ExpertPlan& plan) {
   Product p{};
   const ExpertMat& m = q.m[0];
   const ExpertLayout l = expert_layout(m);
@@ -359,7 +376,6 @@ int launch_expert_product(hipStream_t s, const ExpertProduct& q) {
   const bool xfp4 = q.x_scales != nullptr;
   const size_t x_bytes = q.A / q.k * (xfp4 ? m.cols / 2 : m.cols * 2);
   p.x_bytes = uint32_t(x_bytes);
-  const ExpertPlan plan = plan_product(q);
   p.splits = uint32_t(plan.splits);
   p.partial = static_cast<float*>(q.workspace);
   if (plan.tiles) return launch_experts_tiles(s, p, q.mats, m.fp4, xfp4, tiles_of(plan.rows), plan.width, plan.rows);
