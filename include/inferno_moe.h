@@ -301,7 +301,8 @@ int inferno_mxfp4_quantize(void* stream, const void* x, int x_dtype, size_t rows
 
 /* One matrix [rows,cols], or one per expert, in the packed form that
  * inferno_experts_pack writes once, at a multiple of 16 bytes. BF16: cols a multiple of
- * 8. MXFP4: cols a multiple of 32; scales (but for 255) lie between 2^-100 and 2^100.
+ * 8. MXFP4: cols a multiple of 32; scales (but for 255) lie between 2^-100 and 2^100;
+ * the scale of 32 zeros counts for nothing (inferno_mxfp4_quantize gives them 2^-127).
  * experts <= 256, rows and cols <= 2^24, one matrix at most 2^33 values. */
 typedef struct inferno_experts {
   size_t experts;
@@ -331,7 +332,8 @@ int inferno_experts_pack(void* stream, const inferno_experts* w, const void* wei
  * c, rows that lie in the order of the experts (k = 1). offsets = NULL: one
  * matrix and all rows (sorted = NULL).
  *   x       [x_rows, cols] bf16, or with weights in MXFP4 also MXFP4: codes
- *           [x_rows, cols / 2] with x_scales [x_rows, cols / 32] (else NULL)
+ *           [x_rows, cols / 2] with x_scales [x_rows, cols / 32] (else NULL), of any
+ *           magnitude whose results lie in fp32's range
  *   offsets [experts + 1] ascending, at most x_rows k (others write nothing out of
  *           range, but results of their rows may be of anything)
  *   sorted  [x_rows k]; of an index out of range, or of a row in no group, no
