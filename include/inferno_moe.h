@@ -334,8 +334,8 @@ int inferno_experts_pack(void* stream, const inferno_experts* w, const void* wei
  *   x       [x_rows, cols] bf16, or with weights in MXFP4 also MXFP4: codes
  *           [x_rows, cols / 2] with x_scales [x_rows, cols / 32] (else NULL), of any
  *           magnitude whose results lie in fp32's range
- *   offsets [experts + 1] ascending, at most x_rows k (others write nothing out of
- *           range, but results of their rows may be of anything)
+ *   offsets [experts + 1] ascending, at most x_rows k (with others nothing is read or
+ *           written out of range, but any result may be missing or of anything)
  *   sorted  [x_rows k]; of an index out of range, or of a row in no group, no
  *           result is written
  *   out     [x_rows k, rows] F32 or BF16, which may not overlap an input
