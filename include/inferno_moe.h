@@ -301,8 +301,8 @@ int inferno_mxfp4_quantize(void* stream, const void* x, int x_dtype, size_t rows
 
 /* One matrix [rows,cols], or one per expert, in the packed form that
  * inferno_experts_pack writes once, at a multiple of 16 bytes. BF16: cols a multiple of
- * 8. MXFP4: cols a multiple of 32; scales (but for 255) lie between 2^-100 and 2^100;
- * the scale of 32 zeros counts for nothing (inferno_mxfp4_quantize gives them 2^-127).
+ * 8. MXFP4: cols a multiple of 32; scales (but for 255) lie between 2^-100 and 2^100,
+ * or are of 32 zeros, for which they count for nothing (inferno_mxfp4_quantize: 2^-127).
  * experts <= 256, rows and cols <= 2^24, one matrix at most 2^33 values. */
 typedef struct inferno_experts {
   size_t experts;

@@ -8,13 +8,14 @@
 // are four neighbouring values of one result row. Of a workgroup's four wavefronts
 // SHARES take the same weight rows and share the columns; they add their sums in
 // order through LDS. What bounds it is how many bytes are on their way: every
-// wavefront loads kAhead chunks of 128 columns before it uses the first (twice as
-// many, and workgroups of 8 or 16 wavefronts, were slower).
+// wavefront loads kAhead chunks of 128 columns before it uses the first.
 //
 // One token, microseconds of a call among others: down of 8 of 256 experts, 6144 x
-// 2048 in MXFP4, 12.2 (4.4 TB/s); gate and up of 8 of 64 experts, 768 x 2048 in bf16,
-// 11.2 (4.5 TB/s); gate and up of a shared expert, 1536 x 4096 in MXFP4, 8.2, where a
-// launch of nothing takes 6.2.
+// 2048 in MXFP4, 12.0 (4.5 TB/s); gate and up of 8 of 64 experts, 768 x 2048 in bf16,
+// 11.3 (4.5 TB/s); gate and up of a shared expert, 1536 x 4096 in MXFP4, 8.8, where a
+// launch of nothing takes 6.2. With twice as many chunks ahead the three launches take,
+// from one to the next of a graph, 16.2, 15.2 and 6.4 in place of 14.1, 13.3 and 6.6;
+// with four times as many in MXFP4 the first takes 21 and the last 7.2.
 #include <cmath>
 #include <cstdio>
 
@@ -223,7 +224,9 @@ int launch(hipStream_t s, const Product& p, int mats, bool wfp4, bool xfp4, size
 
 // What a form of tiles costs a CU: every workgroup `tile` and for each 256 bytes of a
 // row `stage`, and the first one `first` a stage that nothing overlaps with. The unit
-// is a tenth of the stage of a tile of 64 rows by 128 weight rows, 0.037 us in bf16.
+// is a tenth of the stage of a tile of 64 rows by 128 weight rows. Only the ratios
+// count: of products of 30 us and more a unit was 0.08 us at the median (MXFP4 by bf16
+// 0.05), half of them within a third of that.
 struct TileCost {
   int width, rows;
   double first, stage, tile;
@@ -257,15 +260,19 @@ ExpertPlan named_form(const char* name) {
 }
 
 // The costs were fitted to 1600 products (1 to 256 experts or one matrix, 1 to 8192
-// tokens) timed in every form that the kernels have. Of 400 others the form that is
-// taken was 2.5% slower than the best on the mean, 22% at most. Some of both sides,
-// microseconds, tokens x columns x weight rows of one matrix in bf16: 4096 x 2048 x
-// 2048 by tiles of 128 x 256 37, by 64 x 128 46; 1536 x 2048 x 2048 31 and 22; 768 x
-// 1024 x 1024 by 64 x 128 10, by 32 x 128 9; 384 x 4096 x 512 by 32 x 128 17, with the
-// columns in four shares 13; 100 x 6144 x 1024 in eight shares 14, by this kernel 12.
-// Down of 640 tokens of 8 of 64 experts, 2048 x 768, MXFP4 by MXFP4, by 128 x 256 30,
-// by 64 x 128 23; gate and up of 1024 tokens of 10 of 128 experts, 1536 x 4096, MXFP4
-// by bf16, by 32 x 128 324, by 64 x 256 275.
+// tokens) timed in every form that the kernels have, by such a search as
+// perf/experts_forms.py makes. Of 1600 others, drawn anew, the form that is taken was
+// 4% slower than the fastest of all on the mean, 14% at the 95th percentile and 46% at
+// most: groups of 15 rows by 729 x 6304 in bf16, tiles of 32 rows where 128 rows with
+// the columns in two shares take 31 us in place of 46. (17 rows of one matrix, 4751 x
+// 5872, take 16 rows a workgroup and two wavefronts, 22 us; 32 and four take 16.) Some of
+// both sides, microseconds, tokens x columns x weight rows of one matrix in bf16: 4096 x
+// 2048 x 2048 by tiles of 128 x 256 41, by 64 x 128 49; 1536 x 2048 x 2048 33 and 23;
+// 384 x 4096 x 512 by 32 x 128 17, with the columns in two shares 14; 100 x 6144 x 1024
+// by 32 x 128 23, in four shares 13, by this kernel 12. Down of 640 tokens of 8 of 64
+// experts, 2048 x 768, MXFP4 by MXFP4, by 128 x 256 33, by 64 x 128 27; gate and up of
+// 1024 tokens of 10 of 128 experts, 1536 x 4096, MXFP4 by bf16, by 32 x 128 327, by 64 x
+// 256 293.
 ExpertPlan plan_product(const ExpertProduct& q) {
   const ExpertMat& m = q.m[0];
   const bool xfp4 = q.x_scales != nullptr;
@@ -303,14 +310,13 @@ ExpertPlan plan_product(const ExpertProduct& q) {
   if (q.offsets && rows <= 8 && !only_tiles && !name) {
     // The weights' bytes bound it, the kernels differ by what each CU has on its way.
     // With enough workgroups of the lowest tiles these win (64 tokens of 8 of 64 experts,
-    // gate and up 768 x 2048 in MXFP4 by bf16: 22 against 33 us; 8 tokens: both 18),
+    // gate and up 768 x 2048 in MXFP4 by bf16: 22 against 32 us; 8 tokens: both 18),
     // with fewer this kernel, which needs no barrier between stages (4 tokens in bf16:
-    // 28 against 33).
+    // 30 against 33).
     if (only_rows || tiles(2, 32, 0.5) < 384) {
       // wavefronts on the same weights where that makes workgroups enough, or shortens
-      // long rows (one token of 8 of 64 experts, gate and up 768 x 2048 in bf16: 16
-      // with one, 12 with two, 13 with four; of one matrix, 1536 x 4096, 9.3 with four
-      // and 10.2 with two)
+      // long rows (one token of 8 of 64 experts, gate and up 768 x 2048 in bf16: 15.5
+      // with one, 12 with two, 12.5 with four; 4 tokens 34.5, 30 and 27)
       const double mine = used * std::ceil(N / 32);
       r.width = 1;
       r.shares = mine < 256 || (mine < 1024 && K >= 2048) ? 4 : K >= 1536 ? 2 : 1;

@@ -14,13 +14,16 @@
 // Where the columns are long and the workgroups few, several share a tile's columns;
 // a second launch adds their sums in order.
 //
-// Measured (a large copy moves 5.0 TB/s here, a large bf16 library product reaches 1.39
+// Measured (a large copy moves 4.94 TB/s here, a large bf16 library product reaches 1.35
 // PFLOP/s): gate and up, 1536 x 4096, of 4096 tokens of 10 of 128 experts, MXFP4 by
-// bf16, 854 us: 1.21 PFLOP/s, the matrix cores. Down, 4096 x 1536, of 2048 such tokens
-// in bf16 441 us: 1.6 GB of weights and 336 MB of fp32 results, 4.6 TB/s. Down of 4096
-// tokens of 8 of 256 experts, 6144 x 2048, MXFP4 by MXFP4, 568 us: 1.7 GB and 805 MB, 4.5
-// TB/s. Where rows are few it is the weights' bytes: 512 tokens of those experts' gate
-// and up 581 us, 5.9 TB/s; 64 tokens of 10 of 128 in bf16 508 us, 6.1 TB/s.
+// bf16, 868 us: 1.19 PFLOP/s, the matrix cores; in bf16 1181 us, 0.87 PFLOP/s. Down, 4096
+// x 1536, of 2048 such tokens in bf16 447 us: 1.6 GB of weights and 336 MB of fp32
+// results, 4.5 TB/s. Down of 4096 tokens of 8 of 256 experts, 6144 x 2048, MXFP4 by
+// MXFP4, 568 us: 1.7 GB and 805 MB, 4.5 TB/s. Where rows are few it is the weights'
+// bytes: 512 tokens of those experts' gate and up 579 us, 5.9 TB/s; 64 tokens of 10 of
+// 128 in bf16 507 us, 6.1 TB/s. Short columns pay for each tile's start and end: down of
+// 5620 tokens of 8 of 64 experts, 2048 x 768 in bf16, 204 us, 0.69 PFLOP/s; of 6863 in
+// MXFP4 153 us, 2.0 TB/s.
 // Tiles of 256 rows by eight wavefronts were slower, as were results stored past the
 // caches.
 #include "experts_dev.hpp"
