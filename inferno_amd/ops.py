@@ -269,7 +269,7 @@ class _Packed:
         allocator gives the packed bytes to the stream that they were packed on; of each
         other stream it is told once, and then waits for what is queued there. (Of a
         graph's replays it cannot know: the handle has to outlive the graph.)"""
-        stream = _raw_stream(self.device.index)
+        stream = _raw_stream(_dev(x).get_device())
         if stream not in self._streams:
             with torch.cuda.device(self.device):
                 if not torch.cuda.is_current_stream_capturing():

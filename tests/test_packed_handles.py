@@ -32,12 +32,13 @@ def test_each_other_stream_is_told_of_once(monkeypatch, kind):
     monkeypatch.setattr(torch.cuda, "device", lambda dev: contextlib.nullcontext())
     h = kind.__new__(kind)
     h.device, h.ref, data = torch.device("cuda:0"), object(), _Bytes()
+    x = SimpleNamespace(is_cuda=True, get_device=lambda: 0)
     now["capturing"] = True  # (nothing to wait for here)
     h._hold(data)
     for stream, capturing, told in [(5, False, []), (7, True, []), (7, False, [7]), (7, False, [7]),
                                     (5, False, [7]), (9, False, [7, 9]), (7, True, [7, 9])]:
         now.update(stream=stream, capturing=capturing)
-        assert h._on(None) is h.ref and data.told == told
+        assert h._on(x) is h.ref and data.told == told
 
 
 def _experts(g, fp4):
