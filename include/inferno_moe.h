@@ -344,7 +344,9 @@ int inferno_experts_pack(void* stream, const inferno_experts* w, const void* wei
  * bytes; x_rows k <= 2^22, and with more than 2^24 workgroups, which needs some 10^10
  * results, a call is refused. x_rows = 0 does nothing. The workspace takes
  * inferno_grouped_workspace_bytes at a multiple of 16 bytes (NULL where that is 0,
- * as it is for most products); calls that overlap need one each. */
+ * as it is for most products); calls that overlap need one each. Its matrices is 1
+ * for grouped_matmul and 2 for gate and up, grouped says whether offsets are given; of
+ * arguments that a product refuses it is 0, with an error. */
 size_t inferno_grouped_workspace_bytes(const inferno_experts* w, int matrices, int x_dtype,
                                        size_t x_rows, size_t k, int grouped);
 int inferno_grouped_matmul(void* stream, const inferno_experts* w, const void* x, int x_dtype,

@@ -63,6 +63,22 @@ ExpertProduct product(const inferno_experts* w0, const inferno_experts* w1, cons
   return p;
 }
 
+int check_x_dtype(const inferno_experts* w, int x_dtype) {
+  INF_CHECK_ARG(x_dtype == INFERNO_BF16 || (x_dtype == INFERNO_MXFP4 && w->format == INFERNO_MXFP4),
+                "x dtype must be BF16, or MXFP4 with weights in MXFP4");
+  return INFERNO_OK;
+}
+
+int check_kind(const inferno_experts* w, int matrices, int x_dtype) {
+  INF_CHECK_ARG(matrices == 1 || matrices == 2, "matrices must be 1 or 2");
+  return check_x_dtype(w, x_dtype);
+}
+
+int check_rows(size_t x_rows, size_t k) {
+  INF_CHECK_ARG(x_rows <= kMostRows && k <= kMostRows && x_rows * k <= kMostRows, "too many rows");
+  return INFERNO_OK;
+}
+
 int check_form(const ExpertPlan& plan) {
   INF_CHECK_ARG(plan.width > 0, "INFERNO_EXPERTS_FORM names no form of this product");
   return INFERNO_OK;
@@ -74,14 +90,13 @@ int run_product(void* stream, const inferno_experts* w0, const inferno_experts* 
                 size_t workspace_bytes) {
   INF_CHECK_ARG(out_dtype == INFERNO_F32 || out_dtype == INFERNO_BF16,
                 "out dtype must be F32 or BF16");
-  INF_CHECK_ARG(x_dtype == INFERNO_BF16 || (x_dtype == INFERNO_MXFP4 && w0->format == INFERNO_MXFP4),
-                "x dtype must be BF16, or MXFP4 with weights in MXFP4");
+  if (int st = check_x_dtype(w0, x_dtype)) return st;
   INF_CHECK_ARG(k > 0, "k must be positive");
   INF_CHECK_ARG(k == 1 || sorted, "several result rows per input row need sorted");
   INF_CHECK_ARG(!sorted || offsets, "sorted rows need the experts' offsets");
   INF_CHECK_ARG(offsets || w0->experts == 1, "several experts need offsets");
   if (x_rows == 0) return INFERNO_OK;
-  INF_CHECK_ARG(x_rows <= kMostRows && k <= kMostRows && x_rows * k <= kMostRows, "too many rows");
+  if (int st = check_rows(x_rows, k)) return st;
   INF_CHECK_ARG(x && out, "null pointer");
   INF_CHECK_ARG((x_dtype == INFERNO_MXFP4) == (x_scales != nullptr),
                 "x_scales belong to MXFP4 rows, which need them");
@@ -155,9 +170,8 @@ int inferno_experts_pack(void* stream, const inferno_experts* w, const void* wei
 size_t inferno_grouped_workspace_bytes(const inferno_experts* w, int matrices, int x_dtype,
                                        size_t x_rows, size_t k, int grouped) {
   clear_error();
-  if (check_shape("given", w) || x_rows > kMostRows || k > kMostRows || x_rows * k > kMostRows ||
-      x_rows * k == 0)
-    return 0;
+  if (check_shape("given", w) || check_kind(w, matrices, x_dtype)) return 0;
+  if (check_rows(x_rows, k) || x_rows * k == 0) return 0;
   static const uint8_t scale = 127;  // (only whether there are scales and offsets counts)
   static const uint32_t offset = 0;
   const ExpertProduct p = product(w, matrices == 2 ? w : nullptr,
