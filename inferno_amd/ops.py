@@ -194,14 +194,19 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
-def _run(x, fn, *args):
-    """fn(stream, *args) on x's device and that device's current stream."""
+def _run(x, fn, *args, held=()):
+    """fn(stream, *args) on x's device and that device's current stream, which reads the
+    packed weights of the handles ``held``."""
     dev = _dev(x).get_device()
     if dev == torch.cuda.current_device():
-        check(fn(_raw_stream(dev), *args))
+        stream = _raw_stream(dev)
+        for h in held:
+            if stream not in h._streams:
+                h._tell(stream)
+        check(fn(stream, *args))
     else:
         with torch.cuda.device(dev):
-            check(fn(_raw_stream(dev), *args))
+            _run(x, fn, *args, held=held)
 
 
 def add_rms_norm_q8(x, residual, w, eps, group=0, act_dtype=torch.float32, out=None):
@@ -264,18 +269,15 @@ class _Packed:
             if not capturing:
                 stream.synchronize()
 
-    def _on(self, x):
-        """``ref``, for a call on x's current stream. When the handle goes, the
-        allocator gives the packed bytes to the stream that they were packed on; of each
-        other stream it is told once, and then waits for what is queued there. (Of a
-        graph's replays it cannot know: the handle has to outlive the graph.)"""
-        stream = _raw_stream(_dev(x).get_device())
-        if stream not in self._streams:
-            with torch.cuda.device(self.device):
-                if not torch.cuda.is_current_stream_capturing():
-                    self._data.record_stream(torch.cuda.current_stream(self.device))
-                    self._streams.add(stream)
-        return self.ref
+    def _tell(self, stream):
+        """Of the current stream, another than the packing's, before its first call. When
+        the handle goes, the allocator gives the packed bytes to the stream that they
+        were packed on; of each other one it is told once, and then waits for what is
+        queued there. (Of a graph's replays it cannot know: the handle has to outlive the
+        graph.)"""
+        if not torch.cuda.is_current_stream_capturing():
+            self._data.record_stream(torch.cuda.current_stream(self.device))
+            self._streams.add(stream)
 
 
 class W4(_Packed):
@@ -355,8 +357,8 @@ def w4_matvec_add2(w, x, residual_a=None, residual_b=None, x_scales=None):
     out = torch.empty(T, w.rows, dtype=torch.float32, device=x.device)
     n = lib().inferno_w4_workspace_bytes(T, w.cols)
     ws = _w4_ws(x, n)
-    _run(x, lib().inferno_w4_matvec_add2, w._on(x), _at(x), dt, xs, xg, _at(residual_a),
-         _at(residual_b), T, _at(out), _at(ws), n)
+    _run(x, lib().inferno_w4_matvec_add2, w.ref, _at(x), dt, xs, xg, _at(residual_a),
+         _at(residual_b), T, _at(out), _at(ws), n, held=(w,))
     return out
 
 
@@ -369,8 +371,8 @@ def w4_gate_up_swiglu(gate, up, x, x_scales=None):
     out = torch.empty(T, gate.rows, dtype=torch.float32, device=x.device)
     n = lib().inferno_w4_workspace_bytes(T, gate.cols)
     ws = _w4_ws(x, n)
-    _run(x, lib().inferno_w4_gate_up_swiglu, gate._on(x), up._on(x), _at(x), dt, xs, xg, T,
-         _at(out), _at(ws), n)
+    _run(x, lib().inferno_w4_gate_up_swiglu, gate.ref, up.ref, _at(x), dt, xs, xg, T, _at(out),
+         _at(ws), n, held=(gate, up))
     return out
 
 
@@ -388,8 +390,8 @@ def w4_moe(gate, up, down, x, ids, weights, k, x_scales=None):
     out = torch.empty(T, H, dtype=torch.float32, device=x.device)
     n = lib().inferno_w4_moe_workspace_bytes(T, k, gate.experts, H, gate.rows)
     ws = _w4_ws(x, n)
-    _run(x, lib().inferno_w4_moe, gate._on(x), up._on(x), down._on(x), _at(x), dt, xs, xg,
-         _at(ids), _at(weights), T, k, _at(out), _at(ws), n)
+    _run(x, lib().inferno_w4_moe, gate.ref, up.ref, down.ref, _at(x), dt, xs, xg, _at(ids),
+         _at(weights), T, k, _at(out), _at(ws), n, held=(gate, up, down))
     return out
 
 
@@ -476,8 +478,8 @@ def _grouped(fn, mats, x, x_scales, offsets, sorted_, k, out_dtype, out):
     dt = MXFP4 if fp4 else BF16
     n = lib().inferno_grouped_workspace_bytes(w.ref, len(mats), dt, T, k, offsets is not None)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    _run(x, fn, *(m._on(x) for m in mats), _at(x), dt, _at(x_scales), T, _at(offsets), _at(sorted_),
-         k, _DT[out.dtype], _at(out), _at(ws), n)
+    _run(x, fn, *(m.ref for m in mats), _at(x), dt, _at(x_scales), T, _at(offsets), _at(sorted_), k,
+         _DT[out.dtype], _at(out), _at(ws), n, held=mats)
     return out
 
 

@@ -27,18 +27,20 @@ class _Bytes:
 def test_each_other_stream_is_told_of_once(monkeypatch, kind):
     now = {"stream": 5, "capturing": False}
     monkeypatch.setattr(ops, "_raw_stream", lambda dev: now["stream"])
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: now["stream"])
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
     monkeypatch.setattr(torch.cuda, "device", lambda dev: contextlib.nullcontext())
     h = kind.__new__(kind)
-    h.device, h.ref, data = torch.device("cuda:0"), object(), _Bytes()
-    x = SimpleNamespace(is_cuda=True, get_device=lambda: 0)
+    h.device, data = torch.device("cuda:0"), _Bytes()
+    x, calls = SimpleNamespace(is_cuda=True, get_device=lambda: 0), []
     now["capturing"] = True  # (nothing to wait for here)
     h._hold(data)
     for stream, capturing, told in [(5, False, []), (7, True, []), (7, False, [7]), (7, False, [7]),
                                     (5, False, [7]), (9, False, [7, 9]), (7, True, [7, 9])]:
         now.update(stream=stream, capturing=capturing)
-        assert h._on(x) is h.ref and data.told == told
+        ops._run(x, lambda s, a: calls.append((s, a)) or 0, "a", held=(h, h))
+        assert calls.pop() == (stream, "a") and data.told == told
 
 
 def _experts(g, fp4):
