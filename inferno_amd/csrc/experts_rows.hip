@@ -12,7 +12,7 @@
 //
 // One token, microseconds of a call among others: down of 8 of 256 experts, 6144 x
 // 2048 in MXFP4, 12.0 (4.5 TB/s); gate and up of 8 of 64 experts, 768 x 2048 in bf16,
-// 11.3 (4.5 TB/s); gate and up of a shared expert, 1536 x 4096 in MXFP4, 8.8, where a
+// 11.3 (4.5 TB/s); gate and up of a shared expert, 1536 x 4096 in MXFP4, 8.5, where a
 // launch of nothing takes 6.2. With twice as many chunks ahead the three launches take,
 // from one to the next of a graph, 16.2, 15.2 and 6.4 in place of 14.1, 13.3 and 6.6;
 // with four times as many in MXFP4 the first takes 21 and the last 7.2.
